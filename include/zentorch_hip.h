@@ -346,6 +346,145 @@ int zt_woq_moe(const void *x, int64_t T, int64_t H, const int32_t *topk_ids,
 size_t zt_woq_moe_workspace_size(int64_t T, int64_t H, int64_t topk, int64_t E,
                                  int64_t I);
 
+/*
+ * The paged key / value cache around the quantised linears (no counterpart
+ * in the reference, whose attention keeps no cache of its own).
+ *
+ * One layer's cache holds `pages` pages of page_size tokens for each of its
+ * heads; element d of token `off` of page p and head h is at
+ *   k + p * k_strides[0] + h * k_strides[1] + off * k_strides[2] + d
+ * (strides in elements), and v likewise.  Sequence i's tokens lie in the
+ * pages that row i of block_table [S, W] names, in order, and context_lens[i]
+ * counts them.  A page's reference count is the number of table rows that
+ * name it; a page with count 0 is free.  Page ids, slots and positions come
+ * from the device, so no call can refuse a bad one: each says what it does
+ * with it, and none reads or writes outside the arrays for it.
+ */
+typedef struct zt_kv_cache {
+  void *k, *v;
+  int32_t dtype; /* bf16 or fp32 */
+  int64_t pages, heads, page_size, head_dim;
+  int64_t k_strides[3], v_strides[3]; /* page, head, token */
+} zt_kv_cache;
+
+/*
+ * Rotary positions: pair i of a head row at position p turns by the angle
+ * whose cosine is table[p][i] and sine table[p][R / 2 + i] (any scaling for
+ * long contexts is in the table):
+ *   (a, b) -> (a cos - b sin, b cos + a sin)     in fp32, rounded once.
+ * The pairs are (x[i], x[R / 2 + i]), or (x[2i], x[2i + 1]) if interleaved;
+ * x[R .. D) passes through.
+ *
+ *  x          [T, H, D] bf16 or fp32, token and head strides in elements
+ *  positions  [T] int64.  A negative one marks padding: the row passes
+ *             through.  One past the table gives NaN.
+ *  table      [length, ld_table] fp32, R columns used, R even, R <= D
+ *  out        [T, H, D] contiguous, another array than x
+ */
+int zt_rotary_embedding(const void *x, int32_t dtype, int64_t T, int64_t H, int64_t D,
+                        int64_t ld_token, int64_t ld_head, const int64_t *positions,
+                        const float *table, int64_t length, int64_t R, int64_t ld_table,
+                        int32_t interleaved, void *out, zt_stream_t stream);
+
+/*
+ * A step's new tokens into one layer's cache: q_out = rotary(q), and for
+ * each token the rotated key and the value of every cache head to its slot
+ * (page * page_size + place in the page).  q [T, H, D], k and v
+ * [T, cache->heads, D] in the cache's type, with strides of token and head.
+ * A slot outside the cache marks a padding token: nothing is stored for it.
+ * Two tokens must not share a slot.
+ */
+int zt_rotary_cache_append(const void *q, int64_t T, int64_t H, const int64_t *q_strides,
+                           const void *k, const int64_t *k_strides, const void *v,
+                           const int64_t *v_strides, const int64_t *positions,
+                           const float *table, int64_t length, int64_t R, int64_t ld_table,
+                           int32_t interleaved, const int64_t *slots, const zt_kv_cache *cache,
+                           void *q_out, zt_stream_t stream);
+
+/*
+ * Attention of a chunk of new tokens over one layer's cache, which holds
+ * their keys and values already:
+ *   out_r = sum_j softmax_j(scale * q_r . k_j) v_j
+ * Sequence i's new tokens are rows cu_seqlens[i] .. cu_seqlens[i + 1] of q
+ * and its last ones in the cache.  Query head h reads cache head h / (H /
+ * heads).  Causal: a token sees the positions up to its own, with a window
+ * only the last `window` of them (0: all).  Otherwise it sees all
+ * context_lens[i].  Keys in pages outside the cache are not seen, and a row
+ * that sees no key is zero, as is a row past cu_seqlens[S].
+ * Scores, softmax and sums are fp32.
+ *
+ *  q          [T, H, head_dim] in the cache's type, strides in elements; all
+ *             rows (q, cache, out) start on 16 bytes
+ *  cu_seqlens [S + 1] int32 ascending from 0; context_lens [S] int32
+ *  max_query_len  the longest chunk; it picks the kernels, and too small a
+ *             value costs time, not results
+ *  head_dim   a multiple of 8, at most 256
+ *  workspace  zt_paged_attention_workspace_size(...) bytes, 16-byte aligned
+ */
+int zt_paged_attention(const void *q, int64_t T, int64_t H, int64_t ld_token, int64_t ld_head,
+                       const zt_kv_cache *cache, const int32_t *block_table, int64_t S, int64_t W,
+                       const int32_t *cu_seqlens, const int32_t *context_lens,
+                       int64_t max_query_len, int32_t causal, int64_t window, float scale,
+                       void *out, void *workspace, size_t workspace_bytes, zt_stream_t stream);
+
+size_t zt_paged_attention_workspace_size(int64_t T, int64_t H, const zt_kv_cache *cache, int64_t S,
+                                         int64_t W, int64_t max_query_len);
+
+/*
+ * Pages for a step's new tokens: sequence i grows by cu_seqlens[i + 1] -
+ * cu_seqlens[i] tokens.  Free pages are given out lowest first, sequence by
+ * sequence.  A sequence whose tokens would not fit its table row is not
+ * granted and takes none; from the first one that the free pages do not
+ * suffice for, none is.  A sequence that is not granted keeps its row and
+ * length, and its tokens get position and slot -1.  Every output is written
+ * whole: table_out [S, W], context_out [S], refs_out [pages], and for each
+ * token its position and its slot [T] (-1 for tokens of no sequence).
+ * S <= 4096, W * page_size < 2^31.
+ */
+int zt_cache_extend(const int32_t *block_table, const int32_t *context_lens,
+                    const int32_t *ref_counts, const int32_t *cu_seqlens, int64_t S, int64_t W,
+                    int64_t pages, int64_t page_size, int64_t T, int32_t *table_out,
+                    int32_t *context_out, int32_t *refs_out, int64_t *positions, int64_t *slots,
+                    zt_stream_t stream);
+
+/*
+ * Row i of the next step continues row parents[i] of this one (outside
+ * [0, S): it ends).  Children share their parent's full pages; its partly
+ * filled last page stays with the first child, and each further child gets a
+ * free page (the lowest, in row order, the ended rows' pages among them) to
+ * which copies[i] = (from, to) asks for it to be copied.  Other rows of
+ * copies [S, 2] are -1.  A row that finds no free page ends (length 0).
+ * Outputs as zt_cache_extend's; S <= 4096.
+ */
+int zt_cache_fork(const int32_t *block_table, const int32_t *context_lens,
+                  const int32_t *ref_counts, const int32_t *parents, int64_t S, int64_t W,
+                  int64_t pages, int64_t page_size, int32_t *table_out, int32_t *context_out,
+                  int32_t *refs_out, int32_t *copies, zt_stream_t stream);
+
+/*
+ * The n pages in use gather in the pool's first n: the k-th page in use past
+ * them (ascending) moves to the k-th free page among them.  copies
+ * [pages / 2, 2] holds the (from, to) pairs, then -1; table_out (any number
+ * of entries) and refs_out follow the moves.  The caller copies the pages
+ * (zt_cache_copy_pages) of every layer.
+ */
+int zt_cache_compact(const int32_t *block_table, int64_t entries, const int32_t *ref_counts,
+                     int64_t pages, int32_t *table_out, int32_t *refs_out, int32_t *copies,
+                     void *workspace, size_t workspace_bytes, zt_stream_t stream);
+
+size_t zt_cache_compact_workspace_size(int64_t pages);
+
+/*
+ * Page `to` of every cache becomes a copy of page `from`, for each pair of
+ * copies [n_copies, 2]; a pair with an id outside [0, pages) is none.  caches
+ * is a HOST array of device pointers (read before the call returns), each to
+ * `pages` pages of page_bytes bytes, page_stride_bytes apart.  No `to` may be
+ * another pair's `from` or `to`.
+ */
+int zt_cache_copy_pages(void *const *caches, int64_t n_caches, int64_t pages, int64_t page_bytes,
+                        int64_t page_stride_bytes, const int32_t *copies, int64_t n_copies,
+                        zt_stream_t stream);
+
 /* Message of the calling thread's last failed call ("" if none). */
 const char *zt_last_error_string(void);
 

@@ -29,8 +29,8 @@ ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 HIPCC = os.path.join(ROCM, "bin", "hipcc")
 
 HIP_SOURCES = ["woq_kernels.hip", "woq_prefill.hip", "dynq_kernels.hip", "s8_prefill.hip",
-               "moe_kernels.hip", "capi.hip"]
-TORCH_SOURCES = ["ops.cpp", "shim_cuda_zentorch.cpp"]
+               "moe_kernels.hip", "kv_cache.hip", "paged_attn.hip", "capi.hip", "capi_cache.hip"]
+TORCH_SOURCES = ["ops.cpp", "ops_cache.cpp", "shim_cuda_zentorch.cpp"]
 
 # -packed-fp32-ops: no v_pk_*_f32 from the compiler (hipcc's host pass warns
 # it does not know the feature; that warning is harmless).

@@ -12,6 +12,7 @@
 
 #include <algorithm>
 
+#include "zt_cache.hpp"
 #include "zt_launch.hpp"
 #include "zt_tuning.hpp"
 
@@ -19,14 +20,25 @@ namespace {
 
 thread_local std::string g_last_error;
 
+// Keeps the message; without one where memory is short, so that nothing is
+// thrown through a C entry point.
+int vfail(int code, const char *fmt, va_list ap) {
+  char buf[512];
+  std::vsnprintf(buf, sizeof(buf), fmt, ap);
+  try {
+    g_last_error = buf;
+  } catch (...) {
+    g_last_error.clear();
+  }
+  return code;
+}
+
 int fail(int code, const char *fmt, ...) __attribute__((format(printf, 2, 3)));
 int fail(int code, const char *fmt, ...) {
-  char buf[512];
   va_list ap;
   va_start(ap, fmt);
-  std::vsnprintf(buf, sizeof(buf), fmt, ap);
+  vfail(code, fmt, ap);
   va_end(ap);
-  g_last_error = buf;
   return code;
 }
 
@@ -103,6 +115,14 @@ hipError_t woq_row_blocks(const zt::WoqArgs &a, hipStream_t s) {
 }
 
 }  // namespace
+
+int zt::api_fail(int code, const char *fmt, ...) {
+  va_list ap;
+  va_start(ap, fmt);
+  vfail(code, fmt, ap);
+  va_end(ap);
+  return code;
+}
 
 // ------------------------------------------------------------ tuning knobs
 namespace zt {

@@ -13,11 +13,7 @@
 // There is no CPU kernel: a CPU tensor reaching these ops is an error, not a
 // fallback.
 #include <ATen/ATen.h>
-#include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
-#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <torch/library.h>
-
-#include <rocprofiler-sdk-roctx/roctx.h>
 
 #include <algorithm>
 #include <deque>
@@ -26,45 +22,12 @@
 #include <vector>
 
 #include "ops.hpp"
+#include "ops_util.hpp"
 #include "zentorch_hip.h"
 
 namespace zentorch_hip {
 
 namespace {
-
-int32_t zt_dtype_of(const at::Tensor &t) {
-  switch (t.scalar_type()) {
-  case at::kFloat: return ZT_DT_F32;
-  case at::kBFloat16: return ZT_DT_BF16;
-  case at::kHalf: return ZT_DT_F16;
-  case at::kChar: return ZT_DT_S8;
-  case at::kByte: return ZT_DT_U8;
-  case at::kInt: return ZT_DT_S32;
-  default: return ZT_DT_NONE;
-  }
-}
-
-void check_device(const at::Tensor &t, const at::Tensor &ref, const char *op,
-                  const char *name) {
-  TORCH_CHECK(t.is_cuda(), op, ": ", name,
-              " must be a GPU tensor (zentorch-mi355x has no CPU kernels), got ",
-              t.device());
-  TORCH_CHECK(t.device() == ref.device(), op, ": ", name, " is on ", t.device(),
-              " but input is on ", ref.device());
-}
-
-hipStream_t current_stream() {
-  return c10::hip::getCurrentHIPStreamMasqueradingAsCUDA().stream();
-}
-
-// Device workspace of one call, from torch's stream-ordered caching
-// allocator.  It is released when the call returns; the allocator hands the
-// block to later work on the same stream only, and inside a HIP graph
-// capture it comes from the graph's private pool, so a captured call keeps
-// its own workspace on every replay.
-at::Tensor call_workspace(const at::Tensor &like, size_t bytes) {
-  return at::empty({(int64_t)std::max<size_t>(bytes, 1)}, like.options().dtype(at::kByte));
-}
 
 std::vector<int64_t> out_sizes(const at::Tensor &input, int64_t N) {
   auto s = input.sizes().vec();
@@ -97,14 +60,6 @@ at::Tensor rows_view(const at::Tensor &t, int64_t *ld) {
   *ld = K;
   return as_2d(t);
 }
-
-// The reference hands zentorch_op_name to ZenDNNL's profiler
-// (MatmulUtils.hpp:763); here it names a ROCTx range around the launches,
-// which rocprofv3 --marker-trace records.
-struct OpRange {
-  explicit OpRange(const std::string &name) { roctxRangePushA(name.c_str()); }
-  ~OpRange() { roctxRangePop(); }
-};
 
 // Shared body of every zentorch_woq_linear* op.  post_ids follow the
 // reference's post-op numbering; binary ops take binary_inputs in order.

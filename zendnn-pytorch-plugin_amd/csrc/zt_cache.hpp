@@ -1,0 +1,87 @@
+// Launch interface of the paged key / value cache's kernels (kv_cache.hip,
+// paged_attn.hip), shared with the C-ABI layer (capi_cache.hip).
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "zt_common.hpp"
+
+namespace zt {
+
+// Sets the calling thread's error message and returns `code` (capi.hip).
+int api_fail(int code, const char *fmt, ...) __attribute__((format(printf, 2, 3)));
+
+struct RotaryArgs {
+  const void *q, *k, *v;      // [T, H | KV | KV, D], unit last stride
+  int64_t q_ld[2], k_ld[2], v_ld[2];  // token and head strides, elements
+  void *q_out;                // [T, H, D]
+  void *k_cache, *v_cache;    // strides of page, head, token
+  int64_t kc_ld[3], vc_ld[3];
+  const int64_t *pos, *slots;
+  const float *table;         // [length, R]: cos, then sin
+  int64_t length, table_ld, pages;
+  int64_t T;
+  int H, KV, D, R, page_size;
+  bool interleaved;
+  // units of 16 bytes (or of one element) per rotated row, per copied row and
+  // per token, set by launch_rotary
+  int row_units, copy_units, units;
+};
+hipError_t launch_rotary(RotaryArgs a, int dtype, bool wide, hipStream_t s);
+
+struct ExtendArgs {
+  const int32_t *table, *ctx, *refs, *cu;  // [S, W], [S], [pages], [S + 1]
+  int S, W, page_size;
+  int64_t pages, T;
+  int32_t *table_out, *ctx_out, *refs_out;
+  int64_t *pos_out, *slots;  // [T]
+};
+hipError_t launch_cache_extend(const ExtendArgs &a, hipStream_t s);
+
+struct ForkArgs {
+  const int32_t *table, *ctx, *refs, *parents;
+  int S, W, page_size;
+  int64_t pages;
+  int32_t *table_out, *ctx_out, *refs_out, *copies;  // copies [S, 2]
+};
+hipError_t launch_cache_fork(const ForkArgs &a, hipStream_t s);
+
+struct CompactArgs {
+  const int32_t *table, *refs;
+  int64_t entries, pages;
+  int32_t *table_out, *refs_out, *copies;  // copies [pages / 2, 2]
+  int32_t *to;                             // [pages] workspace
+};
+hipError_t launch_cache_compact(const CompactArgs &a, hipStream_t s);
+
+constexpr int kCopyCaches = 64;  // caches of one launch
+struct CopyArgs {
+  void *caches[kCopyCaches];
+  const int32_t *copies;
+  int64_t pages, page_stride, page_bytes;  // bytes
+  int parts;
+};
+hipError_t launch_copy_pages(CopyArgs a, int caches, int64_t pairs, bool wide, hipStream_t s);
+
+struct AttnArgs {
+  const void *q;  // [T, H, D]
+  int64_t q_ld[2];
+  const void *k, *v;  // strides of page, head, token
+  int64_t k_ld[3], v_ld[3];
+  const int32_t *table, *cu, *ctx;  // [S, W], [S + 1], [S]
+  int64_t T, pages, max_q;
+  int H, KV, D, S, W, page_size;
+  int dtype;
+  bool causal;
+  int64_t window;
+  float scale;
+  void *out;  // [T, H, D]
+};
+size_t paged_attn_workspace(const AttnArgs &a);
+hipError_t launch_paged_attn(const AttnArgs &a, void *workspace, hipStream_t s);
+
+}  // namespace zt

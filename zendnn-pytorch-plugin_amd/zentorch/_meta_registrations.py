@@ -169,3 +169,51 @@ def meta_zentorch_fused_moe(output, input, w13, w2, w13_bias, w2_bias, topk_weig
                             zentorch_op_name="zentorch::zentorch_fused_moe"):
     # writes `output` in place and returns nothing (FusedMoE.cpp:728-736)
     return None
+
+
+@register_meta("zentorch_rotary_embedding")
+def meta_zentorch_rotary_embedding(input, positions, cos_sin, *, interleaved=False,
+                                   zentorch_op_name=""):
+    return input.new_empty(input.size())
+
+
+@register_meta("zentorch_rotary_cache_append")
+def meta_zentorch_rotary_cache_append(query, key, value, positions, cos_sin, slots, key_cache,
+                                      value_cache, *, interleaved=False, zentorch_op_name=""):
+    # the rotated query; the caches are written in place
+    return query.new_empty(query.size())
+
+
+@register_meta("zentorch_paged_attention")
+def meta_zentorch_paged_attention(query, key_cache, value_cache, block_table, cu_seqlens,
+                                  context_lens, max_query_len, *, causal=True, window=0,
+                                  scale=None, zentorch_op_name=""):
+    return query.new_empty(query.size())
+
+
+@register_meta("zentorch_cache_extend")
+def meta_zentorch_cache_extend(block_table, context_lens, ref_counts, cu_seqlens, page_size,
+                               num_tokens, *, zentorch_op_name=""):
+    # the new table, lengths and counts, and each token's position and slot
+    return (block_table.new_empty(block_table.size()), context_lens.new_empty(context_lens.size()),
+            ref_counts.new_empty(ref_counts.size()),
+            block_table.new_empty((num_tokens,), dtype=torch.int64),
+            block_table.new_empty((num_tokens,), dtype=torch.int64))
+
+
+@register_meta("zentorch_cache_fork")
+def meta_zentorch_cache_fork(block_table, context_lens, ref_counts, parents, page_size, *,
+                             zentorch_op_name=""):
+    return (block_table.new_empty(block_table.size()), context_lens.new_empty(context_lens.size()),
+            ref_counts.new_empty(ref_counts.size()), context_lens.new_empty((parents.size(0), 2)))
+
+
+@register_meta("zentorch_cache_compact")
+def meta_zentorch_cache_compact(block_table, ref_counts, *, zentorch_op_name=""):
+    return (block_table.new_empty(block_table.size()), ref_counts.new_empty(ref_counts.size()),
+            ref_counts.new_empty((ref_counts.size(0) // 2, 2)))
+
+
+@register_meta("zentorch_cache_copy_pages")
+def meta_zentorch_cache_copy_pages(caches, copies, *, zentorch_op_name=""):
+    return None
