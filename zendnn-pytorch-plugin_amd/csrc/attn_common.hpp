@@ -1,0 +1,194 @@
+// Device helpers shared by the attention kernels (paged_attn.hip,
+// paged_attn_tile.hip): which keys a tile of rows sees, and how the keys of
+// all tiles are dealt out to the workgroups.
+//
+// A *row* is one query token of one head.  The rows of sequence i that read
+// cache head h are numbered token-major: row x is token x / G, head h * G + x %
+// G, with G = H / KV query heads to a cache head, so a cached key or value is
+// read once for all G of them.  An *item* is a tile of BM such rows (of any
+// one cache head); it needs the keys of blocks [b0, b1) of UK keys.
+//
+// Work is dealt out in units of one block of one item and cache head, laid
+// end to end (item by item, in it head by head, in it block by block), in
+// equal spans, one per workgroup.  The lengths are known on the device only,
+// so each workgroup finds its span by itself.  A span may end inside an
+// (item, head): its workgroups then leave partial results (running maximum,
+// sum and output), which a second launch joins.  That keeps every compute unit
+// busy for one long sequence as for many ragged ones.
+#pragma once
+
+#include "zt_cache.hpp"
+
+namespace zt {
+
+// 1 KB of zeros: what a lane reads in place of a key or value that is not
+// there, so that weights of zero never meet a NaN or an infinity.
+static __device__ const u32x4_t kZeroRow[64] = {};
+
+struct Seq {
+  int q0, q, n;  // first row of the batch, new tokens, all tokens
+};
+
+__device__ __forceinline__ Seq seq_of(const AttnArgs &a, int i) {
+  const int T = (int)a.T;
+  const int q0 = min(max(a.cu[i], 0), T);
+  return {q0, min(max(a.cu[i + 1], q0), T) - q0, min(max(a.ctx[i], 0), a.W * a.page_size)};
+}
+
+// Keys [begin, end) that some row of tile r sees.
+struct KeyRange {
+  int begin, end;
+};
+__device__ __forceinline__ KeyRange keys_of(const AttnArgs &a, const Seq &s, int r, int BM) {
+  KeyRange k{0, s.n};
+  if (a.causal) {
+    const int first = s.n - s.q + (int)fast_div((uint32_t)r * BM, a.div_group);
+    const int last = s.n - s.q + min((int)fast_div((uint32_t)r * BM + BM - 1, a.div_group), s.q - 1);
+    k.end = max(last + 1, 0);
+    if (a.window) k.begin = (int)max((int64_t)first + 1 - a.window, (int64_t)0);
+  }
+  if (k.begin >= k.end) k.begin = k.end = 0;
+  return k;
+}
+__device__ __forceinline__ int blocks_of(const KeyRange &k, int UK) {
+  return k.end > k.begin ? (k.end + UK - 1) / UK - k.begin / UK : 0;
+}
+
+// Exclusive prefix sum over the workgroup; `part` holds N / 64 values.
+template <int N>
+__device__ __forceinline__ int64_t scan64(int64_t v, int64_t *part, int64_t *total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int64_t x = v;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int64_t y = __shfl_up((long long)x, d);
+    if (lane >= d) x += y;
+  }
+  __syncthreads();
+  if (lane == 63) part[wave] = x;
+  __syncthreads();
+  int64_t before = 0, sum = 0;
+#pragma unroll
+  for (int w = 0; w < N / 64; ++w) {
+    const int64_t y = part[w];
+    if (w < wave) before += y;
+    sum += y;
+  }
+  *total = sum;
+  return before + x - v;
+}
+
+struct PlanShared {
+  int64_t part[16];
+  int64_t off;
+  int item;
+};
+
+struct Plan {
+  int items;
+  int64_t per;   // units of a span
+  int64_t todo;  // units of this workgroup's span
+  int item;      // the item of its first unit
+  int64_t off;   // and that unit's place among the item's units
+};
+
+// The sequence of item x: the last i with tile_base[i] <= x.
+__device__ __forceinline__ int seq_of_item(const int *tile_base, int S, int x) {
+  int lo = 0, hi = S - 1;
+  while (lo < hi) {
+    const int m = (lo + hi + 1) / 2;
+    if (tile_base[m] <= x) lo = m;
+    else hi = m - 1;
+  }
+  return lo;
+}
+
+// tile_base[S + 1] (LDS): items before sequence i's.  N threads.
+template <int N>
+__device__ __forceinline__ Plan make_plan(const AttnArgs &a, int BM, int UK, int *tile_base,
+                                          PlanShared *sh) {
+  const int tid = threadIdx.x;
+  Plan p{};
+  int64_t items = 0;
+  for (int i0 = 0; i0 < a.S; i0 += N) {
+    const int i = i0 + tid;
+    int64_t tiles = 0, total;
+    if (i < a.S) tiles = ((int64_t)seq_of(a, i).q * a.group + BM - 1) / BM;
+    const int64_t before = scan64<N>(tiles, sh->part, &total);
+    if (i < a.S) tile_base[i] = (int)(items + before);
+    items += total;
+  }
+  if (tid == 0) tile_base[a.S] = (int)items;
+  __syncthreads();
+  p.items = (int)items;
+  auto units_of = [&](int x) -> int64_t {
+    if (x >= p.items) return 0;
+    const int i = seq_of_item(tile_base, a.S, x);
+    return (int64_t)blocks_of(keys_of(a, seq_of(a, i), x - tile_base[i], BM), UK) * a.KV;
+  };
+  int64_t sum = 0, units = 0, before = 0;
+  for (int x0 = 0; x0 < p.items; x0 += N) {
+    int64_t total;
+    units = units_of(x0 + tid);
+    before = scan64<N>(units, sh->part, &total);
+    sum += total;
+  }
+  p.per = max((sum + gridDim.x - 1) / gridDim.x, (int64_t)1);
+  const int64_t u0 = p.per * blockIdx.x;
+  p.todo = max(min(p.per, sum - u0), (int64_t)0);
+  if (p.todo == 0) return p;
+  if (p.items <= N) {  // the only round's values are still at hand
+    if (u0 >= before && u0 < before + units) sh->item = tid, sh->off = u0 - before;
+  } else {
+    int64_t base = 0;
+    for (int x0 = 0; base <= u0; x0 += N) {
+      int64_t total;
+      units = units_of(x0 + tid);
+      before = base + scan64<N>(units, sh->part, &total);
+      if (u0 >= before && u0 < before + units) sh->item = x0 + tid, sh->off = u0 - before;
+      base += total;
+    }
+  }
+  __syncthreads();
+  p.item = sh->item, p.off = sh->off;
+  return p;
+}
+
+// What a workgroup leaves about the (item, head) that it began and did not
+// finish (rows = 0: none).  Its partial results are in slots 2 * first + (1 if
+// the unit before it is in the same span), 2 * (first + 1), ..
+struct Split {
+  int64_t u0, u1, per;  // its units, counted over everything; units of a span
+  int row0, rows, head;  // its rows of that cache head, from row0 of the sequence on
+  int q0;                // the sequence's first row of the batch
+};
+
+// Zeros for the rows that see no key: those of items without units and those
+// of no sequence.
+template <int N>
+__device__ __forceinline__ void zero_rows(const AttnArgs &a, const Plan &p, int BM, int UK,
+                                          const int *tile_base) {
+  const int esize = a.dtype == ZT_DT_F32 ? 4 : 2, chunks = a.D * esize / 16;  // of 16 bytes a head
+  char *out = static_cast<char *>(a.out);
+  for (int x = blockIdx.x; x < p.items; x += gridDim.x) {
+    const int i = seq_of_item(tile_base, a.S, x);
+    const Seq s = seq_of(a, i);
+    if (blocks_of(keys_of(a, s, x - tile_base[i], BM), UK)) continue;
+    // the item's rows, of every cache head
+    const int r0 = (x - tile_base[i]) * BM, rows = min(BM, s.q * a.group - r0);
+    const int64_t n = (int64_t)rows * a.KV * chunks;
+    for (int64_t e = threadIdx.x; e < n; e += N) {
+      const int c = (int)(e % chunks), y = (int)(e / chunks), h = y / rows, row = r0 + y - h * rows;
+      const int t = (int)fast_div(row, a.div_group);
+      const int64_t at = ((int64_t)(s.q0 + t) * a.H + h * a.group + row - t * a.group) * chunks + c;
+      reinterpret_cast<u32x4_t *>(out)[at] = u32x4_t{0, 0, 0, 0};
+    }
+  }
+  const int64_t T = a.T, lo = a.S ? min(max((int64_t)a.cu[0], (int64_t)0), T) : T;
+  const int64_t hi = a.S ? min(max((int64_t)a.cu[a.S], (int64_t)0), T) : T;
+  const int64_t row = (int64_t)a.H * chunks, n = (lo + T - hi) * row;
+  for (int64_t e = (int64_t)blockIdx.x * N + threadIdx.x; e < n; e += (int64_t)gridDim.x * N)
+    reinterpret_cast<u32x4_t *>(out)[e < lo * row ? e : e - lo * row + hi * row] = u32x4_t{0, 0, 0, 0};
+}
+
+}  // namespace zt

@@ -1,4 +1,5 @@
-// Attention of a chunk of new tokens over a paged cache, for gfx950.
+// Attention of a chunk of new tokens over a paged cache, for gfx950: few rows
+// per cache head (decoding, short chunks), and the launch of both kernels.
 //
 //   o_r = sum_j exp(s_rj - m_r) v_j / sum_j exp(s_rj - m_r),
 //   s_rj = scale * q_r . k_j,  m_r = max_j s_rj
@@ -7,85 +8,447 @@
 // q new tokens of n in all, token a sits at position n - q + a and sees the
 // positions up to its own (causal), and of those the last `window` (if that
 // is not 0).  A row that sees none is zero.
-#include "zt_cache.hpp"
+//
+// Keys come in any order of blocks, with a running maximum m and sum l:
+//   m' = max(m, max_j s_j),  l' = l e^(m - m') + sum_j e^(s_j - m'),
+//   o' = o e^(m - m') + sum_j e^(s_j - m') v_j,
+// and two parts (m, l, o) join the same way.  Scores, weights and sums are
+// fp32; exponentials are powers of two with scale * log2(e) in the exponent.
+#include "attn_common.hpp"
 
 namespace zt {
 
 namespace {
 
-template <typename T>
-__device__ __forceinline__ float elem(const T *p);
-template <>
-__device__ __forceinline__ float elem<float>(const float *p) { return *p; }
-template <>
-__device__ __forceinline__ float elem<uint16_t>(const uint16_t *p) { return bf16_bits_to_f32(*p); }
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+typedef short s16x8_t __attribute__((ext_vector_type(8)));
 
-// One workgroup per row: wave w takes the keys w, w + 4, .., each lane up to
-// four of the head's elements, with a running maximum and sum per wave; the
-// four waves' parts are joined at the end.
-template <typename T>
-__global__ __launch_bounds__(256) void paged_attn_row_kernel(AttnArgs a) {
-  __shared__ float sm_m[4], sm_l[4], sm_o[4][256];
-  const int64_t t = blockIdx.x;
-  const int h = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int lo = 0, hi = a.S + 1;
-  while (lo < hi) {
-    const int m = (lo + hi) / 2;
-    if (a.cu[m] > t) hi = m;
-    else lo = m + 1;
-  }
-  const int i = lo - 1;
-  int64_t begin = 0, end = 0;
-  if (i >= 0 && i < a.S) {
-    const int64_t n = min((int64_t)max(a.ctx[i], 0), (int64_t)a.W * a.page_size);
-    const int64_t pos = n - (a.cu[i + 1] - t);
-    end = a.causal ? min(pos + 1, n) : n;
-    if (a.window) begin = max(pos + 1 - a.window, (int64_t)0);
-  }
-  const T *q = static_cast<const T *>(a.q) + t * a.q_ld[0] + h * a.q_ld[1];
-  const int kvh = h / (a.H / a.KV);
-  float x[4], o[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int c = 0; c < 4; ++c) x[c] = lane + 64 * c < a.D ? elem(q + lane + 64 * c) : 0.f;
-  float m = -INFINITY, l = 0.f;
-  for (int64_t j = begin + wave; j < end; j += 4) {
-    const int64_t col = j / a.page_size, off = j - col * a.page_size;
-    const int page = a.table[(int64_t)i * a.W + col];
-    if (page < 0 || page >= a.pages) continue;
-    const T *k = static_cast<const T *>(a.k) + page * a.k_ld[0] + kvh * a.k_ld[1] + off * a.k_ld[2];
-    const T *v = static_cast<const T *>(a.v) + page * a.v_ld[0] + kvh * a.v_ld[1] + off * a.v_ld[2];
-    float s = 0.f;
-    for (int c = 0; c < 4; ++c)
-      if (lane + 64 * c < a.D) s += x[c] * elem(k + lane + 64 * c);
-    for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d);
-    s *= a.scale;
-    const float mn = fmaxf(m, s), f = mn == -INFINITY ? 0.f : expf(m - mn);
-    const float p = mn == -INFINITY ? 0.f : expf(s - mn);
-    m = mn, l = l * f + p;
-    for (int c = 0; c < 4; ++c)
-      if (lane + 64 * c < a.D) o[c] = o[c] * f + p * elem(v + lane + 64 * c);
-  }
-  if (lane == 0) sm_m[wave] = m, sm_l[wave] = l;
-  for (int c = 0; c < 4; ++c) sm_o[wave][lane + 64 * c] = o[c];
-  __syncthreads();
-  const int d = threadIdx.x;
-  if (d >= a.D) return;
-  float mm = fmaxf(fmaxf(sm_m[0], sm_m[1]), fmaxf(sm_m[2], sm_m[3])), ll = 0.f, oo = 0.f;
-  for (int w = 0; w < 4; ++w) {
-    const float f = sm_m[w] == -INFINITY ? 0.f : expf(sm_m[w] - mm);
-    ll += f * sm_l[w], oo += f * sm_o[w][d];
-  }
-  store_elem(a.out, a.dtype, (t * a.H + h) * a.D + d, ll > 0.f ? oo / ll : 0.f);
+constexpr int kRowThreads = 256;
+
+// log2(e) times the scale's magnitude.  The scale's sign goes to the query
+// (exactly), and a scale of 0 zeroes it, so that the row maximum of the raw
+// products is the maximum of the scores.
+__device__ __forceinline__ float score_factor(float scale) {
+  return scale == 0.f ? 1.f : fabsf(scale) * 1.4426950408889634f;
 }
+__device__ __forceinline__ uint32_t scale_sign(uint32_t w, uint32_t mask, float scale) {
+  return scale == 0.f ? 0u : scale < 0.f ? w ^ mask : w;
+}
+
+__device__ __forceinline__ float max_over_groups(float x) {
+  x = fmaxf(x, __shfl_xor(x, 16));
+  return fmaxf(x, __shfl_xor(x, 32));
+}
+__device__ __forceinline__ float sum_over_groups(float x) {
+  x += __shfl_xor(x, 16);
+  return x + __shfl_xor(x, 32);
+}
+
+// 16 NT rows of one cache head against a span of its keys.
+//
+// Bound by HBM: the keys and values are read once, straight to registers, and
+// each CU needs some 64 KB of them in flight.  So the four waves are
+// independent of each other: wave w takes every fourth strip of KS keys (32,
+// or 16 in fp32: 8 KB of keys and 8 KB of values at head_dim 128), with the
+// next strip's loads issued as soon as the scores have used up the keys'
+// registers; they meet only at the end of an (item, head).
+//
+// The products are taken transposed, S^T = K Q^T and O^T = V^T P^T, on 16x16
+// MFMAs with the rows as columns.  The scores' layout (lane (row, g) holds
+// keys 4 g .. 4 g + 3) then is the layout in which the second product takes
+// its weights, without a move between lanes, if V^T takes its keys in the
+// same order.  V^T needs each lane to hold keys of one column: in fp32 plain
+// LDS reads give that, in bf16 the transposing ds_read_b64_tr_b16 (lane i of
+// 16 gets column i of the four rows whose pieces the 16 lanes point at).  Each
+// wave passes its values through LDS of its own.
+//
+// bf16 weights keep the digits that one bf16 drops in a second MFMA (p = hi +
+// lo): the matrix pipe is idle most of the time here.
+template <typename T, int DP, int NT>
+__global__ __launch_bounds__(kRowThreads) void paged_attn_row_kernel(AttnArgs a) {
+  constexpr bool BF = sizeof(T) == 2;
+  constexpr int ES = sizeof(T);
+  constexpr int BM = 16 * NT;
+  constexpr int KT = BF ? 2 : 1;          // 16-key tiles of a strip
+  constexpr int KS = 16 * KT;             // keys of a strip
+  constexpr int UK = 4 * KS;              // keys of a unit
+  constexpr int KC = DP * ES / 64;        // 16-byte pieces of a key per lane
+  constexpr int CR = DP * ES / 16;        // 16-byte pieces of a row
+  constexpr int NV = KS * CR / 64;        // value pieces per lane
+  constexpr int VP = DP * ES + (BF ? 32 : 16);  // LDS pitch: the reads meet no bank twice
+  constexpr int OP = DP + 4;              // pitch of the joined outputs, floats
+  constexpr int DT = DP / 16;
+  constexpr int kWaveLds = KS * VP > 16 * OP * 4 ? KS * VP : 16 * OP * 4;
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  __shared__ PlanShared sh;
+  __shared__ float sm_m[4][16], sm_l[4][16];
+  int *tile_base = reinterpret_cast<int *>(smem + 4 * kWaveLds);
+
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  unsigned char *vlds = smem + wave * kWaveLds;
+  const Plan plan = make_plan<kRowThreads>(a, BM, UK, tile_base, &sh);
+  zero_rows<kRowThreads>(a, plan, BM, UK, tile_base);
+  Split *split = static_cast<Split *>(a.splits) + blockIdx.x;
+  if (tid == 0) split->rows = 0;
+  if (plan.todo == 0) return;
+
+  const float c = score_factor(a.scale);
+  const int G = a.group, C = a.D * ES / 16;  // 16-byte pieces that a row has
+  const char *zero = reinterpret_cast<const char *>(kZeroRow);
+  const int64_t kps = a.k_ld[0] * ES, kts = a.k_ld[2] * ES, vps = a.v_ld[0] * ES, vts = a.v_ld[2] * ES;
+
+  int64_t todo = plan.todo, off = plan.off, unit = plan.per * blockIdx.x;
+  const int64_t span0 = unit;
+  for (int x = plan.item; todo > 0; ++x, off = 0) {
+    const int i = seq_of_item(tile_base, a.S, x);
+    const Seq s = seq_of(a, i);
+    const int r0 = (x - tile_base[i]) * BM;
+    const KeyRange kr = keys_of(a, s, x - tile_base[i], BM);
+    const int nb = blocks_of(kr, UK), b0 = kr.begin / UK;
+    if (nb == 0) continue;
+    const int *table = a.table + (int64_t)i * a.W;
+    // the lane's rows: token, head, and the keys each sees
+    int row_t[NT], lo[NT], hi[NT];
+    bool live[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const int row = r0 + 16 * t + n;
+      row_t[t] = (int)fast_div(row, a.div_group);
+      live[t] = row_t[t] < s.q;
+      const int pos = s.n - s.q + row_t[t];
+      hi[t] = !live[t] ? INT32_MAX : a.causal ? pos + 1 : s.n;
+      lo[t] = live[t] && a.causal && a.window ? (int)max((int64_t)pos + 1 - a.window, (int64_t)0) : 0;
+    }
+    for (int h = (int)(off / nb), bb = (int)(off - (int64_t)h * nb); h < a.KV && todo > 0; ++h, bb = 0) {
+      const int take = (int)min((int64_t)(nb - bb), todo);
+      // ---- the queries, as B operands: lane (row n, g) holds piece 4 j + g
+      u32x4_t q[NT][KC];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const int row = r0 + 16 * t + n;
+        const char *src = static_cast<const char *>(a.q) +
+            ((int64_t)(s.q0 + row_t[t]) * a.q_ld[0] + (h * G + row - row_t[t] * G) * a.q_ld[1]) * ES;
+#pragma unroll
+        for (int j = 0; j < KC; ++j) {
+          const int p = 4 * j + g;
+          q[t][j] = *reinterpret_cast<const u32x4_t *>(live[t] && p < C ? src + 16 * p : zero);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            q[t][j][e] = scale_sign(q[t][j][e], BF ? 0x80008000u : 0x80000000u, a.scale);
+        }
+      }
+      f32x4_t o[NT][DT];
+      float m[NT], l[NT];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        m[t] = -INFINITY, l[t] = 0.f;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[t][d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      }
+      const char *kbase = static_cast<const char *>(a.k) + h * a.k_ld[1] * ES;
+      const char *vbase = static_cast<const char *>(a.v) + h * a.v_ld[1] * ES;
+      const int kend = (b0 + bb + take) * UK;
+      int k0 = (b0 + bb) * UK + wave * KS;
+
+      // page of key k0 + (lane % KS), or one outside the pool if no row of
+      // the item sees it
+      auto lookup = [&](int at) {
+        const int tok = at + (lane & (KS - 1));
+        const bool in = tok >= kr.begin && tok < kr.end && at < kend;
+        const int page = table[in ? fast_div(tok, a.div_page) : 0];
+        return in ? page : -1;
+      };
+      u32x4_t kreg[KT][KC], vreg[NV];
+      uint64_t there;  // which of the strip's keys there are
+      auto load = [&](int at, int page) {
+        const int tok = at + (lane & (KS - 1));
+        const bool ok = page >= 0 && page < a.pages;
+        there = __ballot(ok);
+        const int in_page = tok - (int)fast_div(tok, a.div_page) * a.page_size;
+        const uint64_t ko = (uint64_t)(ok ? kbase + page * kps + in_page * kts : zero);
+        const uint64_t vo = (uint64_t)(ok ? vbase + page * vps + in_page * vts : zero);
+#pragma unroll
+        for (int t = 0; t < KT; ++t) {
+          const char *src = (const char *)__shfl((unsigned long long)ko, 16 * t + n);
+#pragma unroll
+          for (int j = 0; j < KC; ++j) {
+            const int p = 4 * j + g;
+            kreg[t][j] = *reinterpret_cast<const u32x4_t *>(p < C ? src + 16 * p : zero);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+          const int idx = 64 * j + lane, row = idx / CR, p = idx % CR;
+          const char *src = (const char *)__shfl((unsigned long long)vo, row);
+          vreg[j] = *reinterpret_cast<const u32x4_t *>(p < C ? src + 16 * p : zero);
+        }
+      };
+      int page = lookup(k0);
+      if (k0 < kend) load(k0, page);
+      page = lookup(k0 + UK);
+      for (; k0 < kend; k0 += UK) {
+        // values to the wave's LDS (LDS operations of a wave keep their order)
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+          const int idx = 64 * j + lane, row = idx / CR, p = idx % CR;
+          *reinterpret_cast<u32x4_t *>(vlds + row * VP + 16 * p) = vreg[j];
+        }
+        // scores: lane (row n, g) gets keys 16 u + 4 g .. + 3
+        f32x4_t sc[NT][KT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int u = 0; u < KT; ++u) {
+            f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < KC; ++j) {
+              if constexpr (BF) {
+                acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                    __builtin_bit_cast(bf16x8_t, kreg[u][j]), __builtin_bit_cast(bf16x8_t, q[t][j]), acc, 0, 0, 0);
+              } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  acc = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kreg[u][j][e]),
+                                                             __uint_as_float(q[t][j][e]), acc, 0, 0, 0);
+              }
+            }
+            sc[t][u] = acc;
+          }
+        const uint64_t held = there;
+        const bool whole = (uint32_t)held == (KS == 32 ? ~0u : 0xffffu) || (KS == 16 && (held & 0xffff) == 0xffff);
+        if (k0 + UK < kend) {
+          load(k0 + UK, page);
+          page = lookup(k0 + 2 * UK);
+        }
+        // weights
+        bf16x8_t ph[NT], pl[NT];
+        float pf[NT][4];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          if (!whole || __ballot(lo[t] > k0 || hi[t] < k0 + KS)) {
+#pragma unroll
+            for (int u = 0; u < KT; ++u)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int k = 16 * u + 4 * g + e;
+                if (!(held >> k & 1) || k0 + k < lo[t] || k0 + k >= hi[t]) sc[t][u][e] = -INFINITY;
+              }
+          }
+          float mx = sc[t][0][0];
+#pragma unroll
+          for (int u = 0; u < KT; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mx = fmaxf(mx, sc[t][u][e]);
+          mx = fmaxf(m[t], max_over_groups(mx));
+          if (__ballot(mx > m[t])) {
+            const float f = mx == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[t] * c - mx * c);
+            l[t] *= f;
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[t][d][e] *= f;
+            m[t] = mx;
+          }
+          const float mc = m[t] == -INFINITY ? 0.f : m[t] * c;
+#pragma unroll
+          for (int u = 0; u < KT; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float p = __builtin_amdgcn_exp2f(fmaf(sc[t][u][e], c, -mc));
+              l[t] += p;
+              if constexpr (BF) {
+                const __bf16 hi_part = (__bf16)p;
+                ph[t][4 * u + e] = hi_part;
+                pl[t][4 * u + e] = (__bf16)(p - (float)hi_part);
+              } else {
+                pf[t][e] = p;
+              }
+            }
+        }
+        // O^T += V^T P^T
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          if constexpr (BF) {
+            typedef __attribute__((address_space(3))) s16x4_t *tr_ptr;
+            const unsigned char *at = vlds + (4 * g + n / 4) * VP + 32 * d + 8 * (n & 3);
+            const s16x4_t v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)at);
+            const s16x4_t v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)(at + 16 * VP));
+            const bf16x8_t v = __builtin_bit_cast(
+                bf16x8_t, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+              o[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, ph[t], o[t][d], 0, 0, 0);
+              o[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, pl[t], o[t][d], 0, 0, 0);
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float v = *reinterpret_cast<const float *>(vlds + (4 * g + e) * VP + 4 * (16 * d + n));
+#pragma unroll
+              for (int t = 0; t < NT; ++t)
+                o[t][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, pf[t][e], o[t][d], 0, 0, 0);
+            }
+          }
+        }
+      }
+      // ---- join the four waves, 16 rows at a time
+      const bool complete = bb == 0 && take == nb;
+      const int64_t slot = 2 * (int64_t)blockIdx.x + (unit > span0 ? 1 : 0);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const float lsum = sum_over_groups(l[t]);
+        __syncthreads();  // the waves' values and the previous rows are read
+        if (lane < 16) sm_m[wave][n] = m[t], sm_l[wave][n] = lsum;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+          *reinterpret_cast<f32x4_t *>(vlds + (n * OP + 16 * d + 4 * g) * 4) = o[t][d];
+        __syncthreads();
+        for (int e = tid; e < 16 * DP / 4; e += kRowThreads) {
+          const int row = e / (DP / 4), d = e % (DP / 4) * 4;
+          const int rr = r0 + 16 * t + row;
+          const int tok = (int)fast_div(rr, a.div_group);
+          if (tok >= s.q || d >= a.D) continue;
+          const float mm = fmaxf(fmaxf(sm_m[0][row], sm_m[1][row]), fmaxf(sm_m[2][row], sm_m[3][row]));
+          float ll = 0.f;
+          f32x4_t oo = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const float f = sm_m[w][row] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sm_m[w][row] * c - mm * c);
+            ll += f * sm_l[w][row];
+            const f32x4_t y = *reinterpret_cast<const f32x4_t *>(smem + w * kWaveLds + (row * OP + d) * 4);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) oo[k] += f * y[k];
+          }
+          if (complete) {
+            const float r = ll > 0.f ? 1.f / ll : 0.f;
+            const int64_t at = ((int64_t)(s.q0 + tok) * a.H + h * G + rr - tok * G) * a.D + d;
+            if constexpr (BF) {
+              u32x2_t w;
+              w[0] = pack_bf16x2(oo[0] * r, oo[1] * r), w[1] = pack_bf16x2(oo[2] * r, oo[3] * r);
+              *reinterpret_cast<u32x2_t *>(static_cast<uint16_t *>(a.out) + at) = w;
+            } else {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) oo[k] *= r;
+              *reinterpret_cast<f32x4_t *>(static_cast<float *>(a.out) + at) = oo;
+            }
+          } else {
+            const int64_t pr = slot * BM + 16 * t + row;
+            *reinterpret_cast<f32x4_t *>(a.part_o + pr * a.D + d) = oo;
+            if (d == 0) a.part_ml[2 * pr] = mm, a.part_ml[2 * pr + 1] = ll;
+          }
+        }
+      }
+      __syncthreads();  // before the next strips' values
+      if (tid == 0 && bb == 0 && !complete) {
+        split->u0 = unit, split->u1 = unit + nb, split->per = plan.per;
+        split->row0 = r0, split->rows = min(BM, s.q * G - r0), split->head = h, split->q0 = s.q0;
+      }
+      todo -= take;
+      unit += take;
+    }
+  }
+}
+
+// Joins the parts of the (item, head) that workgroup blockIdx.x of the first
+// launch began and others finished.  A thread takes four outputs of a row.
+template <typename T, int BM>
+__global__ __launch_bounds__(256) void paged_attn_join_kernel(AttnArgs a) {
+  const Split s = static_cast<const Split *>(a.splits)[blockIdx.x];
+  if (s.rows == 0) return;
+  const float c = score_factor(a.scale);
+  const int first = (int)blockIdx.x, last = (int)((s.u1 - 1) / s.per);
+  const int d4 = a.D / 4, G = a.group;
+  for (int e = blockIdx.y * 256 + threadIdx.x; e < s.rows * d4; e += gridDim.y * 256) {
+    const int row = e / d4, d = (e - row * d4) * 4;
+    float m = -INFINITY, l = 0.f;
+    f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+    int64_t slot = 2 * (int64_t)first + (s.u0 > first * s.per ? 1 : 0);
+    for (int w = first; w <= last; ++w, slot = 2 * (int64_t)w) {
+      const float *ml = a.part_ml + 2 * (slot * BM + row);
+      const f32x4_t y = *reinterpret_cast<const f32x4_t *>(a.part_o + (slot * BM + row) * a.D + d);
+      const float mw = ml[0], lw = ml[1], mm = fmaxf(m, mw);
+      const float f0 = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m * c - mm * c);
+      const float f1 = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw * c - mm * c);
+      m = mm, l = l * f0 + lw * f1;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) o[k] = o[k] * f0 + y[k] * f1;
+    }
+    const float r = l > 0.f ? 1.f / l : 0.f;
+    const int rr = s.row0 + row, tok = (int)fast_div(rr, a.div_group);
+    const int64_t at = ((int64_t)(s.q0 + tok) * a.H + s.head * G + rr - tok * G) * a.D + d;
+    if constexpr (sizeof(T) == 2) {
+      u32x2_t w;
+      w[0] = pack_bf16x2(o[0] * r, o[1] * r), w[1] = pack_bf16x2(o[2] * r, o[3] * r);
+      *reinterpret_cast<u32x2_t *>(static_cast<uint16_t *>(a.out) + at) = w;
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) o[k] *= r;
+      *reinterpret_cast<f32x4_t *>(static_cast<float *>(a.out) + at) = o;
+    }
+  }
+}
+
+// Workgroups of the first launch: two per CU.
+constexpr int kRowGrid = 512;
+
+template <typename T, int DP, int NT>
+hipError_t launch_rows(const AttnArgs &a, hipStream_t s) {
+  constexpr int KS = sizeof(T) == 2 ? 32 : 16, VP = DP * (int)sizeof(T) + (sizeof(T) == 2 ? 32 : 16);
+  constexpr int wave = std::max(KS * VP, 16 * (DP + 4) * 4);
+  const size_t lds = 4 * wave + ((size_t)a.S + 1) * 4;
+  auto kernel = paged_attn_row_kernel<T, DP, NT>;
+  if (lds > 64 * 1024) {
+    const hipError_t grown = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
+                                                 hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    if (grown != hipSuccess) return grown;
+  }
+  kernel<<<kRowGrid, kRowThreads, lds, s>>>(a);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  paged_attn_join_kernel<T, 16 * NT><<<dim3(kRowGrid, std::min(NT, 4)), 256, 0, s>>>(a);
+  return hipGetLastError();
+}
+
+template <typename T, int NT>
+hipError_t launch_rows_d(const AttnArgs &a, hipStream_t s) {
+  if (a.D <= 64) return launch_rows<T, 64, NT>(a, s);
+  if (a.D <= 128) return launch_rows<T, 128, NT>(a, s);
+  return launch_rows<T, 256, NT>(a, s);
+}
+
+template <typename T>
+hipError_t launch_rows_n(const AttnArgs &a, int nt, hipStream_t s) {
+  if (nt == 1) return launch_rows_d<T, 1>(a, s);
+  if (nt == 2) return launch_rows_d<T, 2>(a, s);
+  return launch_rows_d<T, 4>(a, s);
+}
+
+int row_tiles(const AttnArgs &a) {
+  const int64_t rows = std::min(std::max<int64_t>(a.max_q, 1), a.T) * (a.H / a.KV);
+  return rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+}
+
+size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
 }  // namespace
 
-size_t paged_attn_workspace(const AttnArgs &) { return 0; }
+size_t paged_attn_workspace(const AttnArgs &a) {
+  if (a.T == 0) return 0;
+  const size_t slots = 2 * (size_t)kRowGrid * 16 * row_tiles(a);
+  return up256(kRowGrid * sizeof(Split)) + up256(slots * 2 * sizeof(float)) + slots * a.D * sizeof(float);
+}
 
-hipError_t launch_paged_attn(const AttnArgs &a, void *, hipStream_t s) {
-  const dim3 grid((unsigned)a.T, (unsigned)a.H);
-  if (a.dtype == ZT_DT_BF16) paged_attn_row_kernel<uint16_t><<<grid, dim3(256), 0, s>>>(a);
-  else paged_attn_row_kernel<float><<<grid, dim3(256), 0, s>>>(a);
-  return hipGetLastError();
+hipError_t launch_paged_attn(AttnArgs a, void *workspace, hipStream_t s) {
+  const int nt = row_tiles(a);
+  const size_t slots = 2 * (size_t)kRowGrid * 16 * nt;
+  a.group = a.H / a.KV;
+  a.div_group = make_div(a.group), a.div_page = make_div(a.page_size);
+  char *at = static_cast<char *>(workspace);
+  a.splits = at, at += up256(kRowGrid * sizeof(Split));
+  a.part_ml = reinterpret_cast<float *>(at), at += up256(slots * 2 * sizeof(float));
+  a.part_o = reinterpret_cast<float *>(at);
+  return a.dtype == ZT_DT_BF16 ? launch_rows_n<uint16_t>(a, nt, s) : launch_rows_n<float>(a, nt, s);
 }
 
 }  // namespace zt

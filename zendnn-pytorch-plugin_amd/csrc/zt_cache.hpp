@@ -67,6 +67,21 @@ struct CopyArgs {
 };
 hipError_t launch_copy_pages(CopyArgs a, int caches, int64_t pairs, bool wide, hipStream_t s);
 
+// Division of n < 2^31 by a fixed d: (n * mul) >> shift, with mul =
+// floor(2^(31 + L) / d) + 1 and shift = 31 + L, L = ceil(log2 d), which is exact
+// for every such n.
+struct FastDiv {
+  uint32_t mul, shift;
+};
+inline FastDiv make_div(uint32_t d) {
+  uint32_t L = 0;
+  while ((1ull << L) < d) ++L;
+  return {(uint32_t)((1ull << (31 + L)) / d + 1), 31 + L};
+}
+__device__ __forceinline__ uint32_t fast_div(uint32_t n, FastDiv d) {
+  return (uint32_t)(((uint64_t)n * d.mul) >> d.shift);
+}
+
 struct AttnArgs {
   const void *q;  // [T, H, D]
   int64_t q_ld[2];
@@ -80,8 +95,13 @@ struct AttnArgs {
   int64_t window;
   float scale;
   void *out;  // [T, H, D]
+  // set by launch_paged_attn
+  int group;                    // H / KV
+  FastDiv div_group, div_page;
+  float *part_ml, *part_o;      // partial results: [slots][BM][2], [slots][BM][D]
+  void *splits;                 // [workgroups] of Split
 };
 size_t paged_attn_workspace(const AttnArgs &a);
-hipError_t launch_paged_attn(const AttnArgs &a, void *workspace, hipStream_t s);
+hipError_t launch_paged_attn(AttnArgs a, void *workspace, hipStream_t s);
 
 }  // namespace zt
