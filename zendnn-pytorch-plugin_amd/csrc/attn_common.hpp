@@ -9,17 +9,49 @@
 // one cache head); it needs the keys of blocks [b0, b1) of UK keys.
 //
 // Work is dealt out in units of one block of one item and cache head, laid
-// end to end (item by item, in it head by head, in it block by block), in
+// end to end (head by head, in it item by item, in it block by block), in
 // equal spans, one per workgroup.  The lengths are known on the device only,
 // so each workgroup finds its span by itself.  A span may end inside an
 // (item, head): its workgroups then leave partial results (running maximum,
 // sum and output), which a second launch joins.  That keeps every compute unit
-// busy for one long sequence as for many ragged ones.
+// busy for one long sequence as for many ragged ones.  Consecutive spans go to
+// one XCD (blocks are dealt round-robin over the eight of them), so the tiles
+// of a head find its keys in one L2.
 #pragma once
 
 #include "zt_cache.hpp"
 
 namespace zt {
+
+// log2(e) times the scale's magnitude.  The scale's sign goes to the query
+// (exactly), and a scale of 0 zeroes it, so that the row maximum of the raw
+// products is the maximum of the scores.
+__device__ __forceinline__ float score_factor(float scale) {
+  return scale == 0.f ? 1.f : fabsf(scale) * 1.4426950408889634f;
+}
+template <typename T>
+__device__ __forceinline__ u32x4_t scale_sign(u32x4_t w, float scale) {
+  const uint32_t mask = scale < 0.f ? (sizeof(T) == 2 ? 0x80008000u : 0x80000000u) : 0u;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) w[e] = scale == 0.f ? 0u : w[e] ^ mask;
+  return w;
+}
+
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+
+// Four fp32 outputs of a row, times r, rounded.
+template <typename T>
+__device__ __forceinline__ void store_out(void *out, int64_t at, f32x4_t o, float r) {
+  if constexpr (sizeof(T) == 2) {
+    u32x2_t w;
+    w[0] = pack_bf16x2(o[0] * r, o[1] * r), w[1] = pack_bf16x2(o[2] * r, o[3] * r);
+    *reinterpret_cast<u32x2_t *>(static_cast<uint16_t *>(out) + at) = w;
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) o[k] *= r;
+    *reinterpret_cast<f32x4_t *>(static_cast<float *>(out) + at) = o;
+  }
+}
 
 // 1 KB of zeros: what a lane reads in place of a key or value that is not
 // there, so that weights of zero never meet a NaN or an infinity.
@@ -80,16 +112,14 @@ __device__ __forceinline__ int64_t scan64(int64_t v, int64_t *part, int64_t *tot
 
 struct PlanShared {
   int64_t part[16];
-  int64_t off;
-  int item;
+  int item, off;
 };
 
 struct Plan {
-  int items;
-  int64_t per;   // units of a span
-  int64_t todo;  // units of this workgroup's span
-  int item;      // the item of its first unit
-  int64_t off;   // and that unit's place among the item's units
+  int items, wg;  // items of a head; this workgroup's place in the order of spans
+  int64_t per;    // units of a span
+  int64_t todo;   // units of this workgroup's span
+  int head, item, off;  // its first unit: block `off` of that item
 };
 
 // The sequence of item x: the last i with tile_base[i] <= x.
@@ -124,7 +154,7 @@ __device__ __forceinline__ Plan make_plan(const AttnArgs &a, int BM, int UK, int
   auto units_of = [&](int x) -> int64_t {
     if (x >= p.items) return 0;
     const int i = seq_of_item(tile_base, a.S, x);
-    return (int64_t)blocks_of(keys_of(a, seq_of(a, i), x - tile_base[i], BM), UK) * a.KV;
+    return blocks_of(keys_of(a, seq_of(a, i), x - tile_base[i], BM), UK);
   };
   int64_t sum = 0, units = 0, before = 0;
   for (int x0 = 0; x0 < p.items; x0 += N) {
@@ -133,19 +163,23 @@ __device__ __forceinline__ Plan make_plan(const AttnArgs &a, int BM, int UK, int
     before = scan64<N>(units, sh->part, &total);
     sum += total;
   }
-  p.per = max((sum + gridDim.x - 1) / gridDim.x, (int64_t)1);
-  const int64_t u0 = p.per * blockIdx.x;
-  p.todo = max(min(p.per, sum - u0), (int64_t)0);
+  p.wg = xcd_contiguous_tile(blockIdx.x, gridDim.x);
+  const int64_t all = sum * a.KV;
+  p.per = max((all + gridDim.x - 1) / gridDim.x, (int64_t)1);
+  const int64_t u0 = p.per * p.wg;
+  p.todo = max(min(p.per, all - u0), (int64_t)0);
   if (p.todo == 0) return p;
+  p.head = (int)(u0 / sum);
+  const int64_t at = u0 - p.head * sum;
   if (p.items <= N) {  // the only round's values are still at hand
-    if (u0 >= before && u0 < before + units) sh->item = tid, sh->off = u0 - before;
+    if (at >= before && at < before + units) sh->item = tid, sh->off = (int)(at - before);
   } else {
     int64_t base = 0;
-    for (int x0 = 0; base <= u0; x0 += N) {
+    for (int x0 = 0; base <= at; x0 += N) {
       int64_t total;
       units = units_of(x0 + tid);
       before = base + scan64<N>(units, sh->part, &total);
-      if (u0 >= before && u0 < before + units) sh->item = x0 + tid, sh->off = u0 - before;
+      if (at >= before && at < before + units) sh->item = x0 + tid, sh->off = (int)(at - before);
       base += total;
     }
   }
@@ -190,5 +224,10 @@ __device__ __forceinline__ void zero_rows(const AttnArgs &a, const Plan &p, int 
   for (int64_t e = (int64_t)blockIdx.x * N + threadIdx.x; e < n; e += (int64_t)gridDim.x * N)
     reinterpret_cast<u32x4_t *>(out)[e < lo * row ? e : e - lo * row + hi * row] = u32x4_t{0, 0, 0, 0};
 }
+
+// The tile kernel (paged_attn_tile.hip): its rows per item and workgroups.
+int tile_rows(const AttnArgs &a);
+int tile_grid(const AttnArgs &a);
+hipError_t launch_tiles(const AttnArgs &a, hipStream_t s);
 
 }  // namespace zt

@@ -20,20 +20,7 @@ namespace zt {
 
 namespace {
 
-typedef short s16x4_t __attribute__((ext_vector_type(4)));
-typedef short s16x8_t __attribute__((ext_vector_type(8)));
-
 constexpr int kRowThreads = 256;
-
-// log2(e) times the scale's magnitude.  The scale's sign goes to the query
-// (exactly), and a scale of 0 zeroes it, so that the row maximum of the raw
-// products is the maximum of the scores.
-__device__ __forceinline__ float score_factor(float scale) {
-  return scale == 0.f ? 1.f : fabsf(scale) * 1.4426950408889634f;
-}
-__device__ __forceinline__ uint32_t scale_sign(uint32_t w, uint32_t mask, float scale) {
-  return scale == 0.f ? 0u : scale < 0.f ? w ^ mask : w;
-}
 
 __device__ __forceinline__ float max_over_groups(float x) {
   x = fmaxf(x, __shfl_xor(x, 16));
@@ -89,7 +76,7 @@ __global__ __launch_bounds__(kRowThreads) void paged_attn_row_kernel(AttnArgs a)
   unsigned char *vlds = smem + wave * kWaveLds;
   const Plan plan = make_plan<kRowThreads>(a, BM, UK, tile_base, &sh);
   zero_rows<kRowThreads>(a, plan, BM, UK, tile_base);
-  Split *split = static_cast<Split *>(a.splits) + blockIdx.x;
+  Split *split = static_cast<Split *>(a.splits) + plan.wg;
   if (tid == 0) split->rows = 0;
   if (plan.todo == 0) return;
 
@@ -98,15 +85,17 @@ __global__ __launch_bounds__(kRowThreads) void paged_attn_row_kernel(AttnArgs a)
   const char *zero = reinterpret_cast<const char *>(kZeroRow);
   const int64_t kps = a.k_ld[0] * ES, kts = a.k_ld[2] * ES, vps = a.v_ld[0] * ES, vts = a.v_ld[2] * ES;
 
-  int64_t todo = plan.todo, off = plan.off, unit = plan.per * blockIdx.x;
+  int64_t todo = plan.todo, unit = plan.per * plan.wg;
   const int64_t span0 = unit;
-  for (int x = plan.item; todo > 0; ++x, off = 0) {
+  for (int h = plan.head, x = plan.item, bb = plan.off; todo > 0; ++x, bb = 0) {
+    if (x == plan.items) ++h, x = 0;
     const int i = seq_of_item(tile_base, a.S, x);
     const Seq s = seq_of(a, i);
     const int r0 = (x - tile_base[i]) * BM;
     const KeyRange kr = keys_of(a, s, x - tile_base[i], BM);
     const int nb = blocks_of(kr, UK), b0 = kr.begin / UK;
     if (nb == 0) continue;
+    const int take = (int)min((int64_t)(nb - bb), todo);
     const int *table = a.table + (int64_t)i * a.W;
     // the lane's rows: token, head, and the keys each sees
     int row_t[NT], lo[NT], hi[NT];
@@ -120,240 +109,225 @@ __global__ __launch_bounds__(kRowThreads) void paged_attn_row_kernel(AttnArgs a)
       hi[t] = !live[t] ? INT32_MAX : a.causal ? pos + 1 : s.n;
       lo[t] = live[t] && a.causal && a.window ? (int)max((int64_t)pos + 1 - a.window, (int64_t)0) : 0;
     }
-    for (int h = (int)(off / nb), bb = (int)(off - (int64_t)h * nb); h < a.KV && todo > 0; ++h, bb = 0) {
-      const int take = (int)min((int64_t)(nb - bb), todo);
-      // ---- the queries, as B operands: lane (row n, g) holds piece 4 j + g
-      u32x4_t q[NT][KC];
+    // ---- the queries, as B operands: lane (row n, g) holds piece 4 j + g
+    u32x4_t q[NT][KC];
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const int row = r0 + 16 * t + n;
-        const char *src = static_cast<const char *>(a.q) +
-            ((int64_t)(s.q0 + row_t[t]) * a.q_ld[0] + (h * G + row - row_t[t] * G) * a.q_ld[1]) * ES;
+    for (int t = 0; t < NT; ++t) {
+      const int row = r0 + 16 * t + n;
+      const char *src = static_cast<const char *>(a.q) +
+          ((int64_t)(s.q0 + row_t[t]) * a.q_ld[0] + (h * G + row - row_t[t] * G) * a.q_ld[1]) * ES;
+#pragma unroll
+      for (int j = 0; j < KC; ++j) {
+        const int p = 4 * j + g;
+        q[t][j] = scale_sign<T>(*reinterpret_cast<const u32x4_t *>(live[t] && p < C ? src + 16 * p : zero), a.scale);
+      }
+    }
+    f32x4_t o[NT][DT];
+    float m[NT], l[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      m[t] = -INFINITY, l[t] = 0.f;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) o[t][d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    }
+    const char *kbase = static_cast<const char *>(a.k) + h * a.k_ld[1] * ES;
+    const char *vbase = static_cast<const char *>(a.v) + h * a.v_ld[1] * ES;
+    const int kend = (b0 + bb + take) * UK;
+    int k0 = (b0 + bb) * UK + wave * KS;
+
+    // page of key k0 + (lane % KS), or one outside the pool if no row of
+    // the item sees it
+    auto lookup = [&](int at) {
+      const int tok = at + (lane & (KS - 1));
+      const bool in = tok >= kr.begin && tok < kr.end && at < kend;
+      const int page = table[in ? fast_div(tok, a.div_page) : 0];
+      return in ? page : -1;
+    };
+    u32x4_t kreg[KT][KC], vreg[NV];
+    uint64_t there;  // which of the strip's keys there are
+    auto load = [&](int at, int page) {
+      const int tok = at + (lane & (KS - 1));
+      const bool ok = page >= 0 && page < a.pages;
+      there = __ballot(ok);
+      const int in_page = tok - (int)fast_div(tok, a.div_page) * a.page_size;
+      const uint64_t ko = (uint64_t)(ok ? kbase + page * kps + in_page * kts : zero);
+      const uint64_t vo = (uint64_t)(ok ? vbase + page * vps + in_page * vts : zero);
+#pragma unroll
+      for (int t = 0; t < KT; ++t) {
+        const char *src = (const char *)__shfl((unsigned long long)ko, 16 * t + n);
 #pragma unroll
         for (int j = 0; j < KC; ++j) {
           const int p = 4 * j + g;
-          q[t][j] = *reinterpret_cast<const u32x4_t *>(live[t] && p < C ? src + 16 * p : zero);
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            q[t][j][e] = scale_sign(q[t][j][e], BF ? 0x80008000u : 0x80000000u, a.scale);
+          kreg[t][j] = *reinterpret_cast<const u32x4_t *>(p < C ? src + 16 * p : zero);
         }
       }
-      f32x4_t o[NT][DT];
-      float m[NT], l[NT];
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        m[t] = -INFINITY, l[t] = 0.f;
-#pragma unroll
-        for (int d = 0; d < DT; ++d) o[t][d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      for (int j = 0; j < NV; ++j) {
+        const int idx = 64 * j + lane, row = idx / CR, p = idx % CR;
+        const char *src = (const char *)__shfl((unsigned long long)vo, row);
+        vreg[j] = *reinterpret_cast<const u32x4_t *>(p < C ? src + 16 * p : zero);
       }
-      const char *kbase = static_cast<const char *>(a.k) + h * a.k_ld[1] * ES;
-      const char *vbase = static_cast<const char *>(a.v) + h * a.v_ld[1] * ES;
-      const int kend = (b0 + bb + take) * UK;
-      int k0 = (b0 + bb) * UK + wave * KS;
-
-      // page of key k0 + (lane % KS), or one outside the pool if no row of
-      // the item sees it
-      auto lookup = [&](int at) {
-        const int tok = at + (lane & (KS - 1));
-        const bool in = tok >= kr.begin && tok < kr.end && at < kend;
-        const int page = table[in ? fast_div(tok, a.div_page) : 0];
-        return in ? page : -1;
-      };
-      u32x4_t kreg[KT][KC], vreg[NV];
-      uint64_t there;  // which of the strip's keys there are
-      auto load = [&](int at, int page) {
-        const int tok = at + (lane & (KS - 1));
-        const bool ok = page >= 0 && page < a.pages;
-        there = __ballot(ok);
-        const int in_page = tok - (int)fast_div(tok, a.div_page) * a.page_size;
-        const uint64_t ko = (uint64_t)(ok ? kbase + page * kps + in_page * kts : zero);
-        const uint64_t vo = (uint64_t)(ok ? vbase + page * vps + in_page * vts : zero);
+    };
+    int page = lookup(k0);
+    if (k0 < kend) load(k0, page);
+    page = lookup(k0 + UK);
+    for (; k0 < kend; k0 += UK) {
+      // values to the wave's LDS (LDS operations of a wave keep their order)
 #pragma unroll
-        for (int t = 0; t < KT; ++t) {
-          const char *src = (const char *)__shfl((unsigned long long)ko, 16 * t + n);
+      for (int j = 0; j < NV; ++j) {
+        const int idx = 64 * j + lane, row = idx / CR, p = idx % CR;
+        *reinterpret_cast<u32x4_t *>(vlds + row * VP + 16 * p) = vreg[j];
+      }
+      // scores: lane (row n, g) gets keys 16 u + 4 g .. + 3
+      f32x4_t sc[NT][KT];
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int u = 0; u < KT; ++u) {
+          f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int j = 0; j < KC; ++j) {
-            const int p = 4 * j + g;
-            kreg[t][j] = *reinterpret_cast<const u32x4_t *>(p < C ? src + 16 * p : zero);
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-          const int idx = 64 * j + lane, row = idx / CR, p = idx % CR;
-          const char *src = (const char *)__shfl((unsigned long long)vo, row);
-          vreg[j] = *reinterpret_cast<const u32x4_t *>(p < C ? src + 16 * p : zero);
-        }
-      };
-      int page = lookup(k0);
-      if (k0 < kend) load(k0, page);
-      page = lookup(k0 + UK);
-      for (; k0 < kend; k0 += UK) {
-        // values to the wave's LDS (LDS operations of a wave keep their order)
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-          const int idx = 64 * j + lane, row = idx / CR, p = idx % CR;
-          *reinterpret_cast<u32x4_t *>(vlds + row * VP + 16 * p) = vreg[j];
-        }
-        // scores: lane (row n, g) gets keys 16 u + 4 g .. + 3
-        f32x4_t sc[NT][KT];
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int u = 0; u < KT; ++u) {
-            f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int j = 0; j < KC; ++j) {
-              if constexpr (BF) {
-                acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                    __builtin_bit_cast(bf16x8_t, kreg[u][j]), __builtin_bit_cast(bf16x8_t, q[t][j]), acc, 0, 0, 0);
-              } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                  acc = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kreg[u][j][e]),
-                                                             __uint_as_float(q[t][j][e]), acc, 0, 0, 0);
-              }
-            }
-            sc[t][u] = acc;
-          }
-        const uint64_t held = there;
-        const bool whole = (uint32_t)held == (KS == 32 ? ~0u : 0xffffu) || (KS == 16 && (held & 0xffff) == 0xffff);
-        if (k0 + UK < kend) {
-          load(k0 + UK, page);
-          page = lookup(k0 + 2 * UK);
-        }
-        // weights
-        bf16x8_t ph[NT], pl[NT];
-        float pf[NT][4];
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          if (!whole || __ballot(lo[t] > k0 || hi[t] < k0 + KS)) {
-#pragma unroll
-            for (int u = 0; u < KT; ++u)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const int k = 16 * u + 4 * g + e;
-                if (!(held >> k & 1) || k0 + k < lo[t] || k0 + k >= hi[t]) sc[t][u][e] = -INFINITY;
-              }
-          }
-          float mx = sc[t][0][0];
-#pragma unroll
-          for (int u = 0; u < KT; ++u)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) mx = fmaxf(mx, sc[t][u][e]);
-          mx = fmaxf(m[t], max_over_groups(mx));
-          if (__ballot(mx > m[t])) {
-            const float f = mx == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[t] * c - mx * c);
-            l[t] *= f;
-#pragma unroll
-            for (int d = 0; d < DT; ++d)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) o[t][d][e] *= f;
-            m[t] = mx;
-          }
-          const float mc = m[t] == -INFINITY ? 0.f : m[t] * c;
-#pragma unroll
-          for (int u = 0; u < KT; ++u)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float p = __builtin_amdgcn_exp2f(fmaf(sc[t][u][e], c, -mc));
-              l[t] += p;
-              if constexpr (BF) {
-                const __bf16 hi_part = (__bf16)p;
-                ph[t][4 * u + e] = hi_part;
-                pl[t][4 * u + e] = (__bf16)(p - (float)hi_part);
-              } else {
-                pf[t][e] = p;
-              }
-            }
-        }
-        // O^T += V^T P^T
-#pragma unroll
-        for (int d = 0; d < DT; ++d) {
-          if constexpr (BF) {
-            typedef __attribute__((address_space(3))) s16x4_t *tr_ptr;
-            const unsigned char *at = vlds + (4 * g + n / 4) * VP + 32 * d + 8 * (n & 3);
-            const s16x4_t v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)at);
-            const s16x4_t v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)(at + 16 * VP));
-            const bf16x8_t v = __builtin_bit_cast(
-                bf16x8_t, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-              o[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, ph[t], o[t][d], 0, 0, 0);
-              o[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, pl[t], o[t][d], 0, 0, 0);
-            }
-          } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float v = *reinterpret_cast<const float *>(vlds + (4 * g + e) * VP + 4 * (16 * d + n));
-#pragma unroll
-              for (int t = 0; t < NT; ++t)
-                o[t][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, pf[t][e], o[t][d], 0, 0, 0);
-            }
-          }
-        }
-      }
-      // ---- join the four waves, 16 rows at a time
-      const bool complete = bb == 0 && take == nb;
-      const int64_t slot = 2 * (int64_t)blockIdx.x + (unit > span0 ? 1 : 0);
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const float lsum = sum_over_groups(l[t]);
-        __syncthreads();  // the waves' values and the previous rows are read
-        if (lane < 16) sm_m[wave][n] = m[t], sm_l[wave][n] = lsum;
-#pragma unroll
-        for (int d = 0; d < DT; ++d)
-          *reinterpret_cast<f32x4_t *>(vlds + (n * OP + 16 * d + 4 * g) * 4) = o[t][d];
-        __syncthreads();
-        for (int e = tid; e < 16 * DP / 4; e += kRowThreads) {
-          const int row = e / (DP / 4), d = e % (DP / 4) * 4;
-          const int rr = r0 + 16 * t + row;
-          const int tok = (int)fast_div(rr, a.div_group);
-          if (tok >= s.q || d >= a.D) continue;
-          const float mm = fmaxf(fmaxf(sm_m[0][row], sm_m[1][row]), fmaxf(sm_m[2][row], sm_m[3][row]));
-          float ll = 0.f;
-          f32x4_t oo = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            const float f = sm_m[w][row] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sm_m[w][row] * c - mm * c);
-            ll += f * sm_l[w][row];
-            const f32x4_t y = *reinterpret_cast<const f32x4_t *>(smem + w * kWaveLds + (row * OP + d) * 4);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) oo[k] += f * y[k];
-          }
-          if (complete) {
-            const float r = ll > 0.f ? 1.f / ll : 0.f;
-            const int64_t at = ((int64_t)(s.q0 + tok) * a.H + h * G + rr - tok * G) * a.D + d;
             if constexpr (BF) {
-              u32x2_t w;
-              w[0] = pack_bf16x2(oo[0] * r, oo[1] * r), w[1] = pack_bf16x2(oo[2] * r, oo[3] * r);
-              *reinterpret_cast<u32x2_t *>(static_cast<uint16_t *>(a.out) + at) = w;
+              acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                  __builtin_bit_cast(bf16x8_t, kreg[u][j]), __builtin_bit_cast(bf16x8_t, q[t][j]), acc, 0, 0, 0);
             } else {
 #pragma unroll
-              for (int k = 0; k < 4; ++k) oo[k] *= r;
-              *reinterpret_cast<f32x4_t *>(static_cast<float *>(a.out) + at) = oo;
+              for (int e = 0; e < 4; ++e)
+                acc = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kreg[u][j][e]),
+                                                           __uint_as_float(q[t][j][e]), acc, 0, 0, 0);
             }
-          } else {
-            const int64_t pr = slot * BM + 16 * t + row;
-            *reinterpret_cast<f32x4_t *>(a.part_o + pr * a.D + d) = oo;
-            if (d == 0) a.part_ml[2 * pr] = mm, a.part_ml[2 * pr + 1] = ll;
+          }
+          sc[t][u] = acc;
+        }
+      const uint64_t held = there;
+      const bool whole = (uint32_t)held == (KS == 32 ? ~0u : 0xffffu) || (KS == 16 && (held & 0xffff) == 0xffff);
+      if (k0 + UK < kend) {
+        load(k0 + UK, page);
+        page = lookup(k0 + 2 * UK);
+      }
+      // weights
+      bf16x8_t ph[NT], pl[NT];
+      float pf[NT][4];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        if (!whole || __ballot(lo[t] > k0 || hi[t] < k0 + KS)) {
+#pragma unroll
+          for (int u = 0; u < KT; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int k = 16 * u + 4 * g + e;
+              if (!(held >> k & 1) || k0 + k < lo[t] || k0 + k >= hi[t]) sc[t][u][e] = -INFINITY;
+            }
+        }
+        float mx = sc[t][0][0];
+#pragma unroll
+        for (int u = 0; u < KT; ++u)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) mx = fmaxf(mx, sc[t][u][e]);
+        mx = fmaxf(m[t], max_over_groups(mx));
+        if (__ballot(mx > m[t])) {
+          const float f = mx == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[t] * c - mx * c);
+          l[t] *= f;
+#pragma unroll
+          for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[t][d][e] *= f;
+          m[t] = mx;
+        }
+        const float mc = m[t] == -INFINITY ? 0.f : m[t] * c;
+#pragma unroll
+        for (int u = 0; u < KT; ++u)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float p = __builtin_amdgcn_exp2f(fmaf(sc[t][u][e], c, -mc));
+            l[t] += p;
+            if constexpr (BF) {
+              const __bf16 hi_part = (__bf16)p;
+              ph[t][4 * u + e] = hi_part;
+              pl[t][4 * u + e] = (__bf16)(p - (float)hi_part);
+            } else {
+              pf[t][e] = p;
+            }
+          }
+      }
+      // O^T += V^T P^T
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        if constexpr (BF) {
+          typedef __attribute__((address_space(3))) s16x4_t *tr_ptr;
+          const unsigned char *at = vlds + (4 * g + n / 4) * VP + 32 * d + 8 * (n & 3);
+          const s16x4_t v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)at);
+          const s16x4_t v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)(at + 16 * VP));
+          const bf16x8_t v = __builtin_bit_cast(
+              bf16x8_t, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            o[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, ph[t], o[t][d], 0, 0, 0);
+            o[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, pl[t], o[t][d], 0, 0, 0);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float v = *reinterpret_cast<const float *>(vlds + (4 * g + e) * VP + 4 * (16 * d + n));
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+              o[t][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, pf[t][e], o[t][d], 0, 0, 0);
           }
         }
       }
-      __syncthreads();  // before the next strips' values
-      if (tid == 0 && bb == 0 && !complete) {
-        split->u0 = unit, split->u1 = unit + nb, split->per = plan.per;
-        split->row0 = r0, split->rows = min(BM, s.q * G - r0), split->head = h, split->q0 = s.q0;
-      }
-      todo -= take;
-      unit += take;
     }
+    // ---- join the four waves, 16 rows at a time
+    const bool complete = bb == 0 && take == nb;
+    const int64_t slot = 2 * (int64_t)plan.wg + (unit > span0 ? 1 : 0);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const float lsum = sum_over_groups(l[t]);
+      __syncthreads();  // the waves' values and the previous rows are read
+      if (lane < 16) sm_m[wave][n] = m[t], sm_l[wave][n] = lsum;
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+        *reinterpret_cast<f32x4_t *>(vlds + (n * OP + 16 * d + 4 * g) * 4) = o[t][d];
+      __syncthreads();
+      for (int e = tid; e < 16 * DP / 4; e += kRowThreads) {
+        const int row = e / (DP / 4), d = e % (DP / 4) * 4;
+        const int rr = r0 + 16 * t + row;
+        const int tok = (int)fast_div(rr, a.div_group);
+        if (tok >= s.q || d >= a.D) continue;
+        const float mm = fmaxf(fmaxf(sm_m[0][row], sm_m[1][row]), fmaxf(sm_m[2][row], sm_m[3][row]));
+        float ll = 0.f;
+        f32x4_t oo = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const float f = sm_m[w][row] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sm_m[w][row] * c - mm * c);
+          ll += f * sm_l[w][row];
+          const f32x4_t y = *reinterpret_cast<const f32x4_t *>(smem + w * kWaveLds + (row * OP + d) * 4);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) oo[k] += f * y[k];
+        }
+        if (complete) {
+          const int64_t at = ((int64_t)(s.q0 + tok) * a.H + h * G + rr - tok * G) * a.D + d;
+          store_out<T>(a.out, at, oo, ll > 0.f ? 1.f / ll : 0.f);
+        } else {
+          const int64_t pr = slot * BM + 16 * t + row;
+          *reinterpret_cast<f32x4_t *>(a.part_o + pr * a.D + d) = oo;
+          if (d == 0) a.part_ml[2 * pr] = mm, a.part_ml[2 * pr + 1] = ll;
+        }
+      }
+    }
+    __syncthreads();  // before the next strips' values
+    if (tid == 0 && bb == 0 && !complete) {
+      split->u0 = unit, split->u1 = unit + nb, split->per = plan.per;
+      split->row0 = r0, split->rows = min(BM, s.q * G - r0), split->head = h, split->q0 = s.q0;
+    }
+    todo -= take;
+    unit += take;
   }
 }
 
 // Joins the parts of the (item, head) that workgroup blockIdx.x of the first
 // launch began and others finished.  A thread takes four outputs of a row.
-template <typename T, int BM>
-__global__ __launch_bounds__(256) void paged_attn_join_kernel(AttnArgs a) {
+template <typename T>
+__global__ __launch_bounds__(256) void paged_attn_join_kernel(AttnArgs a, int BM) {
   const Split s = static_cast<const Split *>(a.splits)[blockIdx.x];
   if (s.rows == 0) return;
   const float c = score_factor(a.scale);
@@ -377,15 +351,7 @@ __global__ __launch_bounds__(256) void paged_attn_join_kernel(AttnArgs a) {
     const float r = l > 0.f ? 1.f / l : 0.f;
     const int rr = s.row0 + row, tok = (int)fast_div(rr, a.div_group);
     const int64_t at = ((int64_t)(s.q0 + tok) * a.H + s.head * G + rr - tok * G) * a.D + d;
-    if constexpr (sizeof(T) == 2) {
-      u32x2_t w;
-      w[0] = pack_bf16x2(o[0] * r, o[1] * r), w[1] = pack_bf16x2(o[2] * r, o[3] * r);
-      *reinterpret_cast<u32x2_t *>(static_cast<uint16_t *>(a.out) + at) = w;
-    } else {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) o[k] *= r;
-      *reinterpret_cast<f32x4_t *>(static_cast<float *>(a.out) + at) = o;
-    }
+    store_out<T>(a.out, at, o, r);
   }
 }
 
@@ -404,9 +370,6 @@ hipError_t launch_rows(const AttnArgs &a, hipStream_t s) {
     if (grown != hipSuccess) return grown;
   }
   kernel<<<kRowGrid, kRowThreads, lds, s>>>(a);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return e;
-  paged_attn_join_kernel<T, 16 * NT><<<dim3(kRowGrid, std::min(NT, 4)), 256, 0, s>>>(a);
   return hipGetLastError();
 }
 
@@ -424,9 +387,18 @@ hipError_t launch_rows_n(const AttnArgs &a, int nt, hipStream_t s) {
   return launch_rows_d<T, 4>(a, s);
 }
 
-int row_tiles(const AttnArgs &a) {
+// Rows of one cache head from which on the tile kernel takes over: there each
+// key costs the row kernel's matrix operations more time than its bytes.
+constexpr int kRowsMost = 64;
+
+struct Shape {
+  bool tiles;
+  int bm, grid;
+};
+Shape shape_of(const AttnArgs &a) {
   const int64_t rows = std::min(std::max<int64_t>(a.max_q, 1), a.T) * (a.H / a.KV);
-  return rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  if (rows > kRowsMost) return {true, tile_rows(a), tile_grid(a)};
+  return {false, rows <= 16 ? 16 : rows <= 32 ? 32 : 64, kRowGrid};
 }
 
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
@@ -435,20 +407,29 @@ size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
 size_t paged_attn_workspace(const AttnArgs &a) {
   if (a.T == 0) return 0;
-  const size_t slots = 2 * (size_t)kRowGrid * 16 * row_tiles(a);
-  return up256(kRowGrid * sizeof(Split)) + up256(slots * 2 * sizeof(float)) + slots * a.D * sizeof(float);
+  const Shape p = shape_of(a);
+  const size_t slots = 2 * (size_t)p.grid * p.bm;
+  return up256(p.grid * sizeof(Split)) + up256(slots * 2 * sizeof(float)) + slots * a.D * sizeof(float);
 }
 
 hipError_t launch_paged_attn(AttnArgs a, void *workspace, hipStream_t s) {
-  const int nt = row_tiles(a);
-  const size_t slots = 2 * (size_t)kRowGrid * 16 * nt;
+  const Shape p = shape_of(a);
+  const size_t slots = 2 * (size_t)p.grid * p.bm;
   a.group = a.H / a.KV;
   a.div_group = make_div(a.group), a.div_page = make_div(a.page_size);
   char *at = static_cast<char *>(workspace);
-  a.splits = at, at += up256(kRowGrid * sizeof(Split));
+  a.splits = at, at += up256(p.grid * sizeof(Split));
   a.part_ml = reinterpret_cast<float *>(at), at += up256(slots * 2 * sizeof(float));
   a.part_o = reinterpret_cast<float *>(at);
-  return a.dtype == ZT_DT_BF16 ? launch_rows_n<uint16_t>(a, nt, s) : launch_rows_n<float>(a, nt, s);
+  const bool bf = a.dtype == ZT_DT_BF16;
+  const hipError_t e = p.tiles ? launch_tiles(a, s)
+                       : bf   ? launch_rows_n<uint16_t>(a, p.bm / 16, s)
+                              : launch_rows_n<float>(a, p.bm / 16, s);
+  if (e != hipSuccess) return e;
+  const dim3 grid(p.grid, std::max(p.bm / 16, 1));
+  if (bf) paged_attn_join_kernel<uint16_t><<<grid, 256, 0, s>>>(a, p.bm);
+  else paged_attn_join_kernel<float><<<grid, 256, 0, s>>>(a, p.bm);
+  return hipGetLastError();
 }
 
 }  // namespace zt
