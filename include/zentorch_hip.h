@@ -418,7 +418,7 @@ int zt_rotary_cache_append(const void *q, int64_t T, int64_t H, const int64_t *q
  *  cu_seqlens [S + 1] int32 ascending from 0; context_lens [S] int32
  *  max_query_len  the longest chunk; it picks the kernels, and too small a
  *             value costs time, not results
- *  head_dim   a multiple of 8, at most 256
+ *  head_dim   a multiple of 8, at most 256; S <= 1024
  *  workspace  zt_paged_attention_workspace_size(...) bytes, 16-byte aligned
  */
 int zt_paged_attention(const void *q, int64_t T, int64_t H, int64_t ld_token, int64_t ld_head,

@@ -61,11 +61,17 @@ struct Seq {
   int q0, q, n;  // first row of the batch, new tokens, all tokens
 };
 
-__device__ __forceinline__ Seq seq_of(const AttnArgs &a, int i) {
-  const int T = (int)a.T;
-  const int q0 = min(max(a.cu[i], 0), T);
-  return {q0, min(max(a.cu[i + 1], q0), T) - q0, min(max(a.ctx[i], 0), a.W * a.page_size)};
-}
+// The batch as the device's arrays give it, held to its bounds, in LDS: read
+// from memory once, because each read there is a round trip that a short call
+// waits for.
+struct Batch {
+  int *tile_base;  // [S + 1] items before sequence i's
+  int *q0, *q, *n; // [S]
+  __device__ __forceinline__ Batch(void *lds, int S)
+      : tile_base(static_cast<int *>(lds)), q0(tile_base + S + 1), q(q0 + S), n(q + S) {}
+  __device__ __forceinline__ Seq operator[](int i) const { return {q0[i], q[i], n[i]}; }
+};
+constexpr int batch_ints(int S) { return 4 * S + 1; }
 
 // Keys [begin, end) that some row of tile r sees.
 struct KeyRange {
@@ -133,9 +139,8 @@ __device__ __forceinline__ int seq_of_item(const int *tile_base, int S, int x) {
   return lo;
 }
 
-// tile_base[S + 1] (LDS): items before sequence i's.  N threads.
 template <int N>
-__device__ __forceinline__ Plan make_plan(const AttnArgs &a, int BM, int UK, int *tile_base,
+__device__ __forceinline__ Plan make_plan(const AttnArgs &a, int BM, int UK, const Batch &batch,
                                           PlanShared *sh) {
   const int tid = threadIdx.x;
   Plan p{};
@@ -143,18 +148,22 @@ __device__ __forceinline__ Plan make_plan(const AttnArgs &a, int BM, int UK, int
   for (int i0 = 0; i0 < a.S; i0 += N) {
     const int i = i0 + tid;
     int64_t tiles = 0, total;
-    if (i < a.S) tiles = ((int64_t)seq_of(a, i).q * a.group + BM - 1) / BM;
+    if (i < a.S) {
+      const int T = (int)a.T, q0 = min(max(a.cu[i], 0), T), q = min(max(a.cu[i + 1], q0), T) - q0;
+      batch.q0[i] = q0, batch.q[i] = q, batch.n[i] = min(max(a.ctx[i], 0), a.W * a.page_size);
+      tiles = (uint32_t)(q * a.group + BM - 1) / (uint32_t)BM;
+    }
     const int64_t before = scan64<N>(tiles, sh->part, &total);
-    if (i < a.S) tile_base[i] = (int)(items + before);
+    if (i < a.S) batch.tile_base[i] = (int)(items + before);
     items += total;
   }
-  if (tid == 0) tile_base[a.S] = (int)items;
+  if (tid == 0) batch.tile_base[a.S] = (int)items;
   __syncthreads();
   p.items = (int)items;
   auto units_of = [&](int x) -> int64_t {
     if (x >= p.items) return 0;
-    const int i = seq_of_item(tile_base, a.S, x);
-    return blocks_of(keys_of(a, seq_of(a, i), x - tile_base[i], BM), UK);
+    const int i = seq_of_item(batch.tile_base, a.S, x);
+    return blocks_of(keys_of(a, batch[i], x - batch.tile_base[i], BM), UK);
   };
   int64_t sum = 0, units = 0, before = 0;
   for (int x0 = 0; x0 < p.items; x0 += N) {
@@ -188,6 +197,24 @@ __device__ __forceinline__ Plan make_plan(const AttnArgs &a, int BM, int UK, int
   return p;
 }
 
+// Where the keys of one sequence are: a lane's lookup of its key's page, kept
+// as it was loaded (a use right behind the load would wait for everything in
+// flight), and the offset of its row of K or V in units of 16 bytes.
+struct Pages {
+  const int *table;
+  int begin, end;  // keys that some row of the item sees
+  __device__ __forceinline__ int lookup(const AttnArgs &a, int tok) const {
+    return table[tok >= begin && tok < end ? fast_div(tok, a.div_page) : 0];
+  }
+  __device__ __forceinline__ bool there(const AttnArgs &a, int tok, int page) const {
+    return tok >= begin && tok < end && page >= 0 && page < a.pages;
+  }
+};
+__device__ __forceinline__ uint32_t row_offset(const AttnArgs &a, const uint32_t (&ld)[2], int tok, int page) {
+  const uint32_t off = tok - fast_div(tok, a.div_page) * a.page_size;
+  return (uint32_t)page * ld[0] + off * ld[1];
+}
+
 // What a workgroup leaves about the (item, head) that it began and did not
 // finish (rows = 0: none).  Its partial results are in slots 2 * first + (1 if
 // the unit before it is in the same span), 2 * (first + 1), ..
@@ -201,15 +228,15 @@ struct Split {
 // of no sequence.
 template <int N>
 __device__ __forceinline__ void zero_rows(const AttnArgs &a, const Plan &p, int BM, int UK,
-                                          const int *tile_base) {
+                                          const Batch &batch) {
   const int esize = a.dtype == ZT_DT_F32 ? 4 : 2, chunks = a.D * esize / 16;  // of 16 bytes a head
   char *out = static_cast<char *>(a.out);
   for (int x = blockIdx.x; x < p.items; x += gridDim.x) {
-    const int i = seq_of_item(tile_base, a.S, x);
-    const Seq s = seq_of(a, i);
-    if (blocks_of(keys_of(a, s, x - tile_base[i], BM), UK)) continue;
+    const int i = seq_of_item(batch.tile_base, a.S, x), tile = x - batch.tile_base[i];
+    const Seq s = batch[i];
+    if (blocks_of(keys_of(a, s, tile, BM), UK)) continue;
     // the item's rows, of every cache head
-    const int r0 = (x - tile_base[i]) * BM, rows = min(BM, s.q * a.group - r0);
+    const int r0 = tile * BM, rows = min(BM, s.q * a.group - r0);
     const int64_t n = (int64_t)rows * a.KV * chunks;
     for (int64_t e = threadIdx.x; e < n; e += N) {
       const int c = (int)(e % chunks), y = (int)(e / chunks), h = y / rows, row = r0 + y - h * rows;
@@ -218,8 +245,7 @@ __device__ __forceinline__ void zero_rows(const AttnArgs &a, const Plan &p, int 
       reinterpret_cast<u32x4_t *>(out)[at] = u32x4_t{0, 0, 0, 0};
     }
   }
-  const int64_t T = a.T, lo = a.S ? min(max((int64_t)a.cu[0], (int64_t)0), T) : T;
-  const int64_t hi = a.S ? min(max((int64_t)a.cu[a.S], (int64_t)0), T) : T;
+  const int64_t T = a.T, lo = a.S ? batch.q0[0] : T, hi = a.S ? batch.q0[a.S - 1] + batch.q[a.S - 1] : T;
   const int64_t row = (int64_t)a.H * chunks, n = (lo + T - hi) * row;
   for (int64_t e = (int64_t)blockIdx.x * N + threadIdx.x; e < n; e += (int64_t)gridDim.x * N)
     reinterpret_cast<u32x4_t *>(out)[e < lo * row ? e : e - lo * row + hi * row] = u32x4_t{0, 0, 0, 0};

@@ -17,6 +17,8 @@ bool is_float_dt(int dt) { return dt == ZT_DT_F32 || dt == ZT_DT_BF16; }
 
 // Rows of a batch that the page kernels hold in LDS.
 constexpr int64_t kMaxRows = 4096;
+// Sequences of an attention call (16 bytes of LDS each).
+constexpr int64_t kMaxSeqs = 1024;
 
 bool divides16(const void *p, std::initializer_list<int64_t> elems, int64_t esize) {
   if (reinterpret_cast<uintptr_t>(p) % 16) return false;
@@ -233,10 +235,10 @@ static int attn_args(const char *op, int64_t T, int64_t H, const zt_kv_cache *ca
   if (window < 0 || (window && !causal))
     return api_fail(ZT_EINVAL, "%s: a window (%lld) must not be negative and needs causal", op,
                     (long long)window);
-  if (H > 65535 || S > kMaxRows || T > (1 << 24) || T * H > INT32_MAX / 2 || W > (1 << 24) ||
+  if (H > 65535 || S > kMaxSeqs || T > (1 << 24) || T * H > INT32_MAX / 2 || W > (1 << 24) ||
       cache->page_size > (1 << 24) || W * cache->page_size > (1 << 30))
     return api_fail(ZT_EUNSUPPORTED, "%s: at most 65535 heads, %lld sequences, 2^24 tokens, 2^30 / "
-                    "heads rows and a table of 2^30 tokens a sequence", op, (long long)kMaxRows);
+                    "heads rows and a table of 2^30 tokens a sequence", op, (long long)kMaxSeqs);
   *a = zt::AttnArgs{};
   a->T = T, a->H = (int)H, a->KV = (int)cache->heads, a->D = (int)cache->head_dim;
   a->S = (int)S, a->W = (int)W, a->page_size = (int)cache->page_size, a->pages = cache->pages;
@@ -269,6 +271,11 @@ int zt_paged_attention(const void *q, int64_t T, int64_t H, int64_t ld_token, in
       !divides16(cache->k, {cache->k_strides[0], cache->k_strides[1], cache->k_strides[2]}, es) ||
       !divides16(cache->v, {cache->v_strides[0], cache->v_strides[1], cache->v_strides[2]}, es))
     return api_fail(ZT_EUNSUPPORTED, "%s: query, output and cache need 16-byte aligned rows", op);
+  // the kernels count a layer's rows in units of 16 bytes, in 32 bits
+  for (const int64_t *st : {cache->k_strides, cache->v_strides})
+    if ((double)cache->pages * (double)st[0] + (double)cache->page_size * (double)st[2] >=
+        4294967295.0 * (16 / es))
+      return api_fail(ZT_EUNSUPPORTED, "%s: one head's keys or values span 64 GB and more", op);
   const size_t need = zt::paged_attn_workspace(a);
   if (need && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16))
     return api_fail(ZT_EINVAL, "%s: 16-byte aligned workspace of %zu bytes needed, %zu given", op, need,

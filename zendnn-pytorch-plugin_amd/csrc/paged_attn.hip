@@ -52,7 +52,7 @@ __device__ __forceinline__ float sum_over_groups(float x) {
 // bf16 weights keep the digits that one bf16 drops in a second MFMA (p = hi +
 // lo): the matrix pipe is idle most of the time here.
 template <typename T, int DP, int NT>
-__global__ __launch_bounds__(kRowThreads) void paged_attn_row_kernel(AttnArgs a) {
+__global__ __launch_bounds__(kRowThreads, NT * DP <= 128 ? 2 : 1) void paged_attn_row_kernel(AttnArgs a) {
   constexpr bool BF = sizeof(T) == 2;
   constexpr int ES = sizeof(T);
   constexpr int BM = 16 * NT;
@@ -69,34 +69,31 @@ __global__ __launch_bounds__(kRowThreads) void paged_attn_row_kernel(AttnArgs a)
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   __shared__ PlanShared sh;
   __shared__ float sm_m[4][16], sm_l[4][16];
-  int *tile_base = reinterpret_cast<int *>(smem + 4 * kWaveLds);
+  const Batch batch(smem + 4 * kWaveLds, a.S);
 
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   unsigned char *vlds = smem + wave * kWaveLds;
-  const Plan plan = make_plan<kRowThreads>(a, BM, UK, tile_base, &sh);
-  zero_rows<kRowThreads>(a, plan, BM, UK, tile_base);
+  const Plan plan = make_plan<kRowThreads>(a, BM, UK, batch, &sh);
   Split *split = static_cast<Split *>(a.splits) + plan.wg;
   if (tid == 0) split->rows = 0;
-  if (plan.todo == 0) return;
 
   const float c = score_factor(a.scale);
   const int G = a.group, C = a.D * ES / 16;  // 16-byte pieces that a row has
   const char *zero = reinterpret_cast<const char *>(kZeroRow);
-  const int64_t kps = a.k_ld[0] * ES, kts = a.k_ld[2] * ES, vps = a.v_ld[0] * ES, vts = a.v_ld[2] * ES;
 
   int64_t todo = plan.todo, unit = plan.per * plan.wg;
   const int64_t span0 = unit;
   for (int h = plan.head, x = plan.item, bb = plan.off; todo > 0; ++x, bb = 0) {
     if (x == plan.items) ++h, x = 0;
-    const int i = seq_of_item(tile_base, a.S, x);
-    const Seq s = seq_of(a, i);
-    const int r0 = (x - tile_base[i]) * BM;
-    const KeyRange kr = keys_of(a, s, x - tile_base[i], BM);
+    const int i = seq_of_item(batch.tile_base, a.S, x), tile = x - batch.tile_base[i];
+    const Seq s = batch[i];
+    const int r0 = tile * BM;
+    const KeyRange kr = keys_of(a, s, tile, BM);
     const int nb = blocks_of(kr, UK), b0 = kr.begin / UK;
     if (nb == 0) continue;
     const int take = (int)min((int64_t)(nb - bb), todo);
-    const int *table = a.table + (int64_t)i * a.W;
+    const Pages pages{a.table + (int64_t)i * a.W, kr.begin, kr.end};
     // the lane's rows: token, head, and the keys each sees
     int row_t[NT], lo[NT], hi[NT];
     bool live[NT];
@@ -135,26 +132,18 @@ __global__ __launch_bounds__(kRowThreads) void paged_attn_row_kernel(AttnArgs a)
     const int kend = (b0 + bb + take) * UK;
     int k0 = (b0 + bb) * UK + wave * KS;
 
-    // page of key k0 + (lane % KS), or one outside the pool if no row of
-    // the item sees it
-    auto lookup = [&](int at) {
-      const int tok = at + (lane & (KS - 1));
-      const bool in = tok >= kr.begin && tok < kr.end && at < kend;
-      const int page = table[in ? fast_div(tok, a.div_page) : 0];
-      return in ? page : -1;
-    };
     u32x4_t kreg[KT][KC], vreg[NV];
     uint64_t there;  // which of the strip's keys there are
     auto load = [&](int at, int page) {
       const int tok = at + (lane & (KS - 1));
-      const bool ok = page >= 0 && page < a.pages;
+      const bool ok = pages.there(a, tok, page);
       there = __ballot(ok);
-      const int in_page = tok - (int)fast_div(tok, a.div_page) * a.page_size;
-      const uint64_t ko = (uint64_t)(ok ? kbase + page * kps + in_page * kts : zero);
-      const uint64_t vo = (uint64_t)(ok ? vbase + page * vps + in_page * vts : zero);
+      const uint32_t ko = ok ? row_offset(a, a.k_row, tok, page) : ~0u;
+      const uint32_t vo = ok ? row_offset(a, a.v_row, tok, page) : ~0u;
 #pragma unroll
       for (int t = 0; t < KT; ++t) {
-        const char *src = (const char *)__shfl((unsigned long long)ko, 16 * t + n);
+        const uint32_t r = __shfl(ko, 16 * t + n);
+        const char *src = r == ~0u ? zero : kbase + (uint64_t)r * 16;
 #pragma unroll
         for (int j = 0; j < KC; ++j) {
           const int p = 4 * j + g;
@@ -164,10 +153,11 @@ __global__ __launch_bounds__(kRowThreads) void paged_attn_row_kernel(AttnArgs a)
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         const int idx = 64 * j + lane, row = idx / CR, p = idx % CR;
-        const char *src = (const char *)__shfl((unsigned long long)vo, row);
-        vreg[j] = *reinterpret_cast<const u32x4_t *>(p < C ? src + 16 * p : zero);
+        const uint32_t r = __shfl(vo, row);
+        vreg[j] = *reinterpret_cast<const u32x4_t *>(r != ~0u && p < C ? vbase + (uint64_t)r * 16 + 16 * p : zero);
       }
     };
+    auto lookup = [&](int at) { return pages.lookup(a, at + (lane & (KS - 1))); };
     int page = lookup(k0);
     if (k0 < kend) load(k0, page);
     page = lookup(k0 + UK);
@@ -211,13 +201,15 @@ __global__ __launch_bounds__(kRowThreads) void paged_attn_row_kernel(AttnArgs a)
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         if (!whole || __ballot(lo[t] > k0 || hi[t] < k0 + KS)) {
+          // bit 16 u + e of `seen`: the lane's e-th key of 16
+          const int from = min(max(lo[t] - k0, 0), 32), to = min(max(hi[t] - k0, 0), 32);
+          const uint64_t range = (1ull << to) - (1ull << min(from, to));
+          const uint32_t seen = ((uint32_t)range & (uint32_t)held) >> (4 * g);
 #pragma unroll
           for (int u = 0; u < KT; ++u)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int k = 16 * u + 4 * g + e;
-              if (!(held >> k & 1) || k0 + k < lo[t] || k0 + k >= hi[t]) sc[t][u][e] = -INFINITY;
-            }
+            for (int e = 0; e < 4; ++e)
+              if (!(seen & (1u << (16 * u + e)))) sc[t][u][e] = -INFINITY;
         }
         float mx = sc[t][0][0];
 #pragma unroll
@@ -322,6 +314,7 @@ __global__ __launch_bounds__(kRowThreads) void paged_attn_row_kernel(AttnArgs a)
     todo -= take;
     unit += take;
   }
+  zero_rows<kRowThreads>(a, plan, BM, UK, batch);
 }
 
 // Joins the parts of the (item, head) that workgroup blockIdx.x of the first
@@ -337,16 +330,33 @@ __global__ __launch_bounds__(256) void paged_attn_join_kernel(AttnArgs a, int BM
     const int row = e / d4, d = (e - row * d4) * 4;
     float m = -INFINITY, l = 0.f;
     f32x4_t o = {0.f, 0.f, 0.f, 0.f};
-    int64_t slot = 2 * (int64_t)first + (s.u0 > first * s.per ? 1 : 0);
-    for (int w = first; w <= last; ++w, slot = 2 * (int64_t)w) {
-      const float *ml = a.part_ml + 2 * (slot * BM + row);
-      const f32x4_t y = *reinterpret_cast<const f32x4_t *>(a.part_o + (slot * BM + row) * a.D + d);
-      const float mw = ml[0], lw = ml[1], mm = fmaxf(m, mw);
-      const float f0 = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m * c - mm * c);
-      const float f1 = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw * c - mm * c);
-      m = mm, l = l * f0 + lw * f1;
+    const int odd = s.u0 > first * s.per;  // the first part's place in its pair of slots
+    for (int w0 = first; w0 <= last; w0 += 8) {  // eight parts' loads at once
+      float mw[8], lw[8];
+      f32x4_t y[8];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) o[k] = o[k] * f0 + y[k] * f1;
+      for (int k = 0; k < 8; ++k) {
+        const int w = min(w0 + k, last);
+        const int64_t at = (2 * (int64_t)w + (w == first ? odd : 0)) * BM + row;
+        mw[k] = w0 + k <= last ? a.part_ml[2 * at] : -INFINITY;
+        lw[k] = a.part_ml[2 * at + 1];
+        y[k] = *reinterpret_cast<const f32x4_t *>(a.part_o + at * a.D + d);
+      }
+      float mm = m;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) mm = fmaxf(mm, mw[k]);
+      if (mm == -INFINITY) continue;
+      const float f0 = __builtin_amdgcn_exp2f(m * c - mm * c);
+      m = mm, l *= f0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] *= f0;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float f = __builtin_amdgcn_exp2f(mw[k] * c - mm * c);
+        l += lw[k] * f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] += y[k][e] * f;
+      }
     }
     const float r = l > 0.f ? 1.f / l : 0.f;
     const int rr = s.row0 + row, tok = (int)fast_div(rr, a.div_group);
@@ -362,7 +372,7 @@ template <typename T, int DP, int NT>
 hipError_t launch_rows(const AttnArgs &a, hipStream_t s) {
   constexpr int KS = sizeof(T) == 2 ? 32 : 16, VP = DP * (int)sizeof(T) + (sizeof(T) == 2 ? 32 : 16);
   constexpr int wave = std::max(KS * VP, 16 * (DP + 4) * 4);
-  const size_t lds = 4 * wave + ((size_t)a.S + 1) * 4;
+  const size_t lds = 4 * wave + batch_ints(a.S) * 4;
   auto kernel = paged_attn_row_kernel<T, DP, NT>;
   if (lds > 64 * 1024) {
     const hipError_t grown = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
@@ -417,6 +427,9 @@ hipError_t launch_paged_attn(AttnArgs a, void *workspace, hipStream_t s) {
   const size_t slots = 2 * (size_t)p.grid * p.bm;
   a.group = a.H / a.KV;
   a.div_group = make_div(a.group), a.div_page = make_div(a.page_size);
+  const int64_t per16 = a.dtype == ZT_DT_F32 ? 4 : 8;
+  for (int i = 0; i < 2; ++i)
+    a.k_row[i] = (uint32_t)(a.k_ld[2 * i] / per16), a.v_row[i] = (uint32_t)(a.v_ld[2 * i] / per16);
   char *at = static_cast<char *>(workspace);
   a.splits = at, at += up256(p.grid * sizeof(Split));
   a.part_ml = reinterpret_cast<float *>(at), at += up256(slots * 2 * sizeof(float));

@@ -51,9 +51,9 @@ __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32);
 //
 // bf16 weights are rounded once for the second product (half a step each, 2^-8,
 // and independent, so the sum of n of them is off by much less); their sum is
-// taken before the rounding.
+// taken of the rounded ones, so that a row's weights still add up to one.
 template <typename T, int DP, int DC, int NW>
-__global__ __launch_bounds__(64 * NW, NW / 4) void paged_attn_tile_kernel(AttnArgs a) {
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP <= 128 ? 2 : 1, DP <= 128 ? 2 : 1))) void paged_attn_tile_kernel(AttnArgs a) {
   constexpr bool BF = sizeof(T) == 2;
   constexpr int ES = sizeof(T), NTH = 64 * NW, BM = 32 * NW;
   constexpr int KT = BF ? 2 : 1, TK = 32 * KT;  // keys of a tile
@@ -65,71 +65,77 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void paged_attn_tile_kernel(AttnAr
   constexpr int DT = DC / 32;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   __shared__ PlanShared sh;
-  int *tile_base = reinterpret_cast<int *>(smem + 4 * STAGE);
+  const Batch batch(smem + 4 * STAGE, a.S);
 
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const Plan plan = make_plan<NTH>(a, BM, TK, tile_base, &sh);
-  zero_rows<NTH>(a, plan, BM, TK, tile_base);
+  const Plan plan = make_plan<NTH>(a, BM, TK, batch, &sh);
   Split *split = static_cast<Split *>(a.splits) + plan.wg;
   if (tid == 0) split->rows = 0;
-  if (plan.todo == 0) return;
 
   const float c = score_factor(a.scale);
   const int G = a.group, C = a.D * ES / 16;
   const char *zero = reinterpret_cast<const char *>(kZeroRow);
-  const int64_t kps = a.k_ld[0] * ES, kts = a.k_ld[2] * ES, vps = a.v_ld[0] * ES, vts = a.v_ld[2] * ES;
   // where a lane's pieces of K and columns of V are in a tile
   auto kswz = [](int row) { return CR >= 16 ? row & 15 : row & 7; };
   auto vswz = [](int row) {
     return !BF ? ((row >> 2) & 1) << 3 : CR >= 16 ? (row & 3) << 2 : ((row >> 1) & 1) << 2;
   };
   const uint32_t lds0 = lds_addr(smem);
+  // what the lane fetches in each of its wave's transfers: row, pieces of K and V
+  int part_row[NI], part_k[NI], part_v[NI];
+#pragma unroll
+  for (int j = 0; j < NI; ++j) {
+    const int idx = (wave * NI + j) * 64 + lane, slot = idx % CR;
+    part_row[j] = idx / CR;
+    part_k[j] = slot ^ kswz(part_row[j]), part_v[j] = slot ^ vswz(part_row[j]);
+  }
 
   int64_t todo = plan.todo, unit = plan.per * plan.wg;
   const int64_t span0 = unit;
   for (int h = plan.head, x = plan.item, bb = plan.off; todo > 0; ++x, bb = 0) {
     if (x == plan.items) ++h, x = 0;
-    const int i = seq_of_item(tile_base, a.S, x);
-    const Seq s = seq_of(a, i);
-    const int r0 = (x - tile_base[i]) * BM;
-    const KeyRange kr = keys_of(a, s, x - tile_base[i], BM);
+    const int i = seq_of_item(batch.tile_base, a.S, x), tile = x - batch.tile_base[i];
+    const Seq s = batch[i];
+    const int r0 = tile * BM;
+    const KeyRange kr = keys_of(a, s, tile, BM);
     const int nb = blocks_of(kr, TK), b0 = kr.begin / TK;
     if (nb == 0) continue;
     const int take = (int)min((int64_t)(nb - bb), todo);
-    const int *table = a.table + (int64_t)i * a.W;
+    const Pages pages{a.table + (int64_t)i * a.W, kr.begin, kr.end};
     const char *kbase = static_cast<const char *>(a.k) + h * a.k_ld[1] * ES;
     const char *vbase = static_cast<const char *>(a.v) + h * a.v_ld[1] * ES;
 
-    // page of key at + (lane % TK), or -1 if no row of the item sees it
-    auto lookup = [&](int at) {
+    auto lookup = [&](int at) { return pages.lookup(a, at + (lane & (TK - 1))); };
+    // K and V of a tile go to LDS in NI parts: offsets first, then each part's
+    // pieces.  A tile past the span's last is zeros, so that the parts can be
+    // issued between matrix operations without a branch.
+    uint32_t ko, vo;
+    bool gaps;  // some of its keys are not there
+    auto offsets = [&](int at, int page, bool real) -> uint64_t {
       const int tok = at + (lane & (TK - 1));
-      const bool in = tok >= kr.begin && tok < kr.end;
-      const int page = table[in ? fast_div(tok, a.div_page) : 0];
-      return in ? page : -1;
-    };
-    // K and V of the tile at `at` into stage `st`; returns which keys there are
-    auto load = [&](int at, int page, int st) -> uint64_t {
-      const int tok = at + (lane & (TK - 1));
-      const bool ok = page >= 0 && page < a.pages;
-      const int in_page = tok - (int)fast_div(tok, a.div_page) * a.page_size;
-      const uint64_t ko = (uint64_t)(ok ? kbase + page * kps + in_page * kts : zero);
-      const uint64_t vo = (uint64_t)(ok ? vbase + page * vps + in_page * vts : zero);
-#pragma unroll
-      for (int j = 0; j < NI; ++j) {
-        const int idx = (wave * NI + j) * 64 + lane, row = idx / CR, slot = idx % CR;
-        const char *ks = (const char *)__shfl((unsigned long long)ko, row);
-        const char *vs = (const char *)__shfl((unsigned long long)vo, row);
-        const int kp = slot ^ kswz(row), vp = slot ^ vswz(row);
-        load_to_lds(kp < C ? ks + 16 * kp : zero, lds0 + st * 2 * STAGE + (wave * NI + j) * 1024);
-        load_to_lds(vp < C ? vs + 16 * vp : zero, lds0 + st * 2 * STAGE + STAGE + (wave * NI + j) * 1024);
-      }
+      const bool ok = real && pages.there(a, tok, page);
+      ko = ok ? row_offset(a, a.k_row, tok, page) : ~0u;
+      vo = ok ? row_offset(a, a.v_row, tok, page) : ~0u;
       const uint64_t m = __ballot(ok);
+      gaps = m != ~0ull || C != CR;
       return TK == 64 ? m : m & 0xffffffffull;
     };
+    auto issue = [&](int j, int st) {
+      const uint32_t kr16 = __shfl(ko, part_row[j]), vr16 = __shfl(vo, part_row[j]);
+      const char *ks = kbase + (uint64_t)(kr16 + part_k[j]) * 16, *vs = vbase + (uint64_t)(vr16 + part_v[j]) * 16;
+      if (gaps) {
+        ks = kr16 != ~0u && part_k[j] < C ? ks : zero;
+        vs = vr16 != ~0u && part_v[j] < C ? vs : zero;
+      }
+      load_to_lds(ks, lds0 + st * 2 * STAGE + (wave * NI + j) * 1024);
+      load_to_lds(vs, lds0 + st * 2 * STAGE + STAGE + (wave * NI + j) * 1024);
+    };
     const int k_first = (b0 + bb) * TK;
-    uint64_t there = load(k_first, lookup(k_first), 0), there_next = 0;
-    int page = take > 1 ? lookup(k_first + TK) : -1;
+    uint64_t there = offsets(k_first, lookup(k_first), true);
+#pragma unroll
+    for (int j = 0; j < NI; ++j) issue(j, 0);
+    int page = lookup(k_first + TK);
 
     // ---- the wave's rows: lane (row n, half) holds pieces 2 j + half of q
     const int row = r0 + 32 * wave + n;
@@ -163,43 +169,59 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void paged_attn_tile_kernel(AttnAr
     for (int t = 0; t < take; ++t) {
       const int k0 = k_first + t * TK, st = t & 1;
       wait_and_meet();  // the tile is there, and the previous one is done with
-      if (t + 1 < take) {
-        there_next = load(k0 + TK, page, st ^ 1);
-        if (t + 2 < take) page = lookup(k0 + 2 * TK);
-      }
+      const uint64_t there_next = offsets(k0 + TK, page, t + 1 < take);
+      page = lookup(k0 + 2 * TK);
       if (wave_live && k0 < hi_max && k0 + TK > lo_min) {
         const unsigned char *kt = smem + st * 2 * STAGE, *vt = kt + STAGE;
-        // ---- scores
+        // ---- scores.  Keys are read kAhead operands before their use; the
+        // fences keep the compiler from moving each read next to its use.
         f32x16_t sc[KT];
+        {
+          constexpr int kSteps = KT * NQ, kAhead = kSteps < 4 ? kSteps : 4;
+          u32x4_t k[kAhead];
+          auto read = [&](int j) {
+            return *reinterpret_cast<const u32x4_t *>(kt + (32 * (j / NQ) + n) * RB +
+                                                      16 * ((2 * (j % NQ) + half) ^ kswz(n)));
+          };
 #pragma unroll
-        for (int u = 0; u < KT; ++u) {
+          for (int j = 0; j < kAhead; ++j) k[j] = read(j);
+          __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int e = 0; e < 16; ++e) sc[u][e] = 0.f;
+          for (int j = 0; j < kSteps; ++j) {
+            f32x16_t &to = sc[j / NQ];
+            if (j % NQ == 0)
 #pragma unroll
-          for (int j = 0; j < NQ; ++j) {
-            const u32x4_t k = *reinterpret_cast<const u32x4_t *>(
-                kt + (32 * u + n) * RB + 16 * ((2 * j + half) ^ kswz(n)));
+              for (int e = 0; e < 16; ++e) to[e] = 0.f;
             if constexpr (BF) {
-              sc[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-                  __builtin_bit_cast(bf16x8_t, k), __builtin_bit_cast(bf16x8_t, q[j]), sc[u], 0, 0, 0);
+              to = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, k[j % kAhead]),
+                                                           __builtin_bit_cast(bf16x8_t, q[j % NQ]), to, 0, 0, 0);
             } else {
 #pragma unroll
               for (int e = 0; e < 4; ++e)
-                sc[u] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(k[e]), __uint_as_float(q[j][e]),
-                                                             sc[u], 0, 0, 0);
+                to = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(k[j % kAhead][e]),
+                                                          __uint_as_float(q[j % NQ][e]), to, 0, 0, 0);
             }
+            if (j + kAhead < kSteps) k[j % kAhead] = read(j + kAhead);
+            // the next tile's transfers one at a time: all at once they hold
+            // up the wave that issues them
+            constexpr int kEvery = kSteps / NI;
+            if (j % kEvery == kEvery / 2 && j / kEvery < NI) issue(j / kEvery, st ^ 1);
+            __builtin_amdgcn_sched_barrier(0);
           }
         }
         // ---- weights
         const bool whole = there == (TK == 64 ? ~0ull : 0xffffffffull);
         if (!whole || k0 + TK > hi_min || k0 < lo_max) {
+          // bit 8 (i / 4) + i % 4 of `seen`: the lane's i-th key of 32
 #pragma unroll
-          for (int u = 0; u < KT; ++u)
+          for (int u = 0; u < KT; ++u) {
+            const int from = min(max(lo - k0 - 32 * u, 0), 32), to = min(max(hi - k0 - 32 * u, 0), 32);
+            const uint64_t range = (1ull << to) - (1ull << min(from, to));
+            const uint32_t seen = ((uint32_t)range & (uint32_t)(there >> (32 * u))) >> (4 * half);
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const int k = 32 * u + 8 * (e / 4) + 4 * half + e % 4;
-              if (!(there >> k & 1) || k0 + k < lo || k0 + k >= hi) sc[u][e] = -INFINITY;
-            }
+            for (int e = 0; e < 16; ++e)
+              if (!(seen & (1u << (8 * (e / 4) + e % 4)))) sc[u][e] = -INFINITY;
+          }
         }
         float mx = sc[0][0];
 #pragma unroll
@@ -218,47 +240,73 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void paged_attn_tile_kernel(AttnAr
           m = to;
         }
         const float mc = m == -INFINITY ? 0.f : m * c;
-#pragma unroll
-        for (int u = 0; u < KT; ++u)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            sc[u][e] = __builtin_amdgcn_exp2f(fmaf(sc[u][e], c, -mc));
-            l += sc[u][e];
-          }
-        // ---- O^T += V^T P^T
+        // ---- O^T += V^T P^T, a step of keys at a time (16, or one of each half
+        // in fp32): beside its MFMAs go the next step's weights and the reads
+        // of the operands kAhead MFMAs on
+        auto weight = [&](int e) {
+          return __builtin_amdgcn_exp2f(fmaf(sc[e / 16][e % 16], c, -mc));
+        };
+        constexpr int kAhead = 3;
         if constexpr (BF) {
           typedef __attribute__((address_space(3))) s16x4_t *tr_ptr;
-          u32x4_t p[2 * KT];
-#pragma unroll
-          for (int k = 0; k < 2 * KT; ++k)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              p[k][e] = pack_bf16x2(sc[k / 2][8 * (k % 2) + 2 * e], sc[k / 2][8 * (k % 2) + 2 * e + 1]);
+          constexpr int kKeys = 2 * KT, kSteps = kKeys * DT;
           const int i16 = lane & 15, r = 4 * half + i16 / 4;
           const int piece = 2 * ((lane >> 4) & 1) + (i16 & 3) / 2;
+          auto read = [&](int j) {
+            const unsigned char *at = vt + (16 * (j / DT) + r) * RB +
+                16 * ((4 * (j % DT) + piece) ^ vswz(r)) + 8 * (i16 & 1);
+            const s16x4_t v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)at);
+            const s16x4_t v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)(at + 8 * RB));
+            return __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+          };
+          auto weights = [&](int k, int from, int to, u32x4_t &p) {  // pairs of step k
 #pragma unroll
-          for (int d = 0; d < DT; ++d) {
-            const unsigned char *at = vt + r * RB + 16 * ((4 * d + piece) ^ vswz(r)) + 8 * (i16 & 1);
-#pragma unroll
-            for (int k = 0; k < 2 * KT; ++k) {
-              const s16x4_t v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)(at + 16 * k * RB));
-              const s16x4_t v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)(at + (16 * k + 8) * RB));
-              o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-                  __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7)),
-                  __builtin_bit_cast(bf16x8_t, p[k]), o[d], 0, 0, 0);
+            for (int e = from; e < to; ++e) {
+              const float p0 = weight(8 * k + 2 * e), p1 = weight(8 * k + 2 * e + 1);
+              const uint32_t both = pack_bf16x2(p0, p1);
+              p[e] = both;
+              l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, both), bf16x2_t{1.f, 1.f}, l, false);
             }
+          };
+          bf16x8_t v[kAhead];
+          u32x4_t p[2];
+#pragma unroll
+          for (int j = 0; j < kAhead; ++j) v[j] = read(j);
+          weights(0, 0, 4, p[0]);
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int j = 0; j < kSteps; ++j) {
+            const int k = j / DT, d = j % DT;
+            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[j % kAhead], __builtin_bit_cast(bf16x8_t, p[k & 1]),
+                                                           o[d], 0, 0, 0);
+            if (j + kAhead < kSteps) v[j % kAhead] = read(j + kAhead);
+            if (k + 1 < kKeys) weights(k + 1, 4 * d / DT, 4 * (d + 1) / DT, p[(k + 1) & 1]);
+            __builtin_amdgcn_sched_barrier(0);
           }
         } else {
+          constexpr int kSteps = 16 * DT;
+          auto read = [&](int j) {
+            const int e = j / DT, r = 8 * (e / 4) + 4 * half + e % 4;
+            return *reinterpret_cast<const float *>(vt + r * RB + 16 * ((8 * (j % DT) + n / 4) ^ vswz(r)) +
+                                                    4 * (n & 3));
+          };
+          float v[kAhead], p[2];
 #pragma unroll
-          for (int d = 0; d < DT; ++d)
+          for (int j = 0; j < kAhead; ++j) v[j] = read(j);
+          l += p[0] = weight(0);
+          __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const int r = 8 * (e / 4) + 4 * half + e % 4;
-              const float v = *reinterpret_cast<const float *>(
-                  vt + r * RB + 16 * ((8 * d + n / 4) ^ vswz(r)) + 4 * (n & 3));
-              o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, sc[0][e], o[d], 0, 0, 0);
-            }
+          for (int j = 0; j < kSteps; ++j) {
+            const int e = j / DT, d = j % DT;
+            o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(v[j % kAhead], p[e & 1], o[d], 0, 0, 0);
+            if (j + kAhead < kSteps) v[j % kAhead] = read(j + kAhead);
+            if (d == 0 && e + 1 < 16) l += p[(e + 1) & 1] = weight(e + 1);
+            __builtin_amdgcn_sched_barrier(0);
+          }
         }
+      } else {
+#pragma unroll
+        for (int j = 0; j < NI; ++j) issue(j, st ^ 1);
       }
       there = there_next;
     }
@@ -290,12 +338,13 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void paged_attn_tile_kernel(AttnAr
     unit += take;
     __syncthreads();  // the last tile is done with
   }
+  zero_rows<NTH>(a, plan, BM, TK, batch);
 }
 
 template <typename T, int DP, int DC, int NW>
 hipError_t launch_tiles_as(const AttnArgs &a, int grid, hipStream_t s) {
   constexpr int TK = sizeof(T) == 2 ? 64 : 32;
-  const size_t lds = 4 * (size_t)TK * DP * sizeof(T) + ((size_t)a.S + 1) * 4;
+  const size_t lds = 4 * (size_t)TK * DP * sizeof(T) + batch_ints(a.S) * 4;
   auto kernel = paged_attn_tile_kernel<T, DP, DC, NW>;
   if (lds > 64 * 1024) {
     const hipError_t grown = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
@@ -308,17 +357,17 @@ hipError_t launch_tiles_as(const AttnArgs &a, int grid, hipStream_t s) {
 
 template <typename T>
 hipError_t launch_tiles_t(const AttnArgs &a, int grid, hipStream_t s) {
-  if (a.D <= 64) return launch_tiles_as<T, 64, 64, 8>(a, grid, s);
-  if (a.D <= 96) return launch_tiles_as<T, 128, 96, 8>(a, grid, s);
-  if (a.D <= 128) return launch_tiles_as<T, 128, 128, 8>(a, grid, s);
+  if (a.D <= 64) return launch_tiles_as<T, 64, 64, 4>(a, grid, s);
+  if (a.D <= 96) return launch_tiles_as<T, 128, 96, 4>(a, grid, s);
+  if (a.D <= 128) return launch_tiles_as<T, 128, 128, 4>(a, grid, s);
   return launch_tiles_as<T, 256, 256, 4>(a, grid, s);
 }
 
 }  // namespace
 
 // Past head_dim 128 a wave's queries and outputs need the registers of two.
-int tile_rows(const AttnArgs &a) { return a.D <= 128 ? 256 : 128; }
-int tile_grid(const AttnArgs &) { return 256; }
+int tile_rows(const AttnArgs &) { return 128; }
+int tile_grid(const AttnArgs &a) { return a.D <= 128 ? 512 : 256; }
 
 hipError_t launch_tiles(const AttnArgs &a, hipStream_t s) {
   return a.dtype == ZT_DT_BF16 ? launch_tiles_t<uint16_t>(a, tile_grid(a), s)

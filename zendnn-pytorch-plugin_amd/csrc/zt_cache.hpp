@@ -67,19 +67,19 @@ struct CopyArgs {
 };
 hipError_t launch_copy_pages(CopyArgs a, int caches, int64_t pairs, bool wide, hipStream_t s);
 
-// Division of n < 2^31 by a fixed d: (n * mul) >> shift, with mul =
-// floor(2^(31 + L) / d) + 1 and shift = 31 + L, L = ceil(log2 d), which is exact
-// for every such n.
+// Division of n <= 2^30 by a fixed d >= 1: floor(n * mul / 2^(31 + L)) with
+// mul = floor(2^(31 + L) / d) + 1 and L = ceil(log2 d), which is exact for every
+// n < 2^31; 2 n * mul is taken so that the high word is all that is needed.
 struct FastDiv {
   uint32_t mul, shift;
 };
 inline FastDiv make_div(uint32_t d) {
   uint32_t L = 0;
   while ((1ull << L) < d) ++L;
-  return {(uint32_t)((1ull << (31 + L)) / d + 1), 31 + L};
+  return {(uint32_t)((1ull << (31 + L)) / d + 1), L};
 }
 __device__ __forceinline__ uint32_t fast_div(uint32_t n, FastDiv d) {
-  return (uint32_t)(((uint64_t)n * d.mul) >> d.shift);
+  return __umulhi(2 * n, d.mul) >> d.shift;
 }
 
 struct AttnArgs {
@@ -98,6 +98,7 @@ struct AttnArgs {
   // set by launch_paged_attn
   int group;                    // H / KV
   FastDiv div_group, div_page;
+  uint32_t k_row[2], v_row[2];  // strides of page and token in units of 16 bytes
   float *part_ml, *part_o;      // partial results: [slots][BM][2], [slots][BM][D]
   void *splits;                 // [workgroups] of Split
 };
