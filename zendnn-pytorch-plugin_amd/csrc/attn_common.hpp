@@ -8,15 +8,16 @@
 // read once for all G of them.  An *item* is a tile of BM such rows (of any
 // one cache head); it needs the keys of blocks [b0, b1) of UK keys.
 //
-// Work is dealt out in units of one block of one item and cache head, laid
-// end to end (head by head, in it item by item, in it block by block), in
-// equal spans, one per workgroup.  The lengths are known on the device only,
-// so each workgroup finds its span by itself.  A span may end inside an
-// (item, head): its workgroups then leave partial results (running maximum,
-// sum and output), which a second launch joins.  That keeps every compute unit
-// busy for one long sequence as for many ragged ones.  Consecutive spans go to
-// one XCD (blocks are dealt round-robin over the eight of them), so the tiles
-// of a head find its keys in one L2.
+// Work is dealt out by its cost: an (item, head) costs kLead for its beginning
+// and end and w for each of its blocks, and lies on a line of all of them (head
+// by head, in it item by item).  Each workgroup takes an equal span of the line
+// and works on the blocks that start in it.  The lengths are known on the device
+// only, so each workgroup finds its span by itself.  A span may end inside an
+// (item, head): its workgroups then leave partial results (running maximum, sum
+// and output), which a second launch joins.  That keeps every compute unit busy
+// for one long sequence as for many ragged ones.  Consecutive spans go to one
+// XCD (blocks are dealt round-robin over the eight of them), so the tiles of a
+// head find its keys in one L2.
 #pragma once
 
 #include "zt_cache.hpp"
@@ -94,21 +95,21 @@ __device__ __forceinline__ int blocks_of(const KeyRange &k, int UK) {
 
 // Exclusive prefix sum over the workgroup; `part` holds N / 64 values.
 template <int N>
-__device__ __forceinline__ int64_t scan64(int64_t v, int64_t *part, int64_t *total) {
+__device__ __forceinline__ int scan(int v, int *part, int *total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int64_t x = v;
+  int x = v;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
-    const int64_t y = __shfl_up((long long)x, d);
+    const int y = __shfl_up(x, d);
     if (lane >= d) x += y;
   }
   __syncthreads();
   if (lane == 63) part[wave] = x;
   __syncthreads();
-  int64_t before = 0, sum = 0;
+  int before = 0, sum = 0;
 #pragma unroll
   for (int w = 0; w < N / 64; ++w) {
-    const int64_t y = part[w];
+    const int y = part[w];
     if (w < wave) before += y;
     sum += y;
   }
@@ -117,15 +118,16 @@ __device__ __forceinline__ int64_t scan64(int64_t v, int64_t *part, int64_t *tot
 }
 
 struct PlanShared {
-  int64_t part[16];
-  int item, off;
+  int part[16];
+  int item, before, most;
 };
 
 struct Plan {
-  int items, wg;  // items of a head; this workgroup's place in the order of spans
-  int64_t per;    // units of a span
-  int64_t todo;   // units of this workgroup's span
-  int head, item, off;  // its first unit: block `off` of that item
+  int items, wg;       // items of a head; this workgroup's place in the order of spans
+  int64_t per;         // length of a span
+  int64_t from, to;    // this workgroup's
+  int head, item;      // the (item, head) that `from` lies in
+  int64_t base;        // and where that begins
 };
 
 // The sequence of item x: the last i with tile_base[i] <= x.
@@ -139,63 +141,137 @@ __device__ __forceinline__ int seq_of_item(const int *tile_base, int S, int x) {
   return lo;
 }
 
-template <int N>
+// The cost of a block of an item of `rows` rows.
+struct RowCost {  // every row kernel's unit is the same bytes
+  static constexpr int kLead = 1, kMost = 1;
+  static __device__ __forceinline__ int of(int) { return 1; }
+};
+
+template <int N, typename Cost>
 __device__ __forceinline__ Plan make_plan(const AttnArgs &a, int BM, int UK, const Batch &batch,
                                           PlanShared *sh) {
   const int tid = threadIdx.x;
   Plan p{};
-  int64_t items = 0;
   for (int i0 = 0; i0 < a.S; i0 += N) {
     const int i = i0 + tid;
-    int64_t tiles = 0, total;
+    int tiles = 0, total;
     if (i < a.S) {
       const int T = (int)a.T, q0 = min(max(a.cu[i], 0), T), q = min(max(a.cu[i + 1], q0), T) - q0;
       batch.q0[i] = q0, batch.q[i] = q, batch.n[i] = min(max(a.ctx[i], 0), a.W * a.page_size);
-      tiles = (uint32_t)(q * a.group + BM - 1) / (uint32_t)BM;
+      tiles = (int)((uint32_t)(q * a.group + BM - 1) / (uint32_t)BM);
     }
-    const int64_t before = scan64<N>(tiles, sh->part, &total);
-    if (i < a.S) batch.tile_base[i] = (int)(items + before);
-    items += total;
+    const int before = scan<N>(tiles, sh->part, &total);
+    if (i < a.S) batch.tile_base[i] = p.items + before;
+    p.items += total;
   }
-  if (tid == 0) batch.tile_base[a.S] = (int)items;
+  if (tid == 0) batch.tile_base[a.S] = p.items;
   __syncthreads();
-  p.items = (int)items;
-  auto units_of = [&](int x) -> int64_t {
+  auto cost_of = [&](int x) {
     if (x >= p.items) return 0;
-    const int i = seq_of_item(batch.tile_base, a.S, x);
-    return blocks_of(keys_of(a, batch[i], x - batch.tile_base[i], BM), UK);
+    const int i = seq_of_item(batch.tile_base, a.S, x), tile = x - batch.tile_base[i];
+    const Seq s = batch[i];
+    const int nb = blocks_of(keys_of(a, s, tile, BM), UK);
+    return nb ? Cost::kLead + nb * Cost::of(min(BM, s.q * a.group - tile * BM)) : 0;
   };
-  int64_t sum = 0, units = 0, before = 0;
+  int sum = 0, cost = 0, before = 0;
   for (int x0 = 0; x0 < p.items; x0 += N) {
-    int64_t total;
-    units = units_of(x0 + tid);
-    before = scan64<N>(units, sh->part, &total);
+    int total;
+    cost = cost_of(x0 + tid);
+    before = scan<N>(cost, sh->part, &total);
     sum += total;
   }
   p.wg = xcd_contiguous_tile(blockIdx.x, gridDim.x);
-  const int64_t all = sum * a.KV;
-  p.per = max((all + gridDim.x - 1) / gridDim.x, (int64_t)1);
-  const int64_t u0 = p.per * p.wg;
-  p.todo = max(min(p.per, all - u0), (int64_t)0);
-  if (p.todo == 0) return p;
-  p.head = (int)(u0 / sum);
-  const int64_t at = u0 - p.head * sum;
+  // About as many (item, head)s as workgroups, of about one length: each
+  // workgroup takes a whole one, and nothing has to be joined.  What is uneven
+  // about them the two workgroups of a CU share, so the second half of an
+  // XCD's workgroups takes its items from the far end.
+  const int pairs = p.items * a.KV, grid = (int)gridDim.x;
+  if (p.items <= N && pairs <= grid && 32 * (int64_t)pairs >= 31 * (int64_t)grid) {
+    if (tid == 0) sh->most = 0;
+    __syncthreads();
+    if (cost) atomicMax(&sh->most, cost);
+    __syncthreads();
+    if ((int64_t)sh->most * p.items <= (int64_t)sum + sum / 4) {
+      const int xcd = blockIdx.x & 7, each = grid / 8, i = blockIdx.x >> 3;
+      if (grid % 16 == 0 && i >= each / 2) p.wg = xcd * each + each / 2 + each - 1 - i;
+      if (p.wg >= pairs) return p;
+      p.head = p.wg / p.items, p.item = p.wg - p.head * p.items;
+      if (p.item == tid) sh->before = before, sh->item = cost;
+      __syncthreads();
+      p.base = p.from = (int64_t)p.head * sum + sh->before, p.to = p.from + sh->item;
+      p.per = max(sh->item, 1);
+      return p;
+    }
+  }
+  const int64_t all = (int64_t)sum * a.KV;
+  // no span without the start of a block inside a long item
+  p.per = max((all + gridDim.x - 1) / gridDim.x, (int64_t)Cost::kMost);
+  p.from = p.per * p.wg, p.to = min(p.from + p.per, all);
+  if (p.from >= p.to) {  // nothing is left: an empty span at the line's start
+    p.from = p.to = 0;
+    return p;
+  }
+  p.head = (int)(p.from / sum);
+  const int at = (int)(p.from - (int64_t)p.head * sum);
   if (p.items <= N) {  // the only round's values are still at hand
-    if (at >= before && at < before + units) sh->item = tid, sh->off = (int)(at - before);
+    if (at >= before && at < before + cost) sh->item = tid, sh->before = before;
   } else {
-    int64_t base = 0;
+    int base = 0;
     for (int x0 = 0; base <= at; x0 += N) {
-      int64_t total;
-      units = units_of(x0 + tid);
-      before = base + scan64<N>(units, sh->part, &total);
-      if (at >= before && at < before + units) sh->item = x0 + tid, sh->off = (int)(at - before);
+      int total;
+      cost = cost_of(x0 + tid);
+      before = base + scan<N>(cost, sh->part, &total);
+      if (at >= before && at < before + cost) sh->item = x0 + tid, sh->before = before;
       base += total;
     }
   }
   __syncthreads();
-  p.item = sh->item, p.off = sh->off;
+  p.item = sh->item, p.base = (int64_t)p.head * sum + sh->before;
   return p;
 }
+
+// A workgroup's way along its span: for each (item, head) the blocks [bb, bb +
+// take) of its nb.
+struct Segment {
+  int head, tile, seq;
+  KeyRange keys;
+  int b0, nb, bb, take;  // first block of the sequence, blocks, the span's
+  int64_t slot;          // of its partial result
+  int64_t last;          // the workgroup that has the item's last block
+  bool complete;
+};
+template <typename Cost>
+struct Walk {
+  int head, item;
+  int64_t base;
+  __device__ __forceinline__ explicit Walk(const Plan &p) : head(p.head), item(p.item), base(p.base) {}
+  __device__ __forceinline__ bool next(const AttnArgs &a, const Plan &p, const Batch &batch, int BM, int UK,
+                                       Segment *g) {
+    while (base < p.to) {
+      if (item == p.items) ++head, item = 0;
+      g->head = head;
+      g->seq = seq_of_item(batch.tile_base, a.S, item), g->tile = item - batch.tile_base[g->seq];
+      const Seq s = batch[g->seq];
+      g->keys = keys_of(a, s, g->tile, BM);
+      g->nb = blocks_of(g->keys, UK), g->b0 = g->keys.begin / UK;
+      ++item;
+      if (g->nb == 0) continue;
+      const int w = Cost::of(min(BM, s.q * a.group - g->tile * BM));
+      const int64_t first = base + Cost::kLead, odd = base > p.from;
+      // blocks that start in [from, to)
+      const int64_t lo = max(p.from - first, (int64_t)0), hi = p.to - first;
+      const int b = (int)min((lo + w - 1) / w, (int64_t)g->nb), e = hi > 0 ? (int)min((hi + w - 1) / w, (int64_t)g->nb) : 0;
+      base = first + (int64_t)g->nb * w;
+      if (b >= e) continue;
+      g->bb = b, g->take = e - b;
+      g->slot = 2 * (int64_t)p.wg + odd;
+      g->complete = g->take == g->nb;
+      g->last = (first + (int64_t)(g->nb - 1) * w) / p.per;
+      return true;
+    }
+    return false;
+  }
+};
 
 // Where the keys of one sequence are: a lane's lookup of its key's page, kept
 // as it was loaded (a use right behind the load would wait for everything in
@@ -216,10 +292,10 @@ __device__ __forceinline__ uint32_t row_offset(const AttnArgs &a, const uint32_t
 }
 
 // What a workgroup leaves about the (item, head) that it began and did not
-// finish (rows = 0: none).  Its partial results are in slots 2 * first + (1 if
-// the unit before it is in the same span), 2 * (first + 1), ..
+// finish (rows = 0: none): the partial results are in slots `slot` and 2 * w for
+// each workgroup w after it up to `last`.
 struct Split {
-  int64_t u0, u1, per;  // its units, counted over everything; units of a span
+  int64_t slot, last;
   int row0, rows, head;  // its rows of that cache head, from row0 of the sequence on
   int q0;                // the sequence's first row of the batch
 };
@@ -254,6 +330,7 @@ __device__ __forceinline__ void zero_rows(const AttnArgs &a, const Plan &p, int 
 // The tile kernel (paged_attn_tile.hip): its rows per item and workgroups.
 int tile_rows(const AttnArgs &a);
 int tile_grid(const AttnArgs &a);
-hipError_t launch_tiles(const AttnArgs &a, hipStream_t s);
+hipError_t launch_tiles(const AttnArgs &a, int grid, hipStream_t s);
+constexpr int kTileCostLead = 15, kTileCostMost = 6;  // the most of TileCost
 
 }  // namespace zt

@@ -243,6 +243,8 @@ static int attn_args(const char *op, int64_t T, int64_t H, const zt_kv_cache *ca
   a->T = T, a->H = (int)H, a->KV = (int)cache->heads, a->D = (int)cache->head_dim;
   a->S = (int)S, a->W = (int)W, a->page_size = (int)cache->page_size, a->pages = cache->pages;
   a->dtype = cache->dtype, a->max_q = max_query_len, a->causal = causal != 0, a->window = window;
+  if (T > 0 && !zt::paged_attn_countable(*a))
+    return api_fail(ZT_EUNSUPPORTED, "%s: too many tokens over too long tables for one call", op);
   return ZT_OK;
 }
 

@@ -14,6 +14,8 @@
 //   o' = o e^(m - m') + sum_j e^(s_j - m') v_j,
 // and two parts (m, l, o) join the same way.  Scores, weights and sums are
 // fp32; exponentials are powers of two with scale * log2(e) in the exponent.
+#include <cmath>
+
 #include "attn_common.hpp"
 
 namespace zt {
@@ -53,6 +55,7 @@ __device__ __forceinline__ float sum_over_groups(float x) {
 // lo): the matrix pipe is idle most of the time here.
 template <typename T, int DP, int NT>
 __global__ __launch_bounds__(kRowThreads, NT * DP <= 128 ? 2 : 1) void paged_attn_row_kernel(AttnArgs a) {
+  using Cost = RowCost;
   constexpr bool BF = sizeof(T) == 2;
   constexpr int ES = sizeof(T);
   constexpr int BM = 16 * NT;
@@ -74,7 +77,7 @@ __global__ __launch_bounds__(kRowThreads, NT * DP <= 128 ? 2 : 1) void paged_att
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   unsigned char *vlds = smem + wave * kWaveLds;
-  const Plan plan = make_plan<kRowThreads>(a, BM, UK, batch, &sh);
+  const Plan plan = make_plan<kRowThreads, Cost>(a, BM, UK, batch, &sh);
   Split *split = static_cast<Split *>(a.splits) + plan.wg;
   if (tid == 0) split->rows = 0;
 
@@ -82,18 +85,14 @@ __global__ __launch_bounds__(kRowThreads, NT * DP <= 128 ? 2 : 1) void paged_att
   const int G = a.group, C = a.D * ES / 16;  // 16-byte pieces that a row has
   const char *zero = reinterpret_cast<const char *>(kZeroRow);
 
-  int64_t todo = plan.todo, unit = plan.per * plan.wg;
-  const int64_t span0 = unit;
-  for (int h = plan.head, x = plan.item, bb = plan.off; todo > 0; ++x, bb = 0) {
-    if (x == plan.items) ++h, x = 0;
-    const int i = seq_of_item(batch.tile_base, a.S, x), tile = x - batch.tile_base[i];
-    const Seq s = batch[i];
-    const int r0 = tile * BM;
-    const KeyRange kr = keys_of(a, s, tile, BM);
-    const int nb = blocks_of(kr, UK), b0 = kr.begin / UK;
-    if (nb == 0) continue;
-    const int take = (int)min((int64_t)(nb - bb), todo);
-    const Pages pages{a.table + (int64_t)i * a.W, kr.begin, kr.end};
+  Walk<Cost> walk(plan);
+  Segment seg;
+  while (walk.next(a, plan, batch, BM, UK, &seg)) {
+    const int h = seg.head, take = seg.take;
+    const Seq s = batch[seg.seq];
+    const int r0 = seg.tile * BM;
+    const KeyRange kr = seg.keys;
+    const Pages pages{a.table + (int64_t)seg.seq * a.W, kr.begin, kr.end};
     // the lane's rows: token, head, and the keys each sees
     int row_t[NT], lo[NT], hi[NT];
     bool live[NT];
@@ -129,8 +128,8 @@ __global__ __launch_bounds__(kRowThreads, NT * DP <= 128 ? 2 : 1) void paged_att
     }
     const char *kbase = static_cast<const char *>(a.k) + h * a.k_ld[1] * ES;
     const char *vbase = static_cast<const char *>(a.v) + h * a.v_ld[1] * ES;
-    const int kend = (b0 + bb + take) * UK;
-    int k0 = (b0 + bb) * UK + wave * KS;
+    const int kend = (seg.b0 + seg.bb + take) * UK;
+    int k0 = (seg.b0 + seg.bb) * UK + wave * KS;
 
     u32x4_t kreg[KT][KC], vreg[NV];
     uint64_t there;  // which of the strip's keys there are
@@ -269,8 +268,8 @@ __global__ __launch_bounds__(kRowThreads, NT * DP <= 128 ? 2 : 1) void paged_att
       }
     }
     // ---- join the four waves, 16 rows at a time
-    const bool complete = bb == 0 && take == nb;
-    const int64_t slot = 2 * (int64_t)plan.wg + (unit > span0 ? 1 : 0);
+    const bool complete = seg.complete;
+    const int64_t slot = seg.slot;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       const float lsum = sum_over_groups(l[t]);
@@ -307,12 +306,10 @@ __global__ __launch_bounds__(kRowThreads, NT * DP <= 128 ? 2 : 1) void paged_att
       }
     }
     __syncthreads();  // before the next strips' values
-    if (tid == 0 && bb == 0 && !complete) {
-      split->u0 = unit, split->u1 = unit + nb, split->per = plan.per;
+    if (tid == 0 && seg.bb == 0 && !complete) {
+      split->slot = seg.slot, split->last = seg.last;
       split->row0 = r0, split->rows = min(BM, s.q * G - r0), split->head = h, split->q0 = s.q0;
     }
-    todo -= take;
-    unit += take;
   }
   zero_rows<kRowThreads>(a, plan, BM, UK, batch);
 }
@@ -324,20 +321,19 @@ __global__ __launch_bounds__(256) void paged_attn_join_kernel(AttnArgs a, int BM
   const Split s = static_cast<const Split *>(a.splits)[blockIdx.x];
   if (s.rows == 0) return;
   const float c = score_factor(a.scale);
-  const int first = (int)blockIdx.x, last = (int)((s.u1 - 1) / s.per);
+  const int first = (int)blockIdx.x, last = (int)s.last;
   const int d4 = a.D / 4, G = a.group;
   for (int e = blockIdx.y * 256 + threadIdx.x; e < s.rows * d4; e += gridDim.y * 256) {
     const int row = e / d4, d = (e - row * d4) * 4;
     float m = -INFINITY, l = 0.f;
     f32x4_t o = {0.f, 0.f, 0.f, 0.f};
-    const int odd = s.u0 > first * s.per;  // the first part's place in its pair of slots
     for (int w0 = first; w0 <= last; w0 += 8) {  // eight parts' loads at once
       float mw[8], lw[8];
       f32x4_t y[8];
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         const int w = min(w0 + k, last);
-        const int64_t at = (2 * (int64_t)w + (w == first ? odd : 0)) * BM + row;
+        const int64_t at = (w == first ? s.slot : 2 * (int64_t)w) * BM + row;
         mw[k] = w0 + k <= last ? a.part_ml[2 * at] : -INFINITY;
         lw[k] = a.part_ml[2 * at + 1];
         y[k] = *reinterpret_cast<const f32x4_t *>(a.part_o + at * a.D + d);
@@ -365,11 +361,11 @@ __global__ __launch_bounds__(256) void paged_attn_join_kernel(AttnArgs a, int BM
   }
 }
 
-// Workgroups of the first launch: two per CU.
+// Workgroups of the first launch, at most: two per CU.
 constexpr int kRowGrid = 512;
 
 template <typename T, int DP, int NT>
-hipError_t launch_rows(const AttnArgs &a, hipStream_t s) {
+hipError_t launch_rows(const AttnArgs &a, int grid, hipStream_t s) {
   constexpr int KS = sizeof(T) == 2 ? 32 : 16, VP = DP * (int)sizeof(T) + (sizeof(T) == 2 ? 32 : 16);
   constexpr int wave = std::max(KS * VP, 16 * (DP + 4) * 4);
   const size_t lds = 4 * wave + batch_ints(a.S) * 4;
@@ -379,22 +375,22 @@ hipError_t launch_rows(const AttnArgs &a, hipStream_t s) {
                                                  hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     if (grown != hipSuccess) return grown;
   }
-  kernel<<<kRowGrid, kRowThreads, lds, s>>>(a);
+  kernel<<<grid, kRowThreads, lds, s>>>(a);
   return hipGetLastError();
 }
 
 template <typename T, int NT>
-hipError_t launch_rows_d(const AttnArgs &a, hipStream_t s) {
-  if (a.D <= 64) return launch_rows<T, 64, NT>(a, s);
-  if (a.D <= 128) return launch_rows<T, 128, NT>(a, s);
-  return launch_rows<T, 256, NT>(a, s);
+hipError_t launch_rows_d(const AttnArgs &a, int grid, hipStream_t s) {
+  if (a.D <= 64) return launch_rows<T, 64, NT>(a, grid, s);
+  if (a.D <= 128) return launch_rows<T, 128, NT>(a, grid, s);
+  return launch_rows<T, 256, NT>(a, grid, s);
 }
 
 template <typename T>
-hipError_t launch_rows_n(const AttnArgs &a, int nt, hipStream_t s) {
-  if (nt == 1) return launch_rows_d<T, 1>(a, s);
-  if (nt == 2) return launch_rows_d<T, 2>(a, s);
-  return launch_rows_d<T, 4>(a, s);
+hipError_t launch_rows_n(const AttnArgs &a, int nt, int grid, hipStream_t s) {
+  if (nt == 1) return launch_rows_d<T, 1>(a, grid, s);
+  if (nt == 2) return launch_rows_d<T, 2>(a, grid, s);
+  return launch_rows_d<T, 4>(a, grid, s);
 }
 
 // Rows of one cache head from which on the tile kernel takes over: there each
@@ -405,15 +401,29 @@ struct Shape {
   bool tiles;
   int bm, grid;
 };
+double items_most(const AttnArgs &a, int bm) { return std::floor((double)a.T * (a.H / a.KV) / bm) + a.S; }
+double blocks_most(const AttnArgs &a, bool tiles) {
+  const int keys = (tiles ? 64 : 128) / (a.dtype == ZT_DT_F32 ? 2 : 1);
+  return std::floor((double)a.W * a.page_size / keys) + 1;
+}
 Shape shape_of(const AttnArgs &a) {
   const int64_t rows = std::min(std::max<int64_t>(a.max_q, 1), a.T) * (a.H / a.KV);
-  if (rows > kRowsMost) return {true, tile_rows(a), tile_grid(a)};
-  return {false, rows <= 16 ? 16 : rows <= 32 ? 32 : 64, kRowGrid};
+  Shape p{rows > kRowsMost, rows <= 16 ? 16 : rows <= 32 ? 32 : 64, kRowGrid};
+  if (p.tiles) p.bm = tile_rows(a), p.grid = tile_grid(a);
+  // no more workgroups than there can be blocks
+  const double most = items_most(a, p.bm) * a.KV * blocks_most(a, p.tiles);
+  if (most < p.grid) p.grid = std::max((int)most, 1);
+  return p;
 }
 
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
 }  // namespace
+
+bool paged_attn_countable(const AttnArgs &a) {
+  const Shape p = shape_of(a);
+  return items_most(a, p.bm) * (blocks_most(a, p.tiles) * kTileCostMost + kTileCostLead) < 2147483647.0;
+}
 
 size_t paged_attn_workspace(const AttnArgs &a) {
   if (a.T == 0) return 0;
@@ -435,9 +445,9 @@ hipError_t launch_paged_attn(AttnArgs a, void *workspace, hipStream_t s) {
   a.part_ml = reinterpret_cast<float *>(at), at += up256(slots * 2 * sizeof(float));
   a.part_o = reinterpret_cast<float *>(at);
   const bool bf = a.dtype == ZT_DT_BF16;
-  const hipError_t e = p.tiles ? launch_tiles(a, s)
-                       : bf   ? launch_rows_n<uint16_t>(a, p.bm / 16, s)
-                              : launch_rows_n<float>(a, p.bm / 16, s);
+  const hipError_t e = p.tiles ? launch_tiles(a, p.grid, s)
+                       : bf   ? launch_rows_n<uint16_t>(a, p.bm / 16, p.grid, s)
+                              : launch_rows_n<float>(a, p.bm / 16, p.grid, s);
   if (e != hipSuccess) return e;
   const dim3 grid(p.grid, std::max(p.bm / 16, 1));
   if (bf) paged_attn_join_kernel<uint16_t><<<grid, 256, 0, s>>>(a, p.bm);

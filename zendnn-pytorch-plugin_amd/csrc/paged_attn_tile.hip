@@ -26,6 +26,19 @@ __device__ __forceinline__ void wait_and_meet() {
 
 __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32); }
 
+// The cost of a block, and of an item's beginning and end.  A block of few rows
+// takes nearly as long as a full one: in bf16 it waits for its keys (1.9 against
+// 2.2 us, two workgroups a CU), in fp32 for its one wave's share of the matrix
+// operations (4.6 us), which the other workgroup's wave on that SIMD halves.
+// An item's two ends take 5 to 6 us.
+template <typename T>
+struct TileCost {
+  static constexpr int kLead = sizeof(T) == 2 ? 15 : 7, kMost = 6;
+  static __device__ __forceinline__ int of(int rows) {
+    return sizeof(T) == 2 ? 4 + (rows + 63) / 64 : 6;
+  }
+};
+
 // NW waves of 32 rows each against a span of the keys of one cache head.
 //
 // Bound by the matrix pipes and, beside them, by the exponentials.  All waves
@@ -54,6 +67,7 @@ __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32);
 // taken of the rounded ones, so that a row's weights still add up to one.
 template <typename T, int DP, int DC, int NW>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP <= 128 ? 2 : 1, DP <= 128 ? 2 : 1))) void paged_attn_tile_kernel(AttnArgs a) {
+  using Cost = TileCost<T>;
   constexpr bool BF = sizeof(T) == 2;
   constexpr int ES = sizeof(T), NTH = 64 * NW, BM = 32 * NW;
   constexpr int KT = BF ? 2 : 1, TK = 32 * KT;  // keys of a tile
@@ -69,7 +83,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP <= 1
 
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const Plan plan = make_plan<NTH>(a, BM, TK, batch, &sh);
+  const Plan plan = make_plan<NTH, Cost>(a, BM, TK, batch, &sh);
   Split *split = static_cast<Split *>(a.splits) + plan.wg;
   if (tid == 0) split->rows = 0;
 
@@ -91,18 +105,14 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP <= 1
     part_k[j] = slot ^ kswz(part_row[j]), part_v[j] = slot ^ vswz(part_row[j]);
   }
 
-  int64_t todo = plan.todo, unit = plan.per * plan.wg;
-  const int64_t span0 = unit;
-  for (int h = plan.head, x = plan.item, bb = plan.off; todo > 0; ++x, bb = 0) {
-    if (x == plan.items) ++h, x = 0;
-    const int i = seq_of_item(batch.tile_base, a.S, x), tile = x - batch.tile_base[i];
-    const Seq s = batch[i];
-    const int r0 = tile * BM;
-    const KeyRange kr = keys_of(a, s, tile, BM);
-    const int nb = blocks_of(kr, TK), b0 = kr.begin / TK;
-    if (nb == 0) continue;
-    const int take = (int)min((int64_t)(nb - bb), todo);
-    const Pages pages{a.table + (int64_t)i * a.W, kr.begin, kr.end};
+  Walk<Cost> walk(plan);
+  Segment seg;
+  while (walk.next(a, plan, batch, BM, TK, &seg)) {
+    const int h = seg.head, take = seg.take;
+    const Seq s = batch[seg.seq];
+    const int r0 = seg.tile * BM;
+    const KeyRange kr = seg.keys;
+    const Pages pages{a.table + (int64_t)seg.seq * a.W, kr.begin, kr.end};
     const char *kbase = static_cast<const char *>(a.k) + h * a.k_ld[1] * ES;
     const char *vbase = static_cast<const char *>(a.v) + h * a.v_ld[1] * ES;
 
@@ -131,7 +141,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP <= 1
       load_to_lds(ks, lds0 + st * 2 * STAGE + (wave * NI + j) * 1024);
       load_to_lds(vs, lds0 + st * 2 * STAGE + STAGE + (wave * NI + j) * 1024);
     };
-    const int k_first = (b0 + bb) * TK;
+    const int k_first = (seg.b0 + seg.bb) * TK;
     uint64_t there = offsets(k_first, lookup(k_first), true);
 #pragma unroll
     for (int j = 0; j < NI; ++j) issue(j, 0);
@@ -312,10 +322,10 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP <= 1
     }
     // ---- the rows' outputs, or their part: lane (row n, half) holds columns
     // 32 d + 8 k + 4 half .. + 3
-    const bool complete = bb == 0 && take == nb;
+    const bool complete = seg.complete;
     l += other_half(l);
     if (live) {
-      const int64_t slot = 2 * (int64_t)plan.wg + (unit > span0 ? 1 : 0), pr = slot * BM + 32 * wave + n;
+      const int64_t pr = seg.slot * BM + 32 * wave + n;
       const int64_t to = ((int64_t)(s.q0 + row_t) * a.H + h * G + row - row_t * G) * a.D;
       const float r = l > 0.f ? 1.f / l : 0.f;
 #pragma unroll
@@ -330,12 +340,10 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP <= 1
         }
       if (!complete && half == 0) a.part_ml[2 * pr] = m, a.part_ml[2 * pr + 1] = l;
     }
-    if (tid == 0 && bb == 0 && !complete) {
-      split->u0 = unit, split->u1 = unit + nb, split->per = plan.per;
+    if (tid == 0 && seg.bb == 0 && !complete) {
+      split->slot = seg.slot, split->last = seg.last;
       split->row0 = r0, split->rows = min(BM, s.q * G - r0), split->head = h, split->q0 = s.q0;
     }
-    todo -= take;
-    unit += take;
     __syncthreads();  // the last tile is done with
   }
   zero_rows<NTH>(a, plan, BM, TK, batch);
@@ -369,9 +377,9 @@ hipError_t launch_tiles_t(const AttnArgs &a, int grid, hipStream_t s) {
 int tile_rows(const AttnArgs &) { return 128; }
 int tile_grid(const AttnArgs &a) { return a.D <= 128 ? 512 : 256; }
 
-hipError_t launch_tiles(const AttnArgs &a, hipStream_t s) {
-  return a.dtype == ZT_DT_BF16 ? launch_tiles_t<uint16_t>(a, tile_grid(a), s)
-                               : launch_tiles_t<float>(a, tile_grid(a), s);
+hipError_t launch_tiles(const AttnArgs &a, int grid, hipStream_t s) {
+  return a.dtype == ZT_DT_BF16 ? launch_tiles_t<uint16_t>(a, grid, s)
+                               : launch_tiles_t<float>(a, grid, s);
 }
 
 }  // namespace zt

@@ -102,6 +102,8 @@ struct AttnArgs {
   float *part_ml, *part_o;      // partial results: [slots][BM][2], [slots][BM][D]
   void *splits;                 // [workgroups] of Split
 };
+// Whether the work of such a call can be counted in 32 bits.
+bool paged_attn_countable(const AttnArgs &a);
 size_t paged_attn_workspace(const AttnArgs &a);
 hipError_t launch_paged_attn(AttnArgs a, void *workspace, hipStream_t s);
 
