@@ -439,7 +439,7 @@ size_t zt_paged_attention_workspace_size(int64_t T, int64_t H, const zt_kv_cache
  * length, and its tokens get position and slot -1.  Every output is written
  * whole: table_out [S, W], context_out [S], refs_out [pages], and for each
  * token its position and its slot [T] (-1 for tokens of no sequence).
- * S <= 4096, W * page_size < 2^31.
+ * S <= 4096; W * page_size and S * W below 2^30.
  */
 int zt_cache_extend(const int32_t *block_table, const int32_t *context_lens,
                     const int32_t *ref_counts, const int32_t *cu_seqlens, int64_t S, int64_t W,
@@ -454,7 +454,7 @@ int zt_cache_extend(const int32_t *block_table, const int32_t *context_lens,
  * free page (the lowest, in row order, the ended rows' pages among them) to
  * which copies[i] = (from, to) asks for it to be copied.  Other rows of
  * copies [S, 2] are -1.  A row that finds no free page ends (length 0).
- * Outputs as zt_cache_extend's; S <= 4096.
+ * Outputs and bounds as zt_cache_extend's.
  */
 int zt_cache_fork(const int32_t *block_table, const int32_t *context_lens,
                   const int32_t *ref_counts, const int32_t *parents, int64_t S, int64_t W,

@@ -97,12 +97,7 @@ __device__ __forceinline__ int blocks_of(const KeyRange &k, int UK) {
 template <int N>
 __device__ __forceinline__ int scan(int v, int *part, int *total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int x = v;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int y = __shfl_up(x, d);
-    if (lane >= d) x += y;
-  }
+  const int x = wave_scan(v);
   __syncthreads();
   if (lane == 63) part[wave] = x;
   __syncthreads();
@@ -115,6 +110,12 @@ __device__ __forceinline__ int scan(int v, int *part, int *total) {
   }
   *total = sum;
   return before + x - v;
+}
+
+// a / b, in 32 bits where they fit (they do but for the longest calls).
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+  if (((a | b) >> 32) == 0) return (uint32_t)a / (uint32_t)b;
+  return a / b;
 }
 
 struct PlanShared {
@@ -205,13 +206,13 @@ __device__ __forceinline__ Plan make_plan(const AttnArgs &a, int BM, int UK, con
   }
   const int64_t all = (int64_t)sum * a.KV;
   // no span without the start of a block inside a long item
-  p.per = max((all + gridDim.x - 1) / gridDim.x, (int64_t)Cost::kMost);
+  p.per = max(quotient(all + gridDim.x - 1, gridDim.x), (int64_t)Cost::kMost);
   p.from = p.per * p.wg, p.to = min(p.from + p.per, all);
   if (p.from >= p.to) {  // nothing is left: an empty span at the line's start
     p.from = p.to = 0;
     return p;
   }
-  p.head = (int)(p.from / sum);
+  p.head = (int)quotient(p.from, sum);
   const int at = (int)(p.from - (int64_t)p.head * sum);
   if (p.items <= N) {  // the only round's values are still at hand
     if (at >= before && at < before + cost) sh->item = tid, sh->before = before;
@@ -260,13 +261,14 @@ struct Walk {
       const int64_t first = base + Cost::kLead, odd = base > p.from;
       // blocks that start in [from, to)
       const int64_t lo = max(p.from - first, (int64_t)0), hi = p.to - first;
-      const int b = (int)min((lo + w - 1) / w, (int64_t)g->nb), e = hi > 0 ? (int)min((hi + w - 1) / w, (int64_t)g->nb) : 0;
+      const int b = (int)min(quotient(lo + w - 1, w), (int64_t)g->nb);
+      const int e = hi > 0 ? (int)min(quotient(hi + w - 1, w), (int64_t)g->nb) : 0;
       base = first + (int64_t)g->nb * w;
       if (b >= e) continue;
       g->bb = b, g->take = e - b;
       g->slot = 2 * (int64_t)p.wg + odd;
       g->complete = g->take == g->nb;
-      g->last = (first + (int64_t)(g->nb - 1) * w) / p.per;
+      g->last = quotient(first + (int64_t)(g->nb - 1) * w, p.per);
       return true;
     }
     return false;

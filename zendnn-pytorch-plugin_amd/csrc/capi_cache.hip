@@ -128,8 +128,8 @@ int zt_cache_extend(const int32_t *block_table, const int32_t *context_lens,
   if (S < 0 || W < 0 || pages < 0 || page_size <= 0 || T < 0)
     return api_fail(ZT_EINVAL, "%s: need S, W, pages, T >= 0 and page_size > 0", op);
   if (S > kMaxRows) return api_fail(ZT_EUNSUPPORTED, "%s: at most %lld sequences", op, (long long)kMaxRows);
-  if (W > (1 << 24) || pages > INT32_MAX || page_size > (1 << 24) || W * page_size > INT32_MAX ||
-      S * W > INT32_MAX)
+  if (W > (1 << 24) || pages > INT32_MAX || page_size > (1 << 24) || W * page_size >= (1 << 30) ||
+      S * W >= (1 << 30))
     return api_fail(ZT_EUNSUPPORTED, "%s: sizes exceed 32 bits", op);
   if ((S * W > 0 && (!block_table || !table_out)) || (pages > 0 && (!ref_counts || !refs_out)) ||
       (S > 0 && (!context_lens || !context_out)) || !cu_seqlens || (T > 0 && (!positions || !slots)))
@@ -150,8 +150,8 @@ int zt_cache_fork(const int32_t *block_table, const int32_t *context_lens,
   if (S < 0 || W < 0 || pages < 0 || page_size <= 0)
     return api_fail(ZT_EINVAL, "%s: need S, W, pages >= 0 and page_size > 0", op);
   if (S > kMaxRows) return api_fail(ZT_EUNSUPPORTED, "%s: at most %lld rows", op, (long long)kMaxRows);
-  if (W > (1 << 24) || pages > INT32_MAX || page_size > (1 << 24) || W * page_size > INT32_MAX ||
-      S * W > INT32_MAX)
+  if (W > (1 << 24) || pages > INT32_MAX || page_size > (1 << 24) || W * page_size >= (1 << 30) ||
+      S * W >= (1 << 30))
     return api_fail(ZT_EUNSUPPORTED, "%s: sizes exceed 32 bits", op);
   if ((S * W > 0 && (!block_table || !table_out)) || (pages > 0 && (!ref_counts || !refs_out)) ||
       (S > 0 && (!context_lens || !context_out || !parents || !copies)))

@@ -151,16 +151,16 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
 // ------------------------------------------------------------------- pages
 constexpr int kBlock = 1024, kWaves = kBlock / 64;
 
+// This wave's stores and atomics have been carried out in L2, which is where
+// agent-scope atomics of the same XCD meet them (a fence would write back the
+// whole L2 as well).
+__device__ __forceinline__ void counts_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
 // Exclusive prefix sum of v over the workgroup's threads; *total is the sum.
 // `part` is an LDS array of kWaves ints.
 __device__ __forceinline__ int block_scan(int v, int *part, int *total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int x = v;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int y = __shfl_up(x, d);
-    if (lane >= d) x += y;
-  }
+  const int x = wave_scan(v);
   __syncthreads();  // the previous use of part is over
   if (lane == 63) part[wave] = x;
   __syncthreads();
@@ -175,9 +175,6 @@ __device__ __forceinline__ int block_scan(int v, int *part, int *total) {
   return before + x - v;
 }
 
-// n / d rounded up, for 0 <= n < 2^31 and d > 0.
-__device__ __forceinline__ int ceil_div(int n, int d) { return (int)(((unsigned)n + (unsigned)d - 1u) / (unsigned)d); }
-
 // A step's new tokens get their pages.  Sequence i holds have_i = ceil(ctx_i /
 // size) pages and needs want_i = ceil((ctx_i + new_i) / size); need_i = want_i
 // - have_i if want_i fits the table's width, else 0.  The free pages (count 0)
@@ -191,64 +188,91 @@ __device__ __forceinline__ int ceil_div(int n, int d) { return (int)(((unsigned)
 //  * for each free page of its own slice, whose rank among the free pages it
 //    knows, finds the sequence that takes this rank by bisection over the
 //    needs' running sums, and writes the page's table entry, count and slots.
-// So no workgroup waits for another.
+// So no workgroup waits for another.  Bound by round trips to memory: what the
+// steps share (lengths, needs) is read once, into LDS, and the counts four to a
+// load.
 __global__ __launch_bounds__(kBlock) void cache_extend_kernel(ExtendArgs a) {
-  extern __shared__ int sm[];  // end[S]
-  __shared__ int part[kWaves];
-  int *end = sm;
+  extern __shared__ int sm[];  // end[S], ctx[S], cu[S + 1]
+  __shared__ int part[kWaves], part2[kWaves];
   const int tid = threadIdx.x, S = a.S, W = a.W, size = a.page_size;
-  // lengths are held to what a table row can hold (W * size < 2^31), so that
+  int *end = sm, *ctx = sm + S, *cu = sm + 2 * S;
+  // lengths are held to what a table row can hold (W * size < 2^30), so that
   // pages and places come from 32-bit divisions
   const int most = W * size;
-  auto ctx_of = [&](int i) { return max(a.ctx[i], 0); };
-  auto new_of = [&](int i) { return max(a.cu[i + 1] - a.cu[i], 0); };
-  auto fits = [&](int i) { return ctx_of(i) <= most && new_of(i) <= most - ctx_of(i); };
+  for (int i = tid; i <= S; i += kBlock) {
+    cu[i] = a.cu[i];
+    if (i < S) ctx[i] = max(a.ctx[i], 0);
+  }
+  // free pages: all, and those before this workgroup's slice
+  const int64_t slice = ((a.pages + gridDim.x - 1) / gridDim.x + kBlock - 1) / kBlock * kBlock;
+  const int64_t s0 = min((int64_t)blockIdx.x * slice, a.pages), s1 = min(s0 + slice, a.pages);
+  int all = 0, mine = 0;  // s0 is a multiple of 4
+  if (reinterpret_cast<uintptr_t>(a.refs) % 16 == 0) {
+    const i32x4_t *refs = reinterpret_cast<const i32x4_t *>(a.refs);
+#pragma unroll 8
+    for (int64_t p = tid; p < a.pages / 4; p += kBlock) {
+      const i32x4_t r = refs[p];
+      const int f = (r[0] == 0) + (r[1] == 0) + (r[2] == 0) + (r[3] == 0);
+      all += f;
+      mine += 4 * p < s0 ? f : 0;
+    }
+    const int64_t p = a.pages / 4 * 4 + tid;
+    if (p < a.pages) {
+      const int f = a.refs[p] == 0;
+      all += f;
+      mine += p < s0 ? f : 0;
+    }
+  } else {
+    for (int64_t p = tid; p < a.pages; p += kBlock) {
+      const int f = a.refs[p] == 0;
+      all += f;
+      mine += p < s0 ? f : 0;
+    }
+  }
+#pragma unroll
+  for (int d = 32; d; d >>= 1) all += __shfl_xor(all, d), mine += __shfl_xor(mine, d);
+  if ((tid & 63) == 0) part[tid >> 6] = all, part2[tid >> 6] = mine;
+  __syncthreads();
+  int free_pages = 0, rank0 = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) free_pages += part[w], rank0 += part2[w];
+  auto new_of = [&](int i) { return max(cu[i + 1] - cu[i], 0); };
+  auto fits = [&](int i) { return ctx[i] <= most && new_of(i) <= most - ctx[i]; };
+  auto have_of = [&](int i) { return (int)fast_div(ctx[i] + size - 1, a.div_size); };
+  auto want_of = [&](int i) { return (int)fast_div(ctx[i] + new_of(i) + size - 1, a.div_size); };
   // needs and their running sums
   int sum = 0;
   for (int i0 = 0; i0 < S; i0 += kBlock) {
     const int i = i0 + tid;
-    int need = 0;
-    if (i < S && fits(i)) need = ceil_div(ctx_of(i) + new_of(i), size) - ceil_div(ctx_of(i), size);
+    const int need = i < S && fits(i) ? want_of(i) - have_of(i) : 0;
     int total;
     const int before = block_scan(need, part, &total);
     if (i < S) end[i] = sum + before + need;
     sum += total;
   }
-  // free pages: all, and those before this workgroup's slice
-  const int64_t slice = ((a.pages + gridDim.x - 1) / gridDim.x + kBlock - 1) / kBlock * kBlock;
-  const int64_t s0 = min((int64_t)blockIdx.x * slice, a.pages), s1 = min(s0 + slice, a.pages);
-  int all = 0, mine = 0;
-  for (int64_t p = tid; p < a.pages; p += kBlock) {
-    const int f = a.refs[p] == 0;
-    all += f;
-    if (p < s0) mine += f;
-  }
-  int free_pages, rank0;
-  block_scan(all, part, &free_pages);
-  block_scan(mine, part, &rank0);
+  __syncthreads();
   auto granted = [&](int i) { return fits(i) && end[i] <= free_pages; };
-  const int64_t step = (int64_t)gridDim.x * kBlock, first = (int64_t)blockIdx.x * kBlock + tid;
+  const int step = (int)gridDim.x * kBlock, first = (int)blockIdx.x * kBlock + tid;
+#pragma unroll 2
   for (int64_t e = first; e < (int64_t)S * W; e += step) {
-    const int i = (int)e / W, col = (int)e - i * W;
-    if (!(granted(i) && col >= ceil_div(ctx_of(i), size) && col < ceil_div(ctx_of(i) + new_of(i), size)))
-      a.table_out[e] = a.table[e];
+    const int i = (int)fast_div((uint32_t)e, a.div_w), col = (int)e - i * W, page = a.table[e];
+    if (!(granted(i) && col >= have_of(i) && col < want_of(i))) a.table_out[e] = page;
   }
-  for (int64_t i = first; i < S; i += step)
-    a.ctx_out[i] = granted((int)i) ? ctx_of((int)i) + new_of((int)i) : a.ctx[i];
+  for (int i = first; i < S; i += step) a.ctx_out[i] = granted(i) ? ctx[i] + new_of(i) : a.ctx[i];
   for (int64_t t = first; t < a.T; t += step) {
     int lo = 0, hi = S + 1;  // the first j with cu[j] > t
     while (lo < hi) {
       const int m = (lo + hi) / 2;
-      if (a.cu[m] > t) hi = m;
+      if (cu[m] > t) hi = m;
       else lo = m + 1;
     }
     const int i = lo - 1;
     int64_t pos = -1, slot = -1;
     bool fresh = false;
     if (i >= 0 && i < S && granted(i)) {
-      const int c = ctx_of(i), p = c + (int)(t - a.cu[i]), col = p / size;
+      const int p = ctx[i] + (int)(t - cu[i]), col = (int)fast_div(p, a.div_size);
       pos = p;
-      fresh = col >= ceil_div(c, size);
+      fresh = col >= have_of(i);
       if (!fresh) {
         const int page = a.table[(int64_t)i * W + col];
         if (page >= 0 && page < a.pages) slot = (int64_t)page * size + (p - col * size);
@@ -277,13 +301,13 @@ __global__ __launch_bounds__(kBlock) void cache_extend_kernel(ExtendArgs a) {
         else lo = m + 1;
       }
       if (granted(lo)) {
-        const int c = ctx_of(lo), n = c + new_of(lo);
-        const int col = ceil_div(c, size) + rank - (lo ? end[lo - 1] : 0);
+        const int c = ctx[lo], n = c + new_of(lo);
+        const int col = have_of(lo) + rank - (lo ? end[lo - 1] : 0);
         a.table_out[(int64_t)lo * W + col] = (int32_t)p;
         out = 1;
         const int from = col * size, last = n - from < size ? n : from + size;
         for (int pos = max(c, from); pos < last; ++pos) {
-          const int64_t t = (int64_t)a.cu[lo] + (pos - c);
+          const int64_t t = (int64_t)cu[lo] + (pos - c);
           if (t >= 0 && t < a.T) a.slots[t] = p * size + (pos - from);
         }
       }
@@ -300,56 +324,59 @@ __global__ __launch_bounds__(kBlock) void cache_extend_kernel(ExtendArgs a) {
 //
 // One workgroup: the steps depend on each other through the whole pool's
 // counts, and the tables are small (64 rows of 128 pages: 33 KB each way).
+// Bound by round trips to memory, so lengths and parents are kept in LDS and a
+// thread takes kEach table entries at once, their loads before their uses.
 __global__ __launch_bounds__(kBlock) void cache_fork_kernel(ForkArgs a) {
+  constexpr int kEach = 8;
   extern __shared__ int sm[];
   __shared__ int part[kWaves];
   const int tid = threadIdx.x, S = a.S, W = a.W, size = a.page_size;
-  int *children = sm, *first = sm + S, *give = sm + 2 * S;  // give[r]: the r-th free page
-  for (int i = tid; i < S; i += kBlock) children[i] = 0, first[i] = S;
+  // give[r]: the r-th free page; rank[i]: which of them row i gets, -1: none
+  int *children = sm, *first = sm + S, *give = sm + 2 * S, *rank = sm + 3 * S, *ctx = sm + 4 * S, *par = sm + 5 * S;
+  for (int i = tid; i < S; i += kBlock) {
+    const int p = a.parents[i];
+    children[i] = 0, first[i] = S;
+    ctx[i] = min(max(a.ctx[i], 0), W * size);
+    par[i] = p >= 0 && p < S ? p : -1;
+  }
+#pragma unroll 4
   for (int64_t p = tid; p < a.pages; p += kBlock)
     __hip_atomic_store(a.refs_out + p, a.refs[p], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  __threadfence();
+  counts_done();
   __syncthreads();
-  auto parent = [&](int i) {
-    const int p = a.parents[i];
-    return p >= 0 && p < S ? p : -1;
-  };
-  for (int i = tid; i < S; i += kBlock) {
-    const int p = parent(i);
-    if (p >= 0) {
-      atomicAdd(&children[p], 1);
-      atomicMin(&first[p], i);
+  for (int i = tid; i < S; i += kBlock)
+    if (par[i] >= 0) {
+      atomicAdd(&children[par[i]], 1);
+      atomicMin(&first[par[i]], i);
+    }
+  __syncthreads();
+  auto have_of = [&](int i) { return (int)fast_div(ctx[i] + size - 1, a.div_size); };
+  auto partial = [&](int i) { return ctx[i] != (int)fast_div(ctx[i], a.div_size) * size; };
+  auto in_pool = [&](int page) { return page >= 0 && page < a.pages; };
+  const int entries = S * W;
+  // the counts after every child took its parent's pages
+  for (int e0 = 0; e0 < entries; e0 += kEach * kBlock) {
+    int page[kEach];
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) page[k] = a.table[min(e0 + k * kBlock + tid, entries - 1)];
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+      const int e = e0 + k * kBlock + tid;
+      if (e >= entries || !in_pool(page[k])) continue;
+      const int i = (int)fast_div(e, a.div_w), col = e - i * W, have = have_of(i);
+      if (col >= have) continue;
+      const bool last = partial(i) && col == have - 1;
+      const int gain = (last ? (children[i] > 0) : children[i]) - 1;
+      if (gain) atomicAdd(a.refs_out + page[k], gain);
     }
   }
-  __syncthreads();
-  auto ctx_of = [&](int i) { return min(max(a.ctx[i], 0), W * size); };
-  auto page_of = [&](int i, int col) {
-    const int p = a.table[(int64_t)i * W + col];
-    return p >= 0 && p < a.pages ? p : -1;
-  };
-  // the counts after every child took its parent's pages
-  for (int64_t e = tid; e < (int64_t)S * W; e += kBlock) {
-    const int i = (int)e / W, col = (int)e - i * W;
-    const int c = ctx_of(i);
-    const int have = ceil_div(c, size);
-    if (col >= have) continue;
-    const int page = page_of(i, col);
-    if (page < 0) continue;
-    const bool last = c % size != 0 && col == have - 1;
-    const int gain = (last ? (children[i] > 0) : children[i]) - 1;
-    if (gain) atomicAdd(a.refs_out + page, gain);
-  }
-  __threadfence();
+  counts_done();
   // rows that need a page of their own
   int needs = 0;
-  int *rank = sm + 3 * S;  // -1: the row needs none
   for (int i0 = 0; i0 < S; i0 += kBlock) {
     const int i = i0 + tid;
     int need = 0;
-    if (i < S) {
-      const int p = parent(i);
-      need = p >= 0 && ctx_of(p) % size != 0 && first[p] != i;
-    }
+    if (i < S) need = par[i] >= 0 && partial(par[i]) && first[par[i]] != i;
     int total;
     const int before = block_scan(need, part, &total);
     if (i < S) rank[i] = need ? needs + before : -1;
@@ -367,13 +394,12 @@ __global__ __launch_bounds__(kBlock) void cache_fork_kernel(ForkArgs a) {
   }
   __syncthreads();
   for (int i = tid; i < S; i += kBlock) {
-    const int p = parent(i);
+    const int p = par[i];
     const bool lost = p >= 0 && rank[i] >= found;
-    const bool fresh = rank[i] >= 0 && !lost;
     int src = -1, dst = -1;
-    if (fresh) {
-      const int c = ctx_of(p);
-      src = page_of(p, ceil_div(c, size) - 1);
+    if (rank[i] >= 0 && !lost) {
+      src = a.table[(int64_t)p * W + have_of(p) - 1];
+      if (!in_pool(src)) src = -1;
       dst = give[rank[i]];
       atomicAdd(a.refs_out + dst, 1);
     }
@@ -381,27 +407,29 @@ __global__ __launch_bounds__(kBlock) void cache_fork_kernel(ForkArgs a) {
     a.copies[2 * i] = src;
     a.copies[2 * i + 1] = dst;
   }
-  for (int64_t e = tid; e < (int64_t)S * W; e += kBlock) {
-    const int i = (int)e / W, col = (int)e - i * W;
-    const int p = parent(i);
-    int out = -1;
-    if (p >= 0) {
-      const int c = ctx_of(p);
-      const int have = ceil_div(c, size);
-      if (col < have) {
-        const bool last = c % size != 0 && col == have - 1;
-        const bool lost = rank[i] >= found;
-        out = a.table[(int64_t)p * W + col];
-        if (lost) {  // its share of the full pages goes back
-          const int page = page_of(p, col);
-          if (!last && page >= 0) atomicSub(a.refs_out + page, 1);
-          out = -1;
-        } else if (last && rank[i] >= 0) {
-          out = give[rank[i]];
+  for (int e0 = 0; e0 < entries; e0 += kEach * kBlock) {
+    int page[kEach];
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+      const int e = min(e0 + k * kBlock + tid, entries - 1), i = (int)fast_div(e, a.div_w);
+      page[k] = a.table[(int64_t)max(par[i], 0) * W + e - i * W];
+    }
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+      const int e = e0 + k * kBlock + tid;
+      if (e >= entries) continue;
+      const int i = (int)fast_div(e, a.div_w), col = e - i * W, p = par[i];
+      int out = -1;
+      if (p >= 0 && col < have_of(p)) {
+        const bool last = partial(p) && col == have_of(p) - 1;
+        if (rank[i] >= found) {  // a lost row's share of the full pages goes back
+          if (!last && in_pool(page[k])) atomicSub(a.refs_out + page[k], 1);
+        } else {
+          out = last && rank[i] >= 0 ? give[rank[i]] : page[k];
         }
       }
+      a.table_out[e] = out;
     }
-    a.table_out[e] = out;
   }
 }
 
@@ -481,15 +509,24 @@ hipError_t launch_rotary(RotaryArgs a, int dtype, bool wide, hipStream_t s) {
   return wide ? launch_rotary_v<float, 4>(a, s) : launch_rotary_v<float, 1>(a, s);
 }
 
-hipError_t launch_cache_extend(const ExtendArgs &a, hipStream_t s) {
-  const int64_t work = std::max({a.pages, (int64_t)a.S * a.W / 4, a.T});
-  const int grid = (int)std::min<int64_t>(std::max<int64_t>((work + 4 * kBlock - 1) / (4 * kBlock), 1), 256);
-  cache_extend_kernel<<<grid, kBlock, (size_t)std::max(a.S, 1) * sizeof(int), s>>>(a);
+hipError_t launch_cache_extend(ExtendArgs a, hipStream_t s) {
+  // a workgroup's share: one entry, page and token per thread, on 256 CUs
+  const int64_t work = std::max({a.pages, (int64_t)a.S * a.W, a.T});
+  const int grid = (int)std::min<int64_t>(std::max<int64_t>((work + kBlock - 1) / kBlock, 1), 256);
+  a.div_size = make_div(a.page_size), a.div_w = make_div(std::max(a.W, 1));
+  cache_extend_kernel<<<grid, kBlock, (3 * (size_t)a.S + 1) * sizeof(int), s>>>(a);
   return hipGetLastError();
 }
 
-hipError_t launch_cache_fork(const ForkArgs &a, hipStream_t s) {
-  cache_fork_kernel<<<1, kBlock, (size_t)std::max(a.S, 1) * 4 * sizeof(int), s>>>(a);
+hipError_t launch_cache_fork(ForkArgs a, hipStream_t s) {
+  const size_t lds = (size_t)a.S * 6 * sizeof(int);
+  if (lds > 60 * 1024) {
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(cache_fork_kernel),
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    if (e != hipSuccess) return e;
+  }
+  a.div_size = make_div(a.page_size), a.div_w = make_div(std::max(a.W, 1));
+  cache_fork_kernel<<<1, kBlock, lds, s>>>(a);
   return hipGetLastError();
 }
 

@@ -15,6 +15,33 @@ namespace zt {
 // Sets the calling thread's error message and returns `code` (capi.hip).
 int api_fail(int code, const char *fmt, ...) __attribute__((format(printf, 2, 3)));
 
+// Division of n <= 2^30 by a fixed d >= 1: floor(n * mul / 2^(31 + L)) with
+// mul = floor(2^(31 + L) / d) + 1 and L = ceil(log2 d), which is exact for every
+// n < 2^31; 2 n * mul is taken so that the high word is all that is needed.
+struct FastDiv {
+  uint32_t mul, shift;
+};
+inline FastDiv make_div(uint32_t d) {
+  uint32_t L = 0;
+  while ((1ull << L) < d) ++L;
+  return {(uint32_t)((1ull << (31 + L)) / d + 1), L};
+}
+__device__ __forceinline__ uint32_t fast_div(uint32_t n, FastDiv d) {
+  return __umulhi(2 * n, d.mul) >> d.shift;
+}
+
+// Inclusive prefix sum over a wave, by lane moves that cost an addition each
+// (rows of 16 lanes, then the rows' last lanes on).
+__device__ __forceinline__ int wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);   // row_shr 1
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);   // row_shr 2
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);   // row_shr 4
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);   // row_shr 8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row 0 -> 1, 2 -> 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // lane 31 -> rows 2, 3
+  return x;
+}
+
 struct RotaryArgs {
   const void *q, *k, *v;      // [T, H | KV | KV, D], unit last stride
   int64_t q_ld[2], k_ld[2], v_ld[2];  // token and head strides, elements
@@ -39,16 +66,18 @@ struct ExtendArgs {
   int64_t pages, T;
   int32_t *table_out, *ctx_out, *refs_out;
   int64_t *pos_out, *slots;  // [T]
+  FastDiv div_size, div_w;   // set by launch_cache_extend
 };
-hipError_t launch_cache_extend(const ExtendArgs &a, hipStream_t s);
+hipError_t launch_cache_extend(ExtendArgs a, hipStream_t s);
 
 struct ForkArgs {
   const int32_t *table, *ctx, *refs, *parents;
   int S, W, page_size;
   int64_t pages;
   int32_t *table_out, *ctx_out, *refs_out, *copies;  // copies [S, 2]
+  FastDiv div_size, div_w;  // set by launch_cache_fork
 };
-hipError_t launch_cache_fork(const ForkArgs &a, hipStream_t s);
+hipError_t launch_cache_fork(ForkArgs a, hipStream_t s);
 
 struct CompactArgs {
   const int32_t *table, *refs;
@@ -66,21 +95,6 @@ struct CopyArgs {
   int parts;
 };
 hipError_t launch_copy_pages(CopyArgs a, int caches, int64_t pairs, bool wide, hipStream_t s);
-
-// Division of n <= 2^30 by a fixed d >= 1: floor(n * mul / 2^(31 + L)) with
-// mul = floor(2^(31 + L) / d) + 1 and L = ceil(log2 d), which is exact for every
-// n < 2^31; 2 n * mul is taken so that the high word is all that is needed.
-struct FastDiv {
-  uint32_t mul, shift;
-};
-inline FastDiv make_div(uint32_t d) {
-  uint32_t L = 0;
-  while ((1ull << L) < d) ++L;
-  return {(uint32_t)((1ull << (31 + L)) / d + 1), L};
-}
-__device__ __forceinline__ uint32_t fast_div(uint32_t n, FastDiv d) {
-  return __umulhi(2 * n, d.mul) >> d.shift;
-}
 
 struct AttnArgs {
   const void *q;  // [T, H, D]
