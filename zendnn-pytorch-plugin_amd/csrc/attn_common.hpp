@@ -71,6 +71,11 @@ struct Batch {
   __device__ __forceinline__ Batch(void *lds, int S)
       : tile_base(static_cast<int *>(lds)), q0(tile_base + S + 1), q(q0 + S), n(q + S) {}
   __device__ __forceinline__ Seq operator[](int i) const { return {q0[i], q[i], n[i]}; }
+  // the same for an i that all lanes share, in scalar registers
+  __device__ __forceinline__ Seq uniform(int i) const {
+    return {__builtin_amdgcn_readfirstlane(q0[i]), __builtin_amdgcn_readfirstlane(q[i]),
+            __builtin_amdgcn_readfirstlane(n[i])};
+  }
 };
 constexpr int batch_ints(int S) { return 4 * S + 1; }
 
@@ -108,7 +113,7 @@ __device__ __forceinline__ int scan(int v, int *part, int *total) {
     if (w < wave) before += y;
     sum += y;
   }
-  *total = sum;
+  *total = __builtin_amdgcn_readfirstlane(sum);
   return before + x - v;
 }
 
@@ -199,8 +204,9 @@ __device__ __forceinline__ Plan make_plan(const AttnArgs &a, int BM, int UK, con
       p.head = p.wg / p.items, p.item = p.wg - p.head * p.items;
       if (p.item == tid) sh->before = before, sh->item = cost;
       __syncthreads();
-      p.base = p.from = (int64_t)p.head * sum + sh->before, p.to = p.from + sh->item;
-      p.per = max(sh->item, 1);
+      const int length = __builtin_amdgcn_readfirstlane(sh->item);
+      p.base = p.from = (int64_t)p.head * sum + __builtin_amdgcn_readfirstlane(sh->before);
+      p.to = p.from + length, p.per = max(length, 1);
       return p;
     }
   }
@@ -227,7 +233,8 @@ __device__ __forceinline__ Plan make_plan(const AttnArgs &a, int BM, int UK, con
     }
   }
   __syncthreads();
-  p.item = sh->item, p.base = (int64_t)p.head * sum + sh->before;
+  p.item = __builtin_amdgcn_readfirstlane(sh->item);
+  p.base = (int64_t)p.head * sum + __builtin_amdgcn_readfirstlane(sh->before);
   return p;
 }
 
@@ -251,8 +258,9 @@ struct Walk {
     while (base < p.to) {
       if (item == p.items) ++head, item = 0;
       g->head = head;
-      g->seq = seq_of_item(batch.tile_base, a.S, item), g->tile = item - batch.tile_base[g->seq];
-      const Seq s = batch[g->seq];
+      g->seq = __builtin_amdgcn_readfirstlane(seq_of_item(batch.tile_base, a.S, item));
+      g->tile = item - __builtin_amdgcn_readfirstlane(batch.tile_base[g->seq]);
+      const Seq s = batch.uniform(g->seq);
       g->keys = keys_of(a, s, g->tile, BM);
       g->nb = blocks_of(g->keys, UK), g->b0 = g->keys.begin / UK;
       ++item;

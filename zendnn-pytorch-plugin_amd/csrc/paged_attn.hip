@@ -89,7 +89,7 @@ __global__ __launch_bounds__(kRowThreads, NT * DP <= 128 ? 2 : 1) void paged_att
   Segment seg;
   while (walk.next(a, plan, batch, BM, UK, &seg)) {
     const int h = seg.head, take = seg.take;
-    const Seq s = batch[seg.seq];
+    const Seq s = batch.uniform(seg.seq);
     const int r0 = seg.tile * BM;
     const KeyRange kr = seg.keys;
     const Pages pages{a.table + (int64_t)seg.seq * a.W, kr.begin, kr.end};

@@ -109,7 +109,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP <= 1
   Segment seg;
   while (walk.next(a, plan, batch, BM, TK, &seg)) {
     const int h = seg.head, take = seg.take;
-    const Seq s = batch[seg.seq];
+    const Seq s = batch.uniform(seg.seq);
     const int r0 = seg.tile * BM;
     const KeyRange kr = seg.keys;
     const Pages pages{a.table + (int64_t)seg.seq * a.W, kr.begin, kr.end};
