@@ -337,6 +337,65 @@ __device__ __forceinline__ void zero_rows(const AttnArgs &a, const Plan &p, int 
     reinterpret_cast<u32x4_t *>(out)[e < lo * row ? e : e - lo * row + hi * row] = u32x4_t{0, 0, 0, 0};
 }
 
+__device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32); }
+
+// The 32 rows of a wave of the tile kernels, as one lane sees them: its row is
+// n = lane % 32, and of 32 scores it holds those of keys 8 (i / 4) + 4 half +
+// i % 4, half = lane / 32.
+struct Rows32 {
+  int row, token;  // of the sequence's rows and new tokens
+  bool live;
+  int lo, hi;      // the keys it sees
+  bool any;        // over the wave's rows; live ones come first, and their
+  int hi_min, lo_min, hi_max, lo_max;  // tokens ascend with the rows
+
+  __device__ __forceinline__ Rows32(const AttnArgs &a, const Seq &s, int row) : row(row) {
+    token = (int)fast_div(row, a.div_group);
+    live = token < s.q;
+    const int pos = s.n - s.q + token;
+    hi = !live ? INT32_MAX : a.causal ? pos + 1 : s.n;
+    lo = live && a.causal && a.window ? (int)max((int64_t)pos + 1 - a.window, (int64_t)0) : 0;
+    const uint32_t alive = (uint32_t)__ballot(live);
+    any = alive != 0;
+    const int last = 31 - __builtin_clz(alive | 1u);
+    hi_min = __builtin_amdgcn_readlane(hi, 0), lo_min = __builtin_amdgcn_readlane(lo, 0);
+    hi_max = __builtin_amdgcn_readlane(hi, last), lo_max = __builtin_amdgcn_readlane(lo, last);
+  }
+  __device__ __forceinline__ bool see(int k0, int n) const { return any && k0 < hi_max && k0 + n > lo_min; }
+  __device__ __forceinline__ bool see_all(int k0, int n) const { return k0 + n <= hi_min && k0 >= lo_max; }
+  // scores of keys k0 .. k0 + 31 that the row does not see, or that are not there
+  __device__ __forceinline__ void mask(f32x16_t &sc, int k0, uint32_t there) const {
+    const int from = min(max(lo - k0, 0), 32), to = min(max(hi - k0, 0), 32);
+    const uint64_t range = (1ull << to) - (1ull << min(from, to));
+    const uint32_t seen = ((uint32_t)range & there) >> (4 * ((threadIdx.x >> 5) & 1));
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+      if (!(seen & (1u << (8 * (e / 4) + e % 4)))) sc[e] = -INFINITY;
+  }
+  // Outputs, or a part of them: the lane holds columns 32 d + 8 k + 4 half .. + 3.
+  template <typename T, int DT>
+  __device__ __forceinline__ void store(const AttnArgs &a, const Segment &seg, const Seq &s, int BM, int at,
+                                        const f32x16_t (&o)[DT], float m, float l) const {
+    if (!live) return;
+    const int half = (threadIdx.x >> 5) & 1;
+    const int64_t pr = seg.slot * BM + at;
+    const int64_t to =
+        ((int64_t)(s.q0 + token) * a.H + seg.head * a.group + row - token * a.group) * a.D;
+    const float r = l > 0.f ? 1.f / l : 0.f;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int col = 32 * d + 8 * k + 4 * half;
+        const f32x4_t y = {o[d][4 * k], o[d][4 * k + 1], o[d][4 * k + 2], o[d][4 * k + 3]};
+        if (col >= a.D) continue;
+        if (seg.complete) store_out<T>(a.out, to + col, y, r);
+        else *reinterpret_cast<f32x4_t *>(a.part_o + pr * a.D + col) = y;
+      }
+    if (!seg.complete && half == 0) a.part_ml[2 * pr] = m, a.part_ml[2 * pr + 1] = l;
+  }
+};
+
 // The tile kernel (paged_attn_tile.hip): its rows per item and workgroups.
 int tile_rows(const AttnArgs &a);
 int tile_grid(const AttnArgs &a);

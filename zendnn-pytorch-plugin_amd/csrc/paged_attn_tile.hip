@@ -24,8 +24,6 @@ __device__ __forceinline__ void wait_and_meet() {
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
-__device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32); }
-
 // The cost of a block, and of an item's beginning and end.  A block of few rows
 // takes nearly as long as a full one: in bf16 it waits for its keys (1.9 against
 // 2.2 us, two workgroups a CU), in fp32 for its one wave's share of the matrix
@@ -148,25 +146,15 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP <= 1
     int page = lookup(k_first + TK);
 
     // ---- the wave's rows: lane (row n, half) holds pieces 2 j + half of q
-    const int row = r0 + 32 * wave + n;
-    const int row_t = (int)fast_div(row, a.div_group);
-    const bool live = row_t < s.q;
-    const int pos = s.n - s.q + row_t;
-    const int hi = !live ? INT32_MAX : a.causal ? pos + 1 : s.n;
-    const int lo = live && a.causal && a.window ? (int)max((int64_t)pos + 1 - a.window, (int64_t)0) : 0;
-    // over the wave's live rows, which come first: tokens ascend with the rows
-    const bool wave_live = __ballot(live) != 0;
-    const int last_live = 31 - __builtin_clz((uint32_t)__ballot(live) | 1u);
-    const int hi_min = __builtin_amdgcn_readlane(hi, 0), lo_min = __builtin_amdgcn_readlane(lo, 0);
-    const int hi_max = __builtin_amdgcn_readlane(hi, last_live), lo_max = __builtin_amdgcn_readlane(lo, last_live);
+    const Rows32 rows(a, s, r0 + 32 * wave + n);
     u32x4_t q[NQ];
     {
       const char *src = static_cast<const char *>(a.q) +
-          ((int64_t)(s.q0 + row_t) * a.q_ld[0] + (h * G + row - row_t * G) * a.q_ld[1]) * ES;
+          ((int64_t)(s.q0 + rows.token) * a.q_ld[0] + (h * G + rows.row - rows.token * G) * a.q_ld[1]) * ES;
 #pragma unroll
       for (int j = 0; j < NQ; ++j) {
         const int p = 2 * j + half;
-        q[j] = scale_sign<T>(*reinterpret_cast<const u32x4_t *>(live && p < C ? src + 16 * p : zero), a.scale);
+        q[j] = scale_sign<T>(*reinterpret_cast<const u32x4_t *>(rows.live && p < C ? src + 16 * p : zero), a.scale);
       }
     }
     f32x16_t o[DT];
@@ -181,7 +169,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP <= 1
       wait_and_meet();  // the tile is there, and the previous one is done with
       const uint64_t there_next = offsets(k0 + TK, page, t + 1 < take);
       page = lookup(k0 + 2 * TK);
-      if (wave_live && k0 < hi_max && k0 + TK > lo_min) {
+      if (rows.see(k0, TK)) {
         const unsigned char *kt = smem + st * 2 * STAGE, *vt = kt + STAGE;
         // ---- scores.  Keys are read kAhead operands before their use; the
         // fences keep the compiler from moving each read next to its use.
@@ -221,18 +209,9 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP <= 1
         }
         // ---- weights
         const bool whole = there == (TK == 64 ? ~0ull : 0xffffffffull);
-        if (!whole || k0 + TK > hi_min || k0 < lo_max) {
-          // bit 8 (i / 4) + i % 4 of `seen`: the lane's i-th key of 32
+        if (!whole || !rows.see_all(k0, TK))
 #pragma unroll
-          for (int u = 0; u < KT; ++u) {
-            const int from = min(max(lo - k0 - 32 * u, 0), 32), to = min(max(hi - k0 - 32 * u, 0), 32);
-            const uint64_t range = (1ull << to) - (1ull << min(from, to));
-            const uint32_t seen = ((uint32_t)range & (uint32_t)(there >> (32 * u))) >> (4 * half);
-#pragma unroll
-            for (int e = 0; e < 16; ++e)
-              if (!(seen & (1u << (8 * (e / 4) + e % 4)))) sc[u][e] = -INFINITY;
-          }
-        }
+          for (int u = 0; u < KT; ++u) rows.mask(sc[u], k0 + 32 * u, (uint32_t)(there >> (32 * u)));
         float mx = sc[0][0];
 #pragma unroll
         for (int u = 0; u < KT; ++u)
@@ -322,25 +301,9 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP <= 1
     }
     // ---- the rows' outputs, or their part: lane (row n, half) holds columns
     // 32 d + 8 k + 4 half .. + 3
-    const bool complete = seg.complete;
     l += other_half(l);
-    if (live) {
-      const int64_t pr = seg.slot * BM + 32 * wave + n;
-      const int64_t to = ((int64_t)(s.q0 + row_t) * a.H + h * G + row - row_t * G) * a.D;
-      const float r = l > 0.f ? 1.f / l : 0.f;
-#pragma unroll
-      for (int d = 0; d < DT; ++d)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int col = 32 * d + 8 * k + 4 * half;
-          const f32x4_t y = {o[d][4 * k], o[d][4 * k + 1], o[d][4 * k + 2], o[d][4 * k + 3]};
-          if (col >= a.D) continue;
-          if (complete) store_out<T>(a.out, to + col, y, r);
-          else *reinterpret_cast<f32x4_t *>(a.part_o + pr * a.D + col) = y;
-        }
-      if (!complete && half == 0) a.part_ml[2 * pr] = m, a.part_ml[2 * pr + 1] = l;
-    }
-    if (tid == 0 && seg.bb == 0 && !complete) {
+    rows.store<T>(a, seg, s, BM, 32 * wave + n, o, m, l);
+    if (tid == 0 && seg.bb == 0 && !seg.complete) {
       split->slot = seg.slot, split->last = seg.last;
       split->row0 = r0, split->rows = min(BM, s.q * G - r0), split->head = h, split->q0 = s.q0;
     }
