@@ -30,7 +30,7 @@ HIPCC = os.path.join(ROCM, "bin", "hipcc")
 
 HIP_SOURCES = ["woq_kernels.hip", "woq_prefill.hip", "dynq_kernels.hip", "s8_prefill.hip",
                "moe_kernels.hip", "kv_cache.hip", "paged_attn.hip",
-               "paged_attn_tile.hip", "capi.hip", "capi_cache.hip"]
+               "paged_attn_tile.hip", "paged_attn_split.hip", "capi.hip", "capi_cache.hip"]
 TORCH_SOURCES = ["ops.cpp", "ops_cache.cpp", "shim_cuda_zentorch.cpp"]
 
 # -packed-fp32-ops: no v_pk_*_f32 from the compiler (hipcc's host pass warns

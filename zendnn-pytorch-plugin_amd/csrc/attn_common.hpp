@@ -400,6 +400,7 @@ struct Rows32 {
 int tile_rows(const AttnArgs &a);
 int tile_grid(const AttnArgs &a);
 hipError_t launch_tiles(const AttnArgs &a, int grid, hipStream_t s);
+hipError_t launch_split(const AttnArgs &a, int grid, hipStream_t s);  // paged_attn_split.hip
 constexpr int kTileCostLead = 15, kTileCostMost = 6;  // the most of TileCost
 
 }  // namespace zt

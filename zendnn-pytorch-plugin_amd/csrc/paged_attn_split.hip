@@ -1,0 +1,268 @@
+// Attention of a chunk of new tokens over a paged cache, for gfx950: many rows
+// per cache head in fp32, head_dim up to 128, on bf16 MFMAs.  The definitions are in
+// paged_attn.hip.
+#include "attn_common.hpp"
+
+namespace zt {
+
+namespace {
+
+// x = x1 + x2 + x3 with each part a bf16: x1 the nearest to x, x2 to x - x1, x3
+// to what is left (8 of fp32's 24 digits each, so the sum is x again but for
+// numbers whose last part underflows).  Two numbers at a time, packed.
+struct Parts {
+  uint32_t p[3];
+};
+__device__ __forceinline__ Parts split2(float a, float b) {
+  Parts s;
+  s.p[0] = pack_bf16x2(a, b);
+  a -= __uint_as_float(s.p[0] << 16), b -= __uint_as_float(s.p[0] & 0xffff0000u);
+  s.p[1] = pack_bf16x2(a, b);
+  a -= __uint_as_float(s.p[1] << 16), b -= __uint_as_float(s.p[1] & 0xffff0000u);
+  s.p[2] = pack_bf16x2(a, b);
+  return s;
+}
+
+// x y without the terms below fp32's last digit: x1 y1 + (x1 y2 + x2 y1) +
+// (x2 y2 + x1 y3 + x3 y1), smallest first.
+__device__ __forceinline__ f32x16_t mfma_split(const u32x4_t (&x)[3], const u32x4_t (&y)[3], f32x16_t acc) {
+  auto mul = [&](int i, int j) {
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, x[i]),
+                                                  __builtin_bit_cast(bf16x8_t, y[j]), acc, 0, 0, 0);
+  };
+  mul(2, 0), mul(0, 2), mul(1, 1), mul(1, 0), mul(0, 1), mul(0, 0);
+  return acc;
+}
+
+// A block takes nearly the same time whatever rows are live, and an item's two
+// ends about one block's.
+struct SplitCost {
+  static constexpr int kLead = 2, kMost = 2;
+  static __device__ __forceinline__ int of(int) { return 2; }
+};
+
+// NW waves of 32 rows each against a span of the keys of one cache head, as
+// paged_attn_tile.hip's kernel does it for bf16, in tiles of 32 keys.
+//
+// An fp32 MFMA runs at a sixteenth of the bf16 rate, so every number goes in
+// three bf16 parts and a product in six MFMAs, 2.7 times as fast, with every
+// term fp32 can hold.  Keys and values are split once per workgroup on their
+// way to LDS (global memory -> registers while a tile is worked on -> three
+// planes of the next stage), queries once per item, weights as they are made.
+template <int DP, int DC, int NW>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2))) void paged_attn_split_kernel(
+    AttnArgs a) {
+  using Cost = SplitCost;
+  constexpr int NTH = 64 * NW, BM = 32 * NW, TK = 32;
+  constexpr int RB = DP * 2, CR = RB / 16, PLANE = TK * RB, STAGE = 6 * PLANE;
+  constexpr int PR = DP / 4, NL = TK * PR / NTH;  // 16-byte pieces of a row; of a tile, per thread
+  constexpr int NQ = DC / 16, DT = DC / 32;
+  static_assert(NL >= 1 && TK * PR % NTH == 0, "the threads share a tile's pieces evenly");
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  __shared__ PlanShared sh;
+  const Batch batch(smem + 2 * STAGE, a.S);
+
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const Plan plan = make_plan<NTH, Cost>(a, BM, TK, batch, &sh);
+  Split *split = static_cast<Split *>(a.splits) + plan.wg;
+  if (tid == 0) split->rows = 0;
+
+  const float c = score_factor(a.scale);
+  const int G = a.group, C = a.D / 4;
+  const char *zero = reinterpret_cast<const char *>(kZeroRow);
+  // the same permutations of a row's 16-byte pieces as the bf16 kernel's
+  auto kswz = [](int row) { return CR >= 16 ? row & 15 : row & 7; };
+  auto vswz = [](int row) { return CR >= 16 ? (row & 3) << 2 : ((row >> 1) & 1) << 2; };
+
+  Walk<Cost> walk(plan);
+  Segment seg;
+  while (walk.next(a, plan, batch, BM, TK, &seg)) {
+    const int h = seg.head, take = seg.take;
+    const Seq s = batch.uniform(seg.seq);
+    const int r0 = seg.tile * BM, k_first = (seg.b0 + seg.bb) * TK;
+    const Pages pages{a.table + (int64_t)seg.seq * a.W, seg.keys.begin, seg.keys.end};
+    const char *kbase = static_cast<const char *>(a.k) + h * a.k_ld[1] * 4;
+    const char *vbase = static_cast<const char *>(a.v) + h * a.v_ld[1] * 4;
+
+    auto lookup = [&](int at) { return pages.lookup(a, at + n); };
+    u32x4_t kreg[NL], vreg[NL];
+    auto fetch = [&](int at, int page) -> uint32_t {
+      const int tok = at + n;
+      const bool ok = pages.there(a, tok, page);
+      const uint32_t ko = ok ? row_offset(a, a.k_row, tok, page) : ~0u;
+      const uint32_t vo = ok ? row_offset(a, a.v_row, tok, page) : ~0u;
+#pragma unroll
+      for (int j = 0; j < NL; ++j) {
+        const int idx = j * NTH + tid, row = idx / PR, piece = idx % PR;
+        const uint32_t kr = __shfl(ko, row), vr = __shfl(vo, row);
+        kreg[j] = *reinterpret_cast<const u32x4_t *>(
+            kr != ~0u && piece < C ? kbase + (uint64_t)(kr + piece) * 16 : zero);
+        vreg[j] = *reinterpret_cast<const u32x4_t *>(
+            vr != ~0u && piece < C ? vbase + (uint64_t)(vr + piece) * 16 : zero);
+      }
+      return (uint32_t)__ballot(ok);
+    };
+    auto put = [&](unsigned char *to, int swz, int row, int piece, u32x4_t x) {
+      const Parts lo = split2(__uint_as_float(x[0]), __uint_as_float(x[1]));
+      const Parts hi = split2(__uint_as_float(x[2]), __uint_as_float(x[3]));
+      to += row * RB + 16 * ((piece / 2) ^ swz) + 8 * (piece & 1);
+#pragma unroll
+      for (int p = 0; p < 3; ++p) *reinterpret_cast<u32x2_t *>(to + p * PLANE) = u32x2_t{lo.p[p], hi.p[p]};
+    };
+    auto keep = [&](int st) {
+#pragma unroll
+      for (int j = 0; j < NL; ++j) {
+        const int idx = j * NTH + tid, row = idx / PR, piece = idx % PR;
+        put(smem + st * STAGE, kswz(row), row, piece, kreg[j]);
+        put(smem + st * STAGE + 3 * PLANE, vswz(row), row, piece, vreg[j]);
+      }
+    };
+    uint32_t there = fetch(k_first, lookup(k_first));
+    int page = lookup(k_first + TK);
+
+    // ---- the wave's rows: lane (row n, half) holds columns 16 j + 8 half .. + 7
+    const Rows32 rows(a, s, r0 + 32 * wave + n);
+    u32x4_t q[NQ][3];
+    {
+      const char *src = static_cast<const char *>(a.q) +
+          ((int64_t)(s.q0 + rows.token) * a.q_ld[0] + (h * G + rows.row - rows.token * G) * a.q_ld[1]) * 4;
+#pragma unroll
+      for (int j = 0; j < NQ; ++j)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int p = 4 * j + 2 * half + e;
+          const u32x4_t x = scale_sign<float>(
+              *reinterpret_cast<const u32x4_t *>(rows.live && p < C ? src + 16 * p : zero), a.scale);
+          const Parts lo = split2(__uint_as_float(x[0]), __uint_as_float(x[1]));
+          const Parts hi = split2(__uint_as_float(x[2]), __uint_as_float(x[3]));
+#pragma unroll
+          for (int k = 0; k < 3; ++k) q[j][k][2 * e] = lo.p[k], q[j][k][2 * e + 1] = hi.p[k];
+        }
+    }
+    f32x16_t o[DT];
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
+    float m = -INFINITY, l = 0.f;
+
+    keep(0);
+    for (int t = 0; t < take; ++t) {
+      const int k0 = k_first + t * TK, st = t & 1;
+      // every wave's part of the tile is in LDS, and the previous tile is done with
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      uint32_t there_next = 0;
+      if (t + 1 < take) {
+        there_next = fetch(k0 + TK, page);
+        page = lookup(k0 + 2 * TK);
+      }
+      if (rows.see(k0, TK)) {
+        const unsigned char *kt = smem + st * STAGE, *vt = kt + 3 * PLANE;
+        // ---- scores; the next step's keys are read before a step's MFMAs
+        f32x16_t sc;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sc[e] = 0.f;
+        auto read_k = [&](int j, u32x4_t (&k)[3]) {
+#pragma unroll
+          for (int p = 0; p < 3; ++p)
+            k[p] = *reinterpret_cast<const u32x4_t *>(kt + p * PLANE + n * RB + 16 * ((2 * j + half) ^ kswz(n)));
+        };
+        u32x4_t k[2][3];
+        read_k(0, k[0]);
+#pragma unroll
+        for (int j = 0; j < NQ; ++j) {
+          if (j + 1 < NQ) read_k(j + 1, k[(j + 1) & 1]);
+          __builtin_amdgcn_sched_barrier(0);
+          sc = mfma_split(k[j & 1], q[j], sc);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        // ---- weights
+        if (there != ~0u || !rows.see_all(k0, TK)) rows.mask(sc, k0, there);
+        float mx = sc[0];
+#pragma unroll
+        for (int e = 1; e < 16; ++e) mx = fmaxf(mx, sc[e]);
+        mx = fmaxf(mx, other_half(mx));
+        if (__ballot(mx != -INFINITY && (mx - m) * c > 8.f)) {
+          const float to = fmaxf(m, mx);
+          const float f = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m * c - to * c);
+          l *= f;
+#pragma unroll
+          for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[d][e] *= f;
+          m = to;
+        }
+        const float mc = m == -INFINITY ? 0.f : m * c;
+        // ---- O^T += V^T P^T, 16 keys and 32 columns a step
+        typedef __attribute__((address_space(3))) s16x4_t *tr_ptr;
+        const int i16 = lane & 15, r = 4 * half + i16 / 4;
+        const int piece = 2 * ((lane >> 4) & 1) + (i16 & 3) / 2;
+        auto read_v = [&](int j, u32x4_t (&v)[3]) {
+#pragma unroll
+          for (int p = 0; p < 3; ++p) {
+            const unsigned char *at = vt + p * PLANE + (16 * (j / DT) + r) * RB +
+                16 * ((4 * (j % DT) + piece) ^ vswz(r)) + 8 * (i16 & 1);
+            const s16x4_t v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)at);
+            const s16x4_t v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)(at + 8 * RB));
+            v[p] = __builtin_bit_cast(u32x4_t, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+          }
+        };
+        u32x4_t p[3], v[2][3];
+        read_v(0, v[0]);
+#pragma unroll
+        for (int j = 0; j < 2 * DT; ++j) {
+          if (j % DT == 0)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int i = 8 * (j / DT) + 2 * e;
+              const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[i], c, -mc));
+              const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[i + 1], c, -mc));
+              l += p0;
+              l += p1;
+              const Parts w = split2(p0, p1);
+#pragma unroll
+              for (int x = 0; x < 3; ++x) p[x][e] = w.p[x];
+            }
+          if (j + 1 < 2 * DT) read_v(j + 1, v[(j + 1) & 1]);
+          __builtin_amdgcn_sched_barrier(0);
+          o[j % DT] = mfma_split(v[j & 1], p, o[j % DT]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      if (t + 1 < take) keep(st ^ 1);
+      there = there_next;
+    }
+    l += other_half(l);
+    rows.store<float>(a, seg, s, BM, 32 * wave + n, o, m, l);
+    if (tid == 0 && seg.bb == 0 && !seg.complete) {
+      split->slot = seg.slot, split->last = seg.last;
+      split->row0 = r0, split->rows = min(BM, s.q * G - r0), split->head = h, split->q0 = s.q0;
+    }
+    __syncthreads();  // the last tile is done with
+  }
+  zero_rows<NTH>(a, plan, BM, TK, batch);
+}
+
+template <int DP, int DC, int NW>
+hipError_t launch_split_as(const AttnArgs &a, int grid, hipStream_t s) {
+  const size_t lds = 2 * 6 * (size_t)32 * DP * 2 + batch_ints(a.S) * 4;
+  auto kernel = paged_attn_split_kernel<DP, DC, NW>;
+  if (lds > 64 * 1024) {
+    const hipError_t grown = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
+                                                 hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    if (grown != hipSuccess) return grown;
+  }
+  kernel<<<grid, 64 * NW, lds, s>>>(a);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_split(const AttnArgs &a, int grid, hipStream_t s) {
+  if (a.D <= 64) return launch_split_as<64, 64, 4>(a, grid, s);
+  if (a.D <= 96) return launch_split_as<128, 96, 8>(a, grid, s);
+  return launch_split_as<128, 128, 8>(a, grid, s);
+}
+
+}  // namespace zt

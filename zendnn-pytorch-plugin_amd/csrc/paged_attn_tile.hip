@@ -326,23 +326,22 @@ hipError_t launch_tiles_as(const AttnArgs &a, int grid, hipStream_t s) {
   return hipGetLastError();
 }
 
-template <typename T>
-hipError_t launch_tiles_t(const AttnArgs &a, int grid, hipStream_t s) {
-  if (a.D <= 64) return launch_tiles_as<T, 64, 64, 4>(a, grid, s);
-  if (a.D <= 96) return launch_tiles_as<T, 128, 96, 4>(a, grid, s);
-  if (a.D <= 128) return launch_tiles_as<T, 128, 128, 4>(a, grid, s);
-  return launch_tiles_as<T, 256, 256, 4>(a, grid, s);
-}
-
 }  // namespace
 
-// Past head_dim 128 a wave's queries and outputs need the registers of two.
-int tile_rows(const AttnArgs &) { return 128; }
-int tile_grid(const AttnArgs &a) { return a.D <= 128 ? 512 : 256; }
+// bf16: two workgroups of four waves a CU; past head_dim 128, where a wave's
+// queries and outputs need the registers of two, one.  fp32 up to head_dim 128
+// goes to the kernel of paged_attn_split.hip: two workgroups of four waves up to
+// 64, then one of eight.
+int tile_rows(const AttnArgs &a) { return a.dtype == ZT_DT_F32 && a.D > 64 && a.D <= 128 ? 256 : 128; }
+int tile_grid(const AttnArgs &a) { return a.D <= (a.dtype == ZT_DT_F32 ? 64 : 128) ? 512 : 256; }
 
 hipError_t launch_tiles(const AttnArgs &a, int grid, hipStream_t s) {
-  return a.dtype == ZT_DT_BF16 ? launch_tiles_t<uint16_t>(a, grid, s)
-                               : launch_tiles_t<float>(a, grid, s);
+  if (a.dtype == ZT_DT_F32)
+    return a.D <= 128 ? launch_split(a, grid, s) : launch_tiles_as<float, 256, 256, 4>(a, grid, s);
+  if (a.D <= 64) return launch_tiles_as<uint16_t, 64, 64, 4>(a, grid, s);
+  if (a.D <= 96) return launch_tiles_as<uint16_t, 128, 96, 4>(a, grid, s);
+  if (a.D <= 128) return launch_tiles_as<uint16_t, 128, 128, 4>(a, grid, s);
+  return launch_tiles_as<uint16_t, 256, 256, 4>(a, grid, s);
 }
 
 }  // namespace zt
