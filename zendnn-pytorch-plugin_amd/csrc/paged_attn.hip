@@ -24,6 +24,12 @@ namespace {
 
 constexpr int kRowThreads = 256;
 
+// Keys and values are read by one workgroup only: past the caches' replacement.
+__device__ __forceinline__ u32x4_t load_once(const char *p) {
+  return __builtin_nontemporal_load(reinterpret_cast<const u32x4_t *>(p));
+}
+
+
 __device__ __forceinline__ float max_over_groups(float x) {
   x = fmaxf(x, __shfl_xor(x, 16));
   return fmaxf(x, __shfl_xor(x, 32));
@@ -146,14 +152,14 @@ __global__ __launch_bounds__(kRowThreads, NT * DP <= 128 ? 2 : 1) void paged_att
 #pragma unroll
         for (int j = 0; j < KC; ++j) {
           const int p = 4 * j + g;
-          kreg[t][j] = *reinterpret_cast<const u32x4_t *>(p < C ? src + 16 * p : zero);
+          kreg[t][j] = load_once(p < C ? src + 16 * p : zero);
         }
       }
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         const int idx = 64 * j + lane, row = idx / CR, p = idx % CR;
         const uint32_t r = __shfl(vo, row);
-        vreg[j] = *reinterpret_cast<const u32x4_t *>(r != ~0u && p < C ? vbase + (uint64_t)r * 16 + 16 * p : zero);
+        vreg[j] = load_once(r != ~0u && p < C ? vbase + (uint64_t)r * 16 + 16 * p : zero);
       }
     };
     auto lookup = [&](int at) { return pages.lookup(a, at + (lane & (KS - 1))); };
