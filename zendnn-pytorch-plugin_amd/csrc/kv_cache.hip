@@ -20,7 +20,7 @@ struct Vec;
 template <>
 struct Vec<uint16_t, 8> {
   static __device__ __forceinline__ void load(const uint16_t *p, float (&f)[8]) {
-    const u32x4_t v = *reinterpret_cast<const u32x4_t *>(p);
+    const u32x4_t v = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t *>(p));
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       f[2 * i] = __uint_as_float(v[i] << 16);
@@ -37,7 +37,7 @@ struct Vec<uint16_t, 8> {
 template <>
 struct Vec<float, 4> {
   static __device__ __forceinline__ void load(const float *p, float (&f)[4]) {
-    const f32x4_t v = *reinterpret_cast<const f32x4_t *>(p);
+    const f32x4_t v = __builtin_nontemporal_load(reinterpret_cast<const f32x4_t *>(p));
 #pragma unroll
     for (int i = 0; i < 4; ++i) f[i] = v[i];
   }
@@ -485,7 +485,8 @@ __global__ __launch_bounds__(256) void copy_pages_kernel(CopyArgs a) {
   const U *from = reinterpret_cast<const U *>(cache + src * a.page_stride);
   U *to = reinterpret_cast<U *>(cache + dst * a.page_stride);
   const int64_t n = a.page_bytes / sizeof(U);
-  for (int64_t i = part * 256 + threadIdx.x; i < n; i += a.parts * 256) to[i] = from[i];
+  for (int64_t i = part * 256 + threadIdx.x; i < n; i += a.parts * 256)
+    __builtin_nontemporal_store(__builtin_nontemporal_load(from + i), to + i);
 }
 
 template <typename T, int V>
