@@ -485,8 +485,17 @@ __global__ __launch_bounds__(256) void copy_pages_kernel(CopyArgs a) {
   const U *from = reinterpret_cast<const U *>(cache + src * a.page_stride);
   U *to = reinterpret_cast<U *>(cache + dst * a.page_stride);
   const int64_t n = a.page_bytes / sizeof(U);
-  for (int64_t i = part * 256 + threadIdx.x; i < n; i += a.parts * 256)
-    __builtin_nontemporal_store(__builtin_nontemporal_load(from + i), to + i);
+  // four loads in flight before the first store, which may alias for all that
+  // the compiler knows
+  const int step = a.parts * 256;
+  for (int64_t i = part * 256 + threadIdx.x; i < n; i += 4 * step) {
+    U x[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[k] = __builtin_nontemporal_load(from + (i + k * step < n ? i + k * step : i));
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (i + k * step < n) __builtin_nontemporal_store(x[k], to + i + k * step);
+  }
 }
 
 template <typename T, int V>
