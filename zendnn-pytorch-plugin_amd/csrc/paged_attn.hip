@@ -323,8 +323,9 @@ __global__ __launch_bounds__(kRowThreads, NT * DP <= 128 ? 2 : 1) void paged_att
 // Joins the parts of the (item, head) that workgroup blockIdx.x of the first
 // launch began and others finished.  A thread takes four outputs of a row.
 template <typename T>
-__global__ __launch_bounds__(256) void paged_attn_join_kernel(AttnArgs a, int BM) {
+__global__ __launch_bounds__(256) void paged_attn_join_kernel(AttnArgs a) {
   const Split s = static_cast<const Split *>(a.splits)[blockIdx.x];
+  const int BM = a.item_rows;
   if (s.rows == 0) return;
   const float c = score_factor(a.scale);
   const int first = (int)blockIdx.x, last = (int)s.last;
@@ -375,6 +376,7 @@ hipError_t launch_rows(const AttnArgs &a, int grid, hipStream_t s) {
   constexpr int KS = sizeof(T) == 2 ? 32 : 16, VP = DP * (int)sizeof(T) + (sizeof(T) == 2 ? 32 : 16);
   constexpr int wave = std::max(KS * VP, 16 * (DP + 4) * 4);
   const size_t lds = 4 * wave + batch_ints(a.S) * 4;
+  if (a.item_rows != 16 * NT) return hipErrorInvalidValue;
   auto kernel = paged_attn_row_kernel<T, DP, NT>;
   if (lds > 64 * 1024) {
     const hipError_t grown = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
@@ -441,7 +443,7 @@ size_t paged_attn_workspace(const AttnArgs &a) {
 hipError_t launch_paged_attn(AttnArgs a, void *workspace, hipStream_t s) {
   const Shape p = shape_of(a);
   const size_t slots = 2 * (size_t)p.grid * p.bm;
-  a.group = a.H / a.KV;
+  a.group = a.H / a.KV, a.item_rows = p.bm;
   a.div_group = make_div(a.group), a.div_page = make_div(a.page_size);
   const int64_t per16 = a.dtype == ZT_DT_F32 ? 4 : 8;
   for (int i = 0; i < 2; ++i)
@@ -456,8 +458,8 @@ hipError_t launch_paged_attn(AttnArgs a, void *workspace, hipStream_t s) {
                               : launch_rows_n<float>(a, p.bm / 16, p.grid, s);
   if (e != hipSuccess) return e;
   const dim3 grid(p.grid, std::max(p.bm / 16, 1));
-  if (bf) paged_attn_join_kernel<uint16_t><<<grid, 256, 0, s>>>(a, p.bm);
-  else paged_attn_join_kernel<float><<<grid, 256, 0, s>>>(a, p.bm);
+  if (bf) paged_attn_join_kernel<uint16_t><<<grid, 256, 0, s>>>(a);
+  else paged_attn_join_kernel<float><<<grid, 256, 0, s>>>(a);
   return hipGetLastError();
 }
 

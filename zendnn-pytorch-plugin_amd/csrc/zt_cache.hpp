@@ -111,6 +111,7 @@ struct AttnArgs {
   void *out;  // [T, H, D]
   // set by launch_paged_attn
   int group;                    // H / KV
+  int item_rows;                // rows of an item, which the partial results are laid out by
   FastDiv div_group, div_page;
   uint32_t k_row[2], v_row[2];  // strides of page and token in units of 16 bytes
   float *part_ml, *part_o;      // partial results: [slots][BM][2], [slots][BM][D]
