@@ -29,7 +29,6 @@ __device__ __forceinline__ u32x4_t load_once(const char *p) {
   return __builtin_nontemporal_load(reinterpret_cast<const u32x4_t *>(p));
 }
 
-
 __device__ __forceinline__ float max_over_groups(float x) {
   x = fmaxf(x, __shfl_xor(x, 16));
   return fmaxf(x, __shfl_xor(x, 32));
@@ -320,51 +319,61 @@ __global__ __launch_bounds__(kRowThreads, NT * DP <= 128 ? 2 : 1) void paged_att
   zero_rows<kRowThreads>(a, plan, BM, UK, batch);
 }
 
+// One row's parts (running maximum, sum, four outputs), K loads at a time.
+template <int K>
+__device__ __forceinline__ f32x4_t join_parts(const AttnArgs &a, const Split &s, int first, int row, int d,
+                                              float c, float *sum) {
+  const int BM = a.item_rows, last = (int)s.last;
+  float m = -INFINITY, l = 0.f;
+  f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+  for (int w0 = first; w0 <= last; w0 += K) {
+    float mw[K], lw[K];
+    f32x4_t y[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int w = min(w0 + k, last);
+      const int64_t at = (w == first ? s.slot : 2 * (int64_t)w) * BM + row;
+      mw[k] = w0 + k <= last ? a.part_ml[2 * at] : -INFINITY;
+      lw[k] = a.part_ml[2 * at + 1];
+      y[k] = *reinterpret_cast<const f32x4_t *>(a.part_o + at * a.D + d);
+    }
+    float mm = m;
+#pragma unroll
+    for (int k = 0; k < K; ++k) mm = fmaxf(mm, mw[k]);
+    if (mm == -INFINITY) continue;
+    const float f0 = __builtin_amdgcn_exp2f(m * c - mm * c);
+    m = mm, l *= f0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] *= f0;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const float f = __builtin_amdgcn_exp2f(mw[k] * c - mm * c);
+      l += lw[k] * f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] += y[k][e] * f;
+    }
+  }
+  *sum = l;
+  return o;
+}
+
 // Joins the parts of the (item, head) that workgroup blockIdx.x of the first
 // launch began and others finished.  A thread takes four outputs of a row.
+// Most are cut once (two parts); a long axis with few rows in dozens.
 template <typename T>
 __global__ __launch_bounds__(256) void paged_attn_join_kernel(AttnArgs a) {
   const Split s = static_cast<const Split *>(a.splits)[blockIdx.x];
-  const int BM = a.item_rows;
   if (s.rows == 0) return;
   const float c = score_factor(a.scale);
-  const int first = (int)blockIdx.x, last = (int)s.last;
-  const int d4 = a.D / 4, G = a.group;
+  const int first = (int)blockIdx.x, d4 = a.D / 4, G = a.group;
+  const bool two = s.last - first < 2;
   for (int e = blockIdx.y * 256 + threadIdx.x; e < s.rows * d4; e += gridDim.y * 256) {
     const int row = e / d4, d = (e - row * d4) * 4;
-    float m = -INFINITY, l = 0.f;
-    f32x4_t o = {0.f, 0.f, 0.f, 0.f};
-    for (int w0 = first; w0 <= last; w0 += 8) {  // eight parts' loads at once
-      float mw[8], lw[8];
-      f32x4_t y[8];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int w = min(w0 + k, last);
-        const int64_t at = (w == first ? s.slot : 2 * (int64_t)w) * BM + row;
-        mw[k] = w0 + k <= last ? a.part_ml[2 * at] : -INFINITY;
-        lw[k] = a.part_ml[2 * at + 1];
-        y[k] = *reinterpret_cast<const f32x4_t *>(a.part_o + at * a.D + d);
-      }
-      float mm = m;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) mm = fmaxf(mm, mw[k]);
-      if (mm == -INFINITY) continue;
-      const float f0 = __builtin_amdgcn_exp2f(m * c - mm * c);
-      m = mm, l *= f0;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] *= f0;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const float f = __builtin_amdgcn_exp2f(mw[k] * c - mm * c);
-        l += lw[k] * f;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] += y[k][e] * f;
-      }
-    }
-    const float r = l > 0.f ? 1.f / l : 0.f;
+    float l;
+    const f32x4_t o = two ? join_parts<2>(a, s, first, row, d, c, &l) : join_parts<8>(a, s, first, row, d, c, &l);
     const int rr = s.row0 + row, tok = (int)fast_div(rr, a.div_group);
     const int64_t at = ((int64_t)(s.q0 + tok) * a.H + s.head * G + rr - tok * G) * a.D + d;
-    store_out<T>(a.out, at, o, r);
+    store_out<T>(a.out, at, o, l > 0.f ? 1.f / l : 0.f);
   }
 }
 
