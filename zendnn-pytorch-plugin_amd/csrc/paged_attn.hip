@@ -58,8 +58,12 @@ __device__ __forceinline__ float sum_over_groups(float x) {
 //
 // bf16 weights keep the digits that one bf16 drops in a second MFMA (p = hi +
 // lo): the matrix pipe is idle most of the time here.
+//
+// Measured (32 query and 8 cache heads of 128, bf16): two sequences of 131072
+// tokens 172-177 us, 6.2 TB/s; 64 ragged ones of up to 8192 129-133 us, 5.8
+// TB/s (a large copy reaches 4.9).  One of 777: 10.8 us, round trips to memory.
 template <typename T, int DP, int NT>
-__global__ __launch_bounds__(kRowThreads, NT * DP <= 128 ? 2 : 1) void paged_attn_row_kernel(AttnArgs a) {
+__global__ __launch_bounds__(kRowThreads, DP <= 128 ? 2 : 1) void paged_attn_row_kernel(AttnArgs a) {
   using Cost = RowCost;
   constexpr bool BF = sizeof(T) == 2;
   constexpr int ES = sizeof(T);
@@ -110,6 +114,10 @@ __global__ __launch_bounds__(kRowThreads, NT * DP <= 128 ? 2 : 1) void paged_att
       hi[t] = !live[t] ? INT32_MAX : a.causal ? pos + 1 : s.n;
       lo[t] = live[t] && a.causal && a.window ? (int)max((int64_t)pos + 1 - a.window, (int64_t)0) : 0;
     }
+    const int kend = (seg.b0 + seg.bb + take) * UK;
+    int k0 = (seg.b0 + seg.bb) * UK + wave * KS;
+    auto lookup = [&](int at) { return pages.lookup(a, at + (lane & (KS - 1))); };
+    int page = lookup(k0);  // on its way while the queries are fetched
     // ---- the queries, as B operands: lane (row n, g) holds piece 4 j + g
     u32x4_t q[NT][KC];
 #pragma unroll
@@ -133,8 +141,6 @@ __global__ __launch_bounds__(kRowThreads, NT * DP <= 128 ? 2 : 1) void paged_att
     }
     const char *kbase = static_cast<const char *>(a.k) + h * a.k_ld[1] * ES;
     const char *vbase = static_cast<const char *>(a.v) + h * a.v_ld[1] * ES;
-    const int kend = (seg.b0 + seg.bb + take) * UK;
-    int k0 = (seg.b0 + seg.bb) * UK + wave * KS;
 
     u32x4_t kreg[KT][KC], vreg[NV];
     uint64_t there;  // which of the strip's keys there are
@@ -161,8 +167,6 @@ __global__ __launch_bounds__(kRowThreads, NT * DP <= 128 ? 2 : 1) void paged_att
         vreg[j] = load_once(r != ~0u && p < C ? vbase + (uint64_t)r * 16 + 16 * p : zero);
       }
     };
-    auto lookup = [&](int at) { return pages.lookup(a, at + (lane & (KS - 1))); };
-    int page = lookup(k0);
     if (k0 < kend) load(k0, page);
     page = lookup(k0 + UK);
     for (; k0 < kend; k0 += UK) {
@@ -359,7 +363,8 @@ __device__ __forceinline__ f32x4_t join_parts(const AttnArgs &a, const Split &s,
 
 // Joins the parts of the (item, head) that workgroup blockIdx.x of the first
 // launch began and others finished.  A thread takes four outputs of a row.
-// Most are cut once (two parts); a long axis with few rows in dozens.
+// Most are cut once (two parts); a long axis with few rows in dozens.  Bound by
+// its round trips (2.4 us for seven parts of 32 rows) or by the parts' bytes.
 template <typename T>
 __global__ __launch_bounds__(256) void paged_attn_join_kernel(AttnArgs a) {
   const Split s = static_cast<const Split *>(a.splits)[blockIdx.x];
@@ -396,23 +401,29 @@ hipError_t launch_rows(const AttnArgs &a, int grid, hipStream_t s) {
   return hipGetLastError();
 }
 
-template <typename T, int NT>
-hipError_t launch_rows_d(const AttnArgs &a, int grid, hipStream_t s) {
-  if (a.D <= 64) return launch_rows<T, 64, NT>(a, grid, s);
-  if (a.D <= 128) return launch_rows<T, 128, NT>(a, grid, s);
-  return launch_rows<T, 256, NT>(a, grid, s);
+hipError_t launch_rows_of(const AttnArgs &a, int grid, hipStream_t s) {
+  if (a.dtype == ZT_DT_BF16) {
+    if (a.D <= 64) return launch_rows<uint16_t, 64, 1>(a, grid, s);
+    if (a.D <= 128) return launch_rows<uint16_t, 128, 1>(a, grid, s);
+    return launch_rows<uint16_t, 256, 1>(a, grid, s);
+  }
+  if (a.D > 128) return launch_rows<float, 256, 1>(a, grid, s);
+  if (a.item_rows == 16)
+    return a.D <= 64 ? launch_rows<float, 64, 1>(a, grid, s) : launch_rows<float, 128, 1>(a, grid, s);
+  return a.D <= 64 ? launch_rows<float, 64, 2>(a, grid, s) : launch_rows<float, 128, 2>(a, grid, s);
 }
 
-template <typename T>
-hipError_t launch_rows_n(const AttnArgs &a, int nt, int grid, hipStream_t s) {
-  if (nt == 1) return launch_rows_d<T, 1>(a, grid, s);
-  if (nt == 2) return launch_rows_d<T, 2>(a, grid, s);
-  return launch_rows_d<T, 4>(a, grid, s);
-}
-
-// Rows of one cache head from which on the tile kernel takes over: there each
-// key costs the row kernel's matrix operations more time than its bytes.
-constexpr int kRowsMost = 64;
+// Rows of one cache head up to which the row kernel is taken.  Measured, row
+// against tile kernel, 8 cache heads, 32 sequences of 2048 tokens, us:
+//   bf16  head_dim 64:  16 rows 34 / 33   32 rows 38 / 36    64 rows 78 / 38
+//         head_dim 128: 16 rows 57 / 56   32 rows 88 / 57    64 rows 121 / 64
+//         head_dim 256: 16 rows 126 / 111 32 rows 278 / 113
+//   fp32  head_dim 64:  16 rows 55 / 88   32 rows 76 / 88    64 rows 156 / 104
+//         head_dim 128: 16 rows 106 / 273 32 rows 166 / 273  64 rows 504 / 278
+//         head_dim 256: 16 rows 228 / 681 32 rows 837 / 681
+// On few long sequences (4 of 32768) the row kernel gains at 16 rows in bf16 too:
+// 99 against 111 us at head_dim 128.
+int rows_most(const AttnArgs &a) { return a.dtype == ZT_DT_F32 && a.D <= 128 ? 32 : 16; }
 
 struct Shape {
   bool tiles;
@@ -425,7 +436,7 @@ double blocks_most(const AttnArgs &a, bool tiles) {
 }
 Shape shape_of(const AttnArgs &a) {
   const int64_t rows = std::min(std::max<int64_t>(a.max_q, 1), a.T) * (a.H / a.KV);
-  Shape p{rows > kRowsMost, rows <= 16 ? 16 : rows <= 32 ? 32 : 64, kRowGrid};
+  Shape p{rows > rows_most(a), rows <= 16 ? 16 : 32, kRowGrid};
   if (p.tiles) p.bm = tile_rows(a), p.grid = tile_grid(a);
   // no more workgroups than there can be blocks
   const double most = items_most(a, p.bm) * a.KV * blocks_most(a, p.tiles);
@@ -462,9 +473,7 @@ hipError_t launch_paged_attn(AttnArgs a, void *workspace, hipStream_t s) {
   a.part_ml = reinterpret_cast<float *>(at), at += up256(slots * 2 * sizeof(float));
   a.part_o = reinterpret_cast<float *>(at);
   const bool bf = a.dtype == ZT_DT_BF16;
-  const hipError_t e = p.tiles ? launch_tiles(a, p.grid, s)
-                       : bf   ? launch_rows_n<uint16_t>(a, p.bm / 16, p.grid, s)
-                              : launch_rows_n<float>(a, p.bm / 16, p.grid, s);
+  const hipError_t e = p.tiles ? launch_tiles(a, p.grid, s) : launch_rows_of(a, p.grid, s);
   if (e != hipSuccess) return e;
   const dim3 grid(p.grid, std::max(p.bm / 16, 1));
   if (bf) paged_attn_join_kernel<uint16_t><<<grid, 256, 0, s>>>(a);

@@ -49,6 +49,10 @@ struct SplitCost {
 // term fp32 can hold.  Keys and values are split once per workgroup on their
 // way to LDS (global memory -> registers while a tile is worked on -> three
 // planes of the next stage), queries once per item, weights as they are made.
+//
+// Measured: eight whole sequences of up to 500 tokens, 16 heads of 64, 52-55 us
+// (fp32 MFMAs: 75); four of 600 to 2000 tokens, 16 heads on 4, head_dim 128 104
+// us (116), head_dim 80 66 us (85).  Past 128 three planes do not fit LDS twice.
 template <int DP, int DC, int NW>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2))) void paged_attn_split_kernel(
     AttnArgs a) {

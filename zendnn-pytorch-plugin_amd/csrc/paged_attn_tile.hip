@@ -63,6 +63,10 @@ struct TileCost {
 // bf16 weights are rounded once for the second product (half a step each, 2^-8,
 // and independent, so the sum of n of them is off by much less); their sum is
 // taken of the rounded ones, so that a row's weights still add up to one.
+//
+// Measured (32 query and 8 cache heads of 128, bf16): 2048 tokens behind 6144
+// 265-276 us, 0.9 PFLOP/s (a large product of the library reaches 1.2 on the
+// same card); the matrix operations with their LDS reads alone 163.
 template <typename T, int DP, int DC, int NW>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP <= 128 ? 2 : 1, DP <= 128 ? 2 : 1))) void paged_attn_tile_kernel(AttnArgs a) {
   using Cost = TileCost<T>;
