@@ -147,9 +147,9 @@ __device__ __forceinline__ int seq_of_item(const int *tile_base, int S, int x) {
   return lo;
 }
 
-// The cost of a block of an item of `rows` rows.
+// The cost of a block of an item of `rows` rows, and the least span.
 struct RowCost {  // every row kernel's unit is the same bytes
-  static constexpr int kLead = 1, kMost = 1;
+  static constexpr int kLead = 1, kMost = 1, kLeast = 1;
   static __device__ __forceinline__ int of(int) { return 1; }
 };
 
@@ -211,8 +211,10 @@ __device__ __forceinline__ Plan make_plan(const AttnArgs &a, int BM, int UK, con
     }
   }
   const int64_t all = (int64_t)sum * a.KV;
-  // no span without the start of a block inside a long item
-  p.per = max(quotient(all + gridDim.x - 1, gridDim.x), (int64_t)Cost::kMost);
+  // kLeast is no shorter than a block, so that every span inside a long item
+  // has the start of one
+  static_assert(Cost::kLeast >= Cost::kMost, "a span may hold no block");
+  p.per = max(quotient(all + gridDim.x - 1, gridDim.x), (int64_t)Cost::kLeast);
   p.from = p.per * p.wg, p.to = min(p.from + p.per, all);
   if (p.from >= p.to) {  // nothing is left: an empty span at the line's start
     p.from = p.to = 0;

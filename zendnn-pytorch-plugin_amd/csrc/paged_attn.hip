@@ -475,7 +475,7 @@ hipError_t launch_paged_attn(AttnArgs a, void *workspace, hipStream_t s) {
   const bool bf = a.dtype == ZT_DT_BF16;
   const hipError_t e = p.tiles ? launch_tiles(a, p.grid, s) : launch_rows_of(a, p.grid, s);
   if (e != hipSuccess) return e;
-  const dim3 grid(p.grid, std::max(p.bm / 16, 1));
+  const dim3 grid(p.grid, std::max(p.bm * a.D / 1024, 1));  // a thread per four outputs
   if (bf) paged_attn_join_kernel<uint16_t><<<grid, 256, 0, s>>>(a);
   else paged_attn_join_kernel<float><<<grid, 256, 0, s>>>(a);
   return hipGetLastError();

@@ -37,7 +37,7 @@ __device__ __forceinline__ f32x16_t mfma_split(const u32x4_t (&x)[3], const u32x
 // A block takes nearly the same time whatever rows are live, and an item's two
 // ends about one block's.
 struct SplitCost {
-  static constexpr int kLead = 2, kMost = 2;
+  static constexpr int kLead = 2, kMost = 2, kLeast = kMost;
   static __device__ __forceinline__ int of(int) { return 2; }
 };
 

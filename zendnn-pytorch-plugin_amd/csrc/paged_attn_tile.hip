@@ -28,10 +28,12 @@ __device__ __forceinline__ void wait_and_meet() {
 // takes nearly as long as a full one: in bf16 it waits for its keys (1.9 against
 // 2.2 us, two workgroups a CU), in fp32 for its one wave's share of the matrix
 // operations (4.6 us), which the other workgroup's wave on that SIMD halves.
-// An item's two ends take 5 to 6 us.
+// An item's two ends take 5 to 6 us.  In bf16 spans have four blocks at least:
+// what a part of 128 rows has to write and the join to read is four blocks'
+// bytes (32 tokens of 32 heads behind 2048: 40 us without, 35 with).
 template <typename T>
 struct TileCost {
-  static constexpr int kLead = sizeof(T) == 2 ? 15 : 7, kMost = 6;
+  static constexpr int kLead = sizeof(T) == 2 ? 15 : 7, kMost = 6, kLeast = sizeof(T) == 2 ? 4 * kMost : kMost;
   static __device__ __forceinline__ int of(int rows) {
     return sizeof(T) == 2 ? 4 + (rows + 63) / 64 : 6;
   }
