@@ -411,10 +411,10 @@ int zt_rotary_cache_append(const void *q, int64_t T, int64_t H, const int64_t *q
  * only the last `window` of them (0: all).  Otherwise it sees all
  * context_lens[i].  Keys in pages outside the cache are not seen, and a row
  * that sees no key is zero, as is a row past cu_seqlens[S].
- * Scores, softmax and sums are fp32.  What no token of a chunk sees (unused
- * places, pages outside the cache, keys behind every window) may hold anything;
- * an infinity or a NaN among the values of a chunk's own later tokens may reach
- * its earlier ones, as weights of zero.
+ * Scores, softmax and sums are fp32.  What a row does not see may hold anything,
+ * infinities and NaN among it.  A row that sees a value that is not finite is
+ * not finite there, or, where the rows of a tile see different keys, NaN as a
+ * whole.
  *
  *  q          [T, H, head_dim] in the cache's type, strides in elements; all
  *             rows (q, cache, out) start on 16 bytes

@@ -173,6 +173,34 @@ def test_attn_bad_pages(q, dtype):
     check(b, causal=False)
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("q,window", [(4, 0), (4, 3), (7, 0), (40, 0), (40, 9), (200, 0), (200, 70)])
+def test_attn_values_that_are_not_finite(q, window, D, dtype):
+    """Keys and values of some of the chunk's own tokens are NaN or infinite:
+    the rows that see none of them keep every bit, the others show it."""
+    lens = [(q, 300), (min(q, 9), 9)]
+    clean, b = (make(lens, 8, 2, D, 16, dtype, seed=D) for _ in "ab")
+    want = check(clean, window=window)
+    bad = {299, 300 - q // 2, 300 - q + 1}
+
+    def put(cache, value, tokens):
+        for p in tokens:
+            cache[b["table"][0, p // 16], :, p % 16] = value
+
+    put(b["v"], math.inf, {299})
+    put(b["v"], math.nan, bad - {299})
+    put(b["k"], math.nan, {299})
+    out = call(b, window=window)
+    pos = torch.arange(300 - q, 300, device=DEV)
+    sees = torch.zeros(q, dtype=torch.bool, device=DEV)
+    for p in bad:
+        sees |= (pos >= p) & ((pos - p < window) if window else True)
+    assert sees.any() and not sees.all()
+    assert torch.equal(out[:q][~sees], want[:q][~sees]) and torch.equal(out[q:], want[q:])
+    assert not torch.isfinite(out[:q][sees]).any()
+
+
 def test_attn_no_pool():
     b = make([(1, 0), (3, 0)], 8, 2, 64, 16, BF, spare=0)
     assert b["k"].size(0) == 0

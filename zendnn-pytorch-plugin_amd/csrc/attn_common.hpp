@@ -54,6 +54,19 @@ __device__ __forceinline__ void store_out(void *out, int64_t at, f32x4_t o, floa
   }
 }
 
+// Whether any of the 16 bytes' numbers is an infinity or a NaN.
+template <typename T>
+__device__ __forceinline__ bool not_finite(u32x4_t x) {
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if constexpr (sizeof(T) == 2)
+      bad |= (x[i] & 0x7f800000u) == 0x7f800000u || (x[i] & 0x7f80u) == 0x7f80u;
+    else
+      bad |= (x[i] & 0x7f800000u) == 0x7f800000u;
+  return bad;
+}
+
 // 1 KB of zeros: what a lane reads in place of a key or value that is not
 // there, so that weights of zero never meet a NaN or an infinity.
 static __device__ const u32x4_t kZeroRow[64] = {};
@@ -303,6 +316,23 @@ __device__ __forceinline__ uint32_t row_offset(const AttnArgs &a, const uint32_t
   return (uint32_t)page * ld[0] + off * ld[1];
 }
 
+// A weight of zero times an infinity or a NaN is a NaN, so where the rows of an
+// item see different keys of a block (an edge of what they see), values that are
+// not finite are taken out of it, and the rows that do see such a key become
+// NaN as a whole.  Whether the item's rows differ, and the keys they all see:
+struct Shared {
+  bool differ;
+  int from, to;
+  __device__ __forceinline__ Shared(const AttnArgs &a, const Seq &s, int tile, int BM) {
+    const int a0 = (int)fast_div((uint32_t)tile * BM, a.div_group);
+    const int a1 = min((int)fast_div((uint32_t)tile * BM + BM - 1, a.div_group), s.q - 1);
+    differ = a.causal && a1 > a0;
+    to = s.n - s.q + a0 + 1;
+    from = a.window ? (int)max((int64_t)s.n - s.q + a1 + 1 - a.window, (int64_t)0) : 0;
+  }
+  __device__ __forceinline__ bool edge(int k0, int n) const { return differ && (k0 + n > to || k0 < from); }
+};
+
 // What a workgroup leaves about the (item, head) that it began and did not
 // finish (rows = 0: none): the partial results are in slots `slot` and 2 * w for
 // each workgroup w after it up to `last`.
@@ -365,6 +395,12 @@ struct Rows32 {
   }
   __device__ __forceinline__ bool see(int k0, int n) const { return any && k0 < hi_max && k0 + n > lo_min; }
   __device__ __forceinline__ bool see_all(int k0, int n) const { return k0 + n <= hi_min && k0 >= lo_max; }
+  // whether the row sees a key of `bad`, bit i being key k0 + i
+  __device__ __forceinline__ bool sees_of(uint64_t bad, int k0) const {
+    const int from = min(max(lo - k0, 0), 64), to = min(max(hi - k0, 0), 64);
+    const uint64_t below = from >= 64 ? ~0ull : (1ull << from) - 1, up = to >= 64 ? ~0ull : (1ull << to) - 1;
+    return live && (bad & up & ~below) != 0;
+  }
   // scores of keys k0 .. k0 + 31 that the row does not see, or that are not there
   __device__ __forceinline__ void mask(f32x16_t &sc, int k0, uint32_t there) const {
     const int from = min(max(lo - k0, 0), 32), to = min(max(hi - k0, 0), 32);

@@ -101,6 +101,7 @@ __global__ __launch_bounds__(kRowThreads, DP <= 128 ? 2 : 1) void paged_attn_row
     const Seq s = batch.uniform(seg.seq);
     const int r0 = seg.tile * BM;
     const KeyRange kr = seg.keys;
+    const Shared shared(a, s, seg.tile, BM);
     const Pages pages{a.table + (int64_t)seg.seq * a.W, kr.begin, kr.end};
     // the lane's rows: token, head, and the keys each sees
     int row_t[NT], lo[NT], hi[NT];
@@ -133,9 +134,10 @@ __global__ __launch_bounds__(kRowThreads, DP <= 128 ? 2 : 1) void paged_attn_row
     }
     f32x4_t o[NT][DT];
     float m[NT], l[NT];
+    bool poisoned[NT];  // the row sees a value that is not finite at an edge
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      m[t] = -INFINITY, l[t] = 0.f;
+      m[t] = -INFINITY, l[t] = 0.f, poisoned[t] = false;
 #pragma unroll
       for (int d = 0; d < DT; ++d) o[t][d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     }
@@ -170,6 +172,15 @@ __global__ __launch_bounds__(kRowThreads, DP <= 128 ? 2 : 1) void paged_attn_row
     if (k0 < kend) load(k0, page);
     page = lookup(k0 + UK);
     for (; k0 < kend; k0 += UK) {
+      uint32_t bad = 0;  // keys whose values are not finite, at an edge
+      if (shared.edge(k0, KS))
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+          const bool is = not_finite<T>(vreg[j]);
+          if (is) vreg[j] = u32x4_t{0, 0, 0, 0};
+          for (uint64_t left = __ballot(is); left; left &= left - 1)
+            bad |= 1u << ((64 * j + __builtin_ctzll(left)) / CR);
+        }
       // values to the wave's LDS (LDS operations of a wave keep their order)
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
@@ -208,6 +219,11 @@ __global__ __launch_bounds__(kRowThreads, DP <= 128 ? 2 : 1) void paged_attn_row
       float pf[NT][4];
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
+        if (bad) {
+          const int from = min(max(lo[t] - k0, 0), 32), to = min(max(hi[t] - k0, 0), 32);
+          const uint64_t range = (1ull << to) - (1ull << min(from, to));
+          poisoned[t] = poisoned[t] || (live[t] && ((uint32_t)range & bad));
+        }
         if (!whole || __ballot(lo[t] > k0 || hi[t] < k0 + KS)) {
           // bit 16 u + e of `seen`: the lane's e-th key of 16
           const int from = min(max(lo[t] - k0, 0), 32), to = min(max(hi[t] - k0, 0), 32);
@@ -282,6 +298,10 @@ __global__ __launch_bounds__(kRowThreads, DP <= 128 ? 2 : 1) void paged_attn_row
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       const float lsum = sum_over_groups(l[t]);
+      if (poisoned[t])
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+          o[t][d] = f32x4_t{NAN, NAN, NAN, NAN};
       __syncthreads();  // the waves' values and the previous rows are read
       if (lane < 16) sm_m[wave][n] = m[t], sm_l[wave][n] = lsum;
 #pragma unroll

@@ -64,6 +64,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
   static_assert(NL >= 1 && TK * PR % NTH == 0, "the threads share a tile's pieces evenly");
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   __shared__ PlanShared sh;
+  __shared__ uint32_t sm_bad[3];  // keys with values that are not finite, of three tiles in turn
   const Batch batch(smem + 2 * STAGE, a.S);
 
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, half = lane >> 5;
@@ -86,6 +87,11 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
     const Seq s = batch.uniform(seg.seq);
     const int r0 = seg.tile * BM, k_first = (seg.b0 + seg.bb) * TK;
     const Pages pages{a.table + (int64_t)seg.seq * a.W, seg.keys.begin, seg.keys.end};
+    const Shared shared(a, s, seg.tile, BM);
+    if (shared.differ) {
+      if (tid < 3) sm_bad[tid] = 0;
+      __syncthreads();
+    }
     const char *kbase = static_cast<const char *>(a.k) + h * a.k_ld[1] * 4;
     const char *vbase = static_cast<const char *>(a.v) + h * a.v_ld[1] * 4;
 
@@ -114,10 +120,15 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
 #pragma unroll
       for (int p = 0; p < 3; ++p) *reinterpret_cast<u32x2_t *>(to + p * PLANE) = u32x2_t{lo.p[p], hi.p[p]};
     };
-    auto keep = [&](int st) {
+    auto keep = [&](int st, int k0, uint32_t *bad) {
+      const bool edge = shared.edge(k0, TK);
 #pragma unroll
       for (int j = 0; j < NL; ++j) {
         const int idx = j * NTH + tid, row = idx / PR, piece = idx % PR;
+        if (edge && not_finite<float>(vreg[j])) {
+          vreg[j] = u32x4_t{0, 0, 0, 0};
+          atomicOr(bad, 1u << row);
+        }
         put(smem + st * STAGE, kswz(row), row, piece, kreg[j]);
         put(smem + st * STAGE + 3 * PLANE, vswz(row), row, piece, vreg[j]);
       }
@@ -150,8 +161,10 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
 #pragma unroll
       for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
     float m = -INFINITY, l = 0.f;
+    bool poisoned = false;  // the row sees a value that is not finite at an edge
 
-    keep(0);
+    keep(0, k_first, sm_bad);
+    int turn = 0;  // t % 3
     for (int t = 0; t < take; ++t) {
       const int k0 = k_first + t * TK, st = t & 1;
       // every wave's part of the tile is in LDS, and the previous tile is done with
@@ -160,6 +173,11 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
       if (t + 1 < take) {
         there_next = fetch(k0 + TK, page);
         page = lookup(k0 + 2 * TK);
+      }
+      const int turn1 = turn == 2 ? 0 : turn + 1;
+      if (shared.differ) {
+        if (tid == 0) sm_bad[3 - turn - turn1] = 0;  // the tile after next's
+        poisoned |= rows.sees_of(sm_bad[turn] & there, k0);
       }
       if (rows.see(k0, TK)) {
         const unsigned char *kt = smem + st * STAGE, *vt = kt + 3 * PLANE;
@@ -234,10 +252,16 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
           __builtin_amdgcn_sched_barrier(0);
         }
       }
-      if (t + 1 < take) keep(st ^ 1);
+      if (t + 1 < take) keep(st ^ 1, k0 + TK, sm_bad + turn1);
       there = there_next;
+      turn = turn1;
     }
     l += other_half(l);
+    if (poisoned)
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[d][e] = __uint_as_float(0x7fc00000u);
     rows.store<float>(a, seg, s, BM, 32 * wave + n, o, m, l);
     if (tid == 0 && seg.bb == 0 && !seg.complete) {
       split->slot = seg.slot, split->last = seg.last;

@@ -83,6 +83,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP <= 1
   constexpr int DT = DC / 32;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   __shared__ PlanShared sh;
+  __shared__ uint32_t sm_bad[NW];
   const Batch batch(smem + 4 * STAGE, a.S);
 
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, half = lane >> 5;
@@ -116,6 +117,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP <= 1
     const Seq s = batch.uniform(seg.seq);
     const int r0 = seg.tile * BM;
     const KeyRange kr = seg.keys;
+    const Shared shared(a, s, seg.tile, BM);
     const Pages pages{a.table + (int64_t)seg.seq * a.W, kr.begin, kr.end};
     const char *kbase = static_cast<const char *>(a.k) + h * a.k_ld[1] * ES;
     const char *vbase = static_cast<const char *>(a.v) + h * a.v_ld[1] * ES;
@@ -170,12 +172,31 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP <= 1
 #pragma unroll
       for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
     float m = -INFINITY, l = 0.f;
+    bool poisoned = false;  // the row sees a value that is not finite at an edge
 
     for (int t = 0; t < take; ++t) {
       const int k0 = k_first + t * TK, st = t & 1;
       wait_and_meet();  // the tile is there, and the previous one is done with
       const uint64_t there_next = offsets(k0 + TK, page, t + 1 < take);
       page = lookup(k0 + 2 * TK);
+      if (shared.edge(k0, TK)) {  // the waves look over TK / NW values each
+        constexpr int ROWS = TK / NW, LANES = 64 / ROWS;
+        unsigned char *at = smem + st * 2 * STAGE + STAGE + (wave * ROWS + lane / LANES) * RB;
+        bool bad = false;
+#pragma unroll
+        for (int j = 0; j < CR / LANES; ++j) {
+          u32x4_t *x = reinterpret_cast<u32x4_t *>(at + 16 * (j * LANES + lane % LANES));
+          if (not_finite<T>(*x)) bad = true, *x = u32x4_t{0, 0, 0, 0};
+        }
+        uint32_t found = 0;
+        for (uint64_t left = __ballot(bad); left; left &= left - 1) found |= 1u << (__builtin_ctzll(left) / LANES);
+        if (lane == 0) sm_bad[wave] = found;
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        uint64_t all = 0;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) all |= (uint64_t)sm_bad[w] << (ROWS * w);
+        poisoned |= rows.sees_of(all & there, k0);
+      }
       if (rows.see(k0, TK)) {
         const unsigned char *kt = smem + st * 2 * STAGE, *vt = kt + STAGE;
         // ---- scores.  Keys are read kAhead operands before their use; the
@@ -316,6 +337,11 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP <= 1
     // workgroup, takes their place
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     l += other_half(l);
+    if (poisoned)
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[d][e] = __uint_as_float(0x7fc00000u);
     rows.store<T>(a, seg, s, BM, 32 * wave + n, o, m, l);
     if (tid == 0 && seg.bb == 0 && !seg.complete) {
       split->slot = seg.slot, split->last = seg.last;
