@@ -192,7 +192,8 @@ __device__ __forceinline__ int block_scan(int v, int *part, int *total) {
 //    needs' running sums, and writes the page's table entry, count and slots.
 // So no workgroup waits for another.  Bound by round trips to memory: what the
 // steps share (lengths, needs) is read once, into LDS, and the counts four to a
-// load (64 sequences of up to 8192 tokens in pages of 16: 6.7 us; 15 with each length read where it is used).
+// load (64 sequences of up to 8192 tokens in pages of 16: 6.7 us; 15 with
+// lengths, counts and table entries read one by one from memory).
 __global__ __launch_bounds__(kBlock) void cache_extend_kernel(ExtendArgs a) {
   extern __shared__ int sm[];  // end[S], ctx[S], cu[S + 1]
   __shared__ int part[kWaves], part2[kWaves];
@@ -328,7 +329,7 @@ __global__ __launch_bounds__(kBlock) void cache_extend_kernel(ExtendArgs a) {
 // counts, and the tables are small (64 rows of 128 pages: 33 KB each way).
 // Bound by round trips to memory, so lengths and parents are kept in LDS and a
 // thread takes kEach table entries at once, their loads before their uses (64
-// rows of 128 pages: 13.8 us; 23.5 one entry at a time).
+// rows of 128 pages: 13.6 us; 23.5 one entry at a time).
 __global__ __launch_bounds__(kBlock) void cache_fork_kernel(ForkArgs a) {
   constexpr int kEach = 8;
   extern __shared__ int sm[];

@@ -50,7 +50,7 @@ struct SplitCost {
 // way to LDS (global memory -> registers while a tile is worked on -> three
 // planes of the next stage), queries once per item, weights as they are made.
 //
-// Measured: eight whole sequences of up to 500 tokens, 16 heads of 64, 54 us
+// Measured: eight whole sequences of up to 500 tokens, 16 heads of 64, 53-55 us
 // (fp32 MFMAs: 75); four of 600 to 2000 tokens, 16 heads on 4, head_dim 128 104
 // us (116), head_dim 80 66 us (85).  Past 128 three planes do not fit LDS twice.
 template <int DP, int DC, int NW>

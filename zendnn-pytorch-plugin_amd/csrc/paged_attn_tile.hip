@@ -67,7 +67,7 @@ struct TileCost {
 // taken of the rounded ones, so that a row's weights still add up to one.
 //
 // Measured (32 query and 8 cache heads of 128, bf16): 2048 tokens behind 6144
-// 262-276 us, 0.9 PFLOP/s (a large product of the library reaches 1.2 on the
+// 266-277 us, 0.9 PFLOP/s (a large product of the library reaches 1.2 on the
 // same card); the matrix operations with their LDS reads alone 163.
 template <typename T, int DP, int DC, int NW>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP <= 128 ? 2 : 1, DP <= 128 ? 2 : 1))) void paged_attn_tile_kernel(AttnArgs a) {
