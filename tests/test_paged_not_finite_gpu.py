@@ -1,0 +1,71 @@
+"""Attention over the paged cache where queries and keys are NaN, in whole items
+and in ones whose keys several workgroups share."""
+import math
+
+import pytest
+import torch
+
+from test_kv_cache_gpu import BF, F32, call, check, make
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def _announce(request):
+    print(f"\n[case] {request.node.name}", flush=True)
+
+
+# (new, all) tokens: few long sequences, whose keys are shared out over dozens
+# of workgroups, and many short ones
+LONG = {1: [(1, 20011), (1, 9973)], 4: [(4, 6007)], 40: [(40, 9973), (1, 70)], 150: [(150, 6007), (150, 700)]}
+KINDS = [(1, False), (1, True), (4, True), (40, False), (40, True), (150, True)]
+
+
+def lens_of(q, long):
+    return LONG[q] if long else [(q, 60 + i % 7) for i in range(90)]
+
+
+def put(cache, b, seq, tokens, value, column=slice(None)):
+    page = cache.size(2)
+    for t in tokens:
+        cache[b["table"][seq, t // page], :, t % page, column] = value
+
+
+def same_but(out, want, rows):
+    """Every row but those of the mask `rows` has the bits of `want`."""
+    return torch.equal(out[~rows], want[~rows])
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("q,long", KINDS)
+def test_nan_query(q, long, D, dtype):
+    """One NaN in a query head: its row is NaN and no other changes."""
+    b = make(lens_of(q, long), 8, 2, D, 64, dtype, seed=q)
+    want = check(b) if q * D < 10000 else call(b)
+    hit = torch.zeros(want.shape[:2], dtype=torch.bool, device=want.device)
+    for t, h in ((0, 3), (want.size(0) - 1, 6)):
+        b["q"][t, h, D // 2] = math.nan
+        hit[t, h] = True
+    out = call(b)
+    assert out[hit].isnan().all()
+    assert same_but(out, want, hit)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("q,long", KINDS)
+@pytest.mark.parametrize("share", ["all", "half"])
+def test_nan_keys(share, q, long, D, dtype):
+    """All keys of the first sequence are NaN, or those of its first half: its
+    rows are NaN, the other sequences' keep every bit."""
+    lens = lens_of(q, long)
+    b = make(lens, 8, 2, D, 64, dtype, seed=q + 1)
+    want = call(b)
+    n = lens[0][1] if share == "all" else lens[0][1] // 2
+    put(b["k"], b, 0, range(n), math.nan)
+    out = call(b)
+    hit = torch.zeros(want.size(0), dtype=torch.bool, device=want.device)
+    hit[:q] = True
+    assert out[:q].isnan().all()
+    assert same_but(out, want, hit)

@@ -343,11 +343,18 @@ __global__ __launch_bounds__(kRowThreads, DP <= 128 ? 2 : 1) void paged_attn_row
   zero_rows<kRowThreads>(a, plan, BM, UK, batch);
 }
 
-// One row's parts (running maximum, sum, four outputs), K loads at a time.
+// One row's parts (running maximum, sum, four outputs), K loads at a time.  A
+// part whose maximum is -inf saw no key, and is all zeros, or only keys whose
+// scores are NaN, and its sums are: it joins parts like it as it is, so that the
+// NaN shows however the keys were cut.
 template <int K>
 __device__ __forceinline__ f32x4_t join_parts(const AttnArgs &a, const Split &s, int first, int row, int d,
                                               float c, float *sum) {
   const int BM = a.item_rows, last = (int)s.last;
+  // from one maximum to another; equal ones, two of -inf among them, change nothing
+  auto factor = [&](float from, float to) {
+    return from == to ? 1.f : __builtin_amdgcn_exp2f(from * c - to * c);
+  };
   float m = -INFINITY, l = 0.f;
   f32x4_t o = {0.f, 0.f, 0.f, 0.f};
   for (int w0 = first; w0 <= last; w0 += K) {
@@ -357,21 +364,23 @@ __device__ __forceinline__ f32x4_t join_parts(const AttnArgs &a, const Split &s,
     for (int k = 0; k < K; ++k) {
       const int w = min(w0 + k, last);
       const int64_t at = (w == first ? s.slot : 2 * (int64_t)w) * BM + row;
-      mw[k] = w0 + k <= last ? a.part_ml[2 * at] : -INFINITY;
+      mw[k] = a.part_ml[2 * at];
       lw[k] = a.part_ml[2 * at + 1];
       y[k] = *reinterpret_cast<const f32x4_t *>(a.part_o + at * a.D + d);
     }
+#pragma unroll
+    for (int k = 1; k < K; ++k)
+      if (w0 + k > last) mw[k] = -INFINITY, lw[k] = 0.f, y[k] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     float mm = m;
 #pragma unroll
     for (int k = 0; k < K; ++k) mm = fmaxf(mm, mw[k]);
-    if (mm == -INFINITY) continue;
-    const float f0 = __builtin_amdgcn_exp2f(m * c - mm * c);
+    const float f0 = factor(m, mm);
     m = mm, l *= f0;
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] *= f0;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const float f = __builtin_amdgcn_exp2f(mw[k] * c - mm * c);
+      const float f = factor(mw[k], mm);
       l += lw[k] * f;
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[e] += y[k][e] * f;
