@@ -1,5 +1,5 @@
-"""Attention over the paged cache where queries and keys are NaN, in whole items
-and in ones whose keys several workgroups share."""
+"""Attention over the paged cache where queries and keys are not finite, in whole
+items and in ones whose keys several workgroups share."""
 import math
 
 import pytest
@@ -69,3 +69,36 @@ def test_nan_keys(share, q, long, D, dtype):
     hit[:q] = True
     assert out[:q].isnan().all()
     assert same_but(out, want, hit)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("q,long", KINDS)
+def test_rows_do_not_feel_each_other(q, long, D, dtype):
+    """A row of far larger scores changes no bit of the rows beside it."""
+    b = make(lens_of(q, long), 8, 2, D, 64, dtype, seed=q)
+    want = call(b)
+    hit = torch.zeros(want.shape[:2], dtype=torch.bool, device=want.device)
+    for t, h in ((0, 3), (want.size(0) - 1, 6)):
+        b["q"][t, h] *= 64
+        hit[t, h] = True
+    out = call(b)
+    assert same_but(out, want, hit) and not torch.equal(out, want)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("q", [4, 12, 40, 200])
+def test_keys_of_infinity(q, D, dtype):
+    """A key whose score is +inf makes the rows that see it NaN."""
+    lens = [(q, 300), (min(q, 9), 9)]
+    b = make(lens, 8, 2, D, 16, dtype, seed=D + 2)
+    b["q"][..., 5] = b["q"][..., 5].abs() + 0.25
+    want = check(b)
+    first = 300 - q // 2
+    put(b["k"], b, 0, [first], math.inf, 5)
+    sees = torch.zeros(want.size(0), dtype=torch.bool, device=want.device)
+    sees[first - 300 + q:q] = True
+    out = call(b)
+    assert out[sees].isnan().all()
+    assert same_but(out, want, sees)

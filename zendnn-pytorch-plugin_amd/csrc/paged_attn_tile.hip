@@ -246,15 +246,16 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP <= 1
 #pragma unroll
           for (int e = 0; e < 16; ++e) mx = fmaxf(mx, sc[u][e]);
         mx = fmaxf(mx, other_half(mx));
-        if (__ballot(mx != -INFINITY && (mx - m) * c > 8.f)) {
-          const float to = fmaxf(m, mx);
-          const float f = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m * c - to * c);
+        // in the rows that grew only, so that no row's bits depend on another's
+        const bool grown = mx != -INFINITY && (mx - m) * c > 8.f;
+        if (__ballot(grown)) {
+          const float f = grown ? __builtin_amdgcn_exp2f(m * c - mx * c) : 1.f;
           l *= f;
 #pragma unroll
           for (int d = 0; d < DT; ++d)
 #pragma unroll
             for (int e = 0; e < 16; ++e) o[d][e] *= f;
-          m = to;
+          m = grown ? mx : m;
         }
         const float mc = m == -INFINITY ? 0.f : m * c;
         // ---- O^T += V^T P^T, a step of keys at a time (16, or one of each half
