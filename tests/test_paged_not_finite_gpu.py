@@ -102,3 +102,21 @@ def test_keys_of_infinity(q, D, dtype):
     out = call(b)
     assert out[sees].isnan().all()
     assert same_but(out, want, sees)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("D", [64, 80, 128, 256])
+@pytest.mark.parametrize("q", [4, 12, 40, 200])
+def test_largest_values_unseen(q, D, dtype):
+    """The type's largest and lowest finite numbers as values of tokens at the
+    chunk's end change no bit of the rows that do not see them."""
+    lens = [(q, 300), (min(q, 9), 9)]
+    clean, b = (make(lens, 8, 2, D, 16, dtype, seed=D) for _ in "ab")
+    want = check(clean)
+    top = torch.finfo(dtype).max
+    first = 300 - q // 2
+    put(b["v"], b, 0, range(first, 300), top, slice(0, D, 2))
+    put(b["v"], b, 0, range(first, 300), -top, slice(1, D, 2))
+    sees = torch.zeros(want.size(0), dtype=torch.bool, device=want.device)
+    sees[first - 300 + q:q] = True
+    assert same_but(call(b), want, sees)

@@ -1,6 +1,8 @@
 // Attention of a chunk of new tokens over a paged cache, for gfx950: many rows
 // per cache head in fp32, head_dim up to 128, on bf16 MFMAs.  The definitions are in
 // paged_attn.hip.
+#include <type_traits>
+
 #include "attn_common.hpp"
 
 namespace zt {
@@ -21,6 +23,35 @@ __device__ __forceinline__ Parts split2(float a, float b) {
   a -= __uint_as_float(s.p[1] << 16), b -= __uint_as_float(s.p[1] & 0xffff0000u);
   s.p[2] = pack_bf16x2(a, b);
   return s;
+}
+
+// The nearest bf16 to a number past bf16's largest is infinite, so those, and
+// numbers that are not finite, are split apart from the others: x1 is x cut
+// short, and an infinity or a NaN goes whole into x1.  mark_past gives them bits
+// of kPast, which it leaves 0 for other pairs.
+constexpr uint32_t kPast = 0x80008000u;
+__device__ __forceinline__ uint32_t mark_past(uint32_t first) { return (first & 0x7f807f80u) + 0x00800080u; }
+__device__ __forceinline__ Parts split2_any(float a, float b) {
+  auto lead = [](float x) -> uint32_t {
+    const uint32_t near = f32_to_bf16_bits(x);
+    return x != x ? 0x7fc0u : (near & 0x7f80u) == 0x7f80u ? __float_as_uint(x) >> 16 : near;
+  };
+  auto rest = [](float x, uint32_t lead) { return fabsf(x) < INFINITY ? x - __uint_as_float(lead << 16) : 0.f; };
+  const uint32_t la = lead(a), lb = lead(b);
+  const float ra = rest(a, la), rb = rest(b, lb);
+  Parts s;
+  s.p[0] = la | lb << 16;
+  s.p[1] = pack_bf16x2(ra, rb);
+  s.p[2] = pack_bf16x2(ra - __uint_as_float(s.p[1] << 16), rb - __uint_as_float(s.p[1] & 0xffff0000u));
+  return s;
+}
+template <bool Any>
+__device__ __forceinline__ void split4(u32x4_t x, Parts (&s)[2]) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const float a = __uint_as_float(x[2 * i]), b = __uint_as_float(x[2 * i + 1]);
+    s[i] = Any ? split2_any(a, b) : split2(a, b);
+  }
 }
 
 // x y without the terms below fp32's last digit: x1 y1 + (x1 y2 + x2 y1) +
@@ -113,25 +144,32 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
       }
       return (uint32_t)__ballot(ok);
     };
-    auto put = [&](unsigned char *to, int swz, int row, int piece, u32x4_t x) {
-      const Parts lo = split2(__uint_as_float(x[0]), __uint_as_float(x[1]));
-      const Parts hi = split2(__uint_as_float(x[2]), __uint_as_float(x[3]));
+    // a piece of a row to the three planes; what it holds past bf16's range
+    auto put = [&](auto any, unsigned char *to, int swz, int row, int piece, u32x4_t x) -> uint32_t {
+      Parts y[2];
+      split4<any>(x, y);
       to += row * RB + 16 * ((piece / 2) ^ swz) + 8 * (piece & 1);
 #pragma unroll
-      for (int p = 0; p < 3; ++p) *reinterpret_cast<u32x2_t *>(to + p * PLANE) = u32x2_t{lo.p[p], hi.p[p]};
+      for (int p = 0; p < 3; ++p) *reinterpret_cast<u32x2_t *>(to + p * PLANE) = u32x2_t{y[0].p[p], y[1].p[p]};
+      return mark_past(y[0].p[0]) | mark_past(y[1].p[0]);
     };
     auto keep = [&](int st, int k0, uint32_t *bad) {
       const bool edge = shared.edge(k0, TK);
+      auto put_all = [&](auto any) {
+        uint32_t past = 0;
 #pragma unroll
-      for (int j = 0; j < NL; ++j) {
-        const int idx = j * NTH + tid, row = idx / PR, piece = idx % PR;
-        if (edge && not_finite<float>(vreg[j])) {
-          vreg[j] = u32x4_t{0, 0, 0, 0};
-          atomicOr(bad, 1u << row);
+        for (int j = 0; j < NL; ++j) {
+          const int idx = j * NTH + tid, row = idx / PR, piece = idx % PR;
+          if (!any && edge && not_finite<float>(vreg[j])) {
+            vreg[j] = u32x4_t{0, 0, 0, 0};
+            atomicOr(bad, 1u << row);
+          }
+          past |= put(any, smem + st * STAGE, kswz(row), row, piece, kreg[j]);
+          past |= put(any, smem + st * STAGE + 3 * PLANE, vswz(row), row, piece, vreg[j]);
         }
-        put(smem + st * STAGE, kswz(row), row, piece, kreg[j]);
-        put(smem + st * STAGE + 3 * PLANE, vswz(row), row, piece, vreg[j]);
-      }
+        return past;
+      };
+      if (__ballot(put_all(std::false_type{}) & kPast)) put_all(std::true_type{});
     };
     uint32_t there = fetch(k_first, lookup(k_first));
     int page = lookup(k_first + TK);
@@ -139,9 +177,10 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
     // ---- the wave's rows: lane (row n, half) holds columns 16 j + 8 half .. + 7
     const Rows32 rows(a, s, r0 + 32 * wave + n);
     u32x4_t q[NQ][3];
-    {
+    auto take_q = [&](auto any) {
       const char *src = static_cast<const char *>(a.q) +
           ((int64_t)(s.q0 + rows.token) * a.q_ld[0] + (h * G + rows.row - rows.token * G) * a.q_ld[1]) * 4;
+      uint32_t past = 0;
 #pragma unroll
       for (int j = 0; j < NQ; ++j)
 #pragma unroll
@@ -149,12 +188,15 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
           const int p = 4 * j + 2 * half + e;
           const u32x4_t x = scale_sign<float>(
               *reinterpret_cast<const u32x4_t *>(rows.live && p < C ? src + 16 * p : zero), a.scale);
-          const Parts lo = split2(__uint_as_float(x[0]), __uint_as_float(x[1]));
-          const Parts hi = split2(__uint_as_float(x[2]), __uint_as_float(x[3]));
+          Parts y[2];
+          split4<any>(x, y);
 #pragma unroll
-          for (int k = 0; k < 3; ++k) q[j][k][2 * e] = lo.p[k], q[j][k][2 * e + 1] = hi.p[k];
+          for (int k = 0; k < 3; ++k) q[j][k][2 * e] = y[0].p[k], q[j][k][2 * e + 1] = y[1].p[k];
+          past |= mark_past(y[0].p[0]) | mark_past(y[1].p[0]);
         }
-    }
+      return past;
+    };
+    if (__ballot(take_q(std::false_type{}) & kPast)) take_q(std::true_type{});
     f32x16_t o[DT];
 #pragma unroll
     for (int d = 0; d < DT; ++d)
