@@ -361,16 +361,13 @@ __device__ __forceinline__ f32x4_t join_parts(const AttnArgs &a, const Split &s,
     float mw[K], lw[K];
     f32x4_t y[K];
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
+    for (int k = 0; k < K; ++k) {  // past the last part: that one again, weighing nothing
       const int w = min(w0 + k, last);
       const int64_t at = (w == first ? s.slot : 2 * (int64_t)w) * BM + row;
-      mw[k] = a.part_ml[2 * at];
+      mw[k] = w0 + k <= last ? a.part_ml[2 * at] : -INFINITY;
       lw[k] = a.part_ml[2 * at + 1];
       y[k] = *reinterpret_cast<const f32x4_t *>(a.part_o + at * a.D + d);
     }
-#pragma unroll
-    for (int k = 1; k < K; ++k)
-      if (w0 + k > last) mw[k] = -INFINITY, lw[k] = 0.f, y[k] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     float mm = m;
 #pragma unroll
     for (int k = 0; k < K; ++k) mm = fmaxf(mm, mw[k]);
