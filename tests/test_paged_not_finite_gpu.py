@@ -120,3 +120,28 @@ def test_largest_values_unseen(q, D, dtype):
     sees = torch.zeros(want.size(0), dtype=torch.bool, device=want.device)
     sees[first - 300 + q:q] = True
     assert same_but(call(b), want, sees)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("D", [64, 80, 128, 256])
+@pytest.mark.parametrize("q", [4, 12, 40, 200])
+def test_largest_values(q, D, dtype):
+    """The type's largest and lowest finite numbers as values of two of the
+    chunk's own tokens: rows that do not see them keep every bit, rows that do
+    stay finite and within the bound."""
+    lens = [(q, 300), (min(q, 9), 9)]
+    clean, b = (make(lens, 8, 2, D, 16, dtype, seed=D) for _ in "ab")
+    want = check(clean)
+    top = torch.finfo(dtype).max
+    first = 300 - q // 2
+    put(b["v"], b, 0, [first], top, slice(0, D, 2))
+    put(b["v"], b, 0, [first], -top, slice(1, D, 2))
+    put(b["v"], b, 0, [299], -top, slice(0, D, 3))
+    sees = torch.zeros(clean["q"].size(0), dtype=torch.bool, device=want.device)
+    sees[first - 300 + q:q] = True
+    out = check(b)
+    assert sees[:q].any() and not sees[:q].all()
+    assert same_but(out, want, sees)
+    # no max_query_len makes such a value infinite
+    for m in (1, 10 ** 6):
+        assert same_but(check(b, max_q=m), call(clean, max_q=m), sees)

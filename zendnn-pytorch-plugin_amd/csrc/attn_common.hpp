@@ -38,6 +38,13 @@ __device__ __forceinline__ u32x4_t scale_sign(u32x4_t w, float scale) {
   return w;
 }
 
+// Weights are held times 2^-40, their sums too, and the division takes it out
+// again: with up to 2^30 keys of weights up to 2^8 the running sums stay below
+// the largest value, so that no finite value becomes infinite on the way.  (A
+// weight underflows at 2^-86 of the largest.)
+constexpr int kHeadroom = 40;
+constexpr float kWeight = 1.f / (1ull << kHeadroom);
+
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
 
 // Four fp32 outputs of a row, times r, rounded.

@@ -255,7 +255,7 @@ __global__ __launch_bounds__(kRowThreads, DP <= 128 ? 2 : 1) void paged_attn_row
         for (int u = 0; u < KT; ++u)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float p = __builtin_amdgcn_exp2f(fmaf(sc[t][u][e], c, -mc));
+            const float p = __builtin_amdgcn_exp2f(fmaf(sc[t][u][e], c, -mc)) * kWeight;
             l[t] += p;
             if constexpr (BF) {
               const __bf16 hi_part = (__bf16)p;

@@ -281,8 +281,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const int i = 8 * (j / DT) + 2 * e;
-              const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[i], c, -mc));
-              const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[i + 1], c, -mc));
+              const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[i], c, -mc)) * kWeight;
+              const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[i + 1], c, -mc)) * kWeight;
               l += p0;
               l += p1;
               const Parts w = split2(p0, p1);
