@@ -145,3 +145,30 @@ def test_largest_values(q, D, dtype):
     # no max_query_len makes such a value infinite
     for m in (1, 10 ** 6):
         assert same_but(check(b, max_q=m), call(clean, max_q=m), sees)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("q,long", KINDS)
+@pytest.mark.parametrize("size", [1e6, 1e9, 1e12, 1e30, "largest"])
+def test_huge_scores(size, q, long, D, dtype):
+    """One key's score stands so far above all others that its value is the
+    output, bit for bit; a very negative one's weighs nothing."""
+    b = make(lens_of(q, long), 8, 2, D, 64, dtype, seed=D + 3)
+    # "largest": the key's number is the type's largest, against small queries
+    top, by = (torch.finfo(dtype).max, 2.0 ** -20) if size == "largest" else (size, 1)
+    b["q"][..., 5] = (b["q"][..., 5].abs() + 0.25) * by
+    clean = call(b)
+    n, t = lens_of(q, long)[0][1], lens_of(q, long)[0][1] - q
+    put(b["k"], b, 0, [t], top, 5)
+    out = call(b)
+    v = b["v"][b["table"][0, t // 64], :, t % 64].repeat_interleave(4, 0)
+    assert torch.equal(out[:q], v.expand_as(out[:q]))
+    assert torch.equal(out[q:], clean[q:])
+    if long:  # a page of very negative ones, against a cache without that page
+        b["k"][b["table"][0, t // 64], :, t % 64, 5] = 0
+        put(b["k"], b, 0, range(192, 256), -top, 5)
+        out = call(b)
+        table = b["table"].clone()
+        table[0, 3] = -1
+        check(b | dict(table=table), out)

@@ -38,6 +38,18 @@ __device__ __forceinline__ u32x4_t scale_sign(u32x4_t w, float scale) {
   return w;
 }
 
+// A weight is 2^(s c - m c), one fused operation per score s.  What the rounding
+// of m c adds to the exponent is the same for all keys of a row and cancels, but
+// for huge scores it is huge itself.  From |m c| = 2^10 on, s - m is taken first.
+constexpr float kFar = 1024.f;
+__device__ __forceinline__ bool is_far(float mc) { return fabsf(mc) >= kFar; }
+// The factor that brings weights from one maximum to a larger one (1 between equal
+// ones, two of -inf among them, whose difference is a NaN that the minimum drops).
+// For huge ones the products' roundings are as the scores' own.
+__device__ __forceinline__ float factor(float from, float to, float c) {
+  return __builtin_amdgcn_exp2f(fminf(from * c - to * c, 0.f));
+}
+
 // Weights are held times 2^-40, their sums too, and the division takes it out
 // again: with up to 2^30 keys of weights up to 2^8 the running sums stay below
 // the largest value, so that no finite value becomes infinite on the way.  (A

@@ -242,7 +242,7 @@ __global__ __launch_bounds__(kRowThreads, DP <= 128 ? 2 : 1) void paged_attn_row
           for (int e = 0; e < 4; ++e) mx = fmaxf(mx, sc[t][u][e]);
         mx = fmaxf(m[t], max_over_groups(mx));
         if (__ballot(mx > m[t])) {
-          const float f = mx == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[t] * c - mx * c);
+          const float f = factor(m[t], mx, c);
           l[t] *= f;
 #pragma unroll
           for (int d = 0; d < DT; ++d)
@@ -250,7 +250,14 @@ __global__ __launch_bounds__(kRowThreads, DP <= 128 ? 2 : 1) void paged_attn_row
             for (int e = 0; e < 4; ++e) o[t][d][e] *= f;
           m[t] = mx;
         }
-        const float mc = m[t] == -INFINITY ? 0.f : m[t] * c;
+        float mc = m[t] == -INFINITY ? 0.f : m[t] * c;
+        if (__ballot(is_far(mc))) {
+#pragma unroll
+          for (int u = 0; u < KT; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sc[t][u][e] -= is_far(mc) ? m[t] : 0.f;
+          mc = is_far(mc) ? 0.f : mc;
+        }
 #pragma unroll
         for (int u = 0; u < KT; ++u)
 #pragma unroll
@@ -318,7 +325,7 @@ __global__ __launch_bounds__(kRowThreads, DP <= 128 ? 2 : 1) void paged_attn_row
         f32x4_t oo = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-          const float f = sm_m[w][row] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sm_m[w][row] * c - mm * c);
+          const float f = factor(sm_m[w][row], mm, c);
           ll += f * sm_l[w][row];
           const f32x4_t y = *reinterpret_cast<const f32x4_t *>(smem + w * kWaveLds + (row * OP + d) * 4);
 #pragma unroll
@@ -351,10 +358,6 @@ template <int K>
 __device__ __forceinline__ f32x4_t join_parts(const AttnArgs &a, const Split &s, int first, int row, int d,
                                               float c, float *sum) {
   const int BM = a.item_rows, last = (int)s.last;
-  // from one maximum to another; equal ones, two of -inf among them, change nothing
-  auto factor = [&](float from, float to) {
-    return from == to ? 1.f : __builtin_amdgcn_exp2f(from * c - to * c);
-  };
   float m = -INFINITY, l = 0.f;
   f32x4_t o = {0.f, 0.f, 0.f, 0.f};
   for (int w0 = first; w0 <= last; w0 += K) {
@@ -371,13 +374,13 @@ __device__ __forceinline__ f32x4_t join_parts(const AttnArgs &a, const Split &s,
     float mm = m;
 #pragma unroll
     for (int k = 0; k < K; ++k) mm = fmaxf(mm, mw[k]);
-    const float f0 = factor(m, mm);
+    const float f0 = factor(m, mm, c);
     m = mm, l *= f0;
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] *= f0;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const float f = factor(mw[k], mm);
+      const float f = factor(mw[k], mm, c);
       l += lw[k] * f;
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[e] += y[k][e] * f;

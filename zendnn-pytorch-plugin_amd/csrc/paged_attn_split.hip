@@ -202,7 +202,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
     for (int d = 0; d < DT; ++d)
 #pragma unroll
       for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
-    float m = -INFINITY, l = 0.f;
+    float m = -INFINITY, mc = 0.f, l = 0.f;
+    bool far = false;  // of some row of the wave
     bool poisoned = false;  // the row sees a value that is not finite at an edge
 
     keep(0, k_first, sm_bad);
@@ -250,15 +251,22 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
         // in the rows that grew only, so that no row's bits depend on another's
         const bool grown = mx != -INFINITY && (mx - m) * c > 8.f;
         if (__ballot(grown)) {
-          const float f = grown ? __builtin_amdgcn_exp2f(m * c - mx * c) : 1.f;
+          const float f = grown ? factor(m, mx, c) : 1.f;
           l *= f;
 #pragma unroll
           for (int d = 0; d < DT; ++d)
 #pragma unroll
             for (int e = 0; e < 16; ++e) o[d][e] *= f;
           m = grown ? mx : m;
+          mc = grown ? mx * c : mc;
+          far = __ballot(is_far(mc)) != 0;
         }
-        const float mc = m == -INFINITY ? 0.f : m * c;
+        float ref = mc;
+        if (far) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) sc[e] -= is_far(mc) ? m : 0.f;
+          ref = is_far(mc) ? 0.f : mc;
+        }
         // ---- O^T += V^T P^T, 16 keys and 32 columns a step
         typedef __attribute__((address_space(3))) s16x4_t *tr_ptr;
         const int i16 = lane & 15, r = 4 * half + i16 / 4;
@@ -281,8 +289,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const int i = 8 * (j / DT) + 2 * e;
-              const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[i], c, -mc)) * kWeight;
-              const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[i + 1], c, -mc)) * kWeight;
+              const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[i], c, -ref)) * kWeight;
+              const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[i + 1], c, -ref)) * kWeight;
               l += p0;
               l += p1;
               const Parts w = split2(p0, p1);

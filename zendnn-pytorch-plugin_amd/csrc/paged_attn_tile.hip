@@ -171,7 +171,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP <= 1
     for (int d = 0; d < DT; ++d)
 #pragma unroll
       for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
-    float m = -INFINITY, l = 0.f;
+    float m = -INFINITY, mc = 0.f, l = 0.f;
+    bool far = false;  // of some row of the wave
     bool poisoned = false;  // the row sees a value that is not finite at an edge
 
     for (int t = 0; t < take; ++t) {
@@ -249,15 +250,24 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP <= 1
         // in the rows that grew only, so that no row's bits depend on another's
         const bool grown = mx != -INFINITY && (mx - m) * c > 8.f;
         if (__ballot(grown)) {
-          const float f = grown ? __builtin_amdgcn_exp2f(m * c - mx * c) : 1.f;
+          const float f = grown ? factor(m, mx, c) : 1.f;
           l *= f;
 #pragma unroll
           for (int d = 0; d < DT; ++d)
 #pragma unroll
             for (int e = 0; e < 16; ++e) o[d][e] *= f;
           m = grown ? mx : m;
+          mc = grown ? mx * c : mc;
+          far = __ballot(is_far(mc)) != 0;
         }
-        const float mc = m == -INFINITY ? 0.f : m * c;
+        float ref = mc;
+        if (far) {
+#pragma unroll
+          for (int u = 0; u < KT; ++u)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) sc[u][e] -= is_far(mc) ? m : 0.f;
+          ref = is_far(mc) ? 0.f : mc;
+        }
         // ---- O^T += V^T P^T, a step of keys at a time (16, or one of each half
         // in fp32): beside its MFMAs go the next step's weights and the reads
         // of the operands kAhead MFMAs on.  A wave that is this far goes before
@@ -266,7 +276,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP <= 1
         __builtin_amdgcn_s_setprio(1);
         // The headroom goes into the exponent in bf16 (its rounding there, 2^-19,
         // is far below the weights'), and is a product in fp32.
-        const float ref = BF ? mc + kHeadroom : mc;
+        if constexpr (BF) ref += kHeadroom;
         auto weight = [&](int e) {
           const float p = __builtin_amdgcn_exp2f(fmaf(sc[e / 16][e % 16], c, -ref));
           return BF ? p : p * kWeight;
