@@ -25,12 +25,16 @@ __device__ __forceinline__ Parts split2(float a, float b) {
   return s;
 }
 
-// The nearest bf16 to a number past bf16's largest is infinite, so those, and
-// numbers that are not finite, are split apart from the others: x1 is x cut
-// short, and an infinity or a NaN goes whole into x1.  mark_past gives them bits
-// of kPast, which it leaves 0 for other pairs.
-constexpr uint32_t kPast = 0x80008000u;
-__device__ __forceinline__ uint32_t mark_past(uint32_t first) { return (first & 0x7f807f80u) + 0x00800080u; }
+// The nearest bf16 to a number of at least kPast is infinite, so pieces that hold
+// one are split apart from the others: its x1 is x cut short, and an infinity
+// or a NaN goes whole into x1.  (A NaN alone shows in all parts of either.)
+constexpr float kPast = 0x1.ffp127f;
+// the larger of m and |x|'s (one operation for two; fmaxf quiets every input)
+__device__ __forceinline__ float largest_of(float m, u32x4_t x) {
+  asm("v_max3_f32 %0, %0, |%1|, |%2|" : "+v"(m) : "v"(x[0]), "v"(x[1]));
+  asm("v_max3_f32 %0, %0, |%1|, |%2|" : "+v"(m) : "v"(x[2]), "v"(x[3]));
+  return m;
+}
 __device__ __forceinline__ Parts split2_any(float a, float b) {
   auto lead = [](float x) -> uint32_t {
     const uint32_t near = f32_to_bf16_bits(x);
@@ -144,19 +148,18 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
       }
       return (uint32_t)__ballot(ok);
     };
-    // a piece of a row to the three planes; what it holds past bf16's range
-    auto put = [&](auto any, unsigned char *to, int swz, int row, int piece, u32x4_t x) -> uint32_t {
+    // a piece of a row to the three planes
+    auto put = [&](auto any, unsigned char *to, int swz, int row, int piece, u32x4_t x) {
       Parts y[2];
       split4<any>(x, y);
       to += row * RB + 16 * ((piece / 2) ^ swz) + 8 * (piece & 1);
 #pragma unroll
       for (int p = 0; p < 3; ++p) *reinterpret_cast<u32x2_t *>(to + p * PLANE) = u32x2_t{y[0].p[p], y[1].p[p]};
-      return mark_past(y[0].p[0]) | mark_past(y[1].p[0]);
     };
     auto keep = [&](int st, int k0, uint32_t *bad) {
       const bool edge = shared.edge(k0, TK);
-      auto put_all = [&](auto any) {
-        uint32_t past = 0;
+      auto put_all = [&](auto any) -> float {
+        float most = 0.f;
 #pragma unroll
         for (int j = 0; j < NL; ++j) {
           const int idx = j * NTH + tid, row = idx / PR, piece = idx % PR;
@@ -164,12 +167,13 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
             vreg[j] = u32x4_t{0, 0, 0, 0};
             atomicOr(bad, 1u << row);
           }
-          past |= put(any, smem + st * STAGE, kswz(row), row, piece, kreg[j]);
-          past |= put(any, smem + st * STAGE + 3 * PLANE, vswz(row), row, piece, vreg[j]);
+          put(any, smem + st * STAGE, kswz(row), row, piece, kreg[j]);
+          put(any, smem + st * STAGE + 3 * PLANE, vswz(row), row, piece, vreg[j]);
+          if (!any) most = largest_of(largest_of(most, kreg[j]), vreg[j]);
         }
-        return past;
+        return most;
       };
-      if (__ballot(put_all(std::false_type{}) & kPast)) put_all(std::true_type{});
+      if (__ballot(!(put_all(std::false_type{}) < kPast))) put_all(std::true_type{});
     };
     uint32_t there = fetch(k_first, lookup(k_first));
     int page = lookup(k_first + TK);
@@ -177,10 +181,10 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
     // ---- the wave's rows: lane (row n, half) holds columns 16 j + 8 half .. + 7
     const Rows32 rows(a, s, r0 + 32 * wave + n);
     u32x4_t q[NQ][3];
-    auto take_q = [&](auto any) {
+    auto take_q = [&](auto any) -> float {
       const char *src = static_cast<const char *>(a.q) +
           ((int64_t)(s.q0 + rows.token) * a.q_ld[0] + (h * G + rows.row - rows.token * G) * a.q_ld[1]) * 4;
-      uint32_t past = 0;
+      float most = 0.f;
 #pragma unroll
       for (int j = 0; j < NQ; ++j)
 #pragma unroll
@@ -192,11 +196,11 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
           split4<any>(x, y);
 #pragma unroll
           for (int k = 0; k < 3; ++k) q[j][k][2 * e] = y[0].p[k], q[j][k][2 * e + 1] = y[1].p[k];
-          past |= mark_past(y[0].p[0]) | mark_past(y[1].p[0]);
+          most = largest_of(most, x);
         }
-      return past;
+      return most;
     };
-    if (__ballot(take_q(std::false_type{}) & kPast)) take_q(std::true_type{});
+    if (__ballot(!(take_q(std::false_type{}) < kPast))) take_q(std::true_type{});
     f32x16_t o[DT];
 #pragma unroll
     for (int d = 0; d < DT; ++d)
