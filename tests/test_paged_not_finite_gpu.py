@@ -172,3 +172,22 @@ def test_huge_scores(size, q, long, D, dtype):
         table = b["table"].clone()
         table[0, 3] = -1
         check(b | dict(table=table), out)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("D", [64, 80, 128, 256])
+@pytest.mark.parametrize("q", [1, 4, 12, 40, 200])
+@pytest.mark.parametrize("all_", [300, 5000])
+def test_keys_of_minus_infinity(all_, q, D, dtype):
+    """Keys whose scores are -inf weigh nothing: the outputs are those of a
+    cache without their pages."""
+    lens = [(q, all_), (min(q, 9), 9)]
+    b = make(lens, 8, 2, D, 16, dtype, seed=D + 1)
+    b["q"][..., 5] = b["q"][..., 5].abs() + 0.25
+    gone = [2, 3, 17]
+    for p in gone:
+        put(b["k"], b, 0, range(16 * p, 16 * p + 16), -math.inf, 5)
+    out = call(b)
+    table = b["table"].clone()
+    table[0, gone] = -1
+    check(b | dict(table=table), out)

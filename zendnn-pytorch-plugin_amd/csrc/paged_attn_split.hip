@@ -1,8 +1,6 @@
 // Attention of a chunk of new tokens over a paged cache, for gfx950: many rows
 // per cache head in fp32, head_dim up to 128, on bf16 MFMAs.  The definitions are in
 // paged_attn.hip.
-#include <type_traits>
-
 #include "attn_common.hpp"
 
 namespace zt {
@@ -25,41 +23,50 @@ __device__ __forceinline__ Parts split2(float a, float b) {
   return s;
 }
 
-// The nearest bf16 to a number of at least kPast is infinite, so pieces that hold
-// one are split apart from the others: its x1 is x cut short, and an infinity
-// or a NaN goes whole into x1.  (A NaN alone shows in all parts of either.)
-constexpr float kPast = 0x1.ffp127f;
-// the larger of m and |x|'s (one operation for two; fmaxf quiets every input)
-__device__ __forceinline__ float largest_of(float m, u32x4_t x) {
-  asm("v_max3_f32 %0, %0, |%1|, |%2|" : "+v"(m) : "v"(x[0]), "v"(x[1]));
-  asm("v_max3_f32 %0, %0, |%1|, |%2|" : "+v"(m) : "v"(x[2]), "v"(x[3]));
-  return m;
-}
-__device__ __forceinline__ Parts split2_any(float a, float b) {
-  auto lead = [](float x) -> uint32_t {
-    const uint32_t near = f32_to_bf16_bits(x);
-    return x != x ? 0x7fc0u : (near & 0x7f80u) == 0x7f80u ? __float_as_uint(x) >> 16 : near;
-  };
-  auto rest = [](float x, uint32_t lead) { return fabsf(x) < INFINITY ? x - __uint_as_float(lead << 16) : 0.f; };
-  const uint32_t la = lead(a), lb = lead(b);
-  const float ra = rest(a, la), rb = rest(b, lb);
+// The same for keys and values, with x1 cut short, so that it is finite where x is
+// (the nearest bf16 to the last 0.2 % below fp32's largest is not): else x2 would
+// be infinite too, and a weight of 0 make NaN of it.  An infinite key is x1 alone:
+// the median takes the NaN that is left of it for 0.
+template <bool Key>
+__device__ __forceinline__ Parts split2_cached(uint32_t a, uint32_t b) {
+  const uint32_t wa = a & 0xffff0000u, wb = b & 0xffff0000u;
   Parts s;
-  s.p[0] = la | lb << 16;
+  s.p[0] = __builtin_amdgcn_perm(wb, wa, 0x07060302u);  // the two high halves
+  float ra = __uint_as_float(a) - __uint_as_float(wa), rb = __uint_as_float(b) - __uint_as_float(wb);
+  if constexpr (Key) {
+    asm("v_med3_f32 %0, %0, 0, %0" : "+v"(ra));
+    asm("v_med3_f32 %0, %0, 0, %0" : "+v"(rb));
+  }
   s.p[1] = pack_bf16x2(ra, rb);
-  s.p[2] = pack_bf16x2(ra - __uint_as_float(s.p[1] << 16), rb - __uint_as_float(s.p[1] & 0xffff0000u));
+  ra -= __uint_as_float(s.p[1] << 16), rb -= __uint_as_float(s.p[1] & 0xffff0000u);
+  s.p[2] = pack_bf16x2(ra, rb);
   return s;
 }
-template <bool Any>
-__device__ __forceinline__ void split4(u32x4_t x, Parts (&s)[2]) {
+
+// The same for a query, all parts cut short and none of them zero (the smallest
+// normal number instead, which adds nothing to a score): an infinite key's score
+// then is infinite with the product's sign, not the NaN of infinities of both
+// signs or of one times 0.  (A query of 0 against an infinite key is a NaN.)
+__device__ __forceinline__ Parts split2_query(uint32_t a, uint32_t b) {
+  typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
+  float ra = __uint_as_float(a), rb = __uint_as_float(b);
+  Parts s;
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const float a = __uint_as_float(x[2 * i]), b = __uint_as_float(x[2 * i + 1]);
-    s[i] = Any ? split2_any(a, b) : split2(a, b);
+  for (int p = 0; p < 3; ++p) {
+    const uint32_t wa = __float_as_uint(ra) & 0xffff0000u, wb = __float_as_uint(rb) & 0xffff0000u;
+    s.p[p] = __builtin_amdgcn_perm(wb, wa, 0x07060302u);
+    ra -= __uint_as_float(wa), rb -= __uint_as_float(wb);
   }
+  const auto least = __builtin_bit_cast(u16x2_t, (s.p[0] & 0x80008000u) | 0x00800080u);
+#pragma unroll
+  for (int p = 1; p < 3; ++p)
+    s.p[p] = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, s.p[p]), least));
+  return s;
 }
 
-// x y without the terms below fp32's last digit: x1 y1 + (x1 y2 + x2 y1) +
-// (x2 y2 + x1 y3 + x3 y1), smallest first.
+// x y without its smallest terms: x1 y1 + (x1 y2 + x2 y1) + (x2 y2 + x1 y3 + x3 y1),
+// smallest first.  Where both are cut short the others are below 2^-21 of x y, 2^-24
+// in the mean; where one is, below 2^-23.
 __device__ __forceinline__ f32x16_t mfma_split(const u32x4_t (&x)[3], const u32x4_t (&y)[3], f32x16_t acc) {
   auto mul = [&](int i, int j) {
     acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, x[i]),
@@ -149,31 +156,25 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
       return (uint32_t)__ballot(ok);
     };
     // a piece of a row to the three planes
-    auto put = [&](auto any, unsigned char *to, int swz, int row, int piece, u32x4_t x) {
-      Parts y[2];
-      split4<any>(x, y);
+    auto put = [&](unsigned char *to, int swz, int row, int piece, const Parts &lo, const Parts &hi) {
       to += row * RB + 16 * ((piece / 2) ^ swz) + 8 * (piece & 1);
 #pragma unroll
-      for (int p = 0; p < 3; ++p) *reinterpret_cast<u32x2_t *>(to + p * PLANE) = u32x2_t{y[0].p[p], y[1].p[p]};
+      for (int p = 0; p < 3; ++p) *reinterpret_cast<u32x2_t *>(to + p * PLANE) = u32x2_t{lo.p[p], hi.p[p]};
     };
     auto keep = [&](int st, int k0, uint32_t *bad) {
       const bool edge = shared.edge(k0, TK);
-      auto put_all = [&](auto any) -> float {
-        float most = 0.f;
 #pragma unroll
-        for (int j = 0; j < NL; ++j) {
-          const int idx = j * NTH + tid, row = idx / PR, piece = idx % PR;
-          if (!any && edge && not_finite<float>(vreg[j])) {
-            vreg[j] = u32x4_t{0, 0, 0, 0};
-            atomicOr(bad, 1u << row);
-          }
-          put(any, smem + st * STAGE, kswz(row), row, piece, kreg[j]);
-          put(any, smem + st * STAGE + 3 * PLANE, vswz(row), row, piece, vreg[j]);
-          if (!any) most = largest_of(largest_of(most, kreg[j]), vreg[j]);
+      for (int j = 0; j < NL; ++j) {
+        const int idx = j * NTH + tid, row = idx / PR, piece = idx % PR;
+        if (edge && not_finite<float>(vreg[j])) {
+          vreg[j] = u32x4_t{0, 0, 0, 0};
+          atomicOr(bad, 1u << row);
         }
-        return most;
-      };
-      if (__ballot(!(put_all(std::false_type{}) < kPast))) put_all(std::true_type{});
+        put(smem + st * STAGE, kswz(row), row, piece, split2_cached<true>(kreg[j][0], kreg[j][1]),
+            split2_cached<true>(kreg[j][2], kreg[j][3]));
+        put(smem + st * STAGE + 3 * PLANE, vswz(row), row, piece, split2_cached<false>(vreg[j][0], vreg[j][1]),
+            split2_cached<false>(vreg[j][2], vreg[j][3]));
+      }
     };
     uint32_t there = fetch(k_first, lookup(k_first));
     int page = lookup(k_first + TK);
@@ -181,10 +182,9 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
     // ---- the wave's rows: lane (row n, half) holds columns 16 j + 8 half .. + 7
     const Rows32 rows(a, s, r0 + 32 * wave + n);
     u32x4_t q[NQ][3];
-    auto take_q = [&](auto any) -> float {
+    {
       const char *src = static_cast<const char *>(a.q) +
           ((int64_t)(s.q0 + rows.token) * a.q_ld[0] + (h * G + rows.row - rows.token * G) * a.q_ld[1]) * 4;
-      float most = 0.f;
 #pragma unroll
       for (int j = 0; j < NQ; ++j)
 #pragma unroll
@@ -192,21 +192,17 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
           const int p = 4 * j + 2 * half + e;
           const u32x4_t x = scale_sign<float>(
               *reinterpret_cast<const u32x4_t *>(rows.live && p < C ? src + 16 * p : zero), a.scale);
-          Parts y[2];
-          split4<any>(x, y);
+          const Parts lo = split2_query(x[0], x[1]), hi = split2_query(x[2], x[3]);
 #pragma unroll
-          for (int k = 0; k < 3; ++k) q[j][k][2 * e] = y[0].p[k], q[j][k][2 * e + 1] = y[1].p[k];
-          most = largest_of(most, x);
+          for (int k = 0; k < 3; ++k) q[j][k][2 * e] = lo.p[k], q[j][k][2 * e + 1] = hi.p[k];
         }
-      return most;
-    };
-    if (__ballot(!(take_q(std::false_type{}) < kPast))) take_q(std::true_type{});
+    }
     f32x16_t o[DT];
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
       for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
-    float m = -INFINITY, mc = 0.f, l = 0.f;
+    float m = -INFINITY, l = 0.f;
     bool far = false;  // of some row of the wave
     bool poisoned = false;  // the row sees a value that is not finite at an edge
 
@@ -262,14 +258,13 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
 #pragma unroll
             for (int e = 0; e < 16; ++e) o[d][e] *= f;
           m = grown ? mx : m;
-          mc = grown ? mx * c : mc;
-          far = __ballot(is_far(mc)) != 0;
+          far = __ballot(m != -INFINITY && is_far(m * c)) != 0;
         }
-        float ref = mc;
+        float ref = m == -INFINITY ? 0.f : m * c;
         if (far) {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) sc[e] -= is_far(mc) ? m : 0.f;
-          ref = is_far(mc) ? 0.f : mc;
+          for (int e = 0; e < 16; ++e) sc[e] -= is_far(ref) ? m : 0.f;
+          ref = is_far(ref) ? 0.f : ref;
         }
         // ---- O^T += V^T P^T, 16 keys and 32 columns a step
         typedef __attribute__((address_space(3))) s16x4_t *tr_ptr;
