@@ -15,10 +15,8 @@ int hip_status(hipError_t e, const char *what) {
 
 bool is_float_dt(int dt) { return dt == ZT_DT_F32 || dt == ZT_DT_BF16; }
 
-// Rows of a batch that the page kernels hold in LDS.
-constexpr int64_t kMaxRows = 4096;
-// Sequences of an attention call (16 bytes of LDS each).
-constexpr int64_t kMaxSeqs = 1024;
+using zt::kMaxRows;
+using zt::kMaxSeqs;
 
 bool divides16(const void *p, std::initializer_list<int64_t> elems, int64_t esize) {
   if (reinterpret_cast<uintptr_t>(p) % 16) return false;

@@ -537,11 +537,9 @@ hipError_t launch_cache_extend(ExtendArgs a, hipStream_t s) {
 
 hipError_t launch_cache_fork(ForkArgs a, hipStream_t s) {
   const size_t lds = (size_t)a.S * 6 * sizeof(int);
-  if (lds > 60 * 1024) {
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(cache_fork_kernel),
-                                             hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-    if (e != hipSuccess) return e;
-  }
+  const hipError_t allowed =
+      allow_lds(reinterpret_cast<const void *>(cache_fork_kernel), lds, kMaxRows * 6 * sizeof(int));
+  if (allowed != hipSuccess) return allowed;
   a.div_size = make_div(a.page_size), a.div_w = make_div(std::max(a.W, 1));
   cache_fork_kernel<<<1, kBlock, lds, s>>>(a);
   return hipGetLastError();

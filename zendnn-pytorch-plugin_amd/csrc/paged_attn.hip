@@ -418,14 +418,11 @@ template <typename T, int DP, int NT>
 hipError_t launch_rows(const AttnArgs &a, int grid, hipStream_t s) {
   constexpr int KS = sizeof(T) == 2 ? 32 : 16, VP = DP * (int)sizeof(T) + (sizeof(T) == 2 ? 32 : 16);
   constexpr int wave = std::max(KS * VP, 16 * (DP + 4) * 4);
-  const size_t lds = 4 * wave + batch_ints(a.S) * 4;
+  const size_t lds = 4 * wave + batch_ints(a.S) * 4, largest = 4 * wave + batch_ints(kMaxSeqs) * 4;
   if (a.item_rows != 16 * NT) return hipErrorInvalidValue;
   auto kernel = paged_attn_row_kernel<T, DP, NT>;
-  if (lds > 64 * 1024) {
-    const hipError_t grown = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
-                                                 hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-    if (grown != hipSuccess) return grown;
-  }
+  const hipError_t allowed = allow_lds(reinterpret_cast<const void *>(kernel), lds, largest);
+  if (allowed != hipSuccess) return allowed;
   kernel<<<grid, kRowThreads, lds, s>>>(a);
   return hipGetLastError();
 }

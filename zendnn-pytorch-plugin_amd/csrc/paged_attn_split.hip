@@ -324,14 +324,12 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
 
 template <int DP, int DC, int NW>
 hipError_t launch_split_as(const AttnArgs &a, int grid, hipStream_t s) {
-  const size_t lds = 2 * 6 * (size_t)32 * DP * 2 + batch_ints(a.S) * 4;
+  const size_t tiles = 2 * 6 * (size_t)32 * DP * 2;
+  const size_t lds = tiles + batch_ints(a.S) * 4, largest = tiles + batch_ints(kMaxSeqs) * 4;
   if (a.item_rows != 32 * NW) return hipErrorInvalidValue;
   auto kernel = paged_attn_split_kernel<DP, DC, NW>;
-  if (lds > 64 * 1024) {
-    const hipError_t grown = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
-                                                 hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-    if (grown != hipSuccess) return grown;
-  }
+  const hipError_t allowed = allow_lds(reinterpret_cast<const void *>(kernel), lds, largest);
+  if (allowed != hipSuccess) return allowed;
   kernel<<<grid, 64 * NW, lds, s>>>(a);
   return hipGetLastError();
 }

@@ -370,14 +370,12 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP <= 1
 template <typename T, int DP, int DC, int NW>
 hipError_t launch_tiles_as(const AttnArgs &a, int grid, hipStream_t s) {
   constexpr int TK = sizeof(T) == 2 ? 64 : 32;
-  const size_t lds = 4 * (size_t)TK * DP * sizeof(T) + batch_ints(a.S) * 4;
+  const size_t tiles = 4 * (size_t)TK * DP * sizeof(T);
+  const size_t lds = tiles + batch_ints(a.S) * 4, largest = tiles + batch_ints(kMaxSeqs) * 4;
   if (a.item_rows != 32 * NW) return hipErrorInvalidValue;
   auto kernel = paged_attn_tile_kernel<T, DP, DC, NW>;
-  if (lds > 64 * 1024) {
-    const hipError_t grown = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
-                                                 hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-    if (grown != hipSuccess) return grown;
-  }
+  const hipError_t allowed = allow_lds(reinterpret_cast<const void *>(kernel), lds, largest);
+  if (allowed != hipSuccess) return allowed;
   kernel<<<grid, 64 * NW, lds, s>>>(a);
   return hipGetLastError();
 }

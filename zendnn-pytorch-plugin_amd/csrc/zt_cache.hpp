@@ -15,6 +15,19 @@ namespace zt {
 // Sets the calling thread's error message and returns `code` (capi.hip).
 int api_fail(int code, const char *fmt, ...) __attribute__((format(printf, 2, 3)));
 
+// Rows of a batch that the page kernels hold in LDS.
+constexpr int64_t kMaxRows = 4096;
+// Sequences of an attention call (16 bytes of LDS each).
+constexpr int64_t kMaxSeqs = 1024;
+
+// Lets a kernel take `bytes` of dynamic LDS.  A call whose size is past what
+// every kernel may take (64 KB) allows the kernel's largest size, always the same:
+// another thread's call to it may be between this and its launch.
+inline hipError_t allow_lds(const void *kernel, size_t bytes, size_t largest) {
+  if (bytes <= 64 * 1024) return hipSuccess;
+  return hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)largest);
+}
+
 // Division of n <= 2^30 by a fixed d >= 1: floor(n * mul / 2^(31 + L)) with
 // mul = floor(2^(31 + L) / d) + 1 and L = ceil(log2 d), which is exact for every
 // n < 2^31; 2 n * mul is taken so that the high word is all that is needed.
