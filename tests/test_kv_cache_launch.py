@@ -97,3 +97,30 @@ def test_lds_sizes_do_not_depend_on_the_call(tmp_path):
             assert rest[4] <= 64 * 1024 or rest[4] <= last[f]
     assert len(allowed) >= 8 and all(len(v) == 1 for v in allowed.values()), allowed
     assert all(largest[f] == max(v) for f, v in allowed.items())
+
+
+def test_launches_stay_below_two_to_the_32_threads(tmp_path):
+    """The runtime leaves out what is past 2^32 threads of a launch, so longer
+    calls are several launches."""
+    got = record(tmp_path, """
+        rc = L.zt_rotary_embedding(p, 1, (1 << 20) + 5, 32, 130, 32 * 130, 130, p, p, 2, 2, 2, 0, p << 20, None)
+        assert rc == 0, L.zt_last_error_string()
+        c = cache(1, 130, heads=16)
+        st = (ctypes.c_int64 * 2)(64 * 130, 130)
+        rc = L.zt_rotary_cache_append(p, (1 << 20) + 5, 32, st, p, st, p, st, p, p, 2, 2, 2, 1, p, ctypes.byref(c),
+                                      p << 20, None)
+        assert rc == 0, L.zt_last_error_string()
+        caches = (ctypes.c_void_p * 70)(*[p] * 70)
+        for n, size in (((1 << 24) + 3, 64), (1 << 20, 1 << 20)):
+            rc = L.zt_cache_copy_pages(caches, 70, 1 << 25, size, size, p, n, None)
+            assert rc == 0, L.zt_last_error_string()
+    """)
+    threads = {}  # by kernel, in the order of the calls
+    for kind, f, x, y, z, block, lds in got:
+        assert kind == "launch" and x * block < 1 << 32
+        threads[f] = threads.get(f, 0) + x * y * z * block
+    T, row = (1 << 20) + 5, 129  # a head row is a pair and 128 single elements
+    rotary, append = T * 32 * row, T * (48 * row + 16 * 130)
+    copies = 256 * 70 * ((1 << 24) + 3 + 64 * (1 << 20))  # 64 workgroups copy a page of 2^20 bytes
+    got = list(threads.values())
+    assert rotary <= got[0] < rotary + 3 * 256 and append <= got[1] < append + 5 * 256 and got[2:] == [copies]

@@ -505,13 +505,25 @@ __global__ __launch_bounds__(256) void copy_pages_kernel(CopyArgs a) {
   }
 }
 
+// Threads of a launch, at most: the runtime counts them in 32 bits and leaves out
+// what is past those without an error.
+constexpr int64_t kMostThreads = 1ll << 31;
+
 template <typename T, int V>
-hipError_t launch_rotary_v(const RotaryArgs &a, hipStream_t s) {
-  const int64_t n = a.T * a.units;
-  const dim3 grid((unsigned)((n + 255) / 256));
-  if (a.interleaved) rotary_kernel<T, V, true><<<grid, dim3(256), 0, s>>>(a);
-  else rotary_kernel<T, V, false><<<grid, dim3(256), 0, s>>>(a);
-  return hipGetLastError();
+hipError_t launch_rotary_v(RotaryArgs a, hipStream_t s) {
+  const int64_t all = a.T, step = std::max<int64_t>(kMostThreads / a.units, 1);
+  auto move = [&](const void *p, int64_t elements) { return static_cast<const T *>(p) + elements; };
+  for (int64_t t = 0; t < all; t += step) {
+    a.T = std::min(step, all - t);
+    const dim3 grid((unsigned)((a.T * a.units + 255) / 256));
+    if (a.interleaved) rotary_kernel<T, V, true><<<grid, dim3(256), 0, s>>>(a);
+    else rotary_kernel<T, V, false><<<grid, dim3(256), 0, s>>>(a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    a.q = move(a.q, step * a.q_ld[0]), a.q_out = static_cast<T *>(a.q_out) + step * a.H * a.D, a.pos += step;
+    if (a.KV) a.k = move(a.k, step * a.k_ld[0]), a.v = move(a.v, step * a.v_ld[0]), a.slots += step;
+  }
+  return hipSuccess;
 }
 
 }  // namespace
@@ -553,10 +565,15 @@ hipError_t launch_cache_compact(const CompactArgs &a, hipStream_t s) {
 hipError_t launch_copy_pages(CopyArgs a, int caches, int64_t pairs, bool wide, hipStream_t s) {
   // four loads of 16 bytes per thread
   a.parts = (int)std::min<int64_t>((a.page_bytes + 16 * 1024 - 1) / (16 * 1024), 64);
-  const dim3 grid((unsigned)(pairs * a.parts), (unsigned)caches);
-  if (wide) copy_pages_kernel<u32x4_t><<<grid, dim3(256), 0, s>>>(a);
-  else copy_pages_kernel<uint8_t><<<grid, dim3(256), 0, s>>>(a);
-  return hipGetLastError();
+  const int64_t step = kMostThreads / 256 / a.parts;
+  for (int64_t k = 0; k < pairs; k += step, a.copies += 2 * step) {
+    const dim3 grid((unsigned)(std::min(step, pairs - k) * a.parts), (unsigned)caches);
+    if (wide) copy_pages_kernel<u32x4_t><<<grid, dim3(256), 0, s>>>(a);
+    else copy_pages_kernel<uint8_t><<<grid, dim3(256), 0, s>>>(a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 }  // namespace zt
