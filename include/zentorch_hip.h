@@ -358,7 +358,9 @@ size_t zt_woq_moe_workspace_size(int64_t T, int64_t H, int64_t topk, int64_t E,
  * counts them.  A page's reference count is the number of table rows that
  * name it; a page with count 0 is free.  Page ids, slots and positions come
  * from the device, so no call can refuse a bad one: each says what it does
- * with it, and none reads or writes outside the arrays for it.
+ * with it, and none reads or writes outside the arrays for it.  Outputs and
+ * workspaces are arrays of their own: one that overlaps an input or another
+ * output is refused.
  */
 typedef struct zt_kv_cache {
   void *k, *v;
@@ -392,7 +394,7 @@ int zt_rotary_embedding(const void *x, int32_t dtype, int64_t T, int64_t H, int6
  * (page * page_size + place in the page).  q [T, H, D], k and v
  * [T, cache->heads, D] in the cache's type, with strides of token and head.
  * A slot outside the cache marks a padding token: nothing is stored for it.
- * Two tokens must not share a slot.
+ * Two tokens must not share a slot.  q_out is contiguous, another array than q.
  */
 int zt_rotary_cache_append(const void *q, int64_t T, int64_t H, const int64_t *q_strides,
                            const void *k, const int64_t *k_strides, const void *v,

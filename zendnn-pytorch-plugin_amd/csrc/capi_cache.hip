@@ -25,6 +25,39 @@ bool divides16(const void *p, std::initializer_list<int64_t> elems, int64_t esiz
   return true;
 }
 
+// The page ops read their inputs while they write their outputs, from many
+// workgroups: no output may lie on an input or on another output.
+struct Span {
+  const void *p;
+  int64_t elems, size;  // of `size` bytes
+};
+bool overlap(const Span &a, const Span &b) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a.p), y = reinterpret_cast<uintptr_t>(b.p);
+  return a.elems > 0 && b.elems > 0 && x < y + (uintptr_t)(b.elems * b.size) &&
+         y < x + (uintptr_t)(a.elems * a.size);
+}
+// Whether s lies on a token's rows [H, D] of a tensor [T, H, D] (it may lie between
+// two tokens', as in a wider buffer that the tensor is a slice of).
+bool touches_rows(const Span &s, const void *x, int64_t T, int64_t H, int64_t D, int64_t ld_token,
+                  int64_t ld_head, int64_t esize) {
+  if (ld_token < 0 || ld_head < 0 || s.elems <= 0) return false;
+  const int64_t token = ((H - 1) * ld_head + D) * esize, ld = ld_token * esize;
+  const int64_t from = (int64_t)(reinterpret_cast<uintptr_t>(s.p) - reinterpret_cast<uintptr_t>(x));
+  const int64_t end = from + s.elems * s.size;
+  // token t's rows are at [t ld, t ld + token): the first that ends past `from`
+  const int64_t t = from < token || ld == 0 ? 0 : (from - token) / ld + 1;
+  return t < T && t * ld < end && t * ld + token > from;
+}
+int check_apart(const char *op, std::initializer_list<Span> in, std::initializer_list<Span> out) {
+  for (auto o = out.begin(); o != out.end(); ++o) {
+    for (const Span &i : in)
+      if (overlap(*o, i)) return api_fail(ZT_EINVAL, "%s: an output overlaps an input", op);
+    for (auto other = out.begin(); other != o; ++other)
+      if (overlap(*o, *other)) return api_fail(ZT_EINVAL, "%s: two outputs overlap", op);
+  }
+  return ZT_OK;
+}
+
 // The sizes and strides of a cache (ZT_OK or the error code).
 int check_cache(const char *op, const zt_kv_cache *c, bool need_data) {
   if (!c) return api_fail(ZT_EINVAL, "%s: null cache", op);
@@ -132,6 +165,10 @@ int zt_cache_extend(const int32_t *block_table, const int32_t *context_lens,
   if ((S * W > 0 && (!block_table || !table_out)) || (pages > 0 && (!ref_counts || !refs_out)) ||
       (S > 0 && (!context_lens || !context_out)) || !cu_seqlens || (T > 0 && (!positions || !slots)))
     return api_fail(ZT_EINVAL, "%s: null tensor pointer", op);
+  if (const int rc = check_apart(
+          op, {{block_table, S * W, 4}, {context_lens, S, 4}, {ref_counts, pages, 4}, {cu_seqlens, S + 1, 4}},
+          {{table_out, S * W, 4}, {context_out, S, 4}, {refs_out, pages, 4}, {positions, T, 8}, {slots, T, 8}}))
+    return rc;
   zt::ExtendArgs a{};
   a.table = block_table, a.ctx = context_lens, a.refs = ref_counts, a.cu = cu_seqlens;
   a.S = (int)S, a.W = (int)W, a.page_size = (int)page_size, a.pages = pages, a.T = T;
@@ -155,6 +192,10 @@ int zt_cache_fork(const int32_t *block_table, const int32_t *context_lens,
       (S > 0 && (!context_lens || !context_out || !parents || !copies)))
     return api_fail(ZT_EINVAL, "%s: null tensor pointer", op);
   if (S == 0 && pages == 0) return ZT_OK;
+  if (const int rc = check_apart(
+          op, {{block_table, S * W, 4}, {context_lens, S, 4}, {ref_counts, pages, 4}, {parents, S, 4}},
+          {{table_out, S * W, 4}, {context_out, S, 4}, {refs_out, pages, 4}, {copies, 2 * S, 4}}))
+    return rc;
   zt::ForkArgs a{};
   a.table = block_table, a.ctx = context_lens, a.refs = ref_counts, a.parents = parents;
   a.S = (int)S, a.W = (int)W, a.page_size = (int)page_size, a.pages = pages;
@@ -180,6 +221,10 @@ int zt_cache_compact(const int32_t *block_table, int64_t entries, const int32_t 
     return api_fail(ZT_EINVAL, "%s: workspace of %zu bytes needed, %zu given", op, need,
                     workspace ? workspace_bytes : (size_t)0);
   if (entries == 0 && pages == 0) return ZT_OK;
+  if (const int rc = check_apart(op, {{block_table, entries, 4}, {ref_counts, pages, 4}},
+                                 {{table_out, entries, 4}, {refs_out, pages, 4}, {copies, pages / 2 * 2, 4},
+                                  {workspace, (int64_t)need, 1}}))
+    return rc;
   zt::CompactArgs a{};
   a.table = block_table, a.refs = ref_counts, a.entries = entries, a.pages = pages;
   a.table_out = table_out, a.refs_out = refs_out, a.copies = copies;
@@ -280,6 +325,10 @@ int zt_paged_attention(const void *q, int64_t T, int64_t H, int64_t ld_token, in
   if (need && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16))
     return api_fail(ZT_EINVAL, "%s: 16-byte aligned workspace of %zu bytes needed, %zu given", op, need,
                     workspace ? workspace_bytes : (size_t)0);
+  const Span to{out, T * H * cache->head_dim, es}, scratch{workspace, (int64_t)need, 1};
+  if (touches_rows(to, q, T, H, cache->head_dim, ld_token, ld_head, es) || overlap(to, scratch) ||
+      touches_rows(scratch, q, T, H, cache->head_dim, ld_token, ld_head, es))
+    return api_fail(ZT_EINVAL, "%s: query, output and workspace must not overlap", op);
   a.q = q, a.q_ld[0] = ld_token, a.q_ld[1] = ld_head;
   a.k = cache->k, a.v = cache->v;
   for (int i = 0; i < 3; ++i) a.k_ld[i] = cache->k_strides[i], a.v_ld[i] = cache->v_strides[i];
