@@ -420,7 +420,8 @@ int zt_rotary_cache_append(const void *q, int64_t T, int64_t H, const int64_t *q
  *
  *  q          [T, H, head_dim] in the cache's type, strides in elements; all
  *             rows (q, cache, out) start on 16 bytes
- *  cu_seqlens [S + 1] int32 ascending from 0; context_lens [S] int32
+ *  cu_seqlens [S + 1] int32 ascending from 0 (held to [0, T]; if it descends
+ *             somewhere, every row is zero); context_lens [S] int32
  *  max_query_len  the longest chunk; it picks the kernels, and too small a
  *             value costs time, not results
  *  head_dim   a multiple of 8, at most 256; S <= 1024

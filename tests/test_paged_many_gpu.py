@@ -8,7 +8,7 @@ import torch
 
 import kv_ref as R
 import zentorch  # noqa: F401
-from test_kv_cache_gpu import BF, F32, check, i32, make, pages_of
+from test_kv_cache_gpu import BF, F32, call, check, i32, make, pages_of
 
 pytestmark = pytest.mark.gpu
 ops = torch.ops.zentorch
@@ -43,6 +43,25 @@ def test_attn_many_items_of_few_sequences(dtype, D):
     """Far more tiles than a round of them, with a window, so that the tiles
     are of like cost and the spans begin in every round."""
     check(make([(5000, 5000), (3, 70), (900, 5000)], 8, 1, D, 16, dtype, seed=D), window=50)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("D,q", [(64, 1), (64, 40), (128, 40), (256, 40)])
+@pytest.mark.parametrize("S", [4, 300])
+def test_attn_cu_seqlens_that_descend(S, D, q, dtype):
+    """Sequences that would overlap: every row is zero.  Ends outside the batch
+    are held to it."""
+    b = make([(q, 50)] * S, 4, 1, D, 16, dtype, seed=S)
+    good = check(b)
+    cu = b["cu"].clone()
+    b["cu"][-1], b["cu"][0] = 2 ** 31 - 1, -5
+    assert torch.equal(call(b), good)
+    for at, value in ((1, 3 * q), (S - 1, 0), (S, -1), (S // 2, -(2 ** 31))):
+        b["cu"] = cu.clone()
+        b["cu"][at] = value
+        assert call(b).eq(0).all(), (at, value)
+    b["cu"] = cu.flip(0).contiguous()
+    assert call(b).eq(0).all()
 
 
 @pytest.mark.parametrize("S", [1025, 4096])

@@ -130,21 +130,25 @@ __device__ __forceinline__ int blocks_of(const KeyRange &k, int UK) {
   return k.end > k.begin ? (k.end + UK - 1) / UK - k.begin / UK : 0;
 }
 
-// Exclusive prefix sum over the workgroup; `part` holds N / 64 values.
+// Exclusive prefix sum over the workgroup of values that are not negative; `part`
+// holds N / 64 values.  `stop`, if given: whether it is set in some thread, where
+// the sums are not to be used.
 template <int N>
-__device__ __forceinline__ int scan(int v, int *part, int *total) {
+__device__ __forceinline__ int scan(int v, int *part, int *total, bool *stop = nullptr) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int x = wave_scan(v);
+  int x = wave_scan(v);
+  if (stop && __ballot(*stop)) x = -1;
   __syncthreads();
   if (lane == 63) part[wave] = x;
   __syncthreads();
-  int before = 0, sum = 0;
+  int before = 0, sum = 0, all = 0;
 #pragma unroll
   for (int w = 0; w < N / 64; ++w) {
     const int y = part[w];
     if (w < wave) before += y;
-    sum += y;
+    sum += y, all |= y;
   }
+  if (stop) *stop = __builtin_amdgcn_readfirstlane(all) < 0;
   *total = __builtin_amdgcn_readfirstlane(sum);
   return before + x - v;
 }
@@ -161,6 +165,7 @@ struct PlanShared {
 };
 
 struct Plan {
+  bool descends;       // cu_seqlens does somewhere: nothing is done
   int items, wg;       // items of a head; this workgroup's place in the order of spans
   int64_t per;         // length of a span
   int64_t from, to;    // this workgroup's
@@ -193,15 +198,20 @@ __device__ __forceinline__ Plan make_plan(const AttnArgs &a, int BM, int UK, con
   for (int i0 = 0; i0 < a.S; i0 += N) {
     const int i = i0 + tid;
     int tiles = 0, total;
+    bool down = false;
     if (i < a.S) {
-      const int T = (int)a.T, q0 = min(max(a.cu[i], 0), T), q = min(max(a.cu[i + 1], q0), T) - q0;
+      const int from = a.cu[i], to = a.cu[i + 1];
+      down = to < from;
+      const int T = (int)a.T, q0 = min(max(from, 0), T), q = min(max(to, q0), T) - q0;
       batch.q0[i] = q0, batch.q[i] = q, batch.n[i] = min(max(a.ctx[i], 0), a.W * a.page_size);
       tiles = (int)((uint32_t)(q * a.group + BM - 1) / (uint32_t)BM);
     }
-    const int before = scan<N>(tiles, sh->part, &total);
+    const int before = scan<N>(tiles, sh->part, &total, &down);
     if (i < a.S) batch.tile_base[i] = p.items + before;
-    p.items += total;
+    p.items += total, p.descends |= down;
   }
+  // Sequences that overlap could be more rows than any count here has room for.
+  if (p.descends) p.items = 0;
   if (tid == 0) batch.tile_base[a.S] = p.items;
   __syncthreads();
   auto cost_of = [&](int x) {
@@ -382,7 +392,8 @@ __device__ __forceinline__ void zero_rows(const AttnArgs &a, const Plan &p, int 
       reinterpret_cast<u32x4_t *>(out)[at] = u32x4_t{0, 0, 0, 0};
     }
   }
-  const int64_t T = a.T, lo = a.S ? batch.q0[0] : T, hi = a.S ? batch.q0[a.S - 1] + batch.q[a.S - 1] : T;
+  const bool none = a.S == 0 || p.descends;
+  const int64_t T = a.T, lo = none ? T : batch.q0[0], hi = none ? T : batch.q0[a.S - 1] + batch.q[a.S - 1];
   const int64_t row = (int64_t)a.H * chunks, n = (lo + T - hi) * row;
   for (int64_t e = (int64_t)blockIdx.x * N + threadIdx.x; e < n; e += (int64_t)gridDim.x * N)
     reinterpret_cast<u32x4_t *>(out)[e < lo * row ? e : e - lo * row + hi * row] = u32x4_t{0, 0, 0, 0};
