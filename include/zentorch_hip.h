@@ -415,8 +415,8 @@ int zt_rotary_cache_append(const void *q, int64_t T, int64_t H, const int64_t *q
  * that sees no key is zero, as is a row past cu_seqlens[S].
  * Scores, softmax and sums are fp32.  What a row does not see may hold anything,
  * infinities and NaN among it.  A row that sees a value that is not finite is
- * not finite there, or, where the rows of a tile see different keys, NaN as a
- * whole.
+ * not finite in that column.  A row with a score of NaN or +inf is NaN; a score
+ * of -inf weighs nothing.
  *
  *  q          [T, H, head_dim] in the cache's type, strides in elements; all
  *             rows (q, cache, out) start on 16 bytes

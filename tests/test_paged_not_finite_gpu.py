@@ -191,3 +191,27 @@ def test_keys_of_minus_infinity(all_, q, D, dtype):
     table = b["table"].clone()
     table[0, gone] = -1
     check(b | dict(table=table), out)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("D", [64, 80, 128, 256])
+@pytest.mark.parametrize("q,n,window", [(1, 300, 0), (4, 300, 0), (7, 300, 3), (12, 300, 0), (40, 300, 0), (40, 300, 9),
+                                        (200, 300, 70), (150, 6007, 0), (4, 6007, 2000)])
+def test_values_that_are_not_finite_by_column(q, n, window, D, dtype):
+    """NaN and infinities in some columns of some values: those columns of the
+    rows that see them are not finite, wherever they lie; every other output
+    keeps its bits."""
+    lens = [(q, n), (min(q, 9), 9)]
+    clean, b = (make(lens, 8, 2, D, 16, dtype, seed=D + q) for _ in "ab")
+    want = call(clean, window=window)
+    pos = torch.arange(n - q, n, device=want.device)
+    hit = torch.zeros(want.shape, dtype=torch.bool, device=want.device)
+    places = [(n - 1, 3, math.inf), (n - q // 2 - 1, 8, math.nan), (n - q // 2 - 1, D - 1, -math.inf),
+              (n - q, 9, math.nan), (n - q - 40, 17, math.nan), (100, 18, math.inf), (5, 10, -math.inf)]
+    for token, column, value in places:
+        put(b["v"], b, 0, [token], value, column)
+        sees = (pos >= token) & ((pos - token < window) if window else True)
+        hit[:q, :, column] |= sees[:, None]
+    out = call(b, window=window)
+    assert torch.equal(out[~hit], want[~hit])
+    assert not torch.isfinite(out[hit]).any()

@@ -86,6 +86,20 @@ __device__ __forceinline__ bool not_finite(u32x4_t x) {
   return bad;
 }
 
+// The 16 bytes' numbers with 0 in place of those that are not finite.
+template <typename T>
+__device__ __forceinline__ u32x4_t finite_of(u32x4_t x) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if constexpr (sizeof(T) == 2) {
+      if ((x[i] & 0x7f800000u) == 0x7f800000u) x[i] &= 0xffffu;
+      if ((x[i] & 0x7f80u) == 0x7f80u) x[i] &= 0xffff0000u;
+    } else if ((x[i] & 0x7f800000u) == 0x7f800000u) {
+      x[i] = 0;
+    }
+  return x;
+}
+
 // 1 KB of zeros: what a lane reads in place of a key or value that is not
 // there, so that weights of zero never meet a NaN or an infinity.
 static __device__ const u32x4_t kZeroRow[64] = {};
@@ -347,8 +361,10 @@ __device__ __forceinline__ uint32_t row_offset(const AttnArgs &a, const uint32_t
 
 // A weight of zero times an infinity or a NaN is a NaN, so where the rows of an
 // item see different keys of a block (an edge of what they see), values that are
-// not finite are taken out of it, and the rows that do see such a key become
-// NaN as a whole.  Whether the item's rows differ, and the keys they all see:
+// not finite are taken out of it.  If there were any, they are added to what the
+// rows that do see them have stored, from memory, at the end of the segment, where
+// that costs the kernels' loops no registers.  Whether the item's rows differ, and
+// the keys they all see:
 struct Shared {
   bool differ;
   int from, to;
@@ -397,6 +413,39 @@ __device__ __forceinline__ void zero_rows(const AttnArgs &a, const Plan &p, int 
   const int64_t row = (int64_t)a.H * chunks, n = (lo + T - hi) * row;
   for (int64_t e = (int64_t)blockIdx.x * N + threadIdx.x; e < n; e += (int64_t)gridDim.x * N)
     reinterpret_cast<u32x4_t *>(out)[e < lo * row ? e : e - lo * row + hi * row] = u32x4_t{0, 0, 0, 0};
+}
+
+// Adds the values that edges left out of the segment's keys [k0, kend), in blocks
+// of n, to four numbers that one row has stored (`at` in its item).
+template <typename T>
+__device__ __forceinline__ void add_edges(const AttnArgs &a, const Segment &seg, const Seq &s, int BM, int at,
+                                          int col, const Shared &shared, const Pages &pages, const char *vbase,
+                                          int k0, int kend, int n) {
+  const int row = seg.tile * BM + at, token = (int)fast_div(row, a.div_group);
+  if (token >= s.q) return;
+  const int pos = s.n - s.q + token, hi = a.causal ? pos + 1 : s.n;
+  const int lo = a.causal && a.window ? (int)max((int64_t)pos + 1 - a.window, (int64_t)0) : 0;
+  for (int k = k0; k < kend; k += n) {
+    if (!shared.edge(k, n)) continue;
+    for (int key = max(k, lo); key < min(k + n, hi); ++key) {
+      const int page = pages.lookup(a, key);
+      if (!pages.there(a, key, page)) continue;
+      const T *v = reinterpret_cast<const T *>(vbase + (uint64_t)row_offset(a, a.v_row, key, page) * 16) + col;
+#pragma unroll 1
+      for (int e = 0; e < 4; ++e) {
+        float x;
+        if constexpr (sizeof(T) == 2) x = bf16_bits_to_f32(v[e]);
+        else x = v[e];
+        if (fabsf(x) < INFINITY) continue;
+        float *part = a.part_o + (seg.slot * BM + at) * a.D + col + e;
+        T *out = static_cast<T *>(a.out) +
+            ((int64_t)(s.q0 + token) * a.H + seg.head * a.group + row - token * a.group) * a.D + col + e;
+        if (!seg.complete) *part += x;
+        else if constexpr (sizeof(T) == 2) *out = (T)f32_to_bf16_bits(bf16_bits_to_f32(*out) + x);
+        else *out += x;
+      }
+    }
+  }
 }
 
 __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32); }

@@ -134,10 +134,10 @@ __global__ __launch_bounds__(kRowThreads, DP <= 128 ? 2 : 1) void paged_attn_row
     }
     f32x4_t o[NT][DT];
     float m[NT], l[NT];
-    bool poisoned[NT];  // the row sees a value that is not finite at an edge
+    bool missed[NT];  // the row sees a value that is not finite at an edge
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      m[t] = -INFINITY, l[t] = 0.f, poisoned[t] = false;
+      m[t] = -INFINITY, l[t] = 0.f, missed[t] = false;
 #pragma unroll
       for (int d = 0; d < DT; ++d) o[t][d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     }
@@ -177,7 +177,7 @@ __global__ __launch_bounds__(kRowThreads, DP <= 128 ? 2 : 1) void paged_attn_row
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
           const bool is = not_finite<T>(vreg[j]);
-          if (is) vreg[j] = u32x4_t{0, 0, 0, 0};
+          if (is) vreg[j] = finite_of<T>(vreg[j]);
           for (uint64_t left = __ballot(is); left; left &= left - 1)
             bad |= 1u << ((64 * j + __builtin_ctzll(left)) / CR);
         }
@@ -222,7 +222,7 @@ __global__ __launch_bounds__(kRowThreads, DP <= 128 ? 2 : 1) void paged_attn_row
         if (bad) {
           const int from = min(max(lo[t] - k0, 0), 32), to = min(max(hi[t] - k0, 0), 32);
           const uint64_t range = (1ull << to) - (1ull << min(from, to));
-          poisoned[t] = poisoned[t] || (live[t] && ((uint32_t)range & bad));
+          missed[t] = missed[t] || (live[t] && ((uint32_t)range & bad));
         }
         if (!whole || __ballot(lo[t] > k0 || hi[t] < k0 + KS)) {
           // bit 16 u + e of `seen`: the lane's e-th key of 16
@@ -305,15 +305,27 @@ __global__ __launch_bounds__(kRowThreads, DP <= 128 ? 2 : 1) void paged_attn_row
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       const float lsum = sum_over_groups(l[t]);
-      if (poisoned[t])
-#pragma unroll
-        for (int d = 0; d < DT; ++d)
-          o[t][d] = f32x4_t{NAN, NAN, NAN, NAN};
       __syncthreads();  // the waves' values and the previous rows are read
       if (lane < 16) sm_m[wave][n] = m[t], sm_l[wave][n] = lsum;
 #pragma unroll
       for (int d = 0; d < DT; ++d)
         *reinterpret_cast<f32x4_t *>(vlds + (n * OP + 16 * d + 4 * g) * 4) = o[t][d];
+      if (__builtin_expect(__ballot(missed[t]) != 0, 0))  // the values that the wave's edges left out
+        for (int k = (seg.b0 + seg.bb) * UK + wave * KS; k < kend; k += UK)
+          for (int key = k; key < k + KS && shared.edge(k, KS); ++key) {
+            const int at = pages.lookup(a, key);
+            if (!pages.there(a, key, at) || !live[t] || key < lo[t] || key >= hi[t]) continue;
+            const T *v = reinterpret_cast<const T *>(vbase + (uint64_t)row_offset(a, a.v_row, key, at) * 16);
+#pragma unroll 1
+            for (int col = 4 * g; col < a.D; col += 16)
+#pragma unroll 1
+              for (int e = 0; e < 4; ++e) {
+                float x;
+                if constexpr (BF) x = bf16_bits_to_f32(v[col + e]);
+                else x = v[col + e];
+                if (!(fabsf(x) < INFINITY)) *reinterpret_cast<float *>(vlds + (n * OP + col + e) * 4) += x;
+              }
+          }
       __syncthreads();
       for (int e = tid; e < 16 * DP / 4; e += kRowThreads) {
         const int row = e / (DP / 4), d = e % (DP / 4) * 4;

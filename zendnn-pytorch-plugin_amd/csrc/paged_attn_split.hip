@@ -166,8 +166,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
 #pragma unroll
       for (int j = 0; j < NL; ++j) {
         const int idx = j * NTH + tid, row = idx / PR, piece = idx % PR;
-        if (edge && not_finite<float>(vreg[j])) {
-          vreg[j] = u32x4_t{0, 0, 0, 0};
+        if (__builtin_expect(edge && not_finite<float>(vreg[j]), 0)) {
+          vreg[j] = finite_of<float>(vreg[j]);
           atomicOr(bad, 1u << row);
         }
         put(smem + st * STAGE, kswz(row), row, piece, split2_cached<true>(kreg[j][0], kreg[j][1]),
@@ -204,7 +204,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
       for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
     float m = -INFINITY, l = 0.f;
     bool far = false;  // of some row of the wave
-    bool poisoned = false;  // the row sees a value that is not finite at an edge
+    bool missed = false;  // the row sees a value that is not finite at an edge
 
     keep(0, k_first, sm_bad);
     int turn = 0;  // t % 3
@@ -220,7 +220,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
       const int turn1 = turn == 2 ? 0 : turn + 1;
       if (shared.differ) {
         if (tid == 0) sm_bad[3 - turn - turn1] = 0;  // the tile after next's
-        poisoned |= rows.sees_of(sm_bad[turn] & there, k0);
+        missed |= rows.sees_of(sm_bad[turn] & there, k0);
       }
       if (rows.see(k0, TK)) {
         const unsigned char *kt = smem + st * STAGE, *vt = kt + 3 * PLANE;
@@ -261,7 +261,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
           far = __ballot(m != -INFINITY && is_far(m * c)) != 0;
         }
         float ref = m == -INFINITY ? 0.f : m * c;
-        if (far) {
+        if (__builtin_expect(far, 0)) {
 #pragma unroll
           for (int e = 0; e < 16; ++e) sc[e] -= is_far(ref) ? m : 0.f;
           ref = is_far(ref) ? 0.f : ref;
@@ -307,12 +307,11 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
       turn = turn1;
     }
     l += other_half(l);
-    if (poisoned)
-#pragma unroll
-      for (int d = 0; d < DT; ++d)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) o[d][e] = __uint_as_float(0x7fc00000u);
     rows.store<float>(a, seg, s, BM, 32 * wave + n, o, m, l);
+    if (__builtin_expect(__ballot(missed) != 0, 0))
+#pragma unroll 1
+      for (int col = 4 * half; col < a.D; col += 8)
+        add_edges<float>(a, seg, s, BM, 32 * wave + n, col, shared, pages, vbase, k_first, k_first + take * TK, TK);
     if (tid == 0 && seg.bb == 0 && !seg.complete) {
       split->slot = seg.slot, split->last = seg.last;
       split->row0 = r0, split->rows = min(BM, s.q * G - r0), split->head = h, split->q0 = s.q0;

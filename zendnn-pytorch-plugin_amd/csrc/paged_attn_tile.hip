@@ -173,21 +173,21 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP <= 1
       for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
     float m = -INFINITY, mc = 0.f, l = 0.f;
     bool far = false;  // of some row of the wave
-    bool poisoned = false;  // the row sees a value that is not finite at an edge
+    bool missed = false;  // the row sees a value that is not finite at an edge
 
     for (int t = 0; t < take; ++t) {
       const int k0 = k_first + t * TK, st = t & 1;
       wait_and_meet();  // the tile is there, and the previous one is done with
       const uint64_t there_next = offsets(k0 + TK, page, t + 1 < take);
       page = lookup(k0 + 2 * TK);
-      if (shared.edge(k0, TK)) {  // the waves look over TK / NW values each
+      if (__builtin_expect(shared.edge(k0, TK), 0)) {  // the waves look over TK / NW values each
         constexpr int ROWS = TK / NW, LANES = 64 / ROWS;
         unsigned char *at = smem + st * 2 * STAGE + STAGE + (wave * ROWS + lane / LANES) * RB;
         bool bad = false;
 #pragma unroll
         for (int j = 0; j < CR / LANES; ++j) {
           u32x4_t *x = reinterpret_cast<u32x4_t *>(at + 16 * (j * LANES + lane % LANES));
-          if (not_finite<T>(*x)) bad = true, *x = u32x4_t{0, 0, 0, 0};
+          if (not_finite<T>(*x)) bad = true, *x = finite_of<T>(*x);
         }
         uint32_t found = 0;
         for (uint64_t left = __ballot(bad); left; left &= left - 1) found |= 1u << (__builtin_ctzll(left) / LANES);
@@ -196,7 +196,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP <= 1
         uint64_t all = 0;
 #pragma unroll
         for (int w = 0; w < NW; ++w) all |= (uint64_t)sm_bad[w] << (ROWS * w);
-        poisoned |= rows.sees_of(all & there, k0);
+        missed |= rows.sees_of(all & there, k0);
       }
       if (rows.see(k0, TK)) {
         const unsigned char *kt = smem + st * 2 * STAGE, *vt = kt + STAGE;
@@ -261,7 +261,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP <= 1
           far = __ballot(is_far(mc)) != 0;
         }
         float ref = mc;
-        if (far) {
+        if (__builtin_expect(far, 0)) {
 #pragma unroll
           for (int u = 0; u < KT; ++u)
 #pragma unroll
@@ -352,12 +352,11 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP <= 1
     // workgroup, takes their place
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     l += other_half(l);
-    if (poisoned)
-#pragma unroll
-      for (int d = 0; d < DT; ++d)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) o[d][e] = __uint_as_float(0x7fc00000u);
     rows.store<T>(a, seg, s, BM, 32 * wave + n, o, m, l);
+    if (__builtin_expect(__ballot(missed) != 0, 0))
+#pragma unroll 1
+      for (int col = 4 * half; col < a.D; col += 8)
+        add_edges<T>(a, seg, s, BM, 32 * wave + n, col, shared, pages, vbase, k_first, k_first + take * TK, TK);
     if (tid == 0 && seg.bb == 0 && !seg.complete) {
       split->slot = seg.slot, split->last = seg.last;
       split->row0 = r0, split->rows = min(BM, s.q * G - r0), split->head = h, split->q0 = s.q0;
