@@ -246,7 +246,16 @@ __device__ __forceinline__ Plan make_plan(const AttnArgs &a, int BM, int UK, con
   // About as many (item, head)s as workgroups, of about one length: each
   // workgroup takes a whole one, and nothing has to be joined.  What is uneven
   // about them the two workgroups of a CU share, so the second half of an
-  // XCD's workgroups takes its items from the far end.
+  // XCD's workgroups takes its items from the far end.  Such are chunks that fill
+  // a budget of tokens (2048 of 32 heads fill the grid of 512), of one sequence or
+  // of several.  Measured, whole items against equal spans, head_dim 128, us:
+  //   2048 tokens behind 6144      273 / 283    2048 behind 30000       1043 / 1110
+  //   2 x 1024 behind 2048         119 / 132    4 x 512 behind 2048      107 / 126
+  //   8 x 256 behind 2048          101 / 116    16 x 128 behind 2048     101 / 99
+  // Below 31 / 32 of the grid the workgroups without an item cost one long
+  // sequence more than that (1984 tokens behind 6144, 496 items: 272 / 275; 1920:
+  // 273 / 265; 1792: 271 / 249), where several short ones would gain further
+  // (4 x 448 behind 2048: 105 / 117).
   const int pairs = p.items * a.KV, grid = (int)gridDim.x;
   if (p.items <= N && pairs <= grid && 32 * (int64_t)pairs >= 31 * (int64_t)grid) {
     if (tid == 0) sh->most = 0;
