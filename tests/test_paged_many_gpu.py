@@ -46,6 +46,15 @@ def test_attn_many_items_of_few_sequences(dtype, D):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("D", [64, 96, 128, 256])
+@pytest.mark.parametrize("rows", [16, 17, 32, 33, 40, 48, 49, 64, 65, 80])
+def test_attn_tens_of_rows(rows, D, dtype):
+    """Chunks around the borders between the kernels for few and for many rows."""
+    check(make([(rows, 300), (rows, rows), (1, 90)], 2, 2, D, 16, dtype, seed=rows))
+    check(make([(-(-rows // 4), 700)], 8, 2, D, 16, dtype, seed=rows + D), window=333)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("D,q", [(64, 1), (64, 40), (128, 40), (256, 40)])
 @pytest.mark.parametrize("S", [4, 300])
 def test_attn_cu_seqlens_that_descend(S, D, q, dtype):

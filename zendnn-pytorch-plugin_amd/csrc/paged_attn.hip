@@ -453,15 +453,24 @@ hipError_t launch_rows_of(const AttnArgs &a, int grid, hipStream_t s) {
 
 // Rows of one cache head up to which the row kernel is taken.  Measured, row
 // against tile kernel, 8 cache heads, 32 sequences of 2048 tokens, us:
-//   bf16  head_dim 64:  16 rows 34 / 33   32 rows 38 / 36    64 rows 78 / 38
-//         head_dim 128: 16 rows 57 / 56   32 rows 88 / 57    64 rows 121 / 64
-//         head_dim 256: 16 rows 126 / 111 32 rows 278 / 113
-//   fp32  head_dim 64:  16 rows 55 / 88   32 rows 76 / 88    64 rows 156 / 104
-//         head_dim 128: 16 rows 106 / 273 32 rows 166 / 273  64 rows 504 / 278
-//         head_dim 256: 16 rows 228 / 681 32 rows 837 / 681
+//   bf16  head_dim 64:  16 rows 34 / 35   32 rows 45 / 36    64 rows 82 / 42
+//         head_dim 128: 16 rows 57 / 56   32 rows 82 / 59    64 rows 153 / 65
+//         head_dim 256: 16 rows 127 / 119 32 rows 169 / 121  64 rows 326 / 123
+//   fp32  head_dim 64:  16 rows 54 / 92   32 rows 79 / 96    48 rows 128 / 115
+//         head_dim 128: 32 rows 179 / 297 64 rows 264 / 303  80 rows 428 / 307
+//         head_dim 256: 32 rows 354 / 766 48 rows 580 / 776  64 rows 669 / 778
+// and at the last two's borders 4 of 32768 503 / 580 (64 rows of 128) and 1004 / 1528
+// (48 of 256), 64 of 500 178 / 190 and 360 / 440, where 64 rows of 256 are 472 / 441.
 // On few long sequences (4 of 32768) the row kernel gains at 16 rows in bf16 too:
 // 99 against 111 us at head_dim 128.
-int rows_most(const AttnArgs &a) { return a.dtype == ZT_DT_F32 && a.D <= 128 ? 32 : 16; }
+int rows_most(const AttnArgs &a) {
+  if (a.dtype == ZT_DT_BF16) return 16;
+  return a.D <= 64 ? 32 : a.D <= 128 ? 64 : 48;
+}
+// Rows of an item of the row kernel: 16, or 32 where two times 16 share the keys.
+int row_item(const AttnArgs &a, int64_t rows) {
+  return a.dtype == ZT_DT_F32 && a.D <= 128 && rows > 16 ? 32 : 16;
+}
 
 struct Shape {
   bool tiles;
@@ -474,7 +483,7 @@ double blocks_most(const AttnArgs &a, bool tiles) {
 }
 Shape shape_of(const AttnArgs &a) {
   const int64_t rows = std::min(std::max<int64_t>(a.max_q, 1), a.T) * (a.H / a.KV);
-  Shape p{rows > rows_most(a), rows <= 16 ? 16 : 32, kRowGrid};
+  Shape p{rows > rows_most(a), row_item(a, rows), kRowGrid};
   if (p.tiles) p.bm = tile_rows(a), p.grid = tile_grid(a);
   // no more workgroups than there can be blocks
   const double most = items_most(a, p.bm) * a.KV * blocks_most(a, p.tiles);
