@@ -61,7 +61,7 @@ __device__ __forceinline__ float sum_over_groups(float x) {
 //
 // Measured (32 query and 8 cache heads of 128, bf16): two sequences of 131072
 // tokens 172-173 us, 6.2 TB/s; 64 ragged ones of up to 8192 129 us, 5.9
-// TB/s (a large copy reaches 4.9).  One of 777: 10.8 us, round trips to memory.
+// TB/s (a large copy reaches 4.9).  One of 777: 10.9 us, round trips to memory.
 template <typename T, int DP, int NT>
 __global__ __launch_bounds__(kRowThreads, DP <= 128 ? 2 : 1) void paged_attn_row_kernel(AttnArgs a) {
   using Cost = RowCost;

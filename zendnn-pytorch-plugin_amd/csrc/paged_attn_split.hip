@@ -87,14 +87,15 @@ struct SplitCost {
 // paged_attn_tile.hip's kernel does it for bf16, in tiles of 32 keys.
 //
 // An fp32 MFMA runs at a sixteenth of the bf16 rate, so every number goes in
-// three bf16 parts and a product in six MFMAs, 2.7 times as fast, with every
-// term fp32 can hold.  Keys and values are split once per workgroup on their
+// three bf16 parts and a product in six MFMAs, 2.7 times as fast, with all
+// but the smallest terms.  Keys and values are split once per workgroup on their
 // way to LDS (global memory -> registers while a tile is worked on -> three
 // planes of the next stage), queries once per item, weights as they are made.
 //
-// Measured: eight whole sequences of up to 500 tokens, 16 heads of 64, 53-55 us
-// (fp32 MFMAs: 75); four of 600 to 2000 tokens, 16 heads on 4, head_dim 128 104
-// us (116), head_dim 80 66 us (85).  Past 128 three planes do not fit LDS twice.
+// Measured: eight whole sequences of up to 500 tokens, 16 heads of 64, 55 us (fp32
+// MFMAs: 75); four causal prompts of 729 to 1765 tokens, 16 heads on 4: head_dim 64 109
+// us, 80 144, 128 210 (109 TFLOP/s; a large fp32 product of the library 143).  Past 128
+// three planes do not fit LDS twice.
 template <int DP, int DC, int NW>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2))) void paged_attn_split_kernel(
     AttnArgs a) {

@@ -26,8 +26,8 @@ __device__ __forceinline__ void wait_and_meet() {
 
 // The cost of a block, and of an item's beginning and end.  A block of few rows
 // takes nearly as long as a full one: in bf16 it waits for its keys (1.9 against
-// 2.2 us, two workgroups a CU), in fp32 for its one wave's share of the matrix
-// operations (4.6 us), which the other workgroup's wave on that SIMD halves.
+// 2.2 us, two workgroups a CU); in fp32 (past head_dim 128, one workgroup a CU) each
+// wave does its own rows' matrix operations, whatever the others have.
 // An item's two ends take 5 to 6 us.  In bf16 spans have four blocks at least:
 // what a part of 128 rows has to write and the join to read is four blocks'
 // bytes (32 tokens of 32 heads behind 2048: 40 us without, 35 with).
@@ -41,10 +41,11 @@ struct TileCost {
 
 // NW waves of 32 rows each against a span of the keys of one cache head.
 //
-// Bound by the matrix pipes and, beside them, by the exponentials.  All waves
-// share tiles of TK keys and values (64, or 32 in fp32) that arrive in LDS by
-// DMA, two tiles deep: while one is worked on the next is on its way, with one
-// barrier per tile.
+// Bound by the matrix operations with their LDS reads, and by the transfers, whose
+// writes to LDS and waits they hide only in part (figures below).  All waves share
+// tiles of TK keys and values (64, or 32 in fp32) that arrive in LDS by DMA, two
+// tiles deep: while one is worked on the next is on its way, with one barrier per
+// tile.
 //
 // The products are taken transposed, S^T = K Q^T and O^T = V^T P^T, on 32x32
 // MFMAs with the rows as columns: a lane holds 16 keys of one row per tile of
@@ -67,8 +68,9 @@ struct TileCost {
 // taken of the rounded ones, so that a row's weights still add up to one.
 //
 // Measured (32 query and 8 cache heads of 128, bf16): 2048 tokens behind 6144
-// 266-277 us, 0.9 PFLOP/s (a large product of the library reaches 1.2 on the
-// same card); the matrix operations with their LDS reads alone 163.
+// 264-275 us, 0.9 PFLOP/s (a large product of the library reaches 1.2 on the
+// same card); copies without the transfers 231, without the exponentials 261, without
+// both 218 beside 272.
 template <typename T, int DP, int DC, int NW>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP <= 128 ? 2 : 1, DP <= 128 ? 2 : 1))) void paged_attn_tile_kernel(AttnArgs a) {
   using Cost = TileCost<T>;
