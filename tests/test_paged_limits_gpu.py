@@ -1,4 +1,5 @@
-"""Calls of the paged-cache ops whose work is more than one launch can count."""
+"""Calls of the paged-cache ops at the edge of what they take: work that is more
+than one launch can count, tables whose rows lie on each other."""
 import pytest
 import torch
 
@@ -47,3 +48,17 @@ def test_rotary_of_many_elements():
         assert torch.equal(y[t], turned), t
     y[T // 2], y[T - 1] = row, row
     assert (y.view(torch.int16) == row.view(torch.int16)).all()
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rotary_table_of_overlapping_rows(interleaved):
+    """One row expanded to every position, and rows that begin inside the one
+    before, as any other table."""
+    x = torch.randn(6, 3, 16, device=DEV)
+    pos = torch.arange(6, device=DEV)
+    one = torch.randn(1, 8, device=DEV)
+    flat = torch.randn(40, device=DEV)
+    for table in (one.expand(9, 8), flat.as_strided((9, 8), (3, 1)), torch.randn(9, 16, device=DEV)[:, ::2],
+                  torch.randn(8, 9, device=DEV).t()):
+        got = ops.zentorch_rotary_embedding(x, pos, table, interleaved=interleaved)
+        assert torch.equal(got, ops.zentorch_rotary_embedding(x, pos, table.contiguous(), interleaved=interleaved))

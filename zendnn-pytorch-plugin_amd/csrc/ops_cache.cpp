@@ -69,7 +69,9 @@ at::Tensor table_rows(const at::Tensor &cos_sin, const at::Tensor &like, const c
   TORCH_CHECK(cos_sin.scalar_type() == at::kFloat && cos_sin.dim() == 2, op,
               ": cos_sin must be a 2D float32 tensor [length, rotated], got ",
               cos_sin.scalar_type(), " ", cos_sin.sizes());
-  return rows_of(cos_sin, false);
+  const at::Tensor t = rows_of(cos_sin, false);
+  // rows that lie on each other (an expanded table) are laid out
+  return t.size(0) > 1 && t.stride(0) < t.size(1) ? t.clone(at::MemoryFormat::Contiguous) : t;
 }
 
 at::Tensor long_1d(const at::Tensor &t, int64_t n, const at::Tensor &like, const char *op,
