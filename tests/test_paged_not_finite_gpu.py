@@ -175,6 +175,16 @@ def test_huge_scores(size, q, long, D, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("q,long", KINDS)
+def test_small_values(q, long, D, dtype):
+    """Values of 2^-100 and less come out as accurate as others."""
+    b = make(lens_of(q, long)[:3], 8, 2, D, 64, dtype, seed=D + 5, poison=False)
+    b["v"] = b["v"] * 2.0 ** -100
+    check(b)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("D", [64, 80, 128, 256])
 @pytest.mark.parametrize("q", [1, 4, 12, 40, 200])
 @pytest.mark.parametrize("all_", [300, 5000])

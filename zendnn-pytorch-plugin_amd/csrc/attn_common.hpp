@@ -50,11 +50,11 @@ __device__ __forceinline__ float factor(float from, float to, float c) {
   return __builtin_amdgcn_exp2f(fminf(from * c - to * c, 0.f));
 }
 
-// Weights are held times 2^-40, their sums too, and the division takes it out
-// again: with up to 2^30 keys of weights up to 2^8 the running sums stay below
-// the largest value, so that no finite value becomes infinite on the way.  (A
-// weight underflows at 2^-86 of the largest.)
-constexpr int kHeadroom = 40;
+// Weights are held times 2^-16, their sums too, and the division takes it out
+// again: weights go up to 2^8, and as long as those of the largest values add up
+// to less than 2^16, no finite value becomes infinite on the way.  More headroom
+// would take it from small values: those of 2^-110 and more keep all their digits.
+constexpr int kHeadroom = 16;
 constexpr float kWeight = 1.f / (1ull << kHeadroom);
 
 typedef short s16x4_t __attribute__((ext_vector_type(4)));

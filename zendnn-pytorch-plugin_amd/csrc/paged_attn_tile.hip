@@ -276,7 +276,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP <= 1
         // the SIMD's other one, so that the two take turns at matrix operations
         // and weights (a chunk of 2048 tokens behind 6144: 283 -> 276 us).
         __builtin_amdgcn_s_setprio(1);
-        // The headroom goes into the exponent in bf16 (its rounding there, 2^-19,
+        // The headroom goes into the exponent in bf16 (its rounding there, 2^-20,
         // is far below the weights'), and is a product in fp32.
         if constexpr (BF) ref += kHeadroom;
         auto weight = [&](int e) {
