@@ -43,8 +43,8 @@ __device__ __forceinline__ Parts split2_cached(uint32_t a, uint32_t b) {
   return s;
 }
 
-// The same for a query, all parts cut short and none of them zero (the smallest
-// normal number instead, which adds nothing to a score): an infinite key's score
+// The same for a query, all parts cut short and none of them zero (bf16's smallest
+// number instead, 2^-133, which adds nothing to a score): an infinite key's score
 // then is infinite with the product's sign, not the NaN of infinities of both
 // signs or of one times 0.  (A query of 0 against an infinite key is a NaN.)
 __device__ __forceinline__ Parts split2_query(uint32_t a, uint32_t b) {
@@ -57,7 +57,7 @@ __device__ __forceinline__ Parts split2_query(uint32_t a, uint32_t b) {
     s.p[p] = __builtin_amdgcn_perm(wb, wa, 0x07060302u);
     ra -= __uint_as_float(wa), rb -= __uint_as_float(wb);
   }
-  const auto least = __builtin_bit_cast(u16x2_t, (s.p[0] & 0x80008000u) | 0x00800080u);
+  const auto least = __builtin_bit_cast(u16x2_t, (s.p[0] & 0x80008000u) | 0x00010001u);
 #pragma unroll
   for (int p = 1; p < 3; ++p)
     s.p[p] = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, s.p[p]), least));
