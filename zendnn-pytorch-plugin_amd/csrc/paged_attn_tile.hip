@@ -68,7 +68,7 @@ struct TileCost {
 // taken of the rounded ones, so that a row's weights still add up to one.
 //
 // Measured (32 query and 8 cache heads of 128, bf16): 2048 tokens behind 6144
-// 264-275 us, 0.9 PFLOP/s (a large product of the library reaches 1.2 on the
+// 264-281 us, 0.9 PFLOP/s (a large product of the library reaches 1.2 on the
 // same card); copies without the transfers 231, without the exponentials 261, without
 // both 218 beside 272.
 template <typename T, int DP, int DC, int NW>
