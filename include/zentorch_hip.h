@@ -496,6 +496,69 @@ int zt_cache_copy_pages(void *const *caches, int64_t n_caches, int64_t pages, in
                         int64_t page_stride_bytes, const int32_t *copies, int64_t n_copies,
                         zt_stream_t stream);
 
+/*
+ * A layer's key / value cache held in 4 bits, in the MXFP4 format.  A head row
+ * is cut into blocks of 32 numbers, the last one filled with zeros; blocks =
+ * ceil(head_dim / 32).  A block has a scale 2^E, kept as the byte E + 127, and
+ * 32 codes of 4 bits, the element of even index in a byte's low half: bit 3 is
+ * the sign, the others name one of 0, 0.5, 1, 1.5, 2, 3, 4, 6, which the scale
+ * multiplies.  Writing picks the E for which the block's largest magnitude is
+ * at least 3.5 and less than 7 scales, held to -125 .. 125, and for each number
+ * the nearest code (of two equally near ones the even one; magnitudes past 6
+ * scales take 6): off by a seventh of the block's largest number at most.  A
+ * block with an infinity or a NaN is written as codes of 0 under the byte 255.
+ * Read, the bytes 253 .. 255 stand for NaN.
+ *
+ * codes [pages, heads, page_size, 16 blocks] bytes, each row on 16 bytes;
+ * scales [pages, heads, page_size, blocks] bytes, anywhere.  The other tensors
+ * are bf16 or fp32.  zt_cache_extend, _fork and _compact serve this cache as
+ * the other one, and zt_cache_copy_pages its codes and its scales.
+ */
+typedef struct zt_kv_cache_mxfp4 {
+  void *k, *v;
+  uint8_t *k_scales, *v_scales;
+  int64_t pages, heads, page_size, head_dim; /* head_dim: a multiple of 8 up to 256 */
+  int64_t k_strides[3], v_strides[3];              /* page, head, token, in bytes */
+  int64_t k_scale_strides[3], v_scale_strides[3];
+} zt_kv_cache_mxfp4;
+
+/*
+ * zt_rotary_cache_append into a cache held in 4 bits.  q_out is fp32's result
+ * rounded once, as there; a key is quantised as its rotation comes out exactly,
+ * without a rounding before.  A row without a position (past the table) is NaN
+ * there too.  Tokens without a slot leave the cache alone, and two tokens must
+ * not share a slot.  The cache's four arrays must not overlap.
+ */
+int zt_rotary_cache_append_mxfp4(const void *q, int32_t dtype, int64_t T, int64_t H, const int64_t *q_strides,
+                                 const void *k, const int64_t *k_strides, const void *v,
+                                 const int64_t *v_strides, const int64_t *positions,
+                                 const float *table, int64_t length, int64_t R, int64_t ld_table,
+                                 int32_t interleaved, const int64_t *slots,
+                                 const zt_kv_cache_mxfp4 *cache, void *q_out, zt_stream_t stream);
+
+/*
+ * The keys and values that the cache holds in slots [n], as [n, heads,
+ * head_dim] contiguous bf16 or fp32, both of which hold them exactly.  A slot
+ * outside the cache gives zeros; slots may repeat.
+ */
+int zt_cache_read_mxfp4(const zt_kv_cache_mxfp4 *cache, const int64_t *slots, int64_t n, int32_t dtype,
+                        void *k_out, void *v_out, zt_stream_t stream);
+
+/*
+ * zt_paged_attention over a cache held in 4 bits: the same sequences, masks,
+ * bounds and rules, with q and out in `dtype`.  Keys and values take part as
+ * the numbers that their codes stand for, without another rounding.
+ */
+int zt_paged_attention_mxfp4(const void *q, int32_t dtype, int64_t T, int64_t H, int64_t ld_token, int64_t ld_head,
+                             const zt_kv_cache_mxfp4 *cache, const int32_t *block_table, int64_t S, int64_t W,
+                             const int32_t *cu_seqlens, const int32_t *context_lens, int64_t max_query_len,
+                             int32_t causal, int64_t window, float scale, void *out, void *workspace,
+                             size_t workspace_bytes, zt_stream_t stream);
+
+size_t zt_paged_attention_mxfp4_workspace_size(int64_t T, int64_t H, int32_t dtype,
+                                               const zt_kv_cache_mxfp4 *cache, int64_t S, int64_t W,
+                                               int64_t max_query_len);
+
 /* Message of the calling thread's last failed call ("" if none). */
 const char *zt_last_error_string(void);
 

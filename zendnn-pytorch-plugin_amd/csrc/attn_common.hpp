@@ -522,6 +522,22 @@ struct Rows32 {
   }
 };
 
+// The partial results of a launch of `grid` workgroups with items of bm rows, in a
+// workspace; and the launch that joins them (paged_attn.hip).
+inline size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+inline size_t parts_bytes(const AttnArgs &a, int grid, int bm) {
+  const size_t slots = 2 * (size_t)grid * bm;
+  return up256(grid * sizeof(Split)) + up256(slots * 2 * sizeof(float)) + slots * a.D * sizeof(float);
+}
+inline void lay_parts(AttnArgs *a, void *workspace, int grid, int bm) {
+  char *at = static_cast<char *>(workspace);
+  a->item_rows = bm;
+  a->splits = at, at += up256(grid * sizeof(Split));
+  a->part_ml = reinterpret_cast<float *>(at), at += up256(2 * (size_t)grid * bm * 2 * sizeof(float));
+  a->part_o = reinterpret_cast<float *>(at);
+}
+hipError_t launch_join(const AttnArgs &a, int grid, hipStream_t s);
+
 // The tile kernel (paged_attn_tile.hip): its rows per item and workgroups.
 int tile_rows(const AttnArgs &a);
 int tile_grid(const AttnArgs &a);

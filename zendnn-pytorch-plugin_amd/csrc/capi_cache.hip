@@ -1,62 +1,10 @@
 // extern "C" entry points of the paged key / value cache (declared in
 // include/zentorch_hip.h): argument validation and launch.
-#include <cmath>
-
-#include "zt_cache.hpp"
+#include "capi_cache.hpp"
 
 namespace {
 
-using zt::api_fail;
-
-int hip_status(hipError_t e, const char *what) {
-  if (e == hipSuccess) return ZT_OK;
-  return api_fail(ZT_EHIP, "%s: HIP error %d (%s)", what, (int)e, hipGetErrorString(e));
-}
-
-bool is_float_dt(int dt) { return dt == ZT_DT_F32 || dt == ZT_DT_BF16; }
-
-using zt::kMaxRows;
-using zt::kMaxSeqs;
-
-bool divides16(const void *p, std::initializer_list<int64_t> elems, int64_t esize) {
-  if (reinterpret_cast<uintptr_t>(p) % 16) return false;
-  for (int64_t e : elems)
-    if (e * esize % 16) return false;
-  return true;
-}
-
-// The page ops read their inputs while they write their outputs, from many
-// workgroups: no output may lie on an input or on another output.
-struct Span {
-  const void *p;
-  int64_t elems, size;  // of `size` bytes
-};
-bool overlap(const Span &a, const Span &b) {
-  const uintptr_t x = reinterpret_cast<uintptr_t>(a.p), y = reinterpret_cast<uintptr_t>(b.p);
-  return a.elems > 0 && b.elems > 0 && x < y + (uintptr_t)(b.elems * b.size) &&
-         y < x + (uintptr_t)(a.elems * a.size);
-}
-// Whether s lies on a token's rows [H, D] of a tensor [T, H, D] (it may lie between
-// two tokens', as in a wider buffer that the tensor is a slice of).
-bool touches_rows(const Span &s, const void *x, int64_t T, int64_t H, int64_t D, int64_t ld_token,
-                  int64_t ld_head, int64_t esize) {
-  if (ld_token < 0 || ld_head < 0 || s.elems <= 0) return false;
-  const int64_t token = ((H - 1) * ld_head + D) * esize, ld = ld_token * esize;
-  const int64_t from = (int64_t)(reinterpret_cast<uintptr_t>(s.p) - reinterpret_cast<uintptr_t>(x));
-  const int64_t end = from + s.elems * s.size;
-  // token t's rows are at [t ld, t ld + token): the first that ends past `from`
-  const int64_t t = from < token || ld == 0 ? 0 : (from - token) / ld + 1;
-  return t < T && t * ld < end && t * ld + token > from;
-}
-int check_apart(const char *op, std::initializer_list<Span> in, std::initializer_list<Span> out) {
-  for (auto o = out.begin(); o != out.end(); ++o) {
-    for (const Span &i : in)
-      if (overlap(*o, i)) return api_fail(ZT_EINVAL, "%s: an output overlaps an input", op);
-    for (auto other = out.begin(); other != o; ++other)
-      if (overlap(*o, *other)) return api_fail(ZT_EINVAL, "%s: two outputs overlap", op);
-  }
-  return ZT_OK;
-}
+using namespace zt;
 
 // The sizes and strides of a cache (ZT_OK or the error code).
 int check_cache(const char *op, const zt_kv_cache *c, bool need_data) {
@@ -73,25 +21,6 @@ int check_cache(const char *op, const zt_kv_cache *c, bool need_data) {
   if (need_data && c->pages > 0 && (!c->k || !c->v))
     return api_fail(ZT_EINVAL, "%s: null cache pointer", op);
   return ZT_OK;
-}
-
-int check_rotary(const char *op, const void *x, int64_t T, int64_t H, int64_t D,
-                 const int64_t *positions, const float *table, int64_t length, int64_t R,
-                 int64_t ld_table, const void *out) {
-  if (T < 0 || H <= 0 || D <= 0) return api_fail(ZT_EINVAL, "%s: need T >= 0 and heads, head_dim > 0", op);
-  if (R <= 0 || R % 2 || R > D)
-    return api_fail(ZT_EINVAL, "%s: the table's width (%lld) must be even, positive and at most "
-                    "head_dim = %lld", op, (long long)R, (long long)D);
-  if (length < 0 || ld_table < R) return api_fail(ZT_EINVAL, "%s: bad table length or row stride", op);
-  if (T > 0 && (!x || !positions || !out || (length > 0 && !table)))
-    return api_fail(ZT_EINVAL, "%s: null tensor pointer", op);
-  return ZT_OK;
-}
-
-// Grids are counted in 32 bits.
-bool too_many(int64_t T, int64_t heads, int64_t D) {
-  return heads > INT32_MAX / 4 || D > (1 << 20) || heads * D > INT32_MAX ||
-         (double)T * (double)heads * (double)D >= 256.0 * 2147483647.0;
 }
 
 }  // namespace
@@ -263,29 +192,10 @@ int zt_cache_copy_pages(void *const *caches, int64_t n_caches, int64_t pages, in
 }
 
 // The checked arguments of an attention call, without its pointers.
-static int attn_args(const char *op, int64_t T, int64_t H, const zt_kv_cache *cache, int64_t S,
-                     int64_t W, int64_t max_query_len, int32_t causal, int64_t window,
-                     zt::AttnArgs *a) {
+static int checked_attn(const char *op, int64_t T, int64_t H, const zt_kv_cache *cache, int64_t S,
+                        int64_t W, int64_t max_query_len, int32_t causal, int64_t window, AttnArgs *a) {
   if (const int rc = check_cache(op, cache, false)) return rc;
-  if (T < 0 || H <= 0 || S < 0 || W < 0 || max_query_len < 0)
-    return api_fail(ZT_EINVAL, "%s: need T, S, W, max_query_len >= 0 and heads > 0", op);
-  if (H % cache->heads)
-    return api_fail(ZT_EINVAL, "%s: query heads (%lld) must be a multiple of the cache's (%lld)", op,
-                    (long long)H, (long long)cache->heads);
-  if (cache->head_dim % 8 || cache->head_dim > 256)
-    return api_fail(ZT_EUNSUPPORTED, "%s: head_dim must be a multiple of 8 up to 256, got %lld", op,
-                    (long long)cache->head_dim);
-  if (window < 0 || (window && !causal))
-    return api_fail(ZT_EINVAL, "%s: a window (%lld) must not be negative and needs causal", op,
-                    (long long)window);
-  if (H > 65535 || S > kMaxSeqs || T > (1 << 24) || T * H > INT32_MAX / 2 || W > (1 << 24) ||
-      cache->page_size > (1 << 24) || W * cache->page_size > (1 << 30))
-    return api_fail(ZT_EUNSUPPORTED, "%s: at most 65535 heads, %lld sequences, 2^24 tokens, 2^30 / "
-                    "heads rows and a table of 2^30 tokens a sequence", op, (long long)kMaxSeqs);
-  *a = zt::AttnArgs{};
-  a->T = T, a->H = (int)H, a->KV = (int)cache->heads, a->D = (int)cache->head_dim;
-  a->S = (int)S, a->W = (int)W, a->page_size = (int)cache->page_size, a->pages = cache->pages;
-  a->dtype = cache->dtype, a->max_q = max_query_len, a->causal = causal != 0, a->window = window;
+  if (const int rc = attn_args(op, T, H, cache, S, W, max_query_len, causal, window, a)) return rc;
   if (T > 0 && !zt::paged_attn_countable(*a))
     return api_fail(ZT_EUNSUPPORTED, "%s: too many tokens over too long tables for one call", op);
   return ZT_OK;
@@ -294,7 +204,7 @@ static int attn_args(const char *op, int64_t T, int64_t H, const zt_kv_cache *ca
 size_t zt_paged_attention_workspace_size(int64_t T, int64_t H, const zt_kv_cache *cache, int64_t S,
                                          int64_t W, int64_t max_query_len) {
   zt::AttnArgs a;
-  if (attn_args("zt_paged_attention_workspace_size", T, H, cache, S, W, max_query_len, 0, 0, &a)) return 0;
+  if (checked_attn("zt_paged_attention_workspace_size", T, H, cache, S, W, max_query_len, 0, 0, &a)) return 0;
   return zt::paged_attn_workspace(a);
 }
 
@@ -305,7 +215,7 @@ int zt_paged_attention(const void *q, int64_t T, int64_t H, int64_t ld_token, in
                        void *out, void *workspace, size_t workspace_bytes, zt_stream_t stream) {
   static const char *op = "zt_paged_attention";
   zt::AttnArgs a;
-  if (const int rc = attn_args(op, T, H, cache, S, W, max_query_len, causal, window, &a)) return rc;
+  if (const int rc = checked_attn(op, T, H, cache, S, W, max_query_len, causal, window, &a)) return rc;
   if (!std::isfinite(scale)) return api_fail(ZT_EINVAL, "%s: scale must be finite", op);
   if (T == 0) return ZT_OK;
   if (!q || !out || !cu_seqlens || (S > 0 && !context_lens) || (S * W > 0 && !block_table) ||

@@ -1,0 +1,254 @@
+// Writing and reading a key / value cache held in 4 bits, for gfx950.  The
+// format is described in mx4.hpp.
+//
+// Both kernels move bytes: they are bound by HBM where the operands are large and
+// by their launch where they are small.  Slots and positions come from the device
+// and are checked before they are used as an address.
+#include "mx4.hpp"
+
+namespace zt {
+
+namespace {
+
+constexpr int kThreads = 256;
+
+// Eight consecutive elements as floats.
+template <typename T, bool WIDE>
+__device__ __forceinline__ void load8(const T *p, float (&f)[8]) {
+  if constexpr (sizeof(T) == 2 && WIDE) {
+    const u32x4_t v = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t *>(p));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[2 * i] = __uint_as_float(v[i] << 16), f[2 * i + 1] = __uint_as_float(v[i] & 0xffff0000u);
+  } else if constexpr (WIDE) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const f32x4_t v = __builtin_nontemporal_load(reinterpret_cast<const f32x4_t *>(p) + j);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f[4 * j + i] = v[i];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if constexpr (sizeof(T) == 2) f[i] = bf16_bits_to_f32(p[i]);
+      else f[i] = p[i];
+  }
+}
+
+// Elements e0 .. e0 + 7 of a row turned to position p: of a pair (a, b) of
+// frequency i, a cos - b sin or b cos + a sin.  The pairs are (x[i], x[R / 2 + i])
+// or, interleaved, (x[2 i], x[2 i + 1]); what is past R is as it was, and so is
+// the row of a negative position.  WIDE: no border of a half lies inside eight
+// elements.  A thread computes its eight elements only, and reads the pairs' other
+// ones beside them, which a neighbour has read.
+template <typename A, typename T, bool IL, bool WIDE, typename Args>
+__device__ __forceinline__ void rotated(const Args &a, const T *src, int e0, int64_t p, A (&y)[8]) {
+  float x[8];
+  load8<T, WIDE>(src + e0, x);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y[i] = x[i];
+  const int R = a.R, half = R / 2;
+  if (p < 0 || e0 >= R) return;
+  const bool inside = p < a.length;
+  const float *row = a.table + p * a.table_ld;
+  const float nan = __uint_as_float(0x7fc00000u);  // no such position: it does not pass unseen
+  if constexpr (IL) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+      const int f = (e0 + i) / 2;
+      if (!WIDE && f >= half) continue;
+      const A c = inside ? row[f] : nan, s = inside ? row[half + f] : nan;
+      y[i] = (A)x[i] * c - (A)x[i + 1] * s, y[i + 1] = (A)x[i + 1] * c + (A)x[i] * s;
+    }
+  } else if constexpr (WIDE) {
+    const bool second = e0 >= half;
+    const int f = second ? e0 - half : e0;
+    float z[8];
+    load8<T, WIDE>(src + (second ? f : e0 + half), z);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const A c = inside ? row[f + i] : nan, s = inside ? row[half + f + i] : nan;
+      const A other = (A)z[i] * s;
+      y[i] = (A)x[i] * c + (second ? other : -other);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int e = e0 + i;
+      if (e >= R) break;
+      const bool second = e >= half;
+      const int f = second ? e - half : e;
+      float z;
+      if constexpr (sizeof(T) == 2) z = bf16_bits_to_f32(src[second ? f : e + half]);
+      else z = src[second ? f : e + half];
+      const A c = inside ? row[f] : nan, s = inside ? row[half + f] : nan;
+      const A other = (A)z * s;
+      y[i] = (A)x[i] * c + (second ? other : -other);
+    }
+  }
+}
+
+// y in fp32, with the last bit set where that is not exact: such a number lies on
+// the same side of every border between two codes (and of 1.75 times a power of
+// two) as y, because those have no digits that far down.
+__device__ __forceinline__ float sticky(double y) {
+  const float f = (float)y;
+  const double back = f;
+  uint32_t b = __float_as_uint(f);
+  if (back != y) b = (fabs(back) > fabs(y) ? b - 1 : b) | 1u;
+  return __uint_as_float(b);
+}
+
+// One thread takes eight elements of a token's row of a query, key or value head,
+// and four threads a block of 32, whose largest magnitude they find among
+// themselves.  Queries are turned in fp32 and rounded once.  Keys are turned in
+// 64 bits, where the products are exact, so that a code next to a border is the
+// nearest one and does not depend on an order of roundings; nothing is rounded
+// between that and the code.
+template <typename T, bool IL, bool WIDE>
+__global__ __launch_bounds__(kThreads) void append_mx4_kernel(Mx4AppendArgs a) {
+  const uint32_t idx = blockIdx.x * kThreads + threadIdx.x;
+  const int64_t t = fast_div(idx, a.div_units);
+  if (t >= a.T) return;
+  int u = (int)(idx - (uint32_t)t * a.units);
+  if (u >= 2 * a.row_threads) {
+    u -= 2 * a.row_threads;
+    const int h = (int)fast_div(u, a.div_q), e0 = 8 * (u - h * (a.D / 8));
+    if (h >= a.H) return;
+    float y[8];
+    rotated<float, T, IL, WIDE>(a, static_cast<const T *>(a.q) + t * a.q_ld[0] + h * a.q_ld[1], e0, a.pos[t], y);
+    T *to = static_cast<T *>(a.q_out) + (t * a.H + h) * a.D + e0;
+    if constexpr (!WIDE) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if constexpr (sizeof(T) == 2) to[i] = (T)f32_to_bf16_bits(y[i]);
+        else to[i] = y[i];
+    } else if constexpr (sizeof(T) == 2) {
+      *reinterpret_cast<u32x4_t *>(to) = u32x4_t{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]),
+                                                 pack_bf16x2(y[4], y[5]), pack_bf16x2(y[6], y[7])};
+    } else {
+      *reinterpret_cast<f32x4_t *>(to) = f32x4_t{y[0], y[1], y[2], y[3]};
+      *reinterpret_cast<f32x4_t *>(to + 4) = f32x4_t{y[4], y[5], y[6], y[7]};
+    }
+    return;
+  }
+  const int64_t slot = a.slots[t];
+  if (slot < 0 || slot >= a.pages * a.page_size) return;  // a padding token, for the whole block
+  const int64_t page = slot / a.page_size, off = slot - page * a.page_size;
+  const bool value = u >= a.row_threads;
+  if (value) u -= a.row_threads;
+  const int h = (int)fast_div(u, a.div_row), w = u - h * (4 * a.NB);  // the row's w-th eight elements
+  float x[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = 0.f;
+  if (8 * w < a.D) {
+    if (value) {
+      load8<T, WIDE>(static_cast<const T *>(a.v) + t * a.v_ld[0] + h * a.v_ld[1] + 8 * w, x);
+    } else {
+      double y[8];
+      rotated<double, T, IL, WIDE>(a, static_cast<const T *>(a.k) + t * a.k_ld[0] + h * a.k_ld[1], 8 * w, a.pos[t], y);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = sticky(y[i]);
+    }
+  }
+  int amax = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) amax = max(amax, (int)(__float_as_uint(x[i]) & 0x7fffffffu));
+  amax = max(amax, __builtin_amdgcn_mov_dpp(amax, 0xb1, 0xf, 0xf, true));  // lanes 1 0 3 2 of four
+  amax = max(amax, __builtin_amdgcn_mov_dpp(amax, 0x4e, 0xf, 0xf, true));  // lanes 2 3 0 1
+  const uint32_t byte = mx_byte((uint32_t)amax);
+  const uint32_t codes = byte == kMxNan ? 0u : mx_codes(x, mx_scale(byte));
+  const Mx4Rows &to = value ? a.values : a.keys;
+  *reinterpret_cast<uint32_t *>(to.codes + page * to.ld[0] + h * to.ld[1] + off * to.ld[2] + 4 * w) = codes;
+  if ((w & 3) == 0) to.scales[page * to.sc_ld[0] + h * to.sc_ld[1] + off * to.sc_ld[2] + w / 4] = (uint8_t)byte;
+}
+
+// One thread gives eight elements of a token's key and of its value.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void read_mx4_kernel(Mx4ReadArgs a) {
+  const uint32_t idx = blockIdx.x * kThreads + threadIdx.x;
+  const int64_t t = fast_div(idx, a.div_units);
+  if (t >= a.n) return;
+  const int u = (int)(idx - (uint32_t)t * a.units);
+  const int h = (int)fast_div(u, a.div_row), w = u - h * (a.D / 8);
+  const int64_t slot = a.slots[t];
+  uint32_t codes[2] = {0u, 0u}, byte[2] = {0u, 0u};
+  if (slot >= 0 && slot < a.pages * a.page_size) {
+    const int64_t page = slot / a.page_size, off = slot - page * a.page_size;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const Mx4Rows &r = i ? a.values : a.keys;
+      codes[i] = *reinterpret_cast<const uint32_t *>(r.codes + page * r.ld[0] + h * r.ld[1] + off * r.ld[2] + 4 * w);
+      byte[i] = r.scales[page * r.sc_ld[0] + h * r.sc_ld[1] + off * r.sc_ld[2] + w / 4];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const u32x4_t y = mx_values(codes[i], mx_scale(byte[i]));
+    T *to = static_cast<T *>(i ? a.v_out : a.k_out) + (t * a.KV + h) * a.D + 8 * w;
+    if constexpr (sizeof(T) == 2) {
+      __builtin_nontemporal_store(y, reinterpret_cast<u32x4_t *>(to));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const u32x4_t z = {y[2 * j] << 16, y[2 * j] & 0xffff0000u, y[2 * j + 1] << 16, y[2 * j + 1] & 0xffff0000u};
+        __builtin_nontemporal_store(z, reinterpret_cast<u32x4_t *>(to) + j);
+      }
+    }
+  }
+}
+
+// Threads of a launch, at most: a thread's number is divided in 31 bits.
+constexpr int64_t kMostThreads = 1 << 30;
+
+}  // namespace
+
+hipError_t launch_append_mx4(Mx4AppendArgs a, int dtype, bool wide, hipStream_t s) {
+  a.row_threads = a.KV * a.NB * 4;
+  a.units = 2 * a.row_threads + (a.H * (a.D / 8) + 3) / 4 * 4;  // whole fours, which share a block
+  a.div_units = make_div(a.units), a.div_row = make_div(4 * a.NB), a.div_q = make_div(a.D / 8);
+  const int64_t T = a.T, most = std::max<int64_t>(kMostThreads / a.units, 1), es = dtype == ZT_DT_F32 ? 4 : 2;
+  const Mx4AppendArgs all = a;
+  for (int64_t t0 = 0; t0 < T; t0 += most) {
+    a = all;
+    a.T = std::min(most, T - t0);
+    a.q = static_cast<const char *>(all.q) + t0 * a.q_ld[0] * es;
+    a.k = static_cast<const char *>(all.k) + t0 * a.k_ld[0] * es;
+    a.v = static_cast<const char *>(all.v) + t0 * a.v_ld[0] * es;
+    a.q_out = static_cast<char *>(all.q_out) + t0 * a.H * a.D * es;
+    a.pos = all.pos + t0, a.slots = all.slots + t0;
+    const int grid = (int)((a.T * a.units + kThreads - 1) / kThreads);
+    auto go = [&](auto kernel) { kernel<<<grid, kThreads, 0, s>>>(a); };
+    if (dtype == ZT_DT_BF16) {
+      if (wide) a.interleaved ? go(append_mx4_kernel<uint16_t, true, true>) : go(append_mx4_kernel<uint16_t, false, true>);
+      else a.interleaved ? go(append_mx4_kernel<uint16_t, true, false>) : go(append_mx4_kernel<uint16_t, false, false>);
+    } else {
+      if (wide) a.interleaved ? go(append_mx4_kernel<float, true, true>) : go(append_mx4_kernel<float, false, true>);
+      else a.interleaved ? go(append_mx4_kernel<float, true, false>) : go(append_mx4_kernel<float, false, false>);
+    }
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+
+hipError_t launch_read_mx4(Mx4ReadArgs a, int dtype, hipStream_t s) {
+  a.units = a.KV * (a.D / 8);
+  a.div_units = make_div(a.units), a.div_row = make_div(a.D / 8);
+  const int64_t n = a.n, most = std::max<int64_t>(kMostThreads / a.units, 1), es = dtype == ZT_DT_F32 ? 4 : 2;
+  const Mx4ReadArgs all = a;
+  for (int64_t t0 = 0; t0 < n; t0 += most) {
+    a = all;
+    a.n = std::min(most, n - t0);
+    a.slots = all.slots + t0;
+    a.k_out = static_cast<char *>(all.k_out) + t0 * a.KV * a.D * es;
+    a.v_out = static_cast<char *>(all.v_out) + t0 * a.KV * a.D * es;
+    const int grid = (int)((a.n * a.units + kThreads - 1) / kThreads);
+    if (dtype == ZT_DT_BF16) read_mx4_kernel<uint16_t><<<grid, kThreads, 0, s>>>(a);
+    else read_mx4_kernel<float><<<grid, kThreads, 0, s>>>(a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+
+}  // namespace zt

@@ -491,8 +491,6 @@ Shape shape_of(const AttnArgs &a) {
   return p;
 }
 
-size_t up256(size_t n) { return (n + 255) / 256 * 256; }
-
 }  // namespace
 
 bool paged_attn_countable(const AttnArgs &a) {
@@ -503,29 +501,27 @@ bool paged_attn_countable(const AttnArgs &a) {
 size_t paged_attn_workspace(const AttnArgs &a) {
   if (a.T == 0) return 0;
   const Shape p = shape_of(a);
-  const size_t slots = 2 * (size_t)p.grid * p.bm;
-  return up256(p.grid * sizeof(Split)) + up256(slots * 2 * sizeof(float)) + slots * a.D * sizeof(float);
+  return parts_bytes(a, p.grid, p.bm);
+}
+
+hipError_t launch_join(const AttnArgs &a, int grid, hipStream_t s) {
+  const dim3 g(grid, std::max(a.item_rows * a.D / 1024, 1));  // a thread per four outputs
+  if (a.dtype == ZT_DT_BF16) paged_attn_join_kernel<uint16_t><<<g, 256, 0, s>>>(a);
+  else paged_attn_join_kernel<float><<<g, 256, 0, s>>>(a);
+  return hipGetLastError();
 }
 
 hipError_t launch_paged_attn(AttnArgs a, void *workspace, hipStream_t s) {
   const Shape p = shape_of(a);
-  const size_t slots = 2 * (size_t)p.grid * p.bm;
-  a.group = a.H / a.KV, a.item_rows = p.bm;
+  a.group = a.H / a.KV;
   a.div_group = make_div(a.group), a.div_page = make_div(a.page_size);
   const int64_t per16 = a.dtype == ZT_DT_F32 ? 4 : 8;
   for (int i = 0; i < 2; ++i)
     a.k_row[i] = (uint32_t)(a.k_ld[2 * i] / per16), a.v_row[i] = (uint32_t)(a.v_ld[2 * i] / per16);
-  char *at = static_cast<char *>(workspace);
-  a.splits = at, at += up256(p.grid * sizeof(Split));
-  a.part_ml = reinterpret_cast<float *>(at), at += up256(slots * 2 * sizeof(float));
-  a.part_o = reinterpret_cast<float *>(at);
-  const bool bf = a.dtype == ZT_DT_BF16;
+  lay_parts(&a, workspace, p.grid, p.bm);
   const hipError_t e = p.tiles ? launch_tiles(a, p.grid, s) : launch_rows_of(a, p.grid, s);
   if (e != hipSuccess) return e;
-  const dim3 grid(p.grid, std::max(p.bm * a.D / 1024, 1));  // a thread per four outputs
-  if (bf) paged_attn_join_kernel<uint16_t><<<grid, 256, 0, s>>>(a);
-  else paged_attn_join_kernel<float><<<grid, 256, 0, s>>>(a);
-  return hipGetLastError();
+  return launch_join(a, p.grid, s);
 }
 
 }  // namespace zt

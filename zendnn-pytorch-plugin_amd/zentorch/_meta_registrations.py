@@ -217,3 +217,25 @@ def meta_zentorch_cache_compact(block_table, ref_counts, *, zentorch_op_name="")
 @register_meta("zentorch_cache_copy_pages")
 def meta_zentorch_cache_copy_pages(caches, copies, *, zentorch_op_name=""):
     return None
+
+
+@register_meta("zentorch_rotary_cache_append_mxfp4")
+def meta_zentorch_rotary_cache_append_mxfp4(query, key, value, positions, cos_sin, slots, key_cache,
+                                            key_scales, value_cache, value_scales, *,
+                                            interleaved=False, zentorch_op_name=""):
+    # the rotated query; the four tensors of the cache are written in place
+    return query.new_empty(query.size())
+
+
+@register_meta("zentorch_cache_read_mxfp4")
+def meta_zentorch_cache_read_mxfp4(key_cache, key_scales, value_cache, value_scales, slots, head_dim,
+                                   *, dtype=torch.bfloat16, zentorch_op_name=""):
+    shape = (slots.size(0), key_cache.size(1), head_dim)
+    return key_cache.new_empty(shape, dtype=dtype), key_cache.new_empty(shape, dtype=dtype)
+
+
+@register_meta("zentorch_paged_attention_mxfp4")
+def meta_zentorch_paged_attention_mxfp4(query, key_cache, key_scales, value_cache, value_scales,
+                                        block_table, cu_seqlens, context_lens, max_query_len, *,
+                                        causal=True, window=0, scale=None, zentorch_op_name=""):
+    return query.new_empty(query.size())
