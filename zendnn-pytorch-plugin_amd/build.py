@@ -31,7 +31,8 @@ HIPCC = os.path.join(ROCM, "bin", "hipcc")
 HIP_SOURCES = ["woq_kernels.hip", "woq_prefill.hip", "dynq_kernels.hip", "s8_prefill.hip",
                "moe_kernels.hip", "kv_cache.hip", "paged_attn.hip",
                "paged_attn_tile.hip", "paged_attn_split.hip", "kv_cache_mx4.hip",
-               "paged_attn_mx4.hip", "capi.hip", "capi_cache.hip", "capi_cache_mx4.hip"]
+               "paged_attn_mx4.hip", "paged_attn_mx4_tile.hip", "capi.hip", "capi_cache.hip",
+               "capi_cache_mx4.hip"]
 TORCH_SOURCES = ["ops.cpp", "ops_cache.cpp", "ops_cache_mx4.cpp", "shim_cuda_zentorch.cpp"]
 
 # -packed-fp32-ops: no v_pk_*_f32 from the compiler (hipcc's host pass warns

@@ -91,6 +91,10 @@ struct Mx4AttnArgs : AttnArgs {
   int NB;         // blocks of a row
   bool sc_words;  // a row's scales are whole aligned words
 };
+// The tile kernel (paged_attn_mx4_tile.hip): its rows per item and workgroups.
+int mx4_tile_rows();
+int mx4_tile_grid(const Mx4AttnArgs &a);
+hipError_t launch_mx4_tiles(const Mx4AttnArgs &a, int grid, hipStream_t s);
 bool paged_attn_mx4_countable(const Mx4AttnArgs &a);
 size_t paged_attn_mx4_workspace(const Mx4AttnArgs &a);
 hipError_t launch_paged_attn_mx4(Mx4AttnArgs a, void *workspace, hipStream_t s);

@@ -369,14 +369,17 @@ hipError_t launch_rows_of(const Mx4AttnArgs &a, int grid, hipStream_t s) {
 }
 
 struct Shape {
+  bool tiles;
   int bm, grid;
 };
 double items_most(const Mx4AttnArgs &a, int bm) { return std::floor((double)a.T * (a.H / a.KV) / bm) + a.S; }
-double blocks_most(const Mx4AttnArgs &a) { return std::floor((double)a.W * a.page_size / 128) + 1; }
+double blocks_most(const Mx4AttnArgs &a, bool tiles) { return std::floor((double)a.W * a.page_size / (tiles ? 64 : 128)) + 1; }
 Shape shape_of(const Mx4AttnArgs &a) {
-  Shape p{BM, kRowGrid};
+  const int64_t rows = std::min(std::max<int64_t>(a.max_q, 1), a.T) * (a.H / a.KV);
+  Shape p{rows > BM, BM, kRowGrid};
+  if (p.tiles) p.bm = mx4_tile_rows(), p.grid = mx4_tile_grid(a);
   // no more workgroups than there can be blocks
-  const double most = items_most(a, p.bm) * a.KV * blocks_most(a);
+  const double most = items_most(a, p.bm) * a.KV * blocks_most(a, p.tiles);
   if (most < p.grid) p.grid = std::max((int)most, 1);
   return p;
 }
@@ -385,7 +388,7 @@ Shape shape_of(const Mx4AttnArgs &a) {
 
 bool paged_attn_mx4_countable(const Mx4AttnArgs &a) {
   const Shape p = shape_of(a);
-  return items_most(a, p.bm) * (blocks_most(a) * kTileCostMost + kTileCostLead) < 2147483647.0;
+  return items_most(a, p.bm) * (blocks_most(a, p.tiles) * kTileCostMost + kTileCostLead) < 2147483647.0;
 }
 
 size_t paged_attn_mx4_workspace(const Mx4AttnArgs &a) {
@@ -401,7 +404,9 @@ hipError_t launch_paged_attn_mx4(Mx4AttnArgs a, void *workspace, hipStream_t s) 
   for (int i = 0; i < 2; ++i)
     a.k_row[i] = (uint32_t)(a.k_ld[2 * i] / 16), a.v_row[i] = (uint32_t)(a.v_ld[2 * i] / 16);
   lay_parts(&a, workspace, p.grid, p.bm);
-  const hipError_t e = a.dtype == ZT_DT_BF16 ? launch_rows_of<uint16_t>(a, p.grid, s) : launch_rows_of<float>(a, p.grid, s);
+  const hipError_t e = p.tiles                   ? launch_mx4_tiles(a, p.grid, s)
+                       : a.dtype == ZT_DT_BF16 ? launch_rows_of<uint16_t>(a, p.grid, s)
+                                               : launch_rows_of<float>(a, p.grid, s);
   if (e != hipSuccess) return e;
   return launch_join(a, p.grid, s);
 }
