@@ -34,6 +34,12 @@ __device__ __forceinline__ float mx_scale(uint32_t byte) {
   return __uint_as_float((byte > kMxLast ? kMxNan : byte) << 23);
 }
 
+// Whether one of a word's four bytes is kMxLast or past it.
+__device__ __forceinline__ bool mx_some_past(uint32_t w) {
+  const uint32_t y = ~w & 0xfcfcfcfcu;  // such a byte is 0 here
+  return ((y - 0x01010101u) & ~y & 0x80808080u) != 0;
+}
+
 // Eight numbers as codes, the first in the lowest bits.
 __device__ __forceinline__ uint32_t mx_codes(const float (&x)[8], float scale) {
   uint32_t w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, x[0], x[1], scale, 0);
@@ -88,8 +94,8 @@ hipError_t launch_read_mx4(Mx4ReadArgs a, int dtype, hipStream_t s);
 struct Mx4AttnArgs : AttnArgs {
   const uint8_t *k_sc, *v_sc;
   int64_t k_sc_ld[3], v_sc_ld[3];
-  int NB;         // blocks of a row
-  bool sc_words;  // a row's scales are whole aligned words
+  int NB;                // blocks of a row
+  bool sc_words, alike;  // set by launch_paged_attn_mx4
 };
 // The tile kernel (paged_attn_mx4_tile.hip): its rows per item and workgroups.
 int mx4_tile_rows();

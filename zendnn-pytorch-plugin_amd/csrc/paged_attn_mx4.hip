@@ -13,10 +13,8 @@ namespace {
 
 constexpr int kRowThreads = 256;
 constexpr int BM = 16;  // rows of an item
+constexpr int row_strip(int dp) { return dp <= 128 ? 64 : 32; }
 
-__device__ __forceinline__ u32x4_t load_once(const uint8_t *p) {
-  return __builtin_nontemporal_load(reinterpret_cast<const u32x4_t *>(p));
-}
 __device__ __forceinline__ float max_over_groups(float x) {
   x = fmaxf(x, __shfl_xor(x, 16));
   return fmaxf(x, __shfl_xor(x, 32));
@@ -38,27 +36,35 @@ __device__ __forceinline__ float top(float x) { return __uint_as_float(__float_a
 // a rounding of keys or values: fp32 queries and weights go in three bf16 parts
 // (cut short, 24 digits), bf16 ones in one and weights in two (p = hi + lo).
 //
-// The four waves are independent, wave w on every fourth strip of 32 keys; codes
-// come straight to registers, the next strip's as soon as they are unpacked.  The
-// products are transposed, S^T = K Q^T and O^T = V^T P^T on 16x16 MFMAs: lane
-// (key n, g) of 16 x 4 unpacks 8 codes of its key to the A operand of an MFMA.  A
-// lane has 16 consecutive bytes of the key, and the queries lie in that order of
-// elements.  Values are unpacked to the wave's LDS, from which the transposing
-// read takes columns.
+// The four waves are independent, wave w on every fourth strip of KS keys (64, or
+// 32 past head_dim 128), whose codes come straight to registers, a part of the next
+// strip's as soon as the part is unpacked.  The products are transposed, S^T = K Q^T
+// and O^T = V^T P^T on 16x16 MFMAs.  Lane (n, g) of 16 x 4 has quarter g of the
+// codes of keys 16 u + n, and of their values: it unpacks 8 codes of its key to the A
+// operand of an MFMA, and the queries lie in that order of elements.  Values are
+// unpacked to the wave's LDS, 32 keys at a time, from which the transposing read
+// takes columns.
+//
+// A key's place is found by the lane of its number, which also has its scales.  A
+// key that is not there is read from the cache's first row: its score is masked by
+// selection, and its value is taken as zeros.
 template <typename T, int DP>
 __global__ __launch_bounds__(kRowThreads, 2) void mx4_row_kernel(Mx4AttnArgs a) {
   using Cost = RowCost;
   constexpr bool BF = sizeof(T) == 2;
   constexpr int QP = BF ? 1 : 3, PP = BF ? 2 : 3;  // parts of a query and of a weight
-  constexpr int KS = 32, UK = 4 * KS;     // keys of a strip and of a unit
-  constexpr int CR = DP / 32;             // blocks of a row: 16 bytes, one scale
-  constexpr int KL = DP <= 128 ? 1 : 2;   // loads of a key per lane
-  constexpr int NV = KS * CR / 64;        // blocks of values per lane
+  constexpr int KS = row_strip(DP), UK = 4 * KS;   // keys of a strip and of a unit
+  constexpr bool WIDE = KS == 64;         // a lane to a key, else lanes 32 .. 63 do the values' part
+  constexpr int KT = KS / 16;             // 16-key tiles of a strip
+  constexpr int WB = DP == 64 ? 2 : 4;    // words of a lane's piece of a row
+  constexpr int KL = DP == 256 ? 2 : 1;   // pieces
   constexpr int NS = DP / 32;             // MFMA steps over a row
+  constexpr int CR = DP / 32;             // blocks of a row
   constexpr int VP = DP * 2 + 32;         // LDS pitch of a row of values
   constexpr int OP = DP + 4;              // pitch of the joined outputs, floats
   constexpr int DT = DP / 16;
-  constexpr int kWaveLds = KS * VP > 16 * OP * 4 ? KS * VP : 16 * OP * 4;
+  constexpr int kWaveLds = 32 * VP > 16 * OP * 4 ? 32 * VP : 16 * OP * 4;
+  typedef unsigned piece_t __attribute__((ext_vector_type(WB)));
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   __shared__ PlanShared sh;
   __shared__ float sm_m[4][16], sm_l[4][16];
@@ -74,13 +80,24 @@ __global__ __launch_bounds__(kRowThreads, 2) void mx4_row_kernel(Mx4AttnArgs a) 
   const float c = score_factor(a.scale);
   const int G = a.group;
   const char *zero = reinterpret_cast<const char *>(kZeroRow);
-  const uint8_t *nothing = reinterpret_cast<const uint8_t *>(kZeroRow);
-  // the element that step t of the lane begins with, and the block it lies in
+  // the lane's i-th piece of a row: its block, and its place; a block past the row's
+  // end has scale 0, and any codes
+  auto block = [&](int i) { return DP == 64 ? g >> 1 : g + 4 * i; };
+  uint32_t place[KL];
+#pragma unroll
+  for (int i = 0; i < KL; ++i) place[i] = block(i) < a.NB ? (DP == 64 ? 8 * g : 16 * (g + 4 * i)) : 0;
+  // the element that step t begins with
   auto element = [&](int t) { return DP == 64 ? 16 * g + 8 * t : 128 * (t / 4) + 32 * g + 8 * (t % 4); };
-  const int kblock = DP == 64 ? g / 2 : g;
-  // the lane's j-th block of values: row and block
-  auto vrow = [&](int j) { return CR == 2 ? lane & 31 : 16 * (j & 1) + n; };
-  auto vblock = [&](int j) { return CR == 2 ? lane >> 5 : g + 4 * (j >> 1); };
+  // Two pieces of 16 bytes change places in rows 4 .. 11 of 16, so that lanes that
+  // write eight rows, and lanes that read four, meet no bank twice.
+  const int flip_w = ((n >> 2 ^ n >> 3) & 1) << 4, flip_r = ((g ^ g >> 1) & 1) << 4;
+  unsigned char *write0 = vlds + n * VP + (DP == 64 ? 32 : 64) * g + flip_w, *write1 = write0 + 16 - 2 * flip_w;
+  const unsigned char *columns = vlds + (4 * g + n / 4) * VP + ((8 * (n & 3)) ^ flip_r);
+  // of a byte of the lane's block in a word of scales
+  const int byte_at = 8 * (block(0) & 3);
+  // what the lane looks after: keys, or values
+  const bool of_v = !WIDE && lane >= 32;
+  const int key_lane = WIDE ? lane : lane & 31;
 
   Walk<Cost> walk(plan);
   Segment seg;
@@ -99,7 +116,7 @@ __global__ __launch_bounds__(kRowThreads, 2) void mx4_row_kernel(Mx4AttnArgs a) 
     const int lo = live && a.causal && a.window ? (int)max((int64_t)pos + 1 - a.window, (int64_t)0) : 0;
     const int kend = (seg.b0 + seg.bb + take) * UK;
     int k0 = (seg.b0 + seg.bb) * UK + wave * KS;
-    auto lookup = [&](int at) { return pages.lookup(a, at + (lane & 31)); };
+    auto lookup = [&](int at) { return pages.lookup(a, at + key_lane); };
     int page = lookup(k0);  // on its way while the queries are fetched
     // ---- the queries, as B operands
     u32x4_t q[QP][NS];
@@ -137,113 +154,157 @@ __global__ __launch_bounds__(kRowThreads, 2) void mx4_row_kernel(Mx4AttnArgs a) 
     for (int d = 0; d < DT; ++d) o[d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     const uint8_t *kbase = static_cast<const uint8_t *>(a.k) + h * a.k_ld[1];
     const uint8_t *vbase = static_cast<const uint8_t *>(a.v) + h * a.v_ld[1];
-    // scales: lane x < 32 has those of key x of the strip, lane 32 + x of value x
-    const uint8_t *sbase = lane < 32 ? a.k_sc + h * a.k_sc_ld[1] : a.v_sc + h * a.v_sc_ld[1];
-    const int64_t s_page = lane < 32 ? a.k_sc_ld[0] : a.v_sc_ld[0], s_tok = lane < 32 ? a.k_sc_ld[2] : a.v_sc_ld[2];
+    const uint8_t *ks_base = a.k_sc + h * a.k_sc_ld[1], *vs_base = a.v_sc + h * a.v_sc_ld[1];
 
-    u32x4_t kreg[2][KL], vreg[NV];
-    uint32_t sreg[CR];
-    uint64_t there;  // which of the strip's keys there are
-    auto load = [&](int at, int page) {
-      const int tok = at + (lane & 31);
+    // Where the strip's keys and values are, and their scales.
+    uint64_t there;         // which of its keys there are
+    uint32_t k_row, v_row;  // of the lane's key, in 16 bytes (v_row alone holds both where lanes share)
+    uint32_t sc[2];         // words of scales: its key's and value's, or two of the one
+    auto words = [&](const uint8_t *p, int first) {
+      if (a.sc_words) {
+        if constexpr (CR == 2) return (uint32_t)*reinterpret_cast<const uint16_t *>(p);
+        else return *reinterpret_cast<const uint32_t *>(p + first);
+      }
+      uint32_t w = 0;
+#pragma unroll
+      for (int i = 0; i < (CR < 4 ? CR : 4); ++i) w |= first + i < a.NB ? (uint32_t)p[first + i] << (8 * i) : 0u;
+      return w;
+    };
+    auto locate = [&](int at, int page) {
+      const int tok = at + key_lane;
       const bool ok = pages.there(a, tok, page);
       there = __ballot(ok);
-      const uint32_t ko = ok ? row_offset(a, a.k_row, tok, page) : ~0u;
-      const uint32_t vo = ok ? row_offset(a, a.v_row, tok, page) : ~0u;
-      const int off = tok - (int)fast_div(tok, a.div_page) * a.page_size;
-      const uint8_t *sc = ok ? sbase + page * s_page + off * s_tok : nothing;
-#pragma unroll
-      for (int i = 0; i < CR; ++i) sreg[i] = i < a.NB ? sc[i] : 0u;
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const uint32_t r = __shfl(ko, 16 * u + n);
-        const uint8_t *src = kbase + (uint64_t)r * 16;
-        if constexpr (DP == 64) {
-          const u32x2_t y = __builtin_nontemporal_load(
-              reinterpret_cast<const u32x2_t *>(r != ~0u && kblock < a.NB ? src + 8 * g : nothing));
-          kreg[u][0][0] = y[0], kreg[u][0][1] = y[1];
+      const int pg = ok ? page : 0, off = ok ? tok - (int)fast_div(tok, a.div_page) * a.page_size : 0;
+      if constexpr (WIDE) {
+        const int64_t to = pg * a.k_sc_ld[0] + off * a.k_sc_ld[2];
+        k_row = pg * a.k_row[0] + off * a.k_row[1];
+        sc[0] = words(ks_base + to, 0);
+        if (a.alike) {
+          v_row = k_row;
+          sc[1] = words(vs_base + to, 0);
         } else {
-#pragma unroll
-          for (int i = 0; i < KL; ++i) kreg[u][i] = load_once(r != ~0u && g + 4 * i < a.NB ? src + 16 * (g + 4 * i) : nothing);
+          v_row = pg * a.v_row[0] + off * a.v_row[1];
+          sc[1] = words(vs_base + pg * a.v_sc_ld[0] + off * a.v_sc_ld[2], 0);
         }
-      }
-#pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        const uint32_t r = __shfl(vo, vrow(j));
-        vreg[j] = load_once(r != ~0u && vblock(j) < a.NB ? vbase + (uint64_t)r * 16 + 16 * vblock(j) : nothing);
+      } else {
+        k_row = v_row = pg * (of_v ? a.v_row[0] : a.k_row[0]) + off * (of_v ? a.v_row[1] : a.k_row[1]);
+        const uint8_t *p = of_v ? vs_base + pg * a.v_sc_ld[0] + off * a.v_sc_ld[2]
+                                : ks_base + pg * a.k_sc_ld[0] + off * a.k_sc_ld[2];
+        sc[0] = words(p, 0), sc[1] = words(p, 4);
       }
     };
-    if (k0 < kend) load(k0, page);
+    auto load = [&](const uint8_t *base, uint32_t row, int i) {
+      return __builtin_nontemporal_load(reinterpret_cast<const piece_t *>(base + (uint64_t)row * 16 + place[i]));
+    };
+    piece_t kreg[KT][KL], vreg[KT][KL];
+    auto load_k = [&] {
+#pragma unroll
+      for (int u = 0; u < KT; ++u) {
+        const uint32_t r = __shfl(k_row, 16 * u + n);
+#pragma unroll
+        for (int i = 0; i < KL; ++i) kreg[u][i] = load(kbase, r, i);
+      }
+    };
+    auto load_v = [&](int from) {  // tiles from, from + 1
+#pragma unroll
+      for (int u = from; u < from + 2; ++u) {
+        const uint32_t r = __shfl(v_row, (WIDE ? 0 : 32) + 16 * u + n);
+#pragma unroll
+        for (int i = 0; i < KL; ++i) vreg[u][i] = load(vbase, r, i);
+      }
+    };
+    if (k0 < kend) {
+      locate(k0, page);
+      load_k();
+#pragma unroll
+      for (int u = 0; u < KT; u += 2) load_v(u);
+    }
     page = lookup(k0 + UK);
     for (; k0 < kend; k0 += UK) {
-      // the lane's scales as words of four
-      uint32_t words[(CR + 3) / 4] = {};
+      const uint64_t held = WIDE ? there : there & 0xffffffffull;
+      const bool whole = held == (WIDE ? ~0ull : 0xffffffffull);
+      const bool edge = shared.edge(k0, KS), more = k0 + UK < kend;
+      // The scales of this strip.  A byte past the last one becomes NaN's.  Values that
+      // are not there get the least scale, which their weight of 0 makes 0, and so do
+      // those of an edge that are not finite.
+      uint32_t now[2] = {sc[0], sc[1]};
+      uint64_t bad = 0;  // keys whose values are not finite, at an edge
+      if (edge || !whole || __ballot(mx_some_past(now[0]) || mx_some_past(now[1]))) {
+        bool is = false;
 #pragma unroll
-      for (int i = 0; i < CR; ++i) words[i / 4] |= sreg[i] << (8 * (i % 4));
-      auto scale_of = [&](int row, int i, int byte) { return (__shfl(words[i], row) >> (8 * byte)) & 255u; };
-      uint32_t bad = 0;  // keys whose values are not finite, at an edge
-      const bool edge = shared.edge(k0, KS);
-      // values to the wave's LDS (LDS operations of a wave keep their order)
+        for (int i = 0; i < 2; ++i) {
+          const bool value = WIDE ? i == 1 : of_v;
 #pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        const int row = vrow(j);
-        uint32_t byte = scale_of(32 + row, j >> 1, CR == 2 ? lane >> 5 : g);
-        bool taken = false;
-        if (edge) {
-          const bool is = byte > kMxLast;
-          if (is) byte = 0, taken = true;
-          for (uint64_t left = __ballot(is); left; left &= left - 1)
-            bad |= 1u << __shfl(row, __builtin_ctzll(left));
+          for (int y = 0; y < 4; ++y)
+            if ((now[i] >> (8 * y) & 255u) > kMxLast) {
+              const bool out = edge && value;
+              is = is || out;
+              now[i] = out ? now[i] & ~(255u << (8 * y)) : now[i] | (255u << (8 * y));
+            }
+          if (value && !((held >> key_lane) & 1)) now[i] = 0;
         }
-        const float sc = mx_scale(byte);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          *reinterpret_cast<u32x4_t *>(vlds + row * VP + ((64 * vblock(j) + 16 * i) ^ ((row & 8) << 1))) =
-              mx_values(taken ? 0u : vreg[j][i], sc);
+        bad = __ballot(is) >> (WIDE ? 0 : 32) & held;
       }
+      auto scale_of = [&](bool v, int u, int i) {
+        const uint32_t w = WIDE ? __shfl(now[v], 16 * u + n) : __shfl(now[i], 32 * v + 16 * u + n);
+        return __uint_as_float((w >> byte_at & 255u) << 23);
+      };
+      // 32 values to the wave's LDS (LDS operations of a wave keep their order)
+      auto unpack_v = [&](int from) {
+#pragma unroll
+        for (int u = from; u < from + 2; ++u)
+#pragma unroll
+          for (int i = 0; i < KL; ++i) {
+            const float x = scale_of(true, u, i);
+#pragma unroll
+            for (int y = 0; y < WB; ++y)
+              *reinterpret_cast<u32x4_t *>((y & 1 ? write1 : write0) + 16 * VP * (u - from) + 32 * (y >> 1) + 256 * i) =
+                  mx_values(vreg[u][i][y], x);
+          }
+      };
+      unpack_v(0);
       // scores: lane (row n, g) gets keys 16 u + 4 g .. + 3
-      f32x4_t sc[2];
+      f32x4_t s4[KT];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
+      for (int u = 0; u < KT; ++u) {
         f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
-        float ks[KL];
+        float x[KL];
 #pragma unroll
-        for (int i = 0; i < KL; ++i) ks[i] = mx_scale(scale_of(16 * u + n, i, kblock));
+        for (int i = 0; i < KL; ++i) x[i] = scale_of(false, u, i);
 #pragma unroll
         for (int t = 0; t < NS; ++t) {
-          const bf16x8_t k = __builtin_bit_cast(bf16x8_t, mx_values(kreg[u][t / 4][t % 4], ks[t / 4]));
+          const bf16x8_t k = __builtin_bit_cast(bf16x8_t, mx_values(kreg[u][t / WB][t % WB], x[t / WB]));
 #pragma unroll
           for (int p = QP - 1; p >= 0; --p)
             acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, __builtin_bit_cast(bf16x8_t, q[p][t]), acc, 0, 0, 0);
         }
-        sc[u] = acc;
+        s4[u] = acc;
+        __builtin_amdgcn_sched_barrier(0);
       }
-      const uint32_t held = (uint32_t)there;
-      if (k0 + UK < kend) {
-        load(k0 + UK, page);
+      if (more) {
+        locate(k0 + UK, page);
+        load_k();
+        load_v(0);
         page = lookup(k0 + 2 * UK);
       }
       // weights
-      const bool some = held != ~0u || __ballot(lo > k0 || hi < k0 + KS);
+      const bool some = !whole || __ballot(lo > k0 || hi < k0 + KS);
       if (some) {
         // bit 16 u + e of `seen`: the lane's e-th key of 16
-        const int from = min(max(lo - k0, 0), 32), to = min(max(hi - k0, 0), 32);
-        const uint32_t range = (uint32_t)((1ull << to) - (1ull << min(from, to)));
-        missed = missed || (live && (range & bad));
-        const uint32_t seen = (range & held) >> (4 * g);
+        const int from = min(max(lo - k0, 0), KS), to = min(max(hi - k0, 0), KS);
+        const uint64_t below = from >= 64 ? ~0ull : (1ull << from) - 1, up = to >= 64 ? ~0ull : (1ull << to) - 1;
+        const uint64_t seen = (up & ~below & held) >> (4 * g);
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int u = 0; u < KT; ++u)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (!(seen & (1u << (16 * u + e)))) sc[u][e] = -INFINITY;
-      } else {
-        missed = missed || (live && bad);
+            if (!(seen & (1ull << (16 * u + e)))) s4[u][e] = -INFINITY;
       }
-      float mx = sc[0][0];
+      float mx = s4[0][0];
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < KT; ++u)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) mx = fmaxf(mx, sc[u][e]);
+        for (int e = 0; e < 4; ++e) mx = fmaxf(mx, s4[u][e]);
       mx = fmaxf(m, max_over_groups(mx));
       if (__ballot(mx > m)) {
         const float f = factor(m, mx, c);
@@ -257,40 +318,64 @@ __global__ __launch_bounds__(kRowThreads, 2) void mx4_row_kernel(Mx4AttnArgs a) 
       float mc = m == -INFINITY ? 0.f : m * c;
       if (__ballot(is_far(mc))) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int u = 0; u < KT; ++u)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) sc[u][e] -= is_far(mc) ? m : 0.f;
+          for (int e = 0; e < 4; ++e) s4[u][e] -= is_far(mc) ? m : 0.f;
         mc = is_far(mc) ? 0.f : mc;
       }
-      u32x4_t pw[PP];
+      // The headroom goes into the exponent in bf16 (its rounding there, 2^-20, is
+      // below the weights'), and is a product in fp32.
+      if constexpr (BF) mc += kHeadroom;
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int half = 0; half < KT / 2; ++half) {
+        u32x4_t pw[PP];
 #pragma unroll
-        for (int e = 0; e < 4; e += 2) {
-          float x[2];
+        for (int u = 0; u < 2; ++u)
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            x[i] = __builtin_amdgcn_exp2f(fmaf(sc[u][e + i], c, -mc)) * kWeight;
-            l += x[i];
+          for (int e = 0; e < 4; e += 2) {
+            float x[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              x[i] = __builtin_amdgcn_exp2f(fmaf(s4[2 * half + u][e + i], c, -mc)) * (BF ? 1.f : kWeight);
+              l += x[i];
+            }
+#pragma unroll
+            for (int p = 0; p < PP; ++p) {
+              pw[p][2 * u + e / 2] = p + 1 < PP ? tops(x[0], x[1]) : pack_bf16x2(x[0], x[1]);
+              x[0] -= top(x[0]), x[1] -= top(x[1]);
+            }
           }
-#pragma unroll
-          for (int p = 0; p < PP; ++p) {
-            pw[p][2 * u + e / 2] = p + 1 < PP ? tops(x[0], x[1]) : pack_bf16x2(x[0], x[1]);
-            x[0] -= top(x[0]), x[1] -= top(x[1]);
-          }
+        if (half) {
+          unpack_v(2 * half);
+          if (more) load_v(2 * half);
         }
-      // O^T += V^T P^T
-      const unsigned char *at0 = vlds + (4 * g + n / 4) * VP;
+        // O^T += V^T P^T, columns read kAhead MFMAs before their use; the fences
+        // keep the compiler from reading them all at once, which costs registers
+        constexpr int kAhead = 3;
+        auto read = [&](int d) {
+          typedef __attribute__((address_space(3))) s16x4_t *tr_ptr;
+          const unsigned char *at = columns + 32 * d;
+          const s16x4_t v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)at);
+          const s16x4_t v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)(at + 16 * VP));
+          return __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+        };
+        bf16x8_t v[kAhead];
 #pragma unroll
-      for (int d = 0; d < DT; ++d) {
-        typedef __attribute__((address_space(3))) s16x4_t *tr_ptr;
-        const unsigned char *at = at0 + ((32 * d + 8 * (n & 3)) ^ ((g & 2) << 3));
-        const s16x4_t v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)at);
-        const s16x4_t v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)(at + 16 * VP));
-        const bf16x8_t v = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+        for (int d = 0; d < kAhead; ++d) v[d] = read(d);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int p = PP - 1; p >= 0; --p)
-          o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, __builtin_bit_cast(bf16x8_t, pw[p]), o[d], 0, 0, 0);
+        for (int d = 0; d < DT; ++d) {
+#pragma unroll
+          for (int p = PP - 1; p >= 0; --p)
+            o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[d % kAhead], __builtin_bit_cast(bf16x8_t, pw[p]), o[d], 0, 0, 0);
+          if (d + kAhead < DT) v[d % kAhead] = read(d + kAhead);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      if (bad) {
+        const int from = min(max(lo - k0, 0), KS), to = min(max(hi - k0, 0), KS);
+        const uint64_t below = from >= 64 ? ~0ull : (1ull << from) - 1, up = to >= 64 ? ~0ull : (1ull << to) - 1;
+        missed = missed || (live && (up & ~below & bad));
       }
     }
     // ---- join the four waves
@@ -307,10 +392,10 @@ __global__ __launch_bounds__(kRowThreads, 2) void mx4_row_kernel(Mx4AttnArgs a) 
           const int at = pages.lookup(a, key);
           if (!pages.there(a, key, at) || !live || key < lo || key >= hi) continue;
           const int off = key - (int)fast_div(key, a.div_page) * a.page_size;
-          const uint8_t *sc = a.v_sc + h * a.v_sc_ld[1] + at * a.v_sc_ld[0] + off * a.v_sc_ld[2];
+          const uint8_t *vs = vs_base + at * a.v_sc_ld[0] + off * a.v_sc_ld[2];
 #pragma unroll 1
           for (int col = 4 * g; col < a.D; col += 16)
-            if (sc[col / kMxBlock] > kMxLast)
+            if (vs[col / kMxBlock] > kMxLast)
 #pragma unroll 1
               for (int e = 0; e < 4; ++e) *reinterpret_cast<float *>(vlds + (n * OP + col + e) * 4) = NAN;
         }
@@ -373,7 +458,7 @@ struct Shape {
   int bm, grid;
 };
 double items_most(const Mx4AttnArgs &a, int bm) { return std::floor((double)a.T * (a.H / a.KV) / bm) + a.S; }
-double blocks_most(const Mx4AttnArgs &a, bool tiles) { return std::floor((double)a.W * a.page_size / (tiles ? 64 : 128)) + 1; }
+double blocks_most(const Mx4AttnArgs &a, bool tiles) { return std::floor((double)a.W * a.page_size / (tiles ? 64 : 4 * row_strip(a.D))) + 1; }
 Shape shape_of(const Mx4AttnArgs &a) {
   const int64_t rows = std::min(std::max<int64_t>(a.max_q, 1), a.T) * (a.H / a.KV);
   Shape p{rows > BM, BM, kRowGrid};
@@ -403,6 +488,15 @@ hipError_t launch_paged_attn_mx4(Mx4AttnArgs a, void *workspace, hipStream_t s) 
   a.div_group = make_div(a.group), a.div_page = make_div(a.page_size);
   for (int i = 0; i < 2; ++i)
     a.k_row[i] = (uint32_t)(a.k_ld[2 * i] / 16), a.v_row[i] = (uint32_t)(a.v_ld[2 * i] / 16);
+  if (a.pages == 0) a.W = 0;  // no key is there, and there is no first row to read in its place
+  // keys and values laid out alike; scales in whole words (or halves: two blocks)
+  a.alike = true, a.sc_words = a.NB == (a.D <= 64 ? 2 : a.D <= 128 ? 4 : 8);
+  const uintptr_t unit = a.NB == 2 ? 2 : 4;
+  for (int i = 0; i < 3; ++i) {
+    a.alike = a.alike && (i == 1 || (a.k_ld[i] == a.v_ld[i] && a.k_sc_ld[i] == a.v_sc_ld[i]));
+    a.sc_words = a.sc_words && a.k_sc_ld[i] % unit == 0 && a.v_sc_ld[i] % unit == 0;
+  }
+  a.sc_words = a.sc_words && reinterpret_cast<uintptr_t>(a.k_sc) % unit == 0 && reinterpret_cast<uintptr_t>(a.v_sc) % unit == 0;
   lay_parts(&a, workspace, p.grid, p.bm);
   const hipError_t e = p.tiles                   ? launch_mx4_tiles(a, p.grid, s)
                        : a.dtype == ZT_DT_BF16 ? launch_rows_of<uint16_t>(a, p.grid, s)
