@@ -94,8 +94,7 @@ hipError_t launch_read_mx4(Mx4ReadArgs a, int dtype, hipStream_t s);
 struct Mx4AttnArgs : AttnArgs {
   const uint8_t *k_sc, *v_sc;
   int64_t k_sc_ld[3], v_sc_ld[3];
-  int NB;                // blocks of a row
-  bool sc_words, alike;  // set by launch_paged_attn_mx4
+  int NB;  // blocks of a row
 };
 // The tile kernel (paged_attn_mx4_tile.hip): its rows per item and workgroups.
 int mx4_tile_rows();

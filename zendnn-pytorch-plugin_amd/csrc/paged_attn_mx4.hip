@@ -48,7 +48,12 @@ __device__ __forceinline__ float top(float x) { return __uint_as_float(__float_a
 // A key's place is found by the lane of its number, which also has its scales.  A
 // key that is not there is read from the cache's first row: its score is masked by
 // selection, and its value is taken as zeros.
-template <typename T, int DP>
+//
+// A loop's every turn issues the same loads, past the last strip too (of the first
+// row then): a load behind a branch makes each wait one for all loads in flight.
+//
+// PLAIN: keys and values are laid out alike, and a row's scales are whole words.
+template <typename T, int DP, bool PLAIN>
 __global__ __launch_bounds__(kRowThreads, 2) void mx4_row_kernel(Mx4AttnArgs a) {
   using Cost = RowCost;
   constexpr bool BF = sizeof(T) == 2;
@@ -161,25 +166,28 @@ __global__ __launch_bounds__(kRowThreads, 2) void mx4_row_kernel(Mx4AttnArgs a) 
     uint32_t k_row, v_row;  // of the lane's key, in 16 bytes (v_row alone holds both where lanes share)
     uint32_t sc[2];         // words of scales: its key's and value's, or two of the one
     auto words = [&](const uint8_t *p, int first) {
-      if (a.sc_words) {
+      if constexpr (PLAIN) {
         if constexpr (CR == 2) return (uint32_t)*reinterpret_cast<const uint16_t *>(p);
         else return *reinterpret_cast<const uint32_t *>(p + first);
       }
       uint32_t w = 0;
 #pragma unroll
-      for (int i = 0; i < (CR < 4 ? CR : 4); ++i) w |= first + i < a.NB ? (uint32_t)p[first + i] << (8 * i) : 0u;
+      for (int i = 0; i < (CR < 4 ? CR : 4); ++i) {
+        const uint32_t y = p[min(first + i, a.NB - 1)];
+        w |= first + i < a.NB ? y << (8 * i) : 0u;
+      }
       return w;
     };
     auto locate = [&](int at, int page) {
       const int tok = at + key_lane;
-      const bool ok = pages.there(a, tok, page);
+      const bool ok = at < kend && pages.there(a, tok, page);
       there = __ballot(ok);
       const int pg = ok ? page : 0, off = ok ? tok - (int)fast_div(tok, a.div_page) * a.page_size : 0;
       if constexpr (WIDE) {
         const int64_t to = pg * a.k_sc_ld[0] + off * a.k_sc_ld[2];
         k_row = pg * a.k_row[0] + off * a.k_row[1];
         sc[0] = words(ks_base + to, 0);
-        if (a.alike) {
+        if constexpr (PLAIN) {
           v_row = k_row;
           sc[1] = words(vs_base + to, 0);
         } else {
@@ -213,17 +221,16 @@ __global__ __launch_bounds__(kRowThreads, 2) void mx4_row_kernel(Mx4AttnArgs a) 
         for (int i = 0; i < KL; ++i) vreg[u][i] = load(vbase, r, i);
       }
     };
-    if (k0 < kend) {
-      locate(k0, page);
-      load_k();
-#pragma unroll
-      for (int u = 0; u < KT; u += 2) load_v(u);
-    }
+    locate(k0, page);
+    load_k();
+    load_v(0);
     page = lookup(k0 + UK);
+#pragma unroll
+    for (int u = 2; u < KT; u += 2) load_v(u);
     for (; k0 < kend; k0 += UK) {
       const uint64_t held = WIDE ? there : there & 0xffffffffull;
       const bool whole = held == (WIDE ? ~0ull : 0xffffffffull);
-      const bool edge = shared.edge(k0, KS), more = k0 + UK < kend;
+      const bool edge = shared.edge(k0, KS);
       // The scales of this strip.  A byte past the last one becomes NaN's.  Values that
       // are not there get the least scale, which their weight of 0 makes 0, and so do
       // those of an edge that are not finite.
@@ -281,12 +288,10 @@ __global__ __launch_bounds__(kRowThreads, 2) void mx4_row_kernel(Mx4AttnArgs a) 
         s4[u] = acc;
         __builtin_amdgcn_sched_barrier(0);
       }
-      if (more) {
-        locate(k0 + UK, page);
-        load_k();
-        load_v(0);
-        page = lookup(k0 + 2 * UK);
-      }
+      locate(k0 + UK, page);
+      load_k();
+      load_v(0);
+      page = lookup(k0 + 2 * UK);
       // weights
       const bool some = !whole || __ballot(lo > k0 || hi < k0 + KS);
       if (some) {
@@ -347,7 +352,7 @@ __global__ __launch_bounds__(kRowThreads, 2) void mx4_row_kernel(Mx4AttnArgs a) 
           }
         if (half) {
           unpack_v(2 * half);
-          if (more) load_v(2 * half);
+          load_v(2 * half);
         }
         // O^T += V^T P^T, columns read kAhead MFMAs before their use; the fences
         // keep the compiler from reading them all at once, which costs registers
@@ -436,21 +441,36 @@ __global__ __launch_bounds__(kRowThreads, 2) void mx4_row_kernel(Mx4AttnArgs a) 
 
 constexpr int kRowGrid = 512;  // workgroups, at most: two per CU
 
-template <typename T, int DP>
+template <typename T, int DP, bool PLAIN>
 hipError_t launch_rows(const Mx4AttnArgs &a, int grid, hipStream_t s) {
   constexpr int wave = std::max(32 * (DP * 2 + 32), 16 * (DP + 4) * 4);
   const size_t lds = 4 * wave + batch_ints(a.S) * 4, largest = 4 * wave + batch_ints(kMaxSeqs) * 4;
-  auto kernel = mx4_row_kernel<T, DP>;
+  auto kernel = mx4_row_kernel<T, DP, PLAIN>;
   const hipError_t allowed = allow_lds(reinterpret_cast<const void *>(kernel), lds, largest);
   if (allowed != hipSuccess) return allowed;
   kernel<<<grid, kRowThreads, lds, s>>>(a);
   return hipGetLastError();
 }
-template <typename T>
+template <typename T, bool PLAIN>
 hipError_t launch_rows_of(const Mx4AttnArgs &a, int grid, hipStream_t s) {
-  if (a.D <= 64) return launch_rows<T, 64>(a, grid, s);
-  if (a.D <= 128) return launch_rows<T, 128>(a, grid, s);
-  return launch_rows<T, 256>(a, grid, s);
+  if (a.D <= 64) return launch_rows<T, 64, PLAIN>(a, grid, s);
+  if (a.D <= 128) return launch_rows<T, 128, PLAIN>(a, grid, s);
+  return launch_rows<T, 256, PLAIN>(a, grid, s);
+}
+// Whether keys and values are laid out alike, and a row's scales in whole words (or
+// a half of one: two blocks).
+bool is_plain(const Mx4AttnArgs &a) {
+  if (a.NB != (a.D <= 64 ? 2 : a.D <= 128 ? 4 : 8)) return false;
+  const int64_t unit = a.NB == 2 ? 2 : 4;
+  for (int i = 0; i < 3; ++i) {
+    if (i != 1 && (a.k_ld[i] != a.v_ld[i] || a.k_sc_ld[i] != a.v_sc_ld[i])) return false;
+    if (a.k_sc_ld[i] % unit || a.v_sc_ld[i] % unit) return false;
+  }
+  return reinterpret_cast<uintptr_t>(a.k_sc) % unit == 0 && reinterpret_cast<uintptr_t>(a.v_sc) % unit == 0;
+}
+template <typename T>
+hipError_t launch_rows_as(const Mx4AttnArgs &a, int grid, hipStream_t s) {
+  return is_plain(a) ? launch_rows_of<T, true>(a, grid, s) : launch_rows_of<T, false>(a, grid, s);
 }
 
 struct Shape {
@@ -489,18 +509,10 @@ hipError_t launch_paged_attn_mx4(Mx4AttnArgs a, void *workspace, hipStream_t s) 
   for (int i = 0; i < 2; ++i)
     a.k_row[i] = (uint32_t)(a.k_ld[2 * i] / 16), a.v_row[i] = (uint32_t)(a.v_ld[2 * i] / 16);
   if (a.pages == 0) a.W = 0;  // no key is there, and there is no first row to read in its place
-  // keys and values laid out alike; scales in whole words (or halves: two blocks)
-  a.alike = true, a.sc_words = a.NB == (a.D <= 64 ? 2 : a.D <= 128 ? 4 : 8);
-  const uintptr_t unit = a.NB == 2 ? 2 : 4;
-  for (int i = 0; i < 3; ++i) {
-    a.alike = a.alike && (i == 1 || (a.k_ld[i] == a.v_ld[i] && a.k_sc_ld[i] == a.v_sc_ld[i]));
-    a.sc_words = a.sc_words && a.k_sc_ld[i] % unit == 0 && a.v_sc_ld[i] % unit == 0;
-  }
-  a.sc_words = a.sc_words && reinterpret_cast<uintptr_t>(a.k_sc) % unit == 0 && reinterpret_cast<uintptr_t>(a.v_sc) % unit == 0;
   lay_parts(&a, workspace, p.grid, p.bm);
   const hipError_t e = p.tiles                   ? launch_mx4_tiles(a, p.grid, s)
-                       : a.dtype == ZT_DT_BF16 ? launch_rows_of<uint16_t>(a, p.grid, s)
-                                               : launch_rows_of<float>(a, p.grid, s);
+                       : a.dtype == ZT_DT_BF16 ? launch_rows_as<uint16_t>(a, p.grid, s)
+                                               : launch_rows_as<float>(a, p.grid, s);
   if (e != hipSuccess) return e;
   return launch_join(a, p.grid, s);
 }
