@@ -15,9 +15,13 @@ constexpr int kRowThreads = 256;
 constexpr int BM = 16;  // rows of an item
 constexpr int row_strip(int dp) { return dp <= 128 ? 64 : 32; }
 
+// Over the four lanes of a row, 16 apart: rows of 16 lanes, then halves of the wave,
+// change places, which costs no trip through LDS.
 __device__ __forceinline__ float max_over_groups(float x) {
-  x = fmaxf(x, __shfl_xor(x, 16));
-  return fmaxf(x, __shfl_xor(x, 32));
+  const u32x2_t a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const u32x2_t b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 __device__ __forceinline__ float sum_over_groups(float x) {
   x += __shfl_xor(x, 16);
@@ -163,7 +167,7 @@ __global__ __launch_bounds__(kRowThreads, 2) void mx4_row_kernel(Mx4AttnArgs a) 
 
     // Where the strip's keys and values are, and their scales.
     uint64_t there;         // which of its keys there are
-    uint32_t k_row, v_row;  // of the lane's key, in 16 bytes (v_row alone holds both where lanes share)
+    uint32_t k_row[KT], v_row[KT];  // of the lane's pieces, in 16 bytes
     uint32_t sc[2];         // words of scales: its key's and value's, or two of the one
     auto words = [&](const uint8_t *p, int first) {
       if constexpr (PLAIN) {
@@ -183,23 +187,24 @@ __global__ __launch_bounds__(kRowThreads, 2) void mx4_row_kernel(Mx4AttnArgs a) 
       const bool ok = at < kend && pages.there(a, tok, page);
       there = __ballot(ok);
       const int pg = ok ? page : 0, off = ok ? tok - (int)fast_div(tok, a.div_page) * a.page_size : 0;
+      uint32_t row, other;  // of the lane's key, and its value where the lane has both
       if constexpr (WIDE) {
         const int64_t to = pg * a.k_sc_ld[0] + off * a.k_sc_ld[2];
-        k_row = pg * a.k_row[0] + off * a.k_row[1];
+        row = pg * a.k_row[0] + off * a.k_row[1];
+        other = PLAIN ? row : pg * a.v_row[0] + off * a.v_row[1];
         sc[0] = words(ks_base + to, 0);
-        if constexpr (PLAIN) {
-          v_row = k_row;
-          sc[1] = words(vs_base + to, 0);
-        } else {
-          v_row = pg * a.v_row[0] + off * a.v_row[1];
-          sc[1] = words(vs_base + pg * a.v_sc_ld[0] + off * a.v_sc_ld[2], 0);
-        }
+        sc[1] = words(vs_base + (PLAIN ? to : pg * a.v_sc_ld[0] + off * a.v_sc_ld[2]), 0);
       } else {
-        k_row = v_row = pg * (of_v ? a.v_row[0] : a.k_row[0]) + off * (of_v ? a.v_row[1] : a.k_row[1]);
+        row = other = pg * (of_v ? a.v_row[0] : a.k_row[0]) + off * (of_v ? a.v_row[1] : a.k_row[1]);
         const uint8_t *p = of_v ? vs_base + pg * a.v_sc_ld[0] + off * a.v_sc_ld[2]
                                 : ks_base + pg * a.k_sc_ld[0] + off * a.k_sc_ld[2];
         sc[0] = words(p, 0), sc[1] = words(p, 4);
       }
+#pragma unroll
+      for (int u = 0; u < KT; ++u) k_row[u] = __shfl(row, 16 * u + n);
+#pragma unroll
+      for (int u = 0; u < KT; ++u)
+        v_row[u] = PLAIN ? k_row[u] : (uint32_t)__shfl(other, (WIDE ? 0 : 32) + 16 * u + n);
     };
     auto load = [&](const uint8_t *base, uint32_t row, int i) {
       return __builtin_nontemporal_load(reinterpret_cast<const piece_t *>(base + (uint64_t)row * 16 + place[i]));
@@ -207,19 +212,15 @@ __global__ __launch_bounds__(kRowThreads, 2) void mx4_row_kernel(Mx4AttnArgs a) 
     piece_t kreg[KT][KL], vreg[KT][KL];
     auto load_k = [&] {
 #pragma unroll
-      for (int u = 0; u < KT; ++u) {
-        const uint32_t r = __shfl(k_row, 16 * u + n);
+      for (int u = 0; u < KT; ++u)
 #pragma unroll
-        for (int i = 0; i < KL; ++i) kreg[u][i] = load(kbase, r, i);
-      }
+        for (int i = 0; i < KL; ++i) kreg[u][i] = load(kbase, k_row[u], i);
     };
     auto load_v = [&](int from) {  // tiles from, from + 1
 #pragma unroll
-      for (int u = from; u < from + 2; ++u) {
-        const uint32_t r = __shfl(v_row, (WIDE ? 0 : 32) + 16 * u + n);
+      for (int u = from; u < from + 2; ++u)
 #pragma unroll
-        for (int i = 0; i < KL; ++i) vreg[u][i] = load(vbase, r, i);
-      }
+        for (int i = 0; i < KL; ++i) vreg[u][i] = load(vbase, v_row[u], i);
     };
     locate(k0, page);
     load_k();
@@ -252,35 +253,38 @@ __global__ __launch_bounds__(kRowThreads, 2) void mx4_row_kernel(Mx4AttnArgs a) 
         }
         bad = __ballot(is) >> (WIDE ? 0 : 32) & held;
       }
-      auto scale_of = [&](bool v, int u, int i) {
-        const uint32_t w = WIDE ? __shfl(now[v], 16 * u + n) : __shfl(now[i], 32 * v + 16 * u + n);
-        return __uint_as_float((w >> byte_at & 255u) << 23);
-      };
+      float k_scale[KT][KL], v_scale[KT][KL];
+#pragma unroll
+      for (int v = 0; v < 2; ++v)
+#pragma unroll
+        for (int u = 0; u < KT; ++u)
+#pragma unroll
+          for (int i = 0; i < KL; ++i) {
+            const uint32_t w = WIDE ? __shfl(now[v], 16 * u + n) : __shfl(now[i], 32 * v + 16 * u + n);
+            (v ? v_scale : k_scale)[u][i] = __uint_as_float((w >> byte_at & 255u) << 23);
+          }
+      __builtin_amdgcn_sched_barrier(0);
       // 32 values to the wave's LDS (LDS operations of a wave keep their order)
       auto unpack_v = [&](int from) {
 #pragma unroll
         for (int u = from; u < from + 2; ++u)
 #pragma unroll
-          for (int i = 0; i < KL; ++i) {
-            const float x = scale_of(true, u, i);
+          for (int i = 0; i < KL; ++i)
 #pragma unroll
             for (int y = 0; y < WB; ++y)
               *reinterpret_cast<u32x4_t *>((y & 1 ? write1 : write0) + 16 * VP * (u - from) + 32 * (y >> 1) + 256 * i) =
-                  mx_values(vreg[u][i][y], x);
-          }
+                  mx_values(vreg[u][i][y], v_scale[u][i]);
       };
+      const int page_after = lookup(k0 + 2 * UK);
       unpack_v(0);
       // scores: lane (row n, g) gets keys 16 u + 4 g .. + 3
       f32x4_t s4[KT];
 #pragma unroll
       for (int u = 0; u < KT; ++u) {
         f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
-        float x[KL];
-#pragma unroll
-        for (int i = 0; i < KL; ++i) x[i] = scale_of(false, u, i);
 #pragma unroll
         for (int t = 0; t < NS; ++t) {
-          const bf16x8_t k = __builtin_bit_cast(bf16x8_t, mx_values(kreg[u][t / WB][t % WB], x[t / WB]));
+          const bf16x8_t k = __builtin_bit_cast(bf16x8_t, mx_values(kreg[u][t / WB][t % WB], k_scale[u][t / WB]));
 #pragma unroll
           for (int p = QP - 1; p >= 0; --p)
             acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, __builtin_bit_cast(bf16x8_t, q[p][t]), acc, 0, 0, 0);
@@ -291,7 +295,8 @@ __global__ __launch_bounds__(kRowThreads, 2) void mx4_row_kernel(Mx4AttnArgs a) 
       locate(k0 + UK, page);
       load_k();
       load_v(0);
-      page = lookup(k0 + 2 * UK);
+      page = page_after;
+      __builtin_amdgcn_sched_barrier(0);
       // weights
       const bool some = !whole || __ballot(lo > k0 || hi < k0 + KS);
       if (some) {
