@@ -73,9 +73,9 @@ struct Mx4AppendArgs {
   int64_t length, table_ld, pages, T;
   int H, KV, D, R, NB, page_size;
   bool interleaved;
-  // set by launch_append_mx4: threads of a token's keys (or values) and of a token
-  int row_threads, units;
-  FastDiv div_units, div_row, div_q;
+  // set by launch_append_mx4: threads of a query's and a key's row, and of a token
+  int q_units, k_units, units;
+  FastDiv div_units, div_k, div_v, div_q, div_page;
 };
 hipError_t launch_append_mx4(Mx4AppendArgs a, int dtype, bool wide, hipStream_t s);
 
@@ -86,7 +86,7 @@ struct Mx4ReadArgs {
   int KV, D, page_size;
   void *k_out, *v_out;  // [n, KV, D]
   int units;            // threads of a token, set by launch_read_mx4
-  FastDiv div_units, div_row;
+  FastDiv div_units, div_row, div_page;
 };
 hipError_t launch_read_mx4(Mx4ReadArgs a, int dtype, hipStream_t s);
 
