@@ -86,24 +86,32 @@ __global__ __launch_bounds__(NTH) __attribute__((amdgpu_waves_per_eu(DP <= 128 ?
     auto lookup = [&](int at) { return pages.lookup(a, at + lane); };
     u32x4_t codes[NP];
     uint32_t scales[NP];
-    // the thread's part of the tile at `at`, and which of its keys there are
+    // The thread's part of the tile at `at`, and which of its keys there are.  What is
+    // not there is read from the cache's first row (no branch: it would make every
+    // wait one for all loads), and gets the least scale: keys are masked by
+    // selection, and a weight of 0 makes the values 0.
     auto load = [&](int at, int page, bool real) -> uint64_t {
       const bool ok = real && pages.there(a, at + lane, page);
       const uint64_t m = __ballot(ok);
-      const int pg = __shfl(page, row);
       const bool mine = (m >> row) & 1;
-      const int tok = at + row, off = tok - (int)fast_div(tok, a.div_page) * a.page_size;
+      const int tok = at + row, its = __shfl(page, row), pg = mine ? its : 0;
+      const int off = mine ? tok - (int)fast_div(tok, a.div_page) * a.page_size : 0;
 #pragma unroll
       for (int j = 0; j < NP; ++j) {
-        const bool v = is_v(j), have = mine && block(j) < a.NB;
+        const bool v = is_v(j);
+        const int b = block(j) < a.NB ? block(j) : 0;
         const uint32_t r = (uint32_t)pg * (v ? a.v_row[0] : a.k_row[0]) + off * (v ? a.v_row[1] : a.k_row[1]);
-        const uint8_t *src = (v ? vbase : kbase) + (uint64_t)r * 16 + 16 * block(j);
-        const uint8_t *sc = (v ? vs_base : ks_base) + pg * (v ? a.v_sc_ld[0] : a.k_sc_ld[0]) +
-            off * (v ? a.v_sc_ld[2] : a.k_sc_ld[2]) + block(j);
-        codes[j] = *reinterpret_cast<const u32x4_t *>(have ? src : nothing);
-        scales[j] = *(have ? sc : nothing);
+        codes[j] = *reinterpret_cast<const u32x4_t *>((v ? vbase : kbase) + (uint64_t)r * 16 + 16 * b);
+        scales[j] = (v ? vs_base : ks_base)[pg * (v ? a.v_sc_ld[0] : a.k_sc_ld[0]) + off * (v ? a.v_sc_ld[2] : a.k_sc_ld[2]) + b];
       }
       return m;
+    };
+    auto settle = [&](uint64_t m) {  // the scales of a tile of which the keys m are there
+#pragma unroll
+      for (int j = 0; j < NP; ++j) {
+        const bool have = ((m >> row) & 1) && block(j) < a.NB;
+        scales[j] = have ? scales[j] : 0u;
+      }
     };
     // and to LDS, a piece of 16 bytes at a time
     auto unpack = [&](int j, int i, int st) {
@@ -117,7 +125,7 @@ __global__ __launch_bounds__(NTH) __attribute__((amdgpu_waves_per_eu(DP <= 128 ?
 #pragma unroll
       for (int j = 0; j < NP; ++j) {
         const bool bad = is_v(j) && scales[j] > kMxLast;
-        if (bad) codes[j] = u32x4_t{0, 0, 0, 0}, scales[j] = 0;
+        if (bad) scales[j] = 0;
         for (uint64_t left = __ballot(bad); left; left &= left - 1)
           found |= 1ull << __builtin_amdgcn_readlane(row, __builtin_ctzll(left));
       }
@@ -166,6 +174,7 @@ __global__ __launch_bounds__(NTH) __attribute__((amdgpu_waves_per_eu(DP <= 128 ?
     bool far = false;  // of some row of the wave
     bool missed = false;  // the row sees a value that is not finite at an edge
 
+    settle(there);
     if (shared.edge(k_first, TK)) take_out(0);
 #pragma unroll
     for (int j = 0; j < NP; ++j)
@@ -183,6 +192,7 @@ __global__ __launch_bounds__(NTH) __attribute__((amdgpu_waves_per_eu(DP <= 128 ?
         for (int w = 0; w < NW; ++w) all |= sm_bad[st][w];
         missed |= rows.sees_of(all & there, k0);
       }
+      settle(there_next);
       if (__builtin_expect(shared.edge(k0 + TK, TK), 0)) take_out(st ^ 1);
       if (rows.see(k0, TK)) {
         const unsigned char *kt = smem + st * 2 * STAGE, *vt = kt + STAGE;
