@@ -95,6 +95,13 @@ struct Mx4AttnArgs : AttnArgs {
   const uint8_t *k_sc, *v_sc;
   int64_t k_sc_ld[3], v_sc_ld[3];
   int NB;  // blocks of a row
+  // Set by launch_paged_attn_mx4.  Most caches are near: keys and values are laid out
+  // alike (strides of page and token in bytes, of codes and of scales), within 2^32
+  // bytes of the first, by strides and numbers of 24 bits, which multiply in one
+  // full-rate instruction.  words: a row's scales are whole aligned words, or a half.
+  bool near, words;
+  uint32_t ld[2], sc_ld[2];
+  int step_off;  // a tile's length less its whole pages
 };
 // The tile kernel (paged_attn_mx4_tile.hip): its rows per item and workgroups.
 int mx4_tile_rows();

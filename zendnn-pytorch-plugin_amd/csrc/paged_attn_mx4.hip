@@ -56,8 +56,9 @@ __device__ __forceinline__ float top(float x) { return __uint_as_float(__float_a
 // A loop's every turn issues the same loads, past the last strip too (of the first
 // row then): a load behind a branch makes each wait one for all loads in flight.
 //
-// PLAIN: keys and values are laid out alike, and a row's scales are whole words.
-template <typename T, int DP, bool PLAIN>
+// NEAR: a near cache's places (mx4.hpp) are found with a third of the instructions.
+// WORDS: a row's scales are loaded together.
+template <typename T, int DP, bool NEAR, bool WORDS>
 __global__ __launch_bounds__(kRowThreads, 2) void mx4_row_kernel(Mx4AttnArgs a) {
   using Cost = RowCost;
   constexpr bool BF = sizeof(T) == 2;
@@ -167,10 +168,10 @@ __global__ __launch_bounds__(kRowThreads, 2) void mx4_row_kernel(Mx4AttnArgs a) 
 
     // Where the strip's keys and values are, and their scales.
     uint64_t there;         // which of its keys there are
-    uint32_t k_row[KT], v_row[KT];  // of the lane's pieces, in 16 bytes
+    uint32_t k_row[KT], v_row[KT];  // of the lane's pieces: bytes if NEAR, else 16 of them
     uint32_t sc[2];         // words of scales: its key's and value's, or two of the one
     auto words = [&](const uint8_t *p, int first) {
-      if constexpr (PLAIN) {
+      if constexpr (WORDS) {
         if constexpr (CR == 2) return (uint32_t)*reinterpret_cast<const uint16_t *>(p);
         else return *reinterpret_cast<const uint32_t *>(p + first);
       }
@@ -188,12 +189,19 @@ __global__ __launch_bounds__(kRowThreads, 2) void mx4_row_kernel(Mx4AttnArgs a) 
       there = __ballot(ok);
       const int pg = ok ? page : 0, off = ok ? tok - (int)fast_div(tok, a.div_page) * a.page_size : 0;
       uint32_t row, other;  // of the lane's key, and its value where the lane has both
-      if constexpr (WIDE) {
-        const int64_t to = pg * a.k_sc_ld[0] + off * a.k_sc_ld[2];
-        row = pg * a.k_row[0] + off * a.k_row[1];
-        other = PLAIN ? row : pg * a.v_row[0] + off * a.v_row[1];
-        sc[0] = words(ks_base + to, 0);
-        sc[1] = words(vs_base + (PLAIN ? to : pg * a.v_sc_ld[0] + off * a.v_sc_ld[2]), 0);
+      if constexpr (NEAR) {
+        row = other = __umul24(pg, a.ld[0]) + __umul24(off, a.ld[1]);
+        const uint32_t to = __umul24(pg, a.sc_ld[0]) + __umul24(off, a.sc_ld[1]);
+        if constexpr (WIDE) {
+          sc[0] = words(ks_base + to, 0), sc[1] = words(vs_base + to, 0);
+        } else {
+          const uint8_t *p = (of_v ? vs_base : ks_base) + to;
+          sc[0] = words(p, 0), sc[1] = words(p, 4);
+        }
+      } else if constexpr (WIDE) {
+        row = pg * a.k_row[0] + off * a.k_row[1], other = pg * a.v_row[0] + off * a.v_row[1];
+        sc[0] = words(ks_base + pg * a.k_sc_ld[0] + off * a.k_sc_ld[2], 0);
+        sc[1] = words(vs_base + pg * a.v_sc_ld[0] + off * a.v_sc_ld[2], 0);
       } else {
         row = other = pg * (of_v ? a.v_row[0] : a.k_row[0]) + off * (of_v ? a.v_row[1] : a.k_row[1]);
         const uint8_t *p = of_v ? vs_base + pg * a.v_sc_ld[0] + off * a.v_sc_ld[2]
@@ -204,10 +212,11 @@ __global__ __launch_bounds__(kRowThreads, 2) void mx4_row_kernel(Mx4AttnArgs a) 
       for (int u = 0; u < KT; ++u) k_row[u] = __shfl(row, 16 * u + n);
 #pragma unroll
       for (int u = 0; u < KT; ++u)
-        v_row[u] = PLAIN ? k_row[u] : (uint32_t)__shfl(other, (WIDE ? 0 : 32) + 16 * u + n);
+        v_row[u] = NEAR ? k_row[u] : (uint32_t)__shfl(other, (WIDE ? 0 : 32) + 16 * u + n);
     };
     auto load = [&](const uint8_t *base, uint32_t row, int i) {
-      return __builtin_nontemporal_load(reinterpret_cast<const piece_t *>(base + (uint64_t)row * 16 + place[i]));
+      const uint8_t *p = NEAR ? base + (row + place[i]) : base + (uint64_t)row * 16 + place[i];
+      return __builtin_nontemporal_load(reinterpret_cast<const piece_t *>(p));
     };
     piece_t kreg[KT][KL], vreg[KT][KL];
     auto load_k = [&] {
@@ -446,36 +455,44 @@ __global__ __launch_bounds__(kRowThreads, 2) void mx4_row_kernel(Mx4AttnArgs a) 
 
 constexpr int kRowGrid = 512;  // workgroups, at most: two per CU
 
-template <typename T, int DP, bool PLAIN>
+template <typename T, int DP, bool NEAR, bool WORDS>
 hipError_t launch_rows(const Mx4AttnArgs &a, int grid, hipStream_t s) {
   constexpr int wave = std::max(32 * (DP * 2 + 32), 16 * (DP + 4) * 4);
   const size_t lds = 4 * wave + batch_ints(a.S) * 4, largest = 4 * wave + batch_ints(kMaxSeqs) * 4;
-  auto kernel = mx4_row_kernel<T, DP, PLAIN>;
+  auto kernel = mx4_row_kernel<T, DP, NEAR, WORDS>;
   const hipError_t allowed = allow_lds(reinterpret_cast<const void *>(kernel), lds, largest);
   if (allowed != hipSuccess) return allowed;
   kernel<<<grid, kRowThreads, lds, s>>>(a);
   return hipGetLastError();
 }
-template <typename T, bool PLAIN>
+template <typename T, bool NEAR, bool WORDS>
 hipError_t launch_rows_of(const Mx4AttnArgs &a, int grid, hipStream_t s) {
-  if (a.D <= 64) return launch_rows<T, 64, PLAIN>(a, grid, s);
-  if (a.D <= 128) return launch_rows<T, 128, PLAIN>(a, grid, s);
-  return launch_rows<T, 256, PLAIN>(a, grid, s);
+  if (a.D <= 64) return launch_rows<T, 64, NEAR, WORDS>(a, grid, s);
+  if (a.D <= 128) return launch_rows<T, 128, NEAR, WORDS>(a, grid, s);
+  return launch_rows<T, 256, NEAR, WORDS>(a, grid, s);
 }
-// Whether keys and values are laid out alike, and a row's scales in whole words (or
-// a half of one: two blocks).
-bool is_plain(const Mx4AttnArgs &a) {
-  if (a.NB != (a.D <= 64 ? 2 : a.D <= 128 ? 4 : 8)) return false;
-  const int64_t unit = a.NB == 2 ? 2 : 4;
+// Whether a cache is near and has its scales in words (mx4.hpp), and its strides.
+void set_near(Mx4AttnArgs *a) {
+  constexpr int64_t k24 = 1 << 24;
+  const int64_t unit = a->NB == 2 ? 2 : 4;
+  a->near = a->pages <= k24 && a->page_size <= k24;
+  a->words = a->NB == (a->D <= 64 ? 2 : a->D <= 128 ? 4 : 8) &&
+             reinterpret_cast<uintptr_t>(a->k_sc) % unit == 0 && reinterpret_cast<uintptr_t>(a->v_sc) % unit == 0;
   for (int i = 0; i < 3; ++i) {
-    if (i != 1 && (a.k_ld[i] != a.v_ld[i] || a.k_sc_ld[i] != a.v_sc_ld[i])) return false;
-    if (a.k_sc_ld[i] % unit || a.v_sc_ld[i] % unit) return false;
+    a->near = a->near && a->k_ld[i] == a->v_ld[i] && a->k_sc_ld[i] == a->v_sc_ld[i];
+    if (i != 1) a->near = a->near && a->k_ld[i] < k24 && a->k_sc_ld[i] < k24;
+    a->words = a->words && a->k_sc_ld[i] % unit == 0 && a->v_sc_ld[i] % unit == 0;
   }
-  return reinterpret_cast<uintptr_t>(a.k_sc) % unit == 0 && reinterpret_cast<uintptr_t>(a.v_sc) % unit == 0;
+  // the last key's last byte, from the head's first
+  a->near = a->near && a->pages * a->k_ld[0] + a->page_size * a->k_ld[2] + 16 * a->NB < (1ll << 32) &&
+            a->pages * a->k_sc_ld[0] + a->page_size * a->k_sc_ld[2] + a->NB < (1ll << 32);
+  for (int i = 0; i < 2; ++i) a->ld[i] = (uint32_t)a->k_ld[2 * i], a->sc_ld[i] = (uint32_t)a->k_sc_ld[2 * i];
+  a->step_off = 64 % a->page_size;
 }
 template <typename T>
 hipError_t launch_rows_as(const Mx4AttnArgs &a, int grid, hipStream_t s) {
-  return is_plain(a) ? launch_rows_of<T, true>(a, grid, s) : launch_rows_of<T, false>(a, grid, s);
+  if (!a.near) return launch_rows_of<T, false, false>(a, grid, s);
+  return a.words ? launch_rows_of<T, true, true>(a, grid, s) : launch_rows_of<T, true, false>(a, grid, s);
 }
 
 struct Shape {
@@ -514,6 +531,7 @@ hipError_t launch_paged_attn_mx4(Mx4AttnArgs a, void *workspace, hipStream_t s) 
   for (int i = 0; i < 2; ++i)
     a.k_row[i] = (uint32_t)(a.k_ld[2 * i] / 16), a.v_row[i] = (uint32_t)(a.v_ld[2 * i] / 16);
   if (a.pages == 0) a.W = 0;  // no key is there, and there is no first row to read in its place
+  set_near(&a);
   lay_parts(&a, workspace, p.grid, p.bm);
   const hipError_t e = p.tiles                   ? launch_mx4_tiles(a, p.grid, s)
                        : a.dtype == ZT_DT_BF16 ? launch_rows_as<uint16_t>(a, p.grid, s)

@@ -34,7 +34,9 @@ constexpr int NW = 4, NTH = 64 * NW, BM = 32 * NW, TK = 64;
 // Scores, weights and outputs are as in paged_attn_tile.hip, on 32x32 MFMAs,
 // transposed.  fp32 queries and weights go in three bf16 parts (cut short, 24
 // digits), three MFMAs a product.
-template <typename T, int DP, int DC>
+//
+// NEAR: a near cache's places (mx4.hpp) are found with a third of the instructions.
+template <typename T, int DP, int DC, bool NEAR>
 __global__ __launch_bounds__(NTH) __attribute__((amdgpu_waves_per_eu(DP <= 128 ? 2 : 1, DP <= 128 ? 2 : 1))) void mx4_tile_kernel(Mx4AttnArgs a) {
   using Cost = Mx4TileCost;
   constexpr bool BF = sizeof(T) == 2;
@@ -84,6 +86,9 @@ __global__ __launch_bounds__(NTH) __attribute__((amdgpu_waves_per_eu(DP <= 128 ?
     const uint8_t *ks_base = a.k_sc + h * a.k_sc_ld[1], *vs_base = a.v_sc + h * a.v_sc_ld[1];
 
     auto lookup = [&](int at) { return pages.lookup(a, at + lane); };
+    const int k_first = (seg.b0 + seg.bb) * TK;
+    // where in its page the thread's row of the next tile to be loaded is
+    int row_off = k_first + row - (int)fast_div(k_first + row, a.div_page) * a.page_size;
     u32x4_t codes[NP];
     uint32_t scales[NP];
     // The thread's part of the tile at `at`, and which of its keys there are.  What is
@@ -94,12 +99,21 @@ __global__ __launch_bounds__(NTH) __attribute__((amdgpu_waves_per_eu(DP <= 128 ?
       const bool ok = real && pages.there(a, at + lane, page);
       const uint64_t m = __ballot(ok);
       const bool mine = (m >> row) & 1;
-      const int tok = at + row, its = __shfl(page, row), pg = mine ? its : 0;
-      const int off = mine ? tok - (int)fast_div(tok, a.div_page) * a.page_size : 0;
+      const int its = __shfl(page, row), pg = mine ? its : 0, off = mine ? row_off : 0;
+      // the next tile's row: a tile on
+      row_off += a.step_off;
+      row_off -= row_off >= a.page_size ? a.page_size : 0;
+      const uint32_t near = __umul24(pg, a.ld[0]) + __umul24(off, a.ld[1]);
+      const uint32_t near_sc = __umul24(pg, a.sc_ld[0]) + __umul24(off, a.sc_ld[1]);
 #pragma unroll
       for (int j = 0; j < NP; ++j) {
         const bool v = is_v(j);
         const int b = block(j) < a.NB ? block(j) : 0;
+        if constexpr (NEAR) {
+          codes[j] = *reinterpret_cast<const u32x4_t *>((v ? vbase : kbase) + (near + 16 * b));
+          scales[j] = (v ? vs_base : ks_base)[near_sc + b];
+          continue;
+        }
         const uint32_t r = (uint32_t)pg * (v ? a.v_row[0] : a.k_row[0]) + off * (v ? a.v_row[1] : a.k_row[1]);
         codes[j] = *reinterpret_cast<const u32x4_t *>((v ? vbase : kbase) + (uint64_t)r * 16 + 16 * b);
         scales[j] = (v ? vs_base : ks_base)[pg * (v ? a.v_sc_ld[0] : a.k_sc_ld[0]) + off * (v ? a.v_sc_ld[2] : a.k_sc_ld[2]) + b];
@@ -131,7 +145,6 @@ __global__ __launch_bounds__(NTH) __attribute__((amdgpu_waves_per_eu(DP <= 128 ?
       }
       if (lane == 0) sm_bad[st][wave] = found;
     };
-    const int k_first = (seg.b0 + seg.bb) * TK;
     uint64_t there = load(k_first, lookup(k_first), true);
     int page = lookup(k_first + TK);
 
@@ -360,23 +373,27 @@ __global__ __launch_bounds__(NTH) __attribute__((amdgpu_waves_per_eu(DP <= 128 ?
   zero_rows<NTH>(a, plan, BM, TK, batch);
 }
 
-template <typename T, int DP, int DC>
+template <typename T, int DP, int DC, bool NEAR>
 hipError_t launch_as(const Mx4AttnArgs &a, int grid, hipStream_t s) {
   const size_t tiles = 4 * (size_t)TK * DP * 2;
   const size_t lds = tiles + batch_ints(a.S) * 4, largest = tiles + batch_ints(kMaxSeqs) * 4;
   if (a.item_rows != BM) return hipErrorInvalidValue;
-  auto kernel = mx4_tile_kernel<T, DP, DC>;
+  auto kernel = mx4_tile_kernel<T, DP, DC, NEAR>;
   const hipError_t allowed = allow_lds(reinterpret_cast<const void *>(kernel), lds, largest);
   if (allowed != hipSuccess) return allowed;
   kernel<<<grid, NTH, lds, s>>>(a);
   return hipGetLastError();
 }
-template <typename T>
+template <typename T, bool NEAR>
 hipError_t launch_of(const Mx4AttnArgs &a, int grid, hipStream_t s) {
-  if (a.D <= 64) return launch_as<T, 64, 64>(a, grid, s);
-  if (a.D <= 96) return launch_as<T, 128, 96>(a, grid, s);
-  if (a.D <= 128) return launch_as<T, 128, 128>(a, grid, s);
-  return launch_as<T, 256, 256>(a, grid, s);
+  if (a.D <= 64) return launch_as<T, 64, 64, NEAR>(a, grid, s);
+  if (a.D <= 96) return launch_as<T, 128, 96, NEAR>(a, grid, s);
+  if (a.D <= 128) return launch_as<T, 128, 128, NEAR>(a, grid, s);
+  return launch_as<T, 256, 256, NEAR>(a, grid, s);
+}
+template <typename T>
+hipError_t launch_by(const Mx4AttnArgs &a, int grid, hipStream_t s) {
+  return a.near ? launch_of<T, true>(a, grid, s) : launch_of<T, false>(a, grid, s);
 }
 
 }  // namespace
@@ -384,7 +401,7 @@ hipError_t launch_of(const Mx4AttnArgs &a, int grid, hipStream_t s) {
 int mx4_tile_rows() { return BM; }
 int mx4_tile_grid(const Mx4AttnArgs &a) { return a.D <= 128 ? 512 : 256; }
 hipError_t launch_mx4_tiles(const Mx4AttnArgs &a, int grid, hipStream_t s) {
-  return a.dtype == ZT_DT_BF16 ? launch_of<uint16_t>(a, grid, s) : launch_of<float>(a, grid, s);
+  return a.dtype == ZT_DT_BF16 ? launch_by<uint16_t>(a, grid, s) : launch_by<float>(a, grid, s);
 }
 
 }  // namespace zt
