@@ -536,7 +536,9 @@ inline void lay_parts(AttnArgs *a, void *workspace, int grid, int bm) {
   a->part_ml = reinterpret_cast<float *>(at), at += up256(2 * (size_t)grid * bm * 2 * sizeof(float));
   a->part_o = reinterpret_cast<float *>(at);
 }
-hipError_t launch_join(const AttnArgs &a, int grid, hipStream_t s);
+// deep: the parts of a long axis 32 at a time, not eight (one round trip for the 32
+// parts of a sequence of 131072, not four).
+hipError_t launch_join(const AttnArgs &a, int grid, bool deep, hipStream_t s);
 
 // The tile kernel (paged_attn_tile.hip): its rows per item and workgroups.
 int tile_rows(const AttnArgs &a);

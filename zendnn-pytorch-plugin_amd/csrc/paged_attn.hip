@@ -406,17 +406,19 @@ __device__ __forceinline__ f32x4_t join_parts(const AttnArgs &a, const Split &s,
 // launch began and others finished.  A thread takes four outputs of a row.
 // Most are cut once (two parts); a long axis with few rows in dozens.  Bound by
 // its round trips (2.4 us for seven parts of 32 rows) or by the parts' bytes.
-template <typename T>
+template <typename T, bool DEEP>
 __global__ __launch_bounds__(256) void paged_attn_join_kernel(AttnArgs a) {
   const Split s = static_cast<const Split *>(a.splits)[blockIdx.x];
   if (s.rows == 0) return;
   const float c = score_factor(a.scale);
   const int first = (int)blockIdx.x, d4 = a.D / 4, G = a.group;
-  const bool two = s.last - first < 2;
+  const int64_t parts = s.last - first;  // but one
   for (int e = blockIdx.y * 256 + threadIdx.x; e < s.rows * d4; e += gridDim.y * 256) {
     const int row = e / d4, d = (e - row * d4) * 4;
     float l;
-    const f32x4_t o = two ? join_parts<2>(a, s, first, row, d, c, &l) : join_parts<8>(a, s, first, row, d, c, &l);
+    const f32x4_t o = parts < 2             ? join_parts<2>(a, s, first, row, d, c, &l)
+                      : DEEP && parts >= 16 ? join_parts<32>(a, s, first, row, d, c, &l)
+                                            : join_parts<8>(a, s, first, row, d, c, &l);
     const int rr = s.row0 + row, tok = (int)fast_div(rr, a.div_group);
     const int64_t at = ((int64_t)(s.q0 + tok) * a.H + s.head * G + rr - tok * G) * a.D + d;
     store_out<T>(a.out, at, o, l > 0.f ? 1.f / l : 0.f);
@@ -504,10 +506,11 @@ size_t paged_attn_workspace(const AttnArgs &a) {
   return parts_bytes(a, p.grid, p.bm);
 }
 
-hipError_t launch_join(const AttnArgs &a, int grid, hipStream_t s) {
+hipError_t launch_join(const AttnArgs &a, int grid, bool deep, hipStream_t s) {
   const dim3 g(grid, std::max(a.item_rows * a.D / 1024, 1));  // a thread per four outputs
-  if (a.dtype == ZT_DT_BF16) paged_attn_join_kernel<uint16_t><<<g, 256, 0, s>>>(a);
-  else paged_attn_join_kernel<float><<<g, 256, 0, s>>>(a);
+  auto go = [&](auto kernel) { kernel<<<g, 256, 0, s>>>(a); };
+  if (a.dtype == ZT_DT_BF16) deep ? go(paged_attn_join_kernel<uint16_t, true>) : go(paged_attn_join_kernel<uint16_t, false>);
+  else deep ? go(paged_attn_join_kernel<float, true>) : go(paged_attn_join_kernel<float, false>);
   return hipGetLastError();
 }
 
@@ -521,7 +524,7 @@ hipError_t launch_paged_attn(AttnArgs a, void *workspace, hipStream_t s) {
   lay_parts(&a, workspace, p.grid, p.bm);
   const hipError_t e = p.tiles ? launch_tiles(a, p.grid, s) : launch_rows_of(a, p.grid, s);
   if (e != hipSuccess) return e;
-  return launch_join(a, p.grid, s);
+  return launch_join(a, p.grid, false, s);
 }
 
 }  // namespace zt
