@@ -537,7 +537,8 @@ inline void lay_parts(AttnArgs *a, void *workspace, int grid, int bm) {
   a->part_o = reinterpret_cast<float *>(at);
 }
 // deep: the parts of a long axis 32 at a time, not eight (one round trip for the 32
-// parts of a sequence of 131072, not four).
+// parts of a sequence of 131072, not four), which takes registers that many rows' parts
+// are better read with (10 us against 16 for those of 33 sequences).
 hipError_t launch_join(const AttnArgs &a, int grid, bool deep, hipStream_t s);
 
 // The tile kernel (paged_attn_tile.hip): its rows per item and workgroups.

@@ -543,7 +543,7 @@ hipError_t launch_paged_attn_mx4(Mx4AttnArgs a, void *workspace, hipStream_t s) 
                        : a.dtype == ZT_DT_BF16 ? launch_rows_as<uint16_t>(a, p.grid, s)
                                                : launch_rows_as<float>(a, p.grid, s);
   if (e != hipSuccess) return e;
-  return launch_join(a, p.grid, true, s);
+  return launch_join(a, p.grid, !p.tiles, s);
 }
 
 }  // namespace zt
