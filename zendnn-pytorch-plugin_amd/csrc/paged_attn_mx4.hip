@@ -64,7 +64,7 @@ __device__ __forceinline__ float top(float x) { return __uint_as_float(__float_a
 //
 // NEAR: a near cache's places (mx4.hpp) are found with a third of the instructions.
 // WORDS: a row's scales are loaded together.
-template <typename T, int DP, bool NEAR, bool WORDS>
+template <typename T, int DP, int DC, bool NEAR, bool WORDS>
 __global__ __launch_bounds__(kRowThreads, 2) void mx4_row_kernel(Mx4AttnArgs a) {
   using Cost = Mx4RowCost;
   constexpr bool BF = sizeof(T) == 2;
@@ -78,7 +78,7 @@ __global__ __launch_bounds__(kRowThreads, 2) void mx4_row_kernel(Mx4AttnArgs a) 
   constexpr int CR = DP / 32;             // blocks of a row
   constexpr int VP = DP * 2 + 32;         // LDS pitch of a row of values
   constexpr int OP = DP + 4;              // pitch of the joined outputs, floats
-  constexpr int DT = DP / 16;
+  constexpr int DT = DC / 16;
   constexpr int kWaveLds = 32 * VP > 16 * OP * 4 ? 32 * VP : 16 * OP * 4;
   typedef unsigned piece_t __attribute__((ext_vector_type(WB)));
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
@@ -425,8 +425,8 @@ __global__ __launch_bounds__(kRowThreads, 2) void mx4_row_kernel(Mx4AttnArgs a) 
               for (int e = 0; e < 4; ++e) *reinterpret_cast<float *>(vlds + (n * OP + col + e) * 4) = NAN;
         }
     __syncthreads();
-    for (int e = tid; e < 16 * DP / 4; e += kRowThreads) {
-      const int row = e / (DP / 4), d = e % (DP / 4) * 4;
+    for (int e = tid; e < 16 * DC / 4; e += kRowThreads) {
+      const int row = e / (DC / 4), d = e % (DC / 4) * 4;
       const int rr = r0 + row;
       const int tok = (int)fast_div(rr, a.div_group);
       if (tok >= s.q || d >= a.D) continue;
@@ -461,11 +461,11 @@ __global__ __launch_bounds__(kRowThreads, 2) void mx4_row_kernel(Mx4AttnArgs a) 
 
 constexpr int kRowGrid = 512;  // workgroups, at most: two per CU
 
-template <typename T, int DP, bool NEAR, bool WORDS>
+template <typename T, int DP, int DC, bool NEAR, bool WORDS>
 hipError_t launch_rows(const Mx4AttnArgs &a, int grid, hipStream_t s) {
   constexpr int wave = std::max(32 * (DP * 2 + 32), 16 * (DP + 4) * 4);
   const size_t lds = 4 * wave + batch_ints(a.S) * 4, largest = 4 * wave + batch_ints(kMaxSeqs) * 4;
-  auto kernel = mx4_row_kernel<T, DP, NEAR, WORDS>;
+  auto kernel = mx4_row_kernel<T, DP, DC, NEAR, WORDS>;
   const hipError_t allowed = allow_lds(reinterpret_cast<const void *>(kernel), lds, largest);
   if (allowed != hipSuccess) return allowed;
   kernel<<<grid, kRowThreads, lds, s>>>(a);
@@ -473,9 +473,11 @@ hipError_t launch_rows(const Mx4AttnArgs &a, int grid, hipStream_t s) {
 }
 template <typename T, bool NEAR, bool WORDS>
 hipError_t launch_rows_of(const Mx4AttnArgs &a, int grid, hipStream_t s) {
-  if (a.D <= 64) return launch_rows<T, 64, NEAR, WORDS>(a, grid, s);
-  if (a.D <= 128) return launch_rows<T, 128, NEAR, WORDS>(a, grid, s);
-  return launch_rows<T, 256, NEAR, WORDS>(a, grid, s);
+  if (a.D <= 64) return launch_rows<T, 64, 64, NEAR, WORDS>(a, grid, s);
+  if constexpr (!WORDS)  // three blocks
+    if (a.D <= 96) return launch_rows<T, 128, 96, NEAR, false>(a, grid, s);
+  if (a.D <= 128) return launch_rows<T, 128, 128, NEAR, WORDS>(a, grid, s);
+  return launch_rows<T, 256, 256, NEAR, WORDS>(a, grid, s);
 }
 // Whether a cache is near and has its scales in words (mx4.hpp), and its strides.
 void set_near(Mx4AttnArgs *a) {
@@ -507,9 +509,24 @@ struct Shape {
 };
 double items_most(const Mx4AttnArgs &a, int bm) { return std::floor((double)a.T * (a.H / a.KV) / bm) + a.S; }
 double blocks_most(const Mx4AttnArgs &a, bool tiles) { return std::floor((double)a.W * a.page_size / (tiles ? 64 : 4 * row_strip(a.D))) + 1; }
+// Rows of one cache head up to which the row kernel is taken, 16 to an item, each of
+// which reads the keys again.  Measured, row against tile kernel, 8 cache heads, 32
+// sequences of 2048 tokens, us:
+//   bf16  head_dim 64:  32 rows 28 / 38    48 rows 40 / 44    64 rows 43 / 44
+//         head_dim 128: 32 rows 36 / 49    48 rows 56 / 56    64 rows 61 / 58
+//         head_dim 256: 32 rows 68 / 110   48 rows 112 / 112  64 rows 122 / 113
+//   fp32  head_dim 64:  20 rows 31 / 50    64 rows 51 / 61    96 rows 73 / 67
+//         head_dim 128: 32 rows 44 / 99    64 rows 78 / 104   96 rows 112 / 110
+// and 4 of 32768 in bf16 at head_dim 128: 20 rows 65 / 72, 48 rows 90 / 85.  Past
+// head_dim 128 the tile kernel's fp32 operands outgrow its registers (1024 rows of one
+// sequence of 2048: 73 / 252, 4096 rows 231 / 655), so there is none.
+int64_t rows_most(const Mx4AttnArgs &a) {
+  if (a.dtype == ZT_DT_BF16) return a.D <= 64 ? 48 : 32;
+  return a.D <= 128 ? 64 : INT64_MAX;
+}
 Shape shape_of(const Mx4AttnArgs &a) {
   const int64_t rows = std::min(std::max<int64_t>(a.max_q, 1), a.T) * (a.H / a.KV);
-  Shape p{rows > BM, BM, kRowGrid};
+  Shape p{rows > rows_most(a), BM, kRowGrid};
   if (p.tiles) p.bm = mx4_tile_rows(), p.grid = mx4_tile_grid(a);
   // no more workgroups than there can be blocks
   const double most = items_most(a, p.bm) * a.KV * blocks_most(a, p.tiles);

@@ -44,6 +44,11 @@ __device__ __forceinline__ void to_e4m3(uint32_t w0, uint32_t w1, float scale, f
 
 constexpr int NW = 4, NTH = 64 * NW, BM = 32 * NW, TK = 64;
 
+// Waves per SIMD, and so workgroups per CU: two, but for sizes whose queries and
+// outputs need the registers of both (fp32, head_dim 128, 512 tokens behind 1536:
+// 76 us with one, 125 with two, which spill; head_dim 96: 64 and 62).
+constexpr int waves(bool bf, int dim) { return dim <= (bf ? 128 : 96) ? 2 : 1; }
+
 // Four waves of 32 rows each against a span of the keys of one cache head.
 //
 // Tiles of 64 keys and values lie in LDS as bf16, which holds a code's value
@@ -57,7 +62,7 @@ constexpr int NW = 4, NTH = 64 * NW, BM = 32 * NW, TK = 64;
 //
 // NEAR: a near cache's places (mx4.hpp) are found with a third of the instructions.
 template <typename T, int DP, int DC, bool NEAR>
-__global__ __launch_bounds__(NTH) __attribute__((amdgpu_waves_per_eu(DP <= 128 ? 2 : 1, DP <= 128 ? 2 : 1))) void mx4_tile_kernel(Mx4AttnArgs a) {
+__global__ __launch_bounds__(NTH) __attribute__((amdgpu_waves_per_eu(waves(sizeof(T) == 2, DC), waves(sizeof(T) == 2, DC)))) void mx4_tile_kernel(Mx4AttnArgs a) {
   using Cost = Mx4TileCost;
   constexpr bool BF = sizeof(T) == 2;
   constexpr int QP = BF ? 1 : 3;                // bf16 parts of a query (not taken for bf16 ones) and of a weight
@@ -514,7 +519,8 @@ hipError_t launch_of(const Mx4AttnArgs &a, int grid, hipStream_t s) {
   if (a.D <= 64) return launch_as<T, 64, 64, NEAR>(a, grid, s);
   if (a.D <= 96) return launch_as<T, 128, 96, NEAR>(a, grid, s);
   if (a.D <= 128) return launch_as<T, 128, 128, NEAR>(a, grid, s);
-  return launch_as<T, 256, 256, NEAR>(a, grid, s);
+  if constexpr (sizeof(T) == 2) return launch_as<T, 256, 256, NEAR>(a, grid, s);
+  return hipErrorInvalidValue;  // fp32 past 128: the row kernel's
 }
 template <typename T>
 hipError_t launch_by(const Mx4AttnArgs &a, int grid, hipStream_t s) {
@@ -524,7 +530,7 @@ hipError_t launch_by(const Mx4AttnArgs &a, int grid, hipStream_t s) {
 }  // namespace
 
 int mx4_tile_rows() { return BM; }
-int mx4_tile_grid(const Mx4AttnArgs &a) { return a.D <= 128 ? 512 : 256; }
+int mx4_tile_grid(const Mx4AttnArgs &a) { return 256 * waves(a.dtype == ZT_DT_BF16, a.D); }
 hipError_t launch_mx4_tiles(const Mx4AttnArgs &a, int grid, hipStream_t s) {
   return a.dtype == ZT_DT_BF16 ? launch_by<uint16_t>(a, grid, s) : launch_by<float>(a, grid, s);
 }
