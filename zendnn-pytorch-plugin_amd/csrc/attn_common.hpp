@@ -200,7 +200,7 @@ __device__ __forceinline__ int seq_of_item(const int *tile_base, int S, int x) {
 
 // The cost of a block of an item of `rows` rows, and the least span.
 struct RowCost {  // every row kernel's unit is the same bytes
-  static constexpr int kLead = 1, kMost = 1, kLeast = 1;
+  static constexpr int kLead = 1, kMost = 1, kLeast = 1, kJoin = 0;
   static __device__ __forceinline__ int of(int) { return 1; }
 };
 
@@ -256,15 +256,25 @@ __device__ __forceinline__ Plan make_plan(const AttnArgs &a, int BM, int UK, con
   // sequence more than that (1984 tokens behind 6144, 496 items: 272 / 275; 1920:
   // 273 / 265; 1792: 271 / 249), where several short ones would gain further
   // (4 x 448 behind 2048: 105 / 117).
+  // A Cost may name what a join is worth (kJoin): fewer (item, head)s than workgroups
+  // then are whole too, if the longest is no longer than an equal span and that; they
+  // are dealt to the XCDs evenly.
   const int pairs = p.items * a.KV, grid = (int)gridDim.x;
-  if (p.items <= N && pairs <= grid && 32 * (int64_t)pairs >= 31 * (int64_t)grid) {
+  bool whole = p.items <= N && pairs <= grid && 32 * (int64_t)pairs >= 31 * (int64_t)grid;
+  const bool few = Cost::kJoin > 0 && !whole && p.items <= N && pairs <= grid;
+  if (whole || few) {
     if (tid == 0) sh->most = 0;
     __syncthreads();
     if (cost) atomicMax(&sh->most, cost);
     __syncthreads();
-    if ((int64_t)sh->most * p.items <= (int64_t)sum + sum / 4) {
+    if (few) whole = (int64_t)(sh->most - Cost::kJoin) * grid <= (int64_t)sum * a.KV;
+    else whole = (int64_t)sh->most * p.items <= (int64_t)sum + sum / 4;
+    if (whole) {
       const int xcd = blockIdx.x & 7, each = grid / 8, i = blockIdx.x >> 3;
-      if (grid % 16 == 0 && i >= each / 2) p.wg = xcd * each + each / 2 + each - 1 - i;
+      const int here = pairs / 8 + (xcd < pairs % 8 ? 1 : 0);  // of this XCD; its others have numbers past the last
+      if (few && i < here) p.wg = xcd_contiguous_tile(blockIdx.x, pairs);
+      else if (few) p.wg = pairs + xcd * each + min(xcd, grid % 8) - xcd * (pairs / 8) - min(xcd, pairs % 8) + i - here;
+      else if (grid % 16 == 0 && i >= each / 2) p.wg = xcd * each + each / 2 + each - 1 - i;
       if (p.wg >= pairs) return p;
       p.head = p.wg / p.items, p.item = p.wg - p.head * p.items;
       if (p.item == tid) sh->before = before, sh->item = cost;

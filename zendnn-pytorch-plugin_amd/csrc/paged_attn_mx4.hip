@@ -16,7 +16,7 @@ constexpr int BM = 16;  // rows of an item
 // An item's beginning and end cost two units of 256 keys, in the trips to memory that
 // nothing hides: 64 ragged sequences 49 us, with one unit 53, with three 50.
 struct Mx4RowCost {
-  static constexpr int kLead = 2, kMost = 1, kLeast = 1;
+  static constexpr int kLead = 2, kMost = 1, kLeast = 1, kJoin = 0;
   static __device__ __forceinline__ int of(int) { return 1; }
 };
 constexpr int row_strip(int dp) { return dp <= 128 ? 64 : 32; }

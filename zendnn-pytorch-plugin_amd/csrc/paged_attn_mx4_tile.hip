@@ -18,7 +18,7 @@ __device__ __forceinline__ uint32_t tops(float lo, float hi) {
 __device__ __forceinline__ float top(float x) { return __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
 
 struct Mx4TileCost {
-  static constexpr int kLead = 15, kMost = kTileCostMost, kLeast = 4 * kMost;
+  static constexpr int kLead = 15, kMost = kTileCostMost, kLeast = 4 * kMost, kJoin = 24;
   static __device__ __forceinline__ int of(int rows) { return 4 + (rows + 63) / 64; }
 };
 

@@ -33,7 +33,7 @@ __device__ __forceinline__ void wait_and_meet() {
 // bytes (32 tokens of 32 heads behind 2048: 40 us without, 35 with).
 template <typename T>
 struct TileCost {
-  static constexpr int kLead = sizeof(T) == 2 ? 15 : 7, kMost = 6, kLeast = sizeof(T) == 2 ? 4 * kMost : kMost;
+  static constexpr int kLead = sizeof(T) == 2 ? 15 : 7, kMost = 6, kLeast = sizeof(T) == 2 ? 4 * kMost : kMost, kJoin = 0;
   static __device__ __forceinline__ int of(int rows) {
     return sizeof(T) == 2 ? 4 + (rows + 63) / 64 : 6;
   }
