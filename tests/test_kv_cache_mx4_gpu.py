@@ -539,3 +539,147 @@ def test_pages_move_with_their_scales():
     for t, w in zip(c, before):
         w[6], w[0] = w[1].clone(), w[3].clone()
         assert torch.equal(t, w)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_a_served_batch(dtype):
+    """Steps as a program makes them: pages for the new tokens, their keys and
+    values written, attention over them, a fork, pages gathered; what the cache
+    holds is followed token by token, and every step's attention checked."""
+    H, KV, D, size, pages, W = 8, 2, 80, 16, 40, 8
+    r = random.Random(3)
+    table = torch.full((4, W), -1, dtype=torch.int32, device=DEV)
+    lens, refs = i32([0] * 4), i32([0] * pages)
+    c = M.cache(pages, KV, size, D, fill=255)
+    held = [[] for _ in range(4)]  # per sequence, its tokens' (key, value)
+    cos_sin = rope(W * size, D)
+    for step, new in enumerate(((37, 5, 64, 18), (1, 1, 1, 1), (3, 1, 2, 1), "fork", (1, 1, 1, 1), (20, 2, 1, 7))):
+        if new == "fork":
+            parents = [0, 0, 2, 0]
+            table, lens, refs, copies = ops.zentorch_cache_fork(table, lens, refs, i32(parents), size)
+            ops.zentorch_cache_copy_pages([c[0], c[2]], copies)
+            ops.zentorch_cache_copy_pages([c[1], c[3]], copies)
+            held = [list(held[p]) for p in parents]
+            table, refs, copies = ops.zentorch_cache_compact(table, refs)
+            ops.zentorch_cache_copy_pages([c[0], c[2]], copies)
+            ops.zentorch_cache_copy_pages([c[1], c[3]], copies)
+            continue
+        T = sum(new)
+        cu = i32([sum(new[:i]) for i in range(5)])
+        table, lens, refs, pos, slots = ops.zentorch_cache_extend(table, lens, refs, cu, size, T)
+        q, k, v = tokens(T, H, KV, D, dtype, seed=10 * step + r.randrange(5))
+        k, v, q = (x / x.double().abs().amax(-1, keepdim=True).to(dtype) for x in (k, v, q))
+        q = ops.zentorch_rotary_cache_append_mxfp4(q, k, v, pos, cos_sin, slots, *c)
+        key, _ = R.rotary(k, pos, cos_sin, False)
+        at = 0
+        for i, n in enumerate(new):
+            held[i] += [(M.values(*M.quantise(key[j]), D), M.values(*M.quantise(v[j].double()), D))
+                        for j in range(at, at + n)]
+            at += n
+        assert lens.tolist() == [len(s) for s in held]
+        for i in range(4):
+            tok = torch.arange(len(held[i]), device=DEV)
+            where = table[i].long()[tok // size] * size + tok % size
+            for got, j in zip(ops.zentorch_cache_read_mxfp4(*c, where, D, dtype=dtype), (0, 1)):
+                assert torch.equal(got.double(), torch.stack([t[j] for t in held[i]]))
+        check(dict(q=q, c=c, table=table, cu=cu, ctx=lens, max_q=max(new)))
+
+
+def test_many_sequences():
+    """As many sequences as a call takes, more items than a round of any loop."""
+    r = random.Random(7)
+    lens = [(1, r.randint(1, 40)) for _ in range(1024)]
+    check(make(lens, 4, 2, 64, 16, BF, seed=7))
+    check(make(lens, 2, 1, 256, 8, F32, seed=8))
+    lens = [(r.randint(1, 30), 30) for _ in range(1023)] + [(400, 700)]
+    check(make(lens, 4, 2, 64, 16, BF, seed=9))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("rows", [16, 17, 32, 33, 48, 49, 64, 65, 80])
+def test_attn_around_the_kernels_borders(rows, D, dtype):
+    check(make([(rows, 300), (1, 40), (min(rows, 7), 7)], 2, 2, D, 16, dtype, seed=rows))
+    check(make([(rows, 150)] * 3, 2, 2, D, 16, dtype, seed=rows + 1), max_q=1)  # too small a value costs time only
+
+
+def test_whole_items():
+    """Fewer items than workgroups, of about one length: none is cut."""
+    for n, kv in ((128, 16), (256, 37), (300, 3), (500, 1)):
+        check(make([(n, n)] * 3, kv, kv, 64, 16, F32, seed=n), causal=False)
+        check(make([(n, n)] * 2, kv, kv, 64, 16, BF, seed=n))
+
+
+def test_two_streams_at_once():
+    """Calls of different sizes on two streams, with nothing between them."""
+    bs = [make([(1, 3000), (1, 77)], 8, 2, 128, 16, BF, seed=1), make([(300, 900)], 8, 2, 256, 16, BF, seed=2)]
+    want = [call(b) for b in bs]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in bs], [[], []]
+    for _ in range(20):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(call(bs[i]))
+    torch.cuda.synchronize()
+    for w, out in zip(want, got):
+        assert all(torch.equal(x, w) for x in out)
+
+
+def test_compiled():
+    """The in-place op under torch.compile, against eager."""
+    x = torch.randn(6, 12, 64, generator=torch.Generator().manual_seed(0)).bfloat16().to(DEV)
+    table, slots, pos = rope(64, 64), i64([3, 40, 7, -1, 9, 20]), i64([0, 5, 9, 3, 1, 2])
+
+    def step(x, kc, ks, vc, vs):
+        q = ops.zentorch_rotary_cache_append_mxfp4(x[:, :8], x[:, 8:10], x[:, 10:], pos, table, slots, kc, ks, vc, vs)
+        k, v = ops.zentorch_cache_read_mxfp4(kc, ks, vc, vs, slots, 64)
+        return q * 2, k, v
+
+    a, b = M.cache(4, 2, 16, 64, fill=3), M.cache(4, 2, 16, 64, fill=3)
+    want = step(x, *a)
+    got = torch.compile(step, backend="aot_eager", fullgraph=True)(x, *b)
+    assert all(torch.equal(y, w) for y, w in zip((*got, *b), (*want, *a)))
+
+
+def refused(word, f, *args, **kw):
+    with pytest.raises(RuntimeError) as e:
+        f(*args, **kw)
+    assert word in str(e.value), str(e.value)
+
+
+def test_refusals():
+    kc, ks, vc, vs = M.filled(4, 2, 16, 64)
+    x = torch.randn(3, 2, 64, device=DEV).bfloat16()
+    q = torch.randn(3, 4, 64, device=DEV).bfloat16()
+    pos, table = i64([0, 1, 2]), rope(8, 64)
+    append, read, attn = (ops.zentorch_rotary_cache_append_mxfp4, ops.zentorch_cache_read_mxfp4,
+                          ops.zentorch_paged_attention_mxfp4)
+    rest = (i32([[0, 1, 2, 3]]), i32([0, 3]), i32([20]), 3)
+    for c, word in (((kc.to(torch.int8), ks, vc, vs), "uint8"), ((kc, ks.float(), vc, vs), "uint8"),
+                    ((kc[..., :16], ks, vc, vs), "32 bytes a row"), ((kc, ks[..., :1], vc, vs), "2 bytes a row"),
+                    ((kc, ks, vc[:3], vs), "pages"), ((kc, ks, vc, vs[:, :1]), "pages"), ((kc[0], ks, vc, vs), "must be"),
+                    ((kc.cpu(), ks, vc, vs), "GPU"), ((kc.transpose(2, 3).contiguous().transpose(2, 3), ks, vc, vs), "dense")):
+        refused(word, attn, q, *c, *rest)
+        refused(word, read, *c, pos, 64)
+        refused(word, append, q, x, x, pos, table, pos, *c)
+    odd = torch.zeros(4 * 2 * 16 * 32 + 8, dtype=torch.uint8, device=DEV)[8:].view(4, 2, 16, 32)
+    for c in ((odd, ks, vc, vs), (kc, ks, odd, vs)):
+        refused("16-byte", attn, q, *c, *rest)
+        refused("16-byte", read, *c, pos, 64)
+    good = kc, ks, vc, vs
+    refused("bytes a row", attn, torch.randn(3, 4, 96, device=DEV), *good, *rest)
+    refused("multiple of 8", read, *good, pos, 60)
+    refused("positive", read, *good, pos, 0)
+    refused("bfloat16 or float32", attn, q.half(), *good, *rest)
+    refused("multiple of the cache's", attn, q[:, :3], *good, *rest)
+    refused("window", attn, q, *good, *rest, causal=False, window=4)
+    refused("int32", attn, q, *good, rest[0].long(), *rest[1:])
+    refused("cu_seqlens", attn, q, *good, rest[0], i32([0, 1, 3]), *rest[2:])
+    refused("dtype", read, *good, pos, 64, dtype=torch.float16)
+    refused("int64", read, *good, pos.int(), 64)
+    refused("one type", append, q, x.float(), x.float(), pos, table, pos, *good)
+    refused("key and value", append, q, x[:2], x[:2], pos, table, pos, *good)
+    refused("int64", append, q, x, x, pos[:2], table, pos, *good)
+    refused("float32", append, q, x, x, pos, table.double(), pos, *good)
+    refused("single memory location", append, q, x, x, pos, table, pos, kc, ks, kc, vs)
+    refused("unsupported operation", append, q, x, x, pos, table, pos, kc[:1].expand(4, 2, 16, 32), ks, vc, vs)

@@ -9,7 +9,9 @@ and compact with the page copies between steps.
 
 Weights are random.  ``python paged_decode.py`` prints the continuations and
 how far the last logits are from those of a cacheless recomputation of every
-whole sequence in plain torch operations.
+whole sequence in plain torch operations.  ``--mxfp4`` holds the cache in 4
+bits: the same steps, with the ops of that format in place of append and
+attention, and codes and scales copied where pages are.
 """
 import math
 import os
@@ -56,12 +58,12 @@ class Decoder:
         of all sequences, sequence i's being cu[i] .. cu[i + 1]."""
         pos, slots = cache.extend(cu, tokens.numel())
         x = self.embed[tokens]
-        for p, (k_cache, v_cache) in zip(self.layers, cache.views):
+        for p, views in zip(self.layers, cache.views):
             h = ops.zentorch_woq_linear(self.norm(x), p["qkv"]["w"], p["qkv"]["s"], None)
             q, k, v = (t.view(tokens.numel(), -1, self.dim) for t in h.split(
                 [self.heads * self.dim, self.kv * self.dim, self.kv * self.dim], dim=1))
-            q = ops.zentorch_rotary_cache_append(q, k, v, pos, cache.cos_sin, slots, k_cache, v_cache)
-            a = ops.zentorch_paged_attention(q, k_cache, v_cache, cache.table, cu, cache.lens, max_query_len)
+            q = cache.append(q, k, v, pos, cache.cos_sin, slots, *views)
+            a = cache.attention(q, *views, cache.table, cu, cache.lens, max_query_len)
             x = ops.zentorch_woq_linear_add(a.flatten(1), p["o"]["w"], p["o"]["s"], None, x)
             m = ops.zentorch_woq_linear_gate_up_silu_mul(self.norm(x), p["gate_up"]["w"], p["gate_up"]["s"], None)
             x = ops.zentorch_woq_linear_add(m, p["down"]["w"], p["down"]["s"], None, x)
@@ -96,11 +98,22 @@ class Decoder:
 class PagedCache:
     """Every layer's pages, one block table for all of them, and its upkeep."""
 
-    def __init__(self, model, rows, pages=96, page_size=16, width=16):
+    def __init__(self, model, rows, pages=96, page_size=16, width=16, mxfp4=False):
         dev, self.size = model.device, page_size
-        self.layers = [torch.zeros(pages, 2, model.kv, page_size, model.dim, dtype=torch.bfloat16, device=dev)
-                       for _ in model.layers]
-        self.views = [c.unbind(1) for c in self.layers]
+
+        def layers(width, dtype):  # a layer's keys and values beside each other
+            return [torch.zeros(pages, 2, model.kv, page_size, width, dtype=dtype, device=dev) for _ in model.layers]
+
+        if mxfp4:
+            blocks = -(-model.dim // 32)
+            codes, scales = layers(16 * blocks, torch.uint8), layers(blocks, torch.uint8)
+            self.parts = [codes, scales]  # what a page's copy has to take along
+            self.views = [(c[:, 0], s[:, 0], c[:, 1], s[:, 1]) for c, s in zip(codes, scales)]
+            self.append, self.attention = ops.zentorch_rotary_cache_append_mxfp4, ops.zentorch_paged_attention_mxfp4
+        else:
+            self.parts = [layers(model.dim, torch.bfloat16)]
+            self.views = [c.unbind(1) for c in self.parts[0]]
+            self.append, self.attention = ops.zentorch_rotary_cache_append, ops.zentorch_paged_attention
         self.table = torch.full((rows, width), -1, dtype=torch.int32, device=dev)
         self.lens = torch.zeros(rows, dtype=torch.int32, device=dev)
         self.refs = torch.zeros(pages, dtype=torch.int32, device=dev)
@@ -114,18 +127,22 @@ class PagedCache:
     def fork(self, parents):
         self.table, self.lens, self.refs, copies = ops.zentorch_cache_fork(
             self.table, self.lens, self.refs, parents, self.size)
-        ops.zentorch_cache_copy_pages(self.layers, copies)
+        self.copy_pages(copies)
 
     def compact(self):
         self.table, self.refs, copies = ops.zentorch_cache_compact(self.table, self.refs)
-        ops.zentorch_cache_copy_pages(self.layers, copies)
+        self.copy_pages(copies)
+
+    def copy_pages(self, copies):
+        for caches in self.parts:
+            ops.zentorch_cache_copy_pages(caches, copies)
 
 
-def run(prompt_lens=(37, 5, 64, 18), steps=6, device="cuda"):
+def run(prompt_lens=(37, 5, 64, 18), steps=6, device="cuda", mxfp4=False):
     """(sequences, the last step's logits, the plain ones, the cache)."""
     model = Decoder(device=device)
     rows = len(prompt_lens)
-    cache = PagedCache(model, rows)
+    cache = PagedCache(model, rows, mxfp4=mxfp4)
     g = torch.Generator().manual_seed(1)
     seqs = [torch.randint(0, 1000, (n,), generator=g).to(device) for n in prompt_lens]
 
@@ -150,7 +167,7 @@ def run(prompt_lens=(37, 5, 64, 18), steps=6, device="cuda"):
 
 
 if __name__ == "__main__":
-    seqs, got, want, cache = run()
+    seqs, got, want, cache = run(mxfp4="--mxfp4" in sys.argv[1:])
     for s in seqs:
         print(len(s), s[-8:].tolist())
     rel = ((got - want).norm() / want.norm()).item()
