@@ -505,7 +505,7 @@ int zt_cache_copy_pages(void *const *caches, int64_t n_caches, int64_t pages, in
  * multiplies.  Writing picks the E for which the block's largest magnitude is
  * at least 3.5 and less than 7 scales, held to -125 .. 125, and for each number
  * the nearest code (of two equally near ones the even one; magnitudes past 6
- * scales take 6): off by a seventh of the block's largest number at most.  A
+ * scales take 6): off by a fifth of the block's largest number at most.  A
  * block with an infinity or a NaN is written as codes of 0 under the byte 255.
  * Read, the bytes 253 .. 255 stand for NaN.
  *
@@ -548,6 +548,12 @@ int zt_cache_read_mxfp4(const zt_kv_cache_mxfp4 *cache, const int64_t *slots, in
  * zt_paged_attention over a cache held in 4 bits: the same sequences, masks,
  * bounds and rules, with q and out in `dtype`.  Keys and values take part as
  * the numbers that their codes stand for, without another rounding.
+ * max_query_len picks the kernels here too.  In fp32 queries and weights keep 24
+ * digits.  In bf16 weights have 16 bits' precision where max_query_len tokens are
+ * up to 32 rows of a cache head (48 up to head_dim 64).  With more they have
+ * bf16's 8, and scores are sums of 8-bit parts of the queries: off by 1e-5 of their
+ * norm, and by 1e-4 of the sum of their products' magnitudes at most, as measured.
+ * A query that is not finite makes its row NaN.
  */
 int zt_paged_attention_mxfp4(const void *q, int32_t dtype, int64_t T, int64_t H, int64_t ld_token, int64_t ld_head,
                              const zt_kv_cache_mxfp4 *cache, const int32_t *block_table, int64_t S, int64_t W,

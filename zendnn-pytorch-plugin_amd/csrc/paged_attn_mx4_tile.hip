@@ -17,6 +17,9 @@ __device__ __forceinline__ uint32_t tops(float lo, float hi) {
 }
 __device__ __forceinline__ float top(float x) { return __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
 
+// As in paged_attn_tile.hip, whose item ends and tiles these resemble.  A join is worth
+// four blocks: eight whole fp32 sequences of up to 500 take 33-38 us in whole items,
+// 40-44 in equal spans; 16 chunks of 100 tokens and the like are the same either way.
 struct Mx4TileCost {
   static constexpr int kLead = 15, kMost = kTileCostMost, kLeast = 4 * kMost, kJoin = 24;
   static __device__ __forceinline__ int of(int rows) { return 4 + (rows + 63) / 64; }
@@ -51,14 +54,33 @@ constexpr int waves(bool bf, int dim) { return dim <= (bf ? 128 : 96) ? 2 : 1; }
 
 // Four waves of 32 rows each against a span of the keys of one cache head.
 //
-// Tiles of 64 keys and values lie in LDS as bf16, which holds a code's value
-// exactly, two tiles deep: each thread has its part of the next tile's codes in
-// registers, unpacks them into the other stage beside the scores' MFMAs, and then
-// loads its part of the tile after that.  One barrier a tile.
+// Bound by the matrix operations with the vector operations beside them.  Tiles of 64
+// keys and values lie in LDS two deep: each thread has its part of the next tile's
+// codes in registers, puts it into the other stage beside the scores' MFMAs, and then
+// loads its part of the tile after that.  One barrier a tile.  Values are unpacked to
+// bf16 on the way, once for the four waves, because their scales run along a token's
+// row, and the second product sums over tokens.
 //
-// Scores, weights and outputs are as in paged_attn_tile.hip, on 32x32 MFMAs,
-// transposed.  fp32 queries and weights go in three bf16 parts (cut short, 24
-// digits), three MFMAs a product.
+// Scores in bf16: scales run along the sum there, as the scaled MFMA takes them (e2m1
+// by e4m3, 32x32x64), so keys stay packed in LDS, a quarter of the bytes to write and
+// read.  A bf16 query is two parts of e4m3, four digits each, at half the time an MFMA:
+// as much matrix time as bf16 keys.  Its sums lose digits below the largest product:
+// measured on normal numbers, scores are off by 8e-6 of their root mean square (1e-4 of
+// the products' sum of magnitudes at most, on random bytes of every size), a
+// hundredth of what the rounding of the weights does.  A chunk of 2048 behind 6144 takes
+// 235-250 us, 257-267 with keys unpacked to bf16; 33 mixed sequences 55, 51 then,
+// because the parts are made once an item.
+//
+// fp32 queries and weights go in three bf16 parts (cut short, 24 digits), three MFMAs a
+// product, with keys unpacked to bf16, which is exact.
+//
+// The running maximum, the weights and the second product are those of
+// paged_attn_tile.hip, on 32x32 MFMAs, transposed.
+//
+// Measured (32 query and 8 cache heads of 128, bf16): the chunk above 0.96-1.02 PFLOP/s
+// (a large product of the library reaches 1.2); copies of the kernel with bf16 keys
+// took 239 without unpacking, 240 without the loads, 242 without the exponentials
+// beside 261.  Eight whole fp32 sequences of up to 500, 16 heads of 64: 33 us.
 //
 // NEAR: a near cache's places (mx4.hpp) are found with a third of the instructions.
 template <typename T, int DP, int DC, bool NEAR>
