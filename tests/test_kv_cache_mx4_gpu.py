@@ -683,3 +683,33 @@ def test_refusals():
     refused("float32", append, q, x, x, pos, table.double(), pos, *good)
     refused("single memory location", append, q, x, x, pos, table, pos, kc, ks, kc, vs)
     refused("unsupported operation", append, q, x, x, pos, table, pos, kc[:1].expand(4, 2, 16, 32), ks, vc, vs)
+
+
+def test_near_cache_past_2_to_the_31():
+    """Keys and values laid out alike, their pages 2.5 GB from first to last."""
+    page, D, pages, stride = 16, 128, 300, 1 << 23
+    buf = torch.empty(pages * stride, dtype=torch.uint8, device=DEV)
+    c = [buf.as_strided((pages, 2, page, b), (stride, page * b, b, 1), at)
+         for b, at in ((64, 0), (4, 65536), (64, 131072), (4, 196608))]
+    for t, x in zip(c, M.filled(pages, 2, page, D, seed=4)):
+        t.copy_(x)
+    g = torch.Generator().manual_seed(0)
+    r = random.Random(1)
+    for q in (1, 90):
+        b = dict(q=torch.randn(2 * q, 8, D, generator=g).bfloat16().to(DEV), c=tuple(c),
+                 table=i32([r.sample(range(256, 300), 8), r.sample(range(300), 7) + [299]]), cu=i32([0, q, 2 * q]),
+                 ctx=i32([120, 128]), max_q=q)
+        check(b)
+        b["q"] = b["q"].float()
+        check(b)
+
+
+def test_slots_past_2_to_the_31():
+    """Every page is the same memory here, which reading allows."""
+    kc, ks, vc, vs = M.filled(1, 2, 4096, 32, seed=2)
+    c = [t.expand(1 << 20, -1, -1, -1) for t in (kc, ks, vc, vs)]
+    slots = i64([((1 << 20) - 1) * 4096 + 5, (1 << 31) - 1, 1 << 31, (1 << 32) - 1, 1 << 32, 7])
+    for got, (codes, scales) in zip(ops.zentorch_cache_read_mxfp4(*c, slots, 32), ((kc, ks), (vc, vs))):
+        want = M.values(codes, scales, 32)[0].transpose(0, 1)[slots % 4096]
+        want[4] = 0  # past the pool
+        assert torch.equal(got.double(), want)

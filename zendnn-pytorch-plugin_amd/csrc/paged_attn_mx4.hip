@@ -106,7 +106,6 @@ __global__ __launch_bounds__(kRowThreads, 2) void mx4_row_kernel(Mx4AttnArgs a) 
 
   const float c = score_factor(a.scale);
   const int G = a.group;
-  const char *zero = reinterpret_cast<const char *>(kZeroRow);
   // the lane's i-th piece of a row: its block, and its place; a block past the row's
   // end has scale 0, and any codes
   auto block = [&](int i) { return DP == 64 ? g >> 1 : g + 4 * i; };
@@ -145,33 +144,17 @@ __global__ __launch_bounds__(kRowThreads, 2) void mx4_row_kernel(Mx4AttnArgs a) 
     int k0 = (seg.b0 + seg.bb) * UK + wave * KS;
     auto lookup = [&](int at) { return pages.lookup(a, at + key_lane); };
     int page = lookup(k0);  // on its way while the queries are fetched
-    // ---- the queries, as B operands
-    u32x4_t q[QP][NS];
+    // ---- the queries, on their way beside the first keys' places (what is not there is
+    // read from the first query)
+    constexpr int kRaw = NS * (BF ? 1 : 2);  // 16 bytes each
+    u32x4_t raw[kRaw];
     {
       const char *src = static_cast<const char *>(a.q) +
           ((int64_t)(s.q0 + row_t) * a.q_ld[0] + (h * G + r0 + n - row_t * G) * a.q_ld[1]) * (int64_t)sizeof(T);
 #pragma unroll
-      for (int t = 0; t < NS; ++t) {
-        const int e = element(t);
-        const char *at = live && e < a.D ? src + e * sizeof(T) : zero;
-        if constexpr (BF) {
-          q[0][t] = scale_sign<T>(*reinterpret_cast<const u32x4_t *>(at), a.scale);
-        } else {
-          float x[8];
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const u32x4_t w = scale_sign<T>(reinterpret_cast<const u32x4_t *>(at)[j], a.scale);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x[4 * j + i] = __uint_as_float(w[i]);
-          }
-#pragma unroll
-          for (int p = 0; p < QP; ++p)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              q[p][t][i] = tops(x[2 * i], x[2 * i + 1]);
-              x[2 * i] -= top(x[2 * i]), x[2 * i + 1] -= top(x[2 * i + 1]);
-            }
-        }
+      for (int y = 0; y < kRaw; ++y) {
+        const int e = BF ? element(y) : element(y / 2) + 4 * (y % 2);
+        raw[y] = *reinterpret_cast<const u32x4_t *>(live && e < a.D ? src + e * sizeof(T) : static_cast<const char *>(a.q));
       }
     }
     f32x4_t o[DT];
@@ -254,6 +237,32 @@ __global__ __launch_bounds__(kRowThreads, 2) void mx4_row_kernel(Mx4AttnArgs a) 
     page = lookup(k0 + UK);
 #pragma unroll
     for (int u = 2; u < KT; u += 2) load_v(u);
+    // ---- the queries, as B operands
+    u32x4_t q[QP][NS];
+#pragma unroll
+    for (int y = 0; y < kRaw; ++y) {
+      const bool have = live && (BF ? element(y) : element(y / 2)) < a.D;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) raw[y][i] = have ? raw[y][i] : 0u;
+      raw[y] = scale_sign<T>(raw[y], a.scale);
+    }
+#pragma unroll
+    for (int t = 0; t < NS; ++t) {
+      if constexpr (BF) {
+        q[0][t] = raw[t];
+      } else {
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(raw[2 * t + i / 4][i % 4]);
+#pragma unroll
+        for (int p = 0; p < QP; ++p)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            q[p][t][i] = tops(x[2 * i], x[2 * i + 1]);
+            x[2 * i] -= top(x[2 * i]), x[2 * i + 1] -= top(x[2 * i + 1]);
+          }
+      }
+    }
     for (; k0 < kend; k0 += UK) {
       const uint64_t held = WIDE ? there : there & 0xffffffffull;
       const bool whole = held == (WIDE ? ~0ull : 0xffffffffull);
