@@ -549,11 +549,9 @@ int zt_cache_read_mxfp4(const zt_kv_cache_mxfp4 *cache, const int64_t *slots, in
  * bounds and rules, with q and out in `dtype`.  Keys and values take part as
  * the numbers that their codes stand for, without another rounding.
  * max_query_len picks the kernels here too.  In fp32 queries and weights keep 24
- * digits.  In bf16 weights have 16 bits' precision where max_query_len tokens are
- * up to 32 rows of a cache head (48 up to head_dim 64).  With more they have
- * bf16's 8, and scores are sums of 8-bit parts of the queries: off by 1e-5 of their
- * norm, and by 1e-4 of the sum of their products' magnitudes at most, as measured;
- * a query that is not finite then makes its row NaN, whatever its scores are.
+ * digits, and a query that is not finite makes its row NaN, whatever its scores are.
+ * In bf16 weights have 16 bits' precision where max_query_len tokens are up to 32
+ * rows of a cache head (48 up to head_dim 64), else bf16's 8.
  */
 int zt_paged_attention_mxfp4(const void *q, int32_t dtype, int64_t T, int64_t H, int64_t ld_token, int64_t ld_head,
                              const zt_kv_cache_mxfp4 *cache, const int32_t *block_table, int64_t S, int64_t W,

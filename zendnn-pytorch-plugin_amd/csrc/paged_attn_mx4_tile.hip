@@ -25,26 +25,6 @@ struct Mx4TileCost {
   static __device__ __forceinline__ int of(int rows) { return 4 + (rows + 63) / 64; }
 };
 
-typedef int i32x8_t __attribute__((ext_vector_type(8)));
-
-typedef short i16x2_t __attribute__((ext_vector_type(2)));
-typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
-
-// Four bf16 numbers over 2^E (up to 256 then) as e4m3, and 16 times what that
-// leaves of them as e4m3; scale is 2^E, by16 is 2^(4 - E).
-__device__ __forceinline__ void to_e4m3(uint32_t w0, uint32_t w1, float scale, float by16, int *high, int *low) {
-  i16x2_t h = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(i16x2_t{0, 0}, __builtin_bit_cast(bf16x2_t, w0), scale, false);
-  h = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(h, __builtin_bit_cast(bf16x2_t, w1), scale, true);
-  const uint32_t hi = __builtin_bit_cast(uint32_t, h);
-  const auto a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hi, 16.f, false);
-  const auto b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hi, 16.f, true);
-  uint32_t lo = __builtin_amdgcn_cvt_pk_fp8_f32(fmaf(__uint_as_float(w0 << 16), by16, -a[0]),
-                                                fmaf(__uint_as_float(w0 & 0xffff0000u), by16, -a[1]), 0, false);
-  lo = __builtin_amdgcn_cvt_pk_fp8_f32(fmaf(__uint_as_float(w1 << 16), by16, -b[0]),
-                                       fmaf(__uint_as_float(w1 & 0xffff0000u), by16, -b[1]), lo, true);
-  *high = (int)hi, *low = (int)lo;
-}
-
 constexpr int NW = 4, NTH = 64 * NW, BM = 32 * NW, TK = 64;
 
 // Waves per SIMD, and so workgroups per CU: two, but for sizes whose queries and
@@ -56,52 +36,42 @@ constexpr int waves(bool bf, int dim) { return dim <= (bf ? 128 : 96) ? 2 : 1; }
 //
 // Bound by the matrix operations with the vector operations beside them.  Tiles of 64
 // keys and values lie in LDS two deep: each thread has its part of the next tile's
-// codes in registers, puts it into the other stage beside the scores' MFMAs, and then
-// loads its part of the tile after that.  One barrier a tile.  Values are unpacked to
-// bf16 on the way, once for the four waves, because their scales run along a token's
-// row, and the second product sums over tokens.
+// codes in registers, unpacks it to the other stage beside the scores' MFMAs, and then
+// loads its part of the tile after that.  One barrier a tile.
 //
-// Scores in bf16: scales run along the sum there, as the scaled MFMA takes them (e2m1
-// by e4m3, 32x32x64), so keys stay packed in LDS, a quarter of the bytes to write and
-// read.  A bf16 query is two parts of e4m3, four digits each, at half the time an MFMA:
-// as much matrix time as bf16 keys.  Its sums lose digits below the largest product:
-// measured on normal numbers, scores are off by 8e-6 of their root mean square (1e-4 of
-// the products' sum of magnitudes at most, on random bytes of every size), a
-// hundredth of what the rounding of the weights does.  A chunk of 2048 behind 6144 takes
-// 235-250 us, 257-267 with keys unpacked to bf16; 33 mixed sequences 55, 51 then,
-// because the parts are made once an item.
-//
-// fp32 queries and weights go in three bf16 parts (cut short, 24 digits), three MFMAs a
-// product, with keys unpacked to bf16, which is exact.
+// A code's value is a bf16 number exactly, so the products are bf16 MFMAs, unpacked
+// once for the four waves, without a rounding of keys or values: bf16 queries go as
+// they are and weights in one part, fp32 queries and weights in three (cut short, 24
+// digits).  Scores by scaled MFMAs over the codes themselves (e2m1 by queries in two
+// parts of e4m3) were 7 % faster on the chunk below and 3 % slower on 33 mixed
+// sequences, but two parts under one scale to 32 numbers lose the digits of those below
+// 2^-13 of the largest: with a channel 2^16 times the others, outputs were off by a tenth.
 //
 // The running maximum, the weights and the second product are those of
 // paged_attn_tile.hip, on 32x32 MFMAs, transposed.
 //
-// Measured (32 query and 8 cache heads of 128, bf16): the chunk above 0.96-1.02 PFLOP/s
-// (a large product of the library reaches 1.2); copies of the kernel with bf16 keys
-// took 239 without unpacking, 240 without the loads, 242 without the exponentials
-// beside 261.  Eight whole fp32 sequences of up to 500, 16 heads of 64: 33 us.
+// Measured (32 query and 8 cache heads of 128, bf16): 2048 tokens behind 6144 264 us, 0.91
+// PFLOP/s (a large product of the library reaches 1.2); copies of the kernel took 239
+// without unpacking, 240 without the loads, 242 without the exponentials beside 261.
+// 33 mixed sequences 53 us.  Eight whole fp32 sequences of up to 500, 16 heads of 64: 33 us.
 //
 // NEAR: a near cache's places (mx4.hpp) are found with a third of the instructions.
 template <typename T, int DP, int DC, bool NEAR>
 __global__ __launch_bounds__(NTH) __attribute__((amdgpu_waves_per_eu(waves(sizeof(T) == 2, DC), waves(sizeof(T) == 2, DC)))) void mx4_tile_kernel(Mx4AttnArgs a) {
   using Cost = Mx4TileCost;
   constexpr bool BF = sizeof(T) == 2;
-  constexpr int QP = BF ? 1 : 3;                // bf16 parts of a query (not taken for bf16 ones) and of a weight
+  constexpr int QP = BF ? 1 : 3;                // bf16 parts of a query and of a weight
   constexpr int KT = TK / 32;                   // 32-key tiles of a tile
   constexpr int CR = DP / 32;                   // blocks of a row: 16 bytes of codes, one scale
   constexpr int RB = DP * 2, PR = RB / 16;      // bytes and 16-byte pieces of an LDS row
-  constexpr int VST = TK * RB, KST = BF ? TK * CR * 16 : VST;  // bytes of a stage's values and keys
-  constexpr int SST = BF ? TK * CR : 0;         // and of its keys' scales
-  constexpr int STAGE = VST + KST + SST;
-  constexpr int KS = (DC + 63) / 64;            // scaled MFMA steps over a row
+  constexpr int STAGE = TK * RB;                // bytes of the values of a tile, and of its keys
   constexpr int NP = 2 * TK * CR / NTH;         // blocks of a tile per thread
   constexpr int NQ = DC / 16;                   // MFMA steps over a row
   constexpr int DT = DC / 32;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   __shared__ PlanShared sh;
   __shared__ uint64_t sm_bad[2][NW];
-  const Batch batch(smem + 2 * STAGE, a.S);
+  const Batch batch(smem + 4 * STAGE, a.S);
 
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -114,7 +84,7 @@ __global__ __launch_bounds__(NTH) __attribute__((amdgpu_waves_per_eu(waves(sizeo
   const char *zero = reinterpret_cast<const char *>(kZeroRow);
   const uint8_t *nothing = reinterpret_cast<const uint8_t *>(kZeroRow);
   // the 16-byte pieces of a row are permuted, so that 16 lanes meet no bank twice
-  auto kswz = [](int row) { return BF ? row / (8 / CR) & (CR - 1) : PR >= 16 ? row & 15 : row & 7; };
+  auto kswz = [](int row) { return PR >= 16 ? row & 15 : row & 7; };
   auto vswz = [](int row) { return PR >= 16 ? (row & 3) << 2 | ((row >> 2) & 3) : ((row >> 1) & 1) << 2; };
   // the thread's blocks of a tile: one row, the blocks of K and V
   const int part = DP == 64 ? (lane >> 4) + 4 * (wave & 1) : lane >> 4;
@@ -177,18 +147,10 @@ __global__ __launch_bounds__(NTH) __attribute__((amdgpu_waves_per_eu(waves(sizeo
         scales[j] = have ? scales[j] : 0u;
       }
     };
-    // and to LDS, a piece of 16 bytes at a time: values (and, for fp32, keys) as bf16,
-    // keys for bf16 queries as they are, with their scales
+    // and to LDS, a piece of 16 bytes at a time
     auto unpack = [&](int j, int i, int st) {
-      unsigned char *to = smem + st * STAGE;
-      if (BF && !is_v(j)) {
-        if (i) return;
-        *reinterpret_cast<u32x4_t *>(to + VST + row * CR * 16 + 16 * (block(j) ^ kswz(row))) = codes[j];
-        to[VST + KST + row * CR + block(j)] = (unsigned char)(scales[j] > kMxLast ? kMxNan : scales[j]);
-        return;
-      }
       const int p = 4 * block(j) + i;
-      to += (is_v(j) ? 0 : VST) + row * RB + 16 * (p ^ (is_v(j) ? vswz(row) : kswz(row)));
+      unsigned char *to = smem + st * 2 * STAGE + (is_v(j) ? 0 : STAGE) + row * RB + 16 * (p ^ (is_v(j) ? vswz(row) : kswz(row)));
       *reinterpret_cast<u32x4_t *>(to) = mx_values(codes[j][i], mx_scale(scales[j]));
     };
     // the values at an edge that are not finite, taken out
@@ -207,9 +169,9 @@ __global__ __launch_bounds__(NTH) __attribute__((amdgpu_waves_per_eu(waves(sizeo
 
     // ---- the wave's rows, and their queries' words, on their way beside the first tile
     const Rows32 rows(a, s, r0 + 32 * wave + n);
-    constexpr int kRaw = BF ? 4 * KS : 2 * NQ;  // 16 bytes each
+    constexpr int kRaw = NQ * (BF ? 1 : 2);  // 16 bytes each
     auto raw_element = [&](int y) {  // that word y of the lane begins with
-      return BF ? 64 * (y / 4) + 32 * (y / 2 % 2) + 16 * half + 8 * (y % 2) : 16 * (y / 2) + 8 * half + 4 * (y % 2);
+      return BF ? 16 * y + 8 * half : 16 * (y / 2) + 8 * half + 4 * (y % 2);
     };
     u32x4_t raw[kRaw];
     {
@@ -232,59 +194,23 @@ __global__ __launch_bounds__(NTH) __attribute__((amdgpu_waves_per_eu(waves(sizeo
     };
     uint64_t there = load(k_first, first_page, true);
     int page = lookup(k_first + TK);
-    u32x4_t q[BF ? 1 : QP][BF ? 1 : NQ];  // fp32: bf16 parts
-    // bf16: two parts of e4m3 (high, low) under scales of 32 elements, as the scaled
-    // MFMA takes them: a lane has 16 elements of each of two blocks, and the scale of
-    // block `half`, of the parts of two steps in a word
-    i32x8_t q8[BF ? 2 : 1][BF ? KS : 1];
-    uint32_t q8_scale[BF ? (KS + 1) / 2 : 1] = {};
-    {
-      settle_raw();
+    u32x4_t q[QP][NQ];
+    settle_raw();
+#pragma unroll
+    for (int j = 0; j < NQ; ++j) {
       if constexpr (BF) {
-#pragma unroll
-        for (int j = 0; j < KS; ++j) {
-          uint32_t mine = 0;
-#pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            const u32x4_t *w = raw + 4 * j + 2 * b;
-            u16x2_t most = {0, 0};
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2_t, w[i / 4][i % 4] & 0x7fff7fffu));
-            int field = max((int)most[0], (int)most[1]) >> 7;  // the largest magnitude's exponent + 127
-            field = max(field, __shfl_xor(field, 32));
-            // The largest magnitude becomes 128 .. 256.  The high part has four digits
-            // of each number, the low one, 16 times finer, the other four of a bf16
-            // number; numbers of 2^-13 of the block's largest and less lose some.
-            const bool finite = field < 255;  // else the row is NaN
-            field = min(max(field, 17), 254);
-            const float scale = __uint_as_float((uint32_t)(field - 7) << 23);
-            const float by16 = __uint_as_float((uint32_t)(127 + 7 + 127 + 4 - field) << 23);
-            const uint32_t bytes = finite ? (uint32_t)(field - 7) | (uint32_t)(field - 11) << 8 : kMxNan * 0x101u;
-            mine = b == half ? bytes : mine;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              int high, low;
-              to_e4m3(w[i / 2][2 * (i & 1)], w[i / 2][2 * (i & 1) + 1], scale, by16, &high, &low);
-              q8[0][j][4 * b + i] = high, q8[1][j][4 * b + i] = low;
-            }
-          }
-          q8_scale[j / 2] |= mine << (16 * (j % 2));
-        }
+        q[0][j] = raw[j];
       } else {
+        float x[8];
 #pragma unroll
-        for (int j = 0; j < NQ; ++j) {
-          float x[8];
+        for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(raw[2 * j + i / 4][i % 4]);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(raw[2 * j + i / 4][i % 4]);
+        for (int p = 0; p < QP; ++p)
 #pragma unroll
-          for (int p = 0; p < QP; ++p)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              q[p][j][i] = tops(x[2 * i], x[2 * i + 1]);
-              x[2 * i] -= top(x[2 * i]), x[2 * i + 1] -= top(x[2 * i + 1]);
-            }
-        }
+          for (int i = 0; i < 4; ++i) {
+            q[p][j][i] = tops(x[2 * i], x[2 * i + 1]);
+            x[2 * i] -= top(x[2 * i]), x[2 * i + 1] -= top(x[2 * i + 1]);
+          }
       }
     }
     settle(there);
@@ -304,7 +230,6 @@ __global__ __launch_bounds__(NTH) __attribute__((amdgpu_waves_per_eu(waves(sizeo
     bool far = false;  // of some row of the wave
     bool missed = false;  // the row sees a value that is not finite at an edge
 
-
     for (int t = 0; t < take; ++t) {
       const int k0 = k_first + t * TK, st = t & 1;
       meet();  // the tile is there, and the previous one is done with
@@ -317,51 +242,9 @@ __global__ __launch_bounds__(NTH) __attribute__((amdgpu_waves_per_eu(waves(sizeo
       settle(there_next);
       if (__builtin_expect(shared.edge(k0 + TK, TK), 0)) take_out(st ^ 1);
       if (rows.see(k0, TK)) {
-        const unsigned char *vt = smem + st * STAGE, *kt = vt + VST;
+        const unsigned char *vt = smem + st * 2 * STAGE, *kt = vt + STAGE;
         f32x16_t sc[KT];
-        if constexpr (BF) {
-          // ---- scores: codes and scales of keys as they are held, the queries' parts
-          // one after the other
-          i32x8_t k[KT * KS];
-          uint32_t ks[KT][(CR + 3) / 4];
-#pragma unroll
-          for (int u = 0; u < KT; ++u) {
-            const int key = 32 * u + n;
-#pragma unroll
-            for (int i = 0; i < (CR + 3) / 4; ++i)
-              if constexpr (CR == 2) ks[u][i] = *reinterpret_cast<const uint16_t *>(kt + KST + key * CR) >> (8 * half);
-              else ks[u][i] = *reinterpret_cast<const uint32_t *>(kt + KST + key * CR + 4 * i) >> (8 * half);
-#pragma unroll
-            for (int j = 0; j < KS; ++j) {
-              const u32x4_t w = *reinterpret_cast<const u32x4_t *>(kt + key * CR * 16 + 16 * ((2 * j + half) ^ kswz(key)));
-              k[u * KS + j] = i32x8_t{(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
-            }
-          }
-          __builtin_amdgcn_sched_barrier(0);
-          constexpr int kSteps = 2 * KT * KS;
-#pragma unroll
-          for (int y = 0; y < kSteps; ++y) {
-            const int p = 1 - y / (KT * KS), u = y % KT, j = y / KT % KS;
-            if (y < KT)
-#pragma unroll
-              for (int e = 0; e < 16; ++e) sc[u][e] = 0.f;
-            // of a word of scales: the block 2 j + half's byte, and the step's part's
-#define MX4_MFMA(A, B) \
-  sc[u] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k[u * KS + j], q8[p][j], sc[u], 4, 0, A, ks[u][j / 2], B, q8_scale[j / 2])
-            if (j % 2 == 0) {
-              if (p == 0) MX4_MFMA(0, 0);
-              else MX4_MFMA(0, 1);
-            } else {
-              if (p == 0) MX4_MFMA(2, 2);
-              else MX4_MFMA(2, 3);
-            }
-#undef MX4_MFMA
-            // the next tile's pieces, evenly
-#pragma unroll
-            for (int i = 4 * NP * y / kSteps; i < 4 * NP * (y + 1) / kSteps; ++i) unpack(i / 4, i % 4, st ^ 1);
-            __builtin_amdgcn_sched_barrier(0);
-          }
-        } else {
+        {
           // ---- scores.  Keys are read kAhead operands before their use; the
           // fences keep the compiler from moving each read next to its use.
           constexpr int kSteps = KT * NQ, kAhead = 4;
@@ -526,8 +409,7 @@ __global__ __launch_bounds__(NTH) __attribute__((amdgpu_waves_per_eu(waves(sizeo
 
 template <typename T, int DP, int DC, bool NEAR>
 hipError_t launch_as(const Mx4AttnArgs &a, int grid, hipStream_t s) {
-  const size_t values = (size_t)TK * DP * 2, keys = sizeof(T) == 2 ? TK * (DP / 32) * 17 : values;
-  const size_t tiles = 2 * (values + keys);
+  const size_t tiles = 4 * (size_t)TK * DP * 2;
   const size_t lds = tiles + batch_ints(a.S) * 4, largest = tiles + batch_ints(kMaxSeqs) * 4;
   if (a.item_rows != BM) return hipErrorInvalidValue;
   auto kernel = mx4_tile_kernel<T, DP, DC, NEAR>;
