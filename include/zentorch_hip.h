@@ -359,8 +359,10 @@ size_t zt_woq_moe_workspace_size(int64_t T, int64_t H, int64_t topk, int64_t E,
  * name it; a page with count 0 is free.  Page ids, slots and positions come
  * from the device, so no call can refuse a bad one: each says what it does
  * with it, and none reads or writes outside the arrays for it.  Outputs and
- * workspaces are arrays of their own: one that overlaps an input or another
- * output is refused.
+ * workspaces are arrays of their own.  Attention, the page ops and the calls on a
+ * cache in 4 bits refuse one that overlaps an input or another output; the two
+ * rotary calls on this cache do not look.  Nor is the cache that an append writes
+ * compared with what it reads: its arrays must be apart from that and each other.
  */
 typedef struct zt_kv_cache {
   void *k, *v;
@@ -527,7 +529,7 @@ typedef struct zt_kv_cache_mxfp4 {
  * rounded once, as there; a key is quantised as its rotation comes out exactly,
  * without a rounding before.  A row without a position (past the table) is NaN
  * there too.  Tokens without a slot leave the cache alone, and two tokens must
- * not share a slot.  The cache's four arrays must not overlap.
+ * not share a slot.
  */
 int zt_rotary_cache_append_mxfp4(const void *q, int32_t dtype, int64_t T, int64_t H, const int64_t *q_strides,
                                  const void *k, const int64_t *k_strides, const void *v,

@@ -239,6 +239,13 @@ int zt_paged_attention(const void *q, int64_t T, int64_t H, int64_t ld_token, in
   if (touches_rows(to, q, T, H, cache->head_dim, ld_token, ld_head, es) || overlap(to, scratch) ||
       touches_rows(scratch, q, T, H, cache->head_dim, ld_token, ld_head, es))
     return api_fail(ZT_EINVAL, "%s: query, output and workspace must not overlap", op);
+  auto held = [&](const void *p, const int64_t *ld) {
+    return Strided{p, cache->head_dim * es, {cache->pages, cache->heads, cache->page_size}, {ld[0] * es, ld[1] * es, ld[2] * es}};
+  };
+  for (const Span &s : {to, scratch})
+    if (touches(s, {{block_table, S * W, 4}, {cu_seqlens, S + 1, 4}, {context_lens, S, 4}},
+                {held(cache->k, cache->k_strides), held(cache->v, cache->v_strides)}))
+      return api_fail(ZT_EINVAL, "%s: output or workspace overlap the cache, the table or the lengths", op);
   a.q = q, a.q_ld[0] = ld_token, a.q_ld[1] = ld_head;
   a.k = cache->k, a.v = cache->v;
   for (int i = 0; i < 3; ++i) a.k_ld[i] = cache->k_strides[i], a.v_ld[i] = cache->v_strides[i];

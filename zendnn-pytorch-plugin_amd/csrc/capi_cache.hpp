@@ -3,6 +3,7 @@
 #pragma once
 
 #include <cmath>
+#include <utility>
 
 #include "zt_cache.hpp"
 
@@ -44,6 +45,41 @@ inline bool touches_rows(const Span &s, const void *x, int64_t T, int64_t H, int
   // token t's rows are at [t ld, t ld + token): the first that ends past `from`
   const int64_t t = from < token || ld == 0 ? 0 : (from - token) / ld + 1;
   return t < T && t * ld < end && t * ld + token > from;
+}
+// Rows of `row` bytes at every sum of its indices' strides (in bytes, not negative).
+struct Strided {
+  const void *p;
+  int64_t row, n[3], ld[3];
+};
+// Whether bytes [from, end) from x's start on lie on its rows, the indices before d at
+// 0.  Strides descend, so that few of an index's entries begin before `from` and reach
+// past it; more than that lie on each other, and are taken as one piece.
+inline bool touches_at(const Strided &x, int d, __int128 from, __int128 end) {
+  __int128 inner = x.row;
+  for (int i = d + 1; i < 3; ++i) inner += (__int128)(x.n[i] - 1) * x.ld[i];
+  const __int128 ld = d < 3 ? x.ld[d] : 0, n = d < 3 ? x.n[d] : 1;
+  if (end <= 0 || from >= inner + (n - 1) * ld) return false;
+  if (d == 3 || from <= 0) return true;  // on the first row
+  if (ld == 0) return touches_at(x, d + 1, from, end);
+  const __int128 first = from < inner ? 0 : (from - inner) / ld + 1;
+  for (__int128 i = first; i < n && i * ld < end; ++i)
+    if (i - first == 64 || touches_at(x, d + 1, from - i * ld, end - i * ld)) return true;
+  return false;
+}
+// Whether s lies on one of x's rows (it may lie between two).
+inline bool touches(const Span &s, Strided x) {
+  if (s.elems <= 0 || x.n[0] <= 0 || x.n[1] <= 0 || x.n[2] <= 0) return false;
+  for (int i : {0, 1, 0})
+    if (x.ld[i] < x.ld[i + 1]) std::swap(x.ld[i], x.ld[i + 1]), std::swap(x.n[i], x.n[i + 1]);
+  const __int128 from = (__int128)reinterpret_cast<uintptr_t>(s.p) - reinterpret_cast<uintptr_t>(x.p);
+  return touches_at(x, 0, from, from + (__int128)s.elems * s.size);
+}
+inline bool touches(const Span &s, std::initializer_list<Span> whole, std::initializer_list<Strided> rows) {
+  for (const Span &x : whole)
+    if (overlap(s, x)) return true;
+  for (const Strided &x : rows)
+    if (touches(s, x)) return true;
+  return false;
 }
 inline int check_apart(const char *op, std::initializer_list<Span> in, std::initializer_list<Span> out) {
   for (auto o = out.begin(); o != out.end(); ++o) {

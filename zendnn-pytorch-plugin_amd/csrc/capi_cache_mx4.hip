@@ -46,6 +46,23 @@ Mx4Rows rows_of(void *codes, const int64_t *ld, uint8_t *scales, const int64_t *
 Mx4Rows keys_of(const zt_kv_cache_mxfp4 *c) { return rows_of(c->k, c->k_strides, c->k_scales, c->k_scale_strides); }
 Mx4Rows values_of(const zt_kv_cache_mxfp4 *c) { return rows_of(c->v, c->v_strides, c->v_scales, c->v_scale_strides); }
 
+
+// The cache's four arrays.
+struct CacheRows {
+  Strided k, v, k_scales, v_scales;
+};
+CacheRows arrays_of(const zt_kv_cache_mxfp4 *c) {
+  auto of = [&](const void *p, int64_t row, const int64_t *ld) {
+    return Strided{p, row * blocks_of_row(c), {c->pages, c->heads, c->page_size}, {ld[0], ld[1], ld[2]}};
+  };
+  return {of(c->k, 16, c->k_strides), of(c->v, 16, c->v_strides), of(c->k_scales, 1, c->k_scale_strides),
+          of(c->v_scales, 1, c->v_scale_strides)};
+}
+bool touches_cache(const Span &s, const zt_kv_cache_mxfp4 *c, std::initializer_list<Span> others) {
+  const CacheRows r = arrays_of(c);
+  return touches(s, others, {r.k, r.v, r.k_scales, r.v_scales});
+}
+
 }  // namespace
 
 extern "C" {
@@ -70,8 +87,10 @@ int zt_rotary_cache_append_mxfp4(const void *q, int32_t dtype, int64_t T, int64_
   const Span out{q_out, T * H * D, es};
   if (touches_rows(out, q, T, H, D, q_strides[0], q_strides[1], es) ||
       touches_rows(out, k, T, KV, D, k_strides[0], k_strides[1], es) ||
-      touches_rows(out, v, T, KV, D, v_strides[0], v_strides[1], es))
-    return api_fail(ZT_EINVAL, "%s: the output overlaps an input", op);
+      touches_rows(out, v, T, KV, D, v_strides[0], v_strides[1], es) ||
+      touches(out, Strided{table, R * 4, {length, 1, 1}, {ld_table * 4, 0, 0}}) ||
+      touches_cache(out, cache, {{positions, T, 8}, {slots, T, 8}}))
+    return api_fail(ZT_EINVAL, "%s: the output overlaps an input or the cache", op);
   Mx4AppendArgs a{};
   a.q = q, a.k = k, a.v = v, a.q_out = q_out;
   for (int i = 0; i < 2; ++i) a.q_ld[i] = q_strides[i], a.k_ld[i] = k_strides[i], a.v_ld[i] = v_strides[i];
@@ -100,6 +119,8 @@ int zt_cache_read_mxfp4(const zt_kv_cache_mxfp4 *cache, const int64_t *slots, in
   if (!divides16(k_out, {}, es) || !divides16(v_out, {}, es))
     return api_fail(ZT_EUNSUPPORTED, "%s: the outputs need 16-byte alignment", op);
   if (const int rc = check_apart(op, {{slots, n, 8}}, {{k_out, rows, es}, {v_out, rows, es}})) return rc;
+  if (touches_cache({k_out, rows, es}, cache, {}) || touches_cache({v_out, rows, es}, cache, {}))
+    return api_fail(ZT_EINVAL, "%s: an output overlaps the cache", op);
   Mx4ReadArgs a{};
   a.keys = keys_of(cache), a.values = values_of(cache);
   a.slots = slots, a.n = n, a.pages = cache->pages, a.page_size = (int)cache->page_size;
@@ -159,6 +180,9 @@ int zt_paged_attention_mxfp4(const void *q, int32_t dtype, int64_t T, int64_t H,
   if (touches_rows(to, q, T, H, cache->head_dim, ld_token, ld_head, es) || overlap(to, scratch) ||
       touches_rows(scratch, q, T, H, cache->head_dim, ld_token, ld_head, es))
     return api_fail(ZT_EINVAL, "%s: query, output and workspace must not overlap", op);
+  for (const Span &s : {to, scratch})
+    if (touches_cache(s, cache, {{block_table, S * W, 4}, {cu_seqlens, S + 1, 4}, {context_lens, S, 4}}))
+      return api_fail(ZT_EINVAL, "%s: output or workspace overlap the cache, the table or the lengths", op);
   a.q = q, a.q_ld[0] = ld_token, a.q_ld[1] = ld_head;
   a.k = cache->k, a.v = cache->v, a.k_sc = cache->k_scales, a.v_sc = cache->v_scales;
   for (int i = 0; i < 3; ++i) {
