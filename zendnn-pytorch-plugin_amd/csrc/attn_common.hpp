@@ -175,7 +175,7 @@ __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
 
 struct PlanShared {
   int part[16];
-  int item, before, most;
+  int item, before, most;  // most: the longest item, or whether one is too long for all to be whole
 };
 
 struct Plan {
@@ -209,6 +209,7 @@ __device__ __forceinline__ Plan make_plan(const AttnArgs &a, int BM, int UK, con
                                           PlanShared *sh) {
   const int tid = threadIdx.x;
   Plan p{};
+  if (Cost::kJoin > 0 && tid == 0) sh->most = 0;
   for (int i0 = 0; i0 < a.S; i0 += N) {
     const int i = i0 + tid;
     int tiles = 0, total;
@@ -258,17 +259,26 @@ __device__ __forceinline__ Plan make_plan(const AttnArgs &a, int BM, int UK, con
   // (4 x 448 behind 2048: 105 / 117).
   // A Cost may name what a join is worth (kJoin): fewer (item, head)s than workgroups
   // then are whole too, if the longest is no longer than an equal span and that; they
-  // are dealt to the XCDs evenly.
+  // are dealt to the XCDs evenly.  (Where the average one is longer, the longest is
+  // not looked at.)
   const int pairs = p.items * a.KV, grid = (int)gridDim.x;
   bool whole = p.items <= N && pairs <= grid && 32 * (int64_t)pairs >= 31 * (int64_t)grid;
-  const bool few = Cost::kJoin > 0 && !whole && p.items <= N && pairs <= grid;
+  const bool few = Cost::kJoin > 0 && !whole && p.items <= N && pairs <= grid &&
+                   ((int64_t)sum - Cost::kJoin * (int64_t)p.items) * grid <= (int64_t)sum * pairs;
   if (whole || few) {
-    if (tid == 0) sh->most = 0;
-    __syncthreads();
-    if (cost) atomicMax(&sh->most, cost);
-    __syncthreads();
-    if (few) whole = (int64_t)(sh->most - Cost::kJoin) * grid <= (int64_t)sum * a.KV;
-    else whole = (int64_t)sh->most * p.items <= (int64_t)sum + sum / 4;
+    if constexpr (Cost::kJoin > 0) {
+      const int64_t limit = few ? (int64_t)sum * a.KV : (int64_t)sum + sum / 4;
+      const bool longer = (int64_t)(cost - (few ? Cost::kJoin : 0)) * (few ? grid : p.items) > limit;
+      if (__ballot(longer) && (tid & 63) == 0) sh->most = 1;
+      __syncthreads();
+      whole = sh->most == 0;
+    } else {
+      if (tid == 0) sh->most = 0;
+      __syncthreads();
+      if (cost) atomicMax(&sh->most, cost);
+      __syncthreads();
+      whole = (int64_t)sh->most * p.items <= (int64_t)sum + sum / 4;
+    }
     if (whole) {
       const int xcd = blockIdx.x & 7, each = grid / 8, i = blockIdx.x >> 3;
       const int here = pairs / 8 + (xcd < pairs % 8 ? 1 : 0);  // of this XCD; its others have numbers past the last

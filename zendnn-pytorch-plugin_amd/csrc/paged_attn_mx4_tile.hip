@@ -18,8 +18,12 @@ __device__ __forceinline__ uint32_t tops(float lo, float hi) {
 __device__ __forceinline__ float top(float x) { return __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
 
 // As in paged_attn_tile.hip, whose item ends and tiles these resemble.  A join is worth
-// four blocks: eight whole fp32 sequences of up to 500 take 33-38 us in whole items,
-// 40-44 in equal spans; 16 chunks of 100 tokens and the like are the same either way.
+// four blocks.  Measured, whole items by that rule against equal spans, us: sequences
+// of one length seen whole, 8 of 500 (16 heads of 64, fp32) 37 / 44, in bf16 25 / 34,
+// causal ones of 400 23 / 28, 4 of 256 (32 heads of 128) 22 / 35.  Where the rule cuts the
+// items its test costs up to 0.5 us: 8 x 128 behind 384 (head_dim 64) 30.6 / 30.1, 16
+// mixed 29.9 / 29.5, 3 causal ones of 500 38.3 / 37.9; one of 512 31.0 / 30.9, one of 1024
+// 48.8 / 48.9.
 struct Mx4TileCost {
   static constexpr int kLead = 15, kMost = kTileCostMost, kLeast = 4 * kMost, kJoin = 24;
   static __device__ __forceinline__ int of(int rows) { return 4 + (rows + 63) / 64; }
