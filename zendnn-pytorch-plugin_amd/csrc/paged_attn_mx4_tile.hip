@@ -109,7 +109,7 @@ __global__ __launch_bounds__(NTH) __attribute__((amdgpu_waves_per_eu(waves(sizeo
     const uint8_t *vbase = static_cast<const uint8_t *>(a.v) + h * a.v_ld[1];
     const uint8_t *ks_base = a.k_sc + h * a.k_sc_ld[1], *vs_base = a.v_sc + h * a.v_sc_ld[1];
 
-    auto lookup = [&](int at) { return pages.lookup(a, at + lane); };
+    auto lookup = [&](int at) { return pages.template lookup<waves(BF, DC) == 2>(a, at + lane); };
     const int k_first = (seg.b0 + seg.bb) * TK;
     // where in its page the thread's row of the next tile to be loaded is
     int row_off = k_first + row - (int)fast_div(k_first + row, a.div_page) * a.page_size;
