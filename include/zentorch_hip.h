@@ -507,8 +507,10 @@ int zt_cache_copy_pages(void *const *caches, int64_t n_caches, int64_t pages, in
  * multiplies.  Writing picks the E for which the block's largest magnitude is
  * at least 3.5 and less than 7 scales, held to -125 .. 125, and for each number
  * the nearest code (of two equally near ones the even one; magnitudes past 6
- * scales take 6): off by a fifth of the block's largest number at most.  A
- * block with an infinity or a NaN is written as codes of 0 under the byte 255.
+ * scales take 6).  A number is off by a fifth of its block's largest at most, where
+ * that is from 3.5 2^-125 on and below 7 2^125; below that by 2^-126 at most, and
+ * above it 6 2^125 is the most that is held.  A block with an infinity or a NaN is
+ * written as codes of 0 under the byte 255.
  * Read, the bytes 253 .. 255 stand for NaN.
  *
  * codes [pages, heads, page_size, 16 blocks] bytes, each row on 16 bytes;
@@ -526,10 +528,10 @@ typedef struct zt_kv_cache_mxfp4 {
 
 /*
  * zt_rotary_cache_append into a cache held in 4 bits.  q_out is fp32's result
- * rounded once, as there; a key is quantised as its rotation comes out exactly,
- * without a rounding before.  A row without a position (past the table) is NaN
- * there too.  Tokens without a slot leave the cache alone, and two tokens must
- * not share a slot.
+ * rounded once, as there; a key is quantised as its rotation comes out in 64 bits,
+ * where the products are exact and their sum is rounded once, to 53 digits.  A row
+ * without a position (past the table) is NaN there too.  Tokens without a slot
+ * leave the cache alone, and two tokens must not share a slot.
  */
 int zt_rotary_cache_append_mxfp4(const void *q, int32_t dtype, int64_t T, int64_t H, const int64_t *q_strides,
                                  const void *k, const int64_t *k_strides, const void *v,

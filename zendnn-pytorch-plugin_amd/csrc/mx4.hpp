@@ -7,7 +7,7 @@
 // one of 0, 0.5, 1, 1.5, 2, 3, 4, 6.  E is such that 3.5 <= amax / 2^E < 7 for the
 // block's largest magnitude (a number is off by one scale at most: from 7 on the next
 // E's codes are nearer), held to -125 .. 125: every value then is a normal bf16
-// number, exactly.  A code is the
+// number, exactly (and the largest fp32 number, of nearly 8 scales, becomes 6).  A code is the
 // nearest one, of two equally near ones the even one.  A block with an infinity or
 // a NaN has the byte 255 and codes of 0.  Read, 255 stands for NaN throughout, and
 // so do 253 and 254, with which some codes' values would be past bf16's largest.
