@@ -58,6 +58,13 @@ __device__ __forceinline__ u32x4_t mx_values(uint32_t w, float scale) {
   return y;
 }
 
+// The upper 16 bits of two numbers, as a pair of bf16, and of one: the first of the
+// bf16 parts that an fp32 number is cut into.
+__device__ __forceinline__ uint32_t tops(float lo, float hi) {
+  return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
+}
+__device__ __forceinline__ float top(float x) { return __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
+
 // Codes and scales of keys or values: strides of page, head and token in bytes.
 struct Mx4Rows {
   uint8_t *codes, *scales;

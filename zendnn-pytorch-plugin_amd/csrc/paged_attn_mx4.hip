@@ -34,12 +34,6 @@ __device__ __forceinline__ float sum_over_groups(float x) {
   return x + __shfl_xor(x, 32);
 }
 
-// The upper 16 bits of two numbers, as a pair of bf16.
-__device__ __forceinline__ uint32_t tops(float lo, float hi) {
-  return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
-}
-__device__ __forceinline__ float top(float x) { return __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
-
 // 16 rows of one cache head against a span of its keys.
 //
 // Bound by HBM on large calls, and by its trips to memory on small ones: a key and its

@@ -12,11 +12,6 @@ namespace {
 // memory stay on their way: what they bring goes to this thread's registers.
 __device__ __forceinline__ void meet() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-__device__ __forceinline__ uint32_t tops(float lo, float hi) {
-  return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
-}
-__device__ __forceinline__ float top(float x) { return __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
-
 // As in paged_attn_tile.hip, whose item ends and tiles these resemble.  A join is worth
 // four blocks.  Measured, whole items by that rule against equal spans, us: sequences
 // of one length seen whole, 8 of 500 (16 heads of 64, fp32) 37 / 44, in bf16 25 / 34,
@@ -85,8 +80,6 @@ __global__ __launch_bounds__(NTH) __attribute__((amdgpu_waves_per_eu(waves(sizeo
 
   const float c = score_factor(a.scale);
   const int G = a.group;
-  const char *zero = reinterpret_cast<const char *>(kZeroRow);
-  const uint8_t *nothing = reinterpret_cast<const uint8_t *>(kZeroRow);
   // the 16-byte pieces of a row are permuted, so that 16 lanes meet no bank twice
   auto kswz = [](int row) { return PR >= 16 ? row & 15 : row & 7; };
   auto vswz = [](int row) { return PR >= 16 ? (row & 3) << 2 | ((row >> 2) & 3) : ((row >> 1) & 1) << 2; };
