@@ -17,8 +17,8 @@ __device__ __forceinline__ void meet() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts
 // of one length seen whole, 8 of 500 (16 heads of 64, fp32) 37 / 44, in bf16 25 / 34,
 // causal ones of 400 23 / 28, 4 of 256 (32 heads of 128) 22 / 35.  Where the rule cuts the
 // items its test costs up to 0.5 us: 8 x 128 behind 384 (head_dim 64) 30.6 / 30.1, 16
-// mixed 29.9 / 29.5, 3 causal ones of 500 38.3 / 37.9; one of 512 31.0 / 30.9, one of 1024
-// 48.8 / 48.9.
+// mixed 30.9 / 30.5, 3 causal ones of 500 38.3 / 37.9; one of 512 31.0 / 30.9, one of 1024
+// 48.8 / 48.9.  Worth 16 or 12 it would cut the eight of 500 and the four of 256 again.
 struct Mx4TileCost {
   static constexpr int kLead = 15, kMost = kTileCostMost, kLeast = 4 * kMost, kJoin = 24;
   static __device__ __forceinline__ int of(int rows) { return 4 + (rows + 63) / 64; }
@@ -28,7 +28,7 @@ constexpr int NW = 4, NTH = 64 * NW, BM = 32 * NW, TK = 64;
 
 // Waves per SIMD, and so workgroups per CU: two, but for sizes whose queries and
 // outputs need the registers of both (fp32, head_dim 128, 512 tokens behind 1536:
-// 76 us with one, 125 with two, which spill; head_dim 96: 64 and 62).
+// 75 us with one, 125 with two, which spill; head_dim 96: 66 and 64).
 constexpr int waves(bool bf, int dim) { return dim <= (bf ? 128 : 96) ? 2 : 1; }
 
 // Four waves of 32 rows each against a span of the keys of one cache head.
@@ -44,13 +44,14 @@ constexpr int waves(bool bf, int dim) { return dim <= (bf ? 128 : 96) ? 2 : 1; }
 // digits).  Scores by scaled MFMAs over the codes themselves (e2m1 by queries in two
 // parts of e4m3) were 7 % faster on the chunk below and 3 % slower on 33 mixed
 // sequences, but two parts under one scale to 32 numbers lose the digits of those below
-// 2^-13 of the largest: with a channel 2^16 times the others, outputs were off by a tenth.
+// 2^-13 of the largest: with a channel 2^16 times the others, outputs were off by more than
+// 0.1 where values are about 1.
 //
 // The running maximum, the weights and the second product are those of
 // paged_attn_tile.hip, on 32x32 MFMAs, transposed.
 //
-// Measured (32 query and 8 cache heads of 128, bf16): 2048 tokens behind 6144 264 us, 0.91
-// PFLOP/s (a large product of the library reaches 1.2); copies of the kernel took 239
+// Measured (32 query and 8 cache heads of 128, bf16): 2048 tokens behind 6144 260-264 us,
+// 0.92 PFLOP/s (a large product of the library reaches 1.2); copies of the kernel took 239
 // without unpacking, 240 without the loads, 242 without the exponentials beside 261.
 // 33 mixed sequences 53 us.  Eight whole fp32 sequences of up to 500, 16 heads of 64: 33 us.
 //
