@@ -510,8 +510,7 @@ int zt_cache_copy_pages(void *const *caches, int64_t n_caches, int64_t pages, in
  * scales take 6).  A number is off by a fifth of its block's largest at most, where
  * that is from 3.5 2^-125 on and below 7 2^125; below that by 2^-126 at most, and
  * above it 6 2^125 is the most that is held.  A block with an infinity or a NaN is
- * written as codes of 0 under the byte 255.
- * Read, the bytes 253 .. 255 stand for NaN.
+ * written as codes of 0 under the byte 255.  Read, the bytes 253 .. 255 stand for NaN.
  *
  * codes [pages, heads, page_size, 16 blocks] bytes, each row on 16 bytes;
  * scales [pages, heads, page_size, blocks] bytes, anywhere.  The other tensors

@@ -46,7 +46,6 @@ Mx4Rows rows_of(void *codes, const int64_t *ld, uint8_t *scales, const int64_t *
 Mx4Rows keys_of(const zt_kv_cache_mxfp4 *c) { return rows_of(c->k, c->k_strides, c->k_scales, c->k_scale_strides); }
 Mx4Rows values_of(const zt_kv_cache_mxfp4 *c) { return rows_of(c->v, c->v_strides, c->v_scales, c->v_scale_strides); }
 
-
 // The cache's four arrays.
 struct CacheRows {
   Strided k, v, k_scales, v_scales;
